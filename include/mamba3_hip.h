@@ -27,6 +27,8 @@
  *                      portable mamba3_step ops.py:825-879 with the step prologue of
  *                      _Mamba3Mixer.step model.py:431-469.
  * m3_linear has no reference hook: it takes the decode step's projection GEMMs (see below).
+ * m3_gated_scan and m3_gated_scan_bwd have no counterpart in the reference: an elementwise gated
+ * recurrence beside the matrix-state one, with its gradients.
  */
 #ifndef MAMBA3_HIP_H
 #define MAMBA3_HIP_H
@@ -261,6 +263,64 @@ typedef struct {
 } m3_rms_norm_args;
 
 int m3_rms_norm(const m3_rms_norm_args* args, hipStream_t stream);
+
+/*
+ * A gated linear recurrence over whole sequences, one FP32 state per channel:
+ *   given form (no gate, no rate):  h_t = exp(decay_t) h_{t-1} + x_t
+ *   gate form (gate and rate):      log a_t = -rate sigmoid(decay_t)
+ *                                   h_t = a_t h_{t-1} + sqrt(1 - a_t^2) sigmoid(gate_t) x_t
+ * out_t = h_t in the activation dtype. length 1 is a decode step; final_state may then (and at
+ * any length) be initial_state itself.
+ * lengths: row b holds max(0, min(lengths[b], L)) tokens; after them out is 0 and the state
+ * stays, whatever x, decay and gate hold there. reset: a token whose byte is not 0 starts from
+ * an empty state (what came before it, NaN and infinities too, is dropped).
+ * rate >= 0; a negative one gives NaN.
+ */
+#define M3_GATED_TILE 128 /* tokens between two of the states that carry holds */
+typedef struct {
+  int32_t batch, length, width;
+  int32_t dtype;           /* of x, decay, gate and out */
+  m3_tensor x, decay;      /* [B, L, C] */
+  m3_tensor gate;          /* [B, L, C], with rate or neither */
+  m3_tensor rate;          /* [C] FP32 */
+  m3_tensor initial_state; /* [B, C] FP32 optional: zeros */
+  const int32_t* lengths;  /* [B] optional: L */
+  const uint8_t* reset;    /* [B, L] optional */
+  int64_t reset_stride;    /* bytes between rows of reset */
+  m3_tensor out;           /* [B, L, C] */
+  m3_tensor final_state;   /* [B, C] FP32 */
+  m3_tensor carry;         /* [ceil(L / M3_GATED_TILE), B, C] FP32 contiguous, optional: the state
+                              after each tile, which m3_gated_scan_bwd reads */
+  void* workspace;
+  size_t workspace_bytes;
+} m3_gated_scan_args;
+
+int m3_gated_scan_workspace_size(const m3_gated_scan_args* args, size_t* bytes);
+int m3_gated_scan(const m3_gated_scan_args* args, hipStream_t stream);
+
+/*
+ * The gradients of m3_gated_scan. fwd holds the forward call's inputs and its carry (out and
+ * final_state are not used; NULL will do); its workspace fields are this call's. With D the
+ * gradient of h:
+ *   D_t = dout_t + a_{t+1} D_{t+1}   (dfinal joins after the last token)
+ *   given form: dx = D, ddecay = D a h_{t-1}
+ *   gate form:  dx = D s q, dgate = D s x q (1 - q), with p, q the gates' sigmoids, s = sqrt(1 - a^2);
+ *               ddecay = -rate p (1 - p) dlog, drate = -sum p dlog,
+ *               dlog = D (a h_{t-1} - q x a^2 / s)
+ * Tokens past a row's length get gradient 0. drate is summed in a fixed order.
+ */
+typedef struct {
+  m3_gated_scan_args fwd;
+  m3_tensor dout;          /* [B, L, C] activation dtype */
+  m3_tensor dfinal;        /* [B, C] FP32 optional: zeros */
+  m3_tensor dx, ddecay;    /* [B, L, C] activation dtype */
+  m3_tensor dgate;         /* [B, L, C] (gate form) */
+  m3_tensor drate;         /* [C] FP32 (gate form) */
+  m3_tensor dinitial;      /* [B, C] FP32 optional */
+} m3_gated_scan_bwd_args;
+
+int m3_gated_scan_bwd_workspace_size(const m3_gated_scan_bwd_args* args, size_t* bytes);
+int m3_gated_scan_bwd(const m3_gated_scan_bwd_args* args, hipStream_t stream);
 
 const char* m3_last_error(void);
 int m3_abi_version(void);

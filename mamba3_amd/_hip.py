@@ -95,9 +95,29 @@ class RmsNormArgs(ctypes.Structure):
     ]
 
 
+class GatedScanArgs(ctypes.Structure):
+    _fields_ = [
+        *[(n, ctypes.c_int32) for n in ("batch", "length", "width", "dtype")],
+        *[(n, _T) for n in ("x", "decay", "gate", "rate", "initial_state")],
+        ("lengths", ctypes.c_void_p), ("reset", ctypes.c_void_p),
+        ("reset_stride", ctypes.c_int64),
+        *[(n, _T) for n in ("out", "final_state", "carry")],
+        ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_size_t),
+    ]
+
+
+class GatedScanBwdArgs(ctypes.Structure):
+    _fields_ = [("fwd", GatedScanArgs),
+                *[(n, _T) for n in ("dout", "dfinal", "dx", "ddecay", "dgate", "drate",
+                                    "dinitial")]]
+
+
 ENTRY_POINTS = ("m3_scan_fwd", "m3_scan_workspace_size", "m3_scan_segments", "m3_scan_fwd_noalloc",
                 "m3_chunk_state", "m3_step", "m3_linear", "m3_linear_workspace_size",
-                "m3_rms_norm", "m3_last_error", "m3_abi_version")
+                "m3_rms_norm", "m3_gated_scan", "m3_gated_scan_workspace_size",
+                "m3_gated_scan_bwd", "m3_gated_scan_bwd_workspace_size", "m3_last_error",
+                "m3_abi_version")
+GATED_TILE = 128  # M3_GATED_TILE: tokens between two of the states a gated scan's carry holds
 SCRATCH_BYTES = 64 << 20  # M3_SCRATCH_BYTES: the no-alloc scan's per-GPU scratch
 
 _lib: ctypes.CDLL | None = None
@@ -113,11 +133,12 @@ def load() -> ctypes.CDLL:
             f"{LIB_PATH} is not built; run `python -m mamba3_amd.build` (hipcc, gfx950)")
     lib = ctypes.CDLL(LIB_PATH)
     for name in ("m3_scan_fwd", "m3_scan_fwd_noalloc", "m3_chunk_state", "m3_step", "m3_linear",
-                 "m3_rms_norm"):
+                 "m3_rms_norm", "m3_gated_scan", "m3_gated_scan_bwd"):
         fn = getattr(lib, name)
         fn.restype = ctypes.c_int
         fn.argtypes = [ctypes.c_void_p, ctypes.c_void_p]
-    for name in ("m3_scan_workspace_size", "m3_linear_workspace_size"):
+    for name in ("m3_scan_workspace_size", "m3_linear_workspace_size",
+                 "m3_gated_scan_workspace_size", "m3_gated_scan_bwd_workspace_size"):
         fn = getattr(lib, name)
         fn.restype = ctypes.c_int
         fn.argtypes = [ctypes.c_void_p, ctypes.POINTER(ctypes.c_size_t)]
@@ -148,6 +169,12 @@ def tensor(t: torch.Tensor | None) -> Tensor:
     return out
 
 
+def row_tensor(t: torch.Tensor) -> Tensor:
+    """``tensor`` for an operand that is present, in one construction (the decode calls' host time
+    is as long as their kernels')."""
+    return Tensor(t.data_ptr() if t.numel() else None, _DTYPE[t.dtype], 0, t.stride())
+
+
 def dtype_code(dtype: torch.dtype) -> int:
     try:
         return _DTYPE[dtype]
@@ -160,17 +187,22 @@ def scan_workspace(args: ctypes.Structure, device: torch.device,
     """Allocate (through torch's caching allocator) the workspace an entry point needs, as
     its ``query`` function reports it, and record it in ``args``; the caller keeps the
     returned tensor alive across the call."""
-    lib = load()
     nbytes = ctypes.c_size_t(0)
-    rc = getattr(lib, query)(ctypes.byref(args), ctypes.byref(nbytes))
-    if rc != 0:
-        raise HipError(query, rc, lib.m3_last_error().decode(errors="replace"))
+    workspace_query(query, args, nbytes)
     if nbytes.value == 0:
         return None
     ws = torch.empty(nbytes.value, dtype=torch.uint8, device=device)
     args.workspace = ws.data_ptr()
     args.workspace_bytes = nbytes.value
     return ws
+
+
+def workspace_query(name: str, args: ctypes.Structure, nbytes: ctypes.c_size_t) -> None:
+    """A workspace query into ``nbytes``; raise on failure."""
+    lib = load()
+    rc = getattr(lib, name)(ctypes.byref(args), ctypes.byref(nbytes))
+    if rc != 0:
+        raise HipError(name, rc, lib.m3_last_error().decode(errors="replace"))
 
 
 def scan_segments(args: ctypes.Structure, concurrent: int) -> int:
@@ -182,6 +214,19 @@ def scan_segments(args: ctypes.Structure, concurrent: int) -> int:
     if rc != 0:
         raise HipError("m3_scan_segments", rc, lib.m3_last_error().decode(errors="replace"))
     return g.value
+
+
+def launch(name: str, args: ctypes.Structure, device: torch.device) -> None:
+    """``call`` on ``device``'s current torch stream, with that device made current if it is not,
+    and without a stream object."""
+    index = device.index
+    if index != torch.cuda.current_device():
+        with torch.cuda.device(device):
+            return call(name, args, device)
+    lib = load()
+    rc = getattr(lib, name)(ctypes.byref(args), torch._C._cuda_getCurrentRawStream(index))
+    if rc != 0:
+        raise HipError(name, rc, lib.m3_last_error().decode(errors="replace"))
 
 
 def call(name: str, args: ctypes.Structure, device: torch.device) -> None:

@@ -15,6 +15,8 @@ step / scan ran on the HIP path (the reference's ``_TRITON_LAST_DISPATCH`` /
 
 from __future__ import annotations
 
+import ctypes
+
 import torch
 
 from . import _hip
@@ -668,6 +670,189 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = NORM_EPS, *,
     return out, s
 
 
+# --------------------------------------------------------------------------- gated recurrence
+
+
+def _validate_gated(x, decay, gate, rate, state, state_name) -> None:
+    if decay.shape != x.shape or (gate is not None and gate.shape != x.shape):
+        raise ValueError("decay and gate must have the shape of x")
+    if x.dtype not in _FLOAT_DTYPES or decay.dtype != x.dtype or (
+            gate is not None and gate.dtype != x.dtype):
+        raise ValueError("x, decay and gate must share one dtype: float32, bfloat16 or float16")
+    if (gate is None) != (rate is None):
+        raise ValueError("gate and rate must be provided together")
+    width = x.shape[-1]
+    if rate is not None and (rate.shape != (width,) or not rate.is_floating_point()):
+        raise ValueError(f"rate must be a floating tensor of shape {(width,)}")
+    if state is not None and (state.shape != (x.shape[0], width) or state.dtype != torch.float32):
+        raise ValueError(f"{state_name} must be float32 of shape {(x.shape[0], width)}")
+
+
+def _rate32(rate: torch.Tensor | None) -> torch.Tensor | None:
+    if rate is None or (rate.dtype == torch.float32 and rate.is_contiguous()):
+        return rate
+    return rate.float().contiguous()
+
+
+def _gated_args(x, decay, gate, rate, state, lengths, reset) -> _hip.GatedScanArgs:
+    """The inputs of a gated scan [B, L, C] as an argument block; the caller keeps the tensors."""
+    batch, length, width = x.shape
+    args = _hip.GatedScanArgs(batch, length, width, _hip.dtype_code(x.dtype), _hip.row_tensor(x),
+                              _hip.row_tensor(decay))
+    if gate is not None:
+        args.gate, args.rate = _hip.row_tensor(gate), _hip.row_tensor(rate)
+    if state is not None:
+        args.initial_state = _hip.row_tensor(state)
+    if lengths is not None:
+        args.lengths = lengths.data_ptr()
+    if reset is not None:
+        args.reset, args.reset_stride = reset.data_ptr(), reset.stride(0)
+    return args
+
+
+def _gated_forward(x, decay, gate, rate, state, lengths, reset, want_carry):
+    batch, length, width = x.shape
+    args = _gated_args(x, decay, gate, rate, state, lengths, reset)
+    out = torch.empty(batch, length, width, dtype=x.dtype, device=x.device)
+    final = torch.empty(batch, width, dtype=torch.float32, device=x.device)
+    carry = None
+    args.out, args.final_state = _hip.row_tensor(out), _hip.row_tensor(final)
+    if want_carry:
+        carry = torch.empty(-(-length // _hip.GATED_TILE), batch, width, dtype=torch.float32,
+                            device=x.device)
+        args.carry = _hip.row_tensor(carry)
+    ws = _hip.scan_workspace(args, x.device, "m3_gated_scan_workspace_size")
+    _hip.launch("m3_gated_scan", args, x.device)
+    del ws
+    return out, final, carry
+
+
+class _GatedScan(torch.autograd.Function):
+    """``gated_scan`` under autograd: the forward call also leaves the state after every
+    ``GATED_TILE`` tokens, from which the backward call recomputes the states between."""
+
+    @staticmethod
+    def forward(ctx, x, decay, gate, rate, state, lengths, reset):
+        out, final, carry = _gated_forward(x, decay, gate, rate, state, lengths, reset, True)
+        ctx.save_for_backward(x, decay, gate, rate, state, lengths, reset, carry)
+        ctx.set_materialize_grads(False)
+        return out, final
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dout, dfinal):
+        x, decay, gate, rate, state, lengths, reset, carry = ctx.saved_tensors
+        if dout is None and dfinal is None:
+            return (None,) * 7
+        dout = torch.zeros(x.shape, dtype=x.dtype, device=x.device) if dout is None else _inner(dout)
+        dfinal = _inner(dfinal)
+        args = _hip.GatedScanBwdArgs(_gated_args(x, decay, gate, rate, state, lengths, reset),
+                                     _hip.row_tensor(dout))
+        args.fwd.carry = _hip.row_tensor(carry)
+        if dfinal is not None:
+            args.dfinal = _hip.row_tensor(dfinal)
+        dx, ddecay = (torch.empty(x.shape, dtype=x.dtype, device=x.device) for _ in range(2))
+        args.dx, args.ddecay = _hip.row_tensor(dx), _hip.row_tensor(ddecay)
+        dgate = drate = dstate = None
+        if gate is not None:
+            dgate, drate = torch.empty_like(dx), torch.empty_like(rate)
+            args.dgate, args.drate = _hip.row_tensor(dgate), _hip.row_tensor(drate)
+        if state is not None:
+            dstate = torch.empty(state.shape, dtype=torch.float32, device=x.device)
+            args.dinitial = _hip.row_tensor(dstate)
+        need = ctypes.c_size_t(0)
+        _hip.workspace_query("m3_gated_scan_bwd_workspace_size", args, need)
+        ws = torch.empty(need.value, dtype=torch.uint8, device=x.device)
+        args.fwd.workspace, args.fwd.workspace_bytes = ws.data_ptr(), need.value
+        _hip.launch("m3_gated_scan_bwd", args, x.device)
+        return dx, ddecay, dgate, drate, dstate, None, None
+
+
+def gated_scan(x: torch.Tensor, decay: torch.Tensor, gate: torch.Tensor | None = None,
+               rate: torch.Tensor | None = None, *, initial_state: torch.Tensor | None = None,
+               lengths: torch.Tensor | None = None, reset: torch.Tensor | None = None):
+    """A gated linear recurrence over ``[B, L, C]``, one FP32 state per channel (``m3_gated_scan``).
+
+    Without ``gate`` and ``rate``, ``decay`` holds log decays: ``h_t = exp(decay_t) h_{t-1} +
+    x_t``. With them ``decay`` and ``gate`` hold logits and ``rate [C]`` (>= 0) the log decay of an
+    open gate: ``a_t = exp(-rate sigmoid(decay_t))``, ``h_t = a_t h_{t-1} + sqrt(1 - a_t^2)
+    sigmoid(gate_t) x_t``. ``x``, ``decay`` and ``gate`` share one dtype and may be slices of one
+    projection. Returns ``(out [B, L, C] = h in x's dtype, final_state [B, C] FP32)``.
+
+    ``initial_state [B, C]`` FP32 continues a sequence. ``lengths [B]`` (integers; clamped to 0..L)
+    ends each row of a padded batch: past its end ``out`` is 0 and the state stays, whatever the
+    padding holds. ``reset [B, L]`` (bool) marks tokens that start from an empty state, as the
+    first token of each document in a packed row does.
+
+    Unlike the Mamba-3 calls of this module this one has a backward pass: gradients reach ``x``,
+    ``decay``, ``gate``, ``rate`` and ``initial_state`` (once: no second derivatives).
+    """
+    if x.ndim != 3:
+        raise ValueError("x must have shape [B, L, C]")
+    _validate_gated(x, decay, gate, rate, initial_state, "initial_state")
+    batch, length, width = x.shape
+    if lengths is not None and (lengths.shape != (batch,) or
+                                lengths.dtype not in (torch.int32, torch.int64)):
+        raise ValueError(f"lengths must be int32 or int64 of shape {(batch,)}")
+    if reset is not None and (reset.shape != (batch, length) or
+                              reset.dtype not in (torch.bool, torch.uint8)):
+        raise ValueError(f"reset must be bool of shape {(batch, length)}")
+    device = _require_device(x, decay, gate, rate, initial_state, lengths, reset)
+    rate = _rate32(rate)
+    if batch == 0 or length == 0 or width == 0:
+        final = (torch.zeros(batch, width, device=device) if initial_state is None
+                 else initial_state.clone())
+        return torch.empty_like(x), final
+    if lengths is not None:
+        lengths = lengths.clamp(0, length).to(torch.int32).contiguous()
+    if reset is not None:
+        reset = _inner(reset)
+        reset = reset.view(torch.uint8) if reset.dtype == torch.bool else reset
+    x, decay, gate, state = _inner(x), _inner(decay), _inner(gate), _inner(initial_state)
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad
+                                       for t in (x, decay, gate, rate, state)):
+        return _GatedScan.apply(x, decay, gate, rate, state, lengths, reset)
+    return _gated_forward(x, decay, gate, rate, state, lengths, reset, False)[:2]
+
+
+def gated_step(x: torch.Tensor, decay: torch.Tensor, state: torch.Tensor,
+               gate: torch.Tensor | None = None, rate: torch.Tensor | None = None, *,
+               inplace: bool = False):
+    """One token of ``gated_scan``: ``x``, ``decay``, ``gate`` ``[B, C]``, ``state [B, C]`` FP32.
+
+    Returns ``(out [B, C], state')``. ``inplace`` writes the new state into ``state`` (the static
+    cache of a captured decode step), which then needs a unit inner stride. No backward.
+    """
+    if x.ndim != 2:
+        raise ValueError("x must have shape [B, C]")
+    _validate_gated(x, decay, gate, rate, state, "state")
+    device = _require_device(x, decay, gate, rate, state)
+    _require_inference(x, decay, gate, rate, state)
+    batch, width = x.shape
+    if inplace and ((width > 1 and state.stride(1) != 1) or
+                    (batch > 1 and state.stride(0) < width)):
+        raise ValueError("state must have a unit innermost stride and rows of its own to be "
+                         "updated in place")
+    out = torch.empty(batch, width, dtype=x.dtype, device=device)
+    new = state if inplace else torch.empty(batch, width, dtype=torch.float32, device=device)
+    if batch == 0 or width == 0:
+        return out, new
+    x, decay, gate, state, rate = (_inner(x), _inner(decay), _inner(gate), _inner(state),
+                                   _rate32(rate))
+    code, tensor = _hip.dtype_code(x.dtype), _hip.Tensor
+    args = _hip.GatedScanArgs(batch, 1, width, code,
+                              tensor(x.data_ptr(), code, 0, (x.stride(0), 0, 1)),
+                              tensor(decay.data_ptr(), code, 0, (decay.stride(0), 0, 1)))
+    if gate is not None:
+        args.gate = tensor(gate.data_ptr(), code, 0, (gate.stride(0), 0, 1))
+        args.rate = tensor(rate.data_ptr(), 0, 0, (1,))
+    args.initial_state = tensor(state.data_ptr(), 0, 0, (state.stride(0), 1))
+    args.out = tensor(out.data_ptr(), code, 0, (width, 0, 1))
+    args.final_state = tensor(new.data_ptr(), 0, 0, (new.stride(0), 1))
+    _hip.launch("m3_gated_scan", args, device)
+    return out, new
+
+
 __all__ = ["heavy_tail_activation", "mamba3_scan", "mamba3_step", "fused_step", "chunk_state",
            "ScanCall", "scan_projection", "step_projection", "split_projection", "linear",
-           "linear_supported", "rms_norm", "rms_norm_supported"]
+           "linear_supported", "rms_norm", "rms_norm_supported", "gated_scan", "gated_step"]
