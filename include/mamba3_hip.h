@@ -28,7 +28,8 @@
  *                      _Mamba3Mixer.step model.py:431-469.
  * m3_linear has no reference hook: it takes the decode step's projection GEMMs (see below).
  * m3_gated_scan and m3_gated_scan_bwd have no counterpart in the reference: an elementwise gated
- * recurrence beside the matrix-state one, with its gradients.
+ * recurrence beside the matrix-state one, with its gradients. Nor has m3_linear4, m3_linear's
+ * product with a weight held in 4 bits.
  */
 #ifndef MAMBA3_HIP_H
 #define MAMBA3_HIP_H
@@ -321,6 +322,35 @@ typedef struct {
 
 int m3_gated_scan_bwd_workspace_size(const m3_gated_scan_bwd_args* args, size_t* bytes);
 int m3_gated_scan_bwd(const m3_gated_scan_bwd_args* args, hipStream_t stream);
+
+/*
+ * m3_linear with a weight held in 4 bits: out[M, N] = x'[M, K] * W[N, K]^T (+ residual[M, N]),
+ *   W[n, k] = (q[n, k] - z[n, k / group]) * scale[n, k / group],  q, z in 0..15,
+ * x' and the residual as in m3_linear (M <= 256, FP32 accumulation, one rounding; the norm at any
+ * M). group is 32, 64 or 128, K a multiple of 32 and of group. No counterpart in the reference.
+ * The weight is laid out once, for reads of 1 KB by a wave, in tiles of 16 rows x 128 columns
+ * (rows and columns past N and K: code 0, scale 0, zero 0), TK = ceil(K / 128) of them a tile row:
+ *   codes [ceil(N / 16), TK, 64, 4] 32-bit words: word i of lane l holds row l % 16, columns
+ *     32 i + 8 (l / 16) + e of its tile, column e = 2 j in bits 4 j, e = 2 j + 1 in bits 4 j + 16
+ *   scales [ceil(N / 16), TK, 128 / group, 16] bf16 or f16
+ *   zeros the same in bytes; NULL: 8 everywhere
+ */
+typedef struct {
+  int64_t m, n, k;
+  int32_t dtype;        /* M3_BF16 or M3_F16: x, norm_weight, residual, out */
+  int32_t scale_dtype;  /* M3_BF16 or M3_F16 */
+  int32_t group;
+  float norm_eps;
+  const void* codes;    /* 16-byte aligned */
+  const void* scales;   /* 8-byte aligned */
+  const void* zeros;    /* 4-byte aligned, optional */
+  m3_tensor x;          /* [M, K], rows 16-byte aligned */
+  m3_tensor norm_weight;/* [K] optional, 16-byte aligned */
+  m3_tensor residual;   /* [M, N] optional */
+  m3_tensor out;        /* [M, N]; may not overlap x or the weight, may equal residual */
+} m3_linear4_args;
+
+int m3_linear4(const m3_linear4_args* args, hipStream_t stream);
 
 const char* m3_last_error(void);
 int m3_abi_version(void);

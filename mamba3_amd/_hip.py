@@ -112,11 +112,21 @@ class GatedScanBwdArgs(ctypes.Structure):
                                     "dinitial")]]
 
 
+class Linear4Args(ctypes.Structure):
+    _fields_ = [
+        *[(n, ctypes.c_int64) for n in ("m", "n", "k")],
+        *[(n, ctypes.c_int32) for n in ("dtype", "scale_dtype", "group")],
+        ("norm_eps", ctypes.c_float),
+        *[(n, ctypes.c_void_p) for n in ("codes", "scales", "zeros")],
+        *[(n, _T) for n in ("x", "norm_weight", "residual", "out")],
+    ]
+
+
 ENTRY_POINTS = ("m3_scan_fwd", "m3_scan_workspace_size", "m3_scan_segments", "m3_scan_fwd_noalloc",
                 "m3_chunk_state", "m3_step", "m3_linear", "m3_linear_workspace_size",
                 "m3_rms_norm", "m3_gated_scan", "m3_gated_scan_workspace_size",
-                "m3_gated_scan_bwd", "m3_gated_scan_bwd_workspace_size", "m3_last_error",
-                "m3_abi_version")
+                "m3_gated_scan_bwd", "m3_gated_scan_bwd_workspace_size", "m3_linear4",
+                "m3_last_error", "m3_abi_version")
 GATED_TILE = 128  # M3_GATED_TILE: tokens between two of the states a gated scan's carry holds
 SCRATCH_BYTES = 64 << 20  # M3_SCRATCH_BYTES: the no-alloc scan's per-GPU scratch
 
@@ -133,7 +143,7 @@ def load() -> ctypes.CDLL:
             f"{LIB_PATH} is not built; run `python -m mamba3_amd.build` (hipcc, gfx950)")
     lib = ctypes.CDLL(LIB_PATH)
     for name in ("m3_scan_fwd", "m3_scan_fwd_noalloc", "m3_chunk_state", "m3_step", "m3_linear",
-                 "m3_rms_norm", "m3_gated_scan", "m3_gated_scan_bwd"):
+                 "m3_rms_norm", "m3_gated_scan", "m3_gated_scan_bwd", "m3_linear4"):
         fn = getattr(lib, name)
         fn.restype = ctypes.c_int
         fn.argtypes = [ctypes.c_void_p, ctypes.c_void_p]

@@ -8,7 +8,8 @@ RMSNorm, dt / A, the bounded phase, bias and rotation, and the chunked SSD or th
 decode step. ``in_proj`` / ``out_proj`` and the residual RMSNorm stay in torch
 (hipBLASLt), except in a decode step of a small batch with 16-bit weights: there both
 projections run on ``ops.linear`` (``m3_linear``), the block's RMSNorm fused into
-``in_proj`` and its residual add into ``out_proj``.
+``in_proj`` and its residual add into ``out_proj`` (``ops.linear4`` after
+``Mamba3.quantize_decode``, with the weights in 4 bits).
 
 Scope: inference (``forward``, ``prefill``, ``step``, ``cuda_graph``) on ROCm devices.
 Autograd through the mixer and CPU execution raise ``RuntimeError``. ``compile`` and
@@ -119,6 +120,27 @@ class _Mamba3Mixer(nn.Module):
             self.register_parameter("direction_logit", None)
         else:
             self.direction_logit = nn.Parameter(torch.zeros(d_model))
+        # 4-bit copies of the projections for decode steps, by name (quantize_decode)
+        self._decode4: dict[str, tuple[ops.Weight4, tuple[object, ...]]] = {}
+
+    def quantize_decode(self, group: int, zeros: bool) -> None:
+        layers = {name: getattr(self, name) for name in ("in_proj", "out_proj")}
+        held = {name: ops.quantize4(layer.weight, group, zeros=zeros)
+                for name, layer in layers.items()}
+        with torch.no_grad():
+            for name, layer in layers.items():
+                layer.weight.copy_(held[name].dequantize(layer.weight.dtype))
+        self._decode4 = {name: (held[name], _storage_signature(layer.weight))
+                         for name, layer in layers.items()}
+
+    def _weight4(self, name: str) -> ops.Weight4 | None:
+        """The projection's 4-bit copy, if there is one; refused once the weight has changed."""
+        if name not in self._decode4:
+            return None
+        held, then = self._decode4[name]
+        if not _same_storage(_storage_signature(getattr(self, name).weight), then):
+            raise RuntimeError(f"{name}.weight changed since quantize_decode; call it again")
+        return held
 
     def _chunk(self) -> int:
         return (self.chunk_size if self.training and torch.is_grad_enabled()
@@ -217,7 +239,12 @@ class _Mamba3Mixer(nn.Module):
         rows = hidden_states[:, 0]
         small = rows.shape[0] <= ops.DECODE_LINEAR_ROWS
         supported = ops.linear_norm_supported if norm is not None else ops.linear_supported
-        if small and supported(rows, self.in_proj.weight):
+        in4, out4 = self._weight4("in_proj"), self._weight4("out_proj")
+        if small and in4 is not None and ops.linear4_supported(rows, in4):
+            proj = ops.linear4(rows, in4, norm_weight=norm.weight if norm is not None else None,
+                               norm_eps=norm.eps if norm is not None else ops.NORM_EPS)
+            proj = proj.unsqueeze(1)
+        elif small and supported(rows, self.in_proj.weight):
             proj = ops.linear(rows, self.in_proj.weight,
                               norm_weight=norm.weight if norm is not None else None,
                               norm_eps=norm.eps if norm is not None else ops.NORM_EPS)
@@ -231,6 +258,11 @@ class _Mamba3Mixer(nn.Module):
             self._validate_cache(cache, hidden_states.shape[0])
         mixed, next_cache = ops.step_projection(proj, self, cache, inplace=inplace)
         mixed = mixed.flatten(-2)
+        if (rows.shape[0] <= ops.DECODE_LINEAR_OUT_ROWS and out4 is not None
+                and ops.linear4_supported(mixed, out4)
+                and (residual is None or residual.dtype == mixed.dtype)):
+            res = residual[:, 0] if residual is not None else None
+            return ops.linear4(mixed, out4, res).unsqueeze(1), next_cache
         if rows.shape[0] <= ops.DECODE_LINEAR_OUT_ROWS and ops.linear_supported(
                 mixed, self.out_proj.weight) and (residual is None or residual.dtype == mixed.dtype):
             res = residual[:, 0] if residual is not None else None
@@ -401,6 +433,29 @@ class Mamba3(nn.Module):
                                           else inference)
         return self
 
+    def quantize_decode(self, group: int = 128, *, zeros: bool = True) -> Mamba3:
+        """Hold every mixer's ``in_proj`` and ``out_proj`` in 4 bits for decode steps.
+
+        The 16-bit weights are rounded to 4-bit codes with a scale (and, with ``zeros``, a zero) for
+        every ``group`` columns (32, 64 or 128; ``ops.quantize4``) and overwritten with the rounded
+        values in their own dtype, so that forward, prefill and steps of more than
+        ``ops.DECODE_LINEAR_ROWS`` rows compute the same model through the general GEMMs. Steps of fewer rows stream the 4-bit
+        copies (``ops.linear4``) instead of the weights. A weight that is replaced or modified
+        afterwards (``load_state_dict``, ``to``, a copy of the model) makes ``step`` raise until
+        this is called again. A step's rows must have the weights' dtype, as ever, to run on it.
+        """
+        for layer in self.layers:
+            for name in ("in_proj", "out_proj"):
+                weight = getattr(layer.mixer, name).weight
+                if weight.dtype not in (torch.bfloat16, torch.float16):
+                    raise ValueError("quantize_decode needs bfloat16 or float16 weights")
+                if group not in ops.LINEAR4_GROUPS or weight.shape[1] % group != 0:
+                    raise ValueError(f"group must be 32, 64 or 128 and divide {name}'s "
+                                     f"{weight.shape[1]} columns")
+        for layer in self.layers:
+            layer.mixer.quantize_decode(group, zeros)
+        return self
+
     def compile_layers(self, **kwargs: object) -> Mamba3:
         """Accepted for API compatibility; the HIP kernels are already fused."""
         return self
@@ -419,6 +474,10 @@ def _storage_signature(w: torch.Tensor) -> tuple[object, ...]:
     ``_parameter_signature`` (``model.py:763-774``: identity, version, data pointer, device,
     dtype, shape), with the object itself kept instead of its ``id``."""
     return (w, w._version, w.data_ptr(), w.device, w.dtype, tuple(w.shape))
+
+
+def _same_storage(now: tuple[object, ...], then: tuple[object, ...]) -> bool:
+    return now[0] is then[0] and now[1:] == then[1:]
 
 
 class _HipGraphDecoder:
@@ -446,6 +505,8 @@ class _HipGraphDecoder:
         # storage it read (address, device, dtype, shape): `Module.to`, `.half()` or
         # `p.data = ...` keep the object and its version but move the storage
         self._captured = [_storage_signature(w) for w in weights]
+        # the 4-bit copies that the graph reads live as long as it does
+        self._weights4 = [dict(layer.mixer._decode4) for layer in model.layers]
         self.input = torch.zeros(batch_size, 1, model.d_model, device=device, dtype=dtype)
         self.cache = [layer.mixer.allocate_cache(batch_size, device=device, dtype=dtype)
                       for layer in model.layers]
@@ -486,8 +547,7 @@ class _HipGraphDecoder:
     def validate(self) -> None:
         current = [_storage_signature(w) for w in self.model.parameters()]
         same = len(current) == len(self._captured) and all(
-            now[0] is then[0] and now[1:] == then[1:]
-            for now, then in zip(current, self._captured))
+            _same_storage(now, then) for now, then in zip(current, self._captured))
         if not same:
             raise RuntimeError("model state changed; recreate the CUDA graph decoder")
 

@@ -670,6 +670,169 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = NORM_EPS, *,
     return out, s
 
 
+# --------------------------------------------------------------------------- 4-bit weights
+
+LINEAR4_GROUPS = (32, 64, 128)
+
+
+class Weight4:
+    """An ``nn.Linear`` weight ``[N, K]`` held in 4 bits, laid out for ``linear4``.
+
+    ``packed [N, K / 2]`` uint8: codes 0..15, the even column in the low four bits. ``scales [N,
+    K / group]`` bfloat16 or float16, ``group`` 32, 64 or 128 by its shape; ``zeros`` of the same
+    shape, uint8 0..15, or ``None`` for 8 everywhere. The weight is ``(code - zero) * scale``.
+    The three are copied into the kernel's tiles once, here (``m3_linear4``'s layout: a wave reads
+    a tile of 16 rows by 128 columns as 1 KB); later changes to them are not seen.
+    """
+
+    def __init__(self, packed: torch.Tensor, scales: torch.Tensor,
+                 zeros: torch.Tensor | None = None) -> None:
+        if packed.ndim != 2 or packed.dtype != torch.uint8 or packed.numel() == 0:
+            raise ValueError("packed must be uint8 of shape [N, K / 2]")
+        n, k = packed.shape[0], 2 * packed.shape[1]
+        if scales.ndim != 2 or scales.shape[0] != n or scales.numel() == 0:
+            raise ValueError("scales must have shape [N, K / group]")
+        if scales.dtype not in (torch.bfloat16, torch.float16):
+            raise ValueError("scales must be bfloat16 or float16")
+        group = k // scales.shape[1]
+        if group not in LINEAR4_GROUPS or group * scales.shape[1] != k:
+            raise ValueError(f"{scales.shape[1]} scales a row of {k}: groups must be of 32, 64 or 128")
+        if zeros is not None and (zeros.shape != scales.shape or zeros.dtype != torch.uint8):
+            raise ValueError("zeros must be uint8 of the scales' shape")
+        if any(t is not None and t.device != packed.device for t in (scales, zeros)):
+            raise ValueError("packed, scales and zeros must be on the same device")
+        self.shape, self.group, self.device = (n, k), group, packed.device
+        self.dtype = scales.dtype
+        tn, tk = -(-n // 16), -(-k // 128)
+        # [N, K] codes -> [tn, row, tk, word i, lane group, e] -> [tn, tk, lane group, row, i, e]
+        codes = torch.stack([packed & 15, packed >> 4], dim=-1).flatten(1)
+        codes = torch.nn.functional.pad(codes, (0, 128 * tk - k, 0, 16 * tn - n))
+        codes = codes.view(tn, 16, tk, 4, 4, 4, 2).permute(0, 2, 4, 1, 3, 6, 5)
+        # a word's nibbles: the even columns, then the odd ones; two to a byte
+        codes = codes.reshape(tn, tk, 64, 4, 8)
+        self.codes = (codes[..., 0::2] | codes[..., 1::2] << 4).contiguous()
+        self.scales = self._tiles(scales, tn, tk)
+        self.zeros = None if zeros is None else self._tiles(zeros.clamp(max=15), tn, tk)
+
+    def _tiles(self, t: torch.Tensor, tn: int, tk: int) -> torch.Tensor:
+        per = 128 // self.group
+        t = torch.nn.functional.pad(t.detach(), (0, per * tk - t.shape[1], 0, 16 * tn - t.shape[0]))
+        return t.view(tn, 16, tk, per).permute(0, 2, 3, 1).contiguous()
+
+    def dequantize(self, dtype: torch.dtype | None = None) -> torch.Tensor:
+        """The weight ``[N, K]`` as ``(code - zero) * scale``, one product in FP32 rounded to
+        ``dtype`` (default: the scales')."""
+        n, k = self.shape
+        tn, tk = self.codes.shape[:2]
+        codes = torch.stack([self.codes & 15, self.codes >> 4], dim=-1)
+        codes = codes.view(tn, tk, 4, 16, 4, 2, 4).permute(0, 3, 1, 4, 2, 6, 5)
+        codes = codes.reshape(16 * tn, -1, self.group).float()
+
+        def rows(t):
+            return t.permute(0, 3, 1, 2).reshape(16 * tn, -1, 1).float()
+
+        zeros = 8.0 if self.zeros is None else rows(self.zeros)
+        weight = ((codes - zeros) * rows(self.scales)).flatten(1)
+        return weight[:n, :k].to(dtype or self.dtype).contiguous()
+
+
+def quantize4(weight: torch.Tensor, group: int = 128, *, zeros: bool = True,
+              dtype: torch.dtype | None = None) -> Weight4:
+    """``weight [N, K]`` rounded to 4 bits in groups of ``group`` columns.
+
+    With ``zeros`` a group's codes span its least to its greatest value (0 among them, which stays
+    exact); without, they are centred on code 8. Scales are ``dtype`` (default: the weight's, or
+    bfloat16 for an FP32 weight), and codes are rounded with the scale as it is held.
+    """
+    if weight.ndim != 2 or weight.dtype not in _FLOAT_DTYPES or weight.numel() == 0:
+        raise ValueError("weight must be a floating [N, K] tensor")
+    if group not in LINEAR4_GROUPS or weight.shape[1] % group != 0:
+        raise ValueError(f"quantize4: K = {weight.shape[1]} must be a multiple of group "
+                         f"{group}, one of {LINEAR4_GROUPS}")
+    dtype = dtype or (torch.bfloat16 if weight.dtype == torch.float32 else weight.dtype)
+    if dtype not in (torch.bfloat16, torch.float16):
+        raise ValueError("scales must be bfloat16 or float16")
+    w = weight.detach().float().unflatten(1, (-1, group))
+    if not bool(torch.isfinite(w).all()):
+        raise ValueError("quantize4: the weight holds NaN or infinities")
+    if zeros:
+        low, high = w.amin(-1, keepdim=True).clamp(max=0), w.amax(-1, keepdim=True).clamp(min=0)
+        scale = (high - low) / 15
+    else:
+        scale = torch.maximum(w.amax(-1, keepdim=True) / 7, -w.amin(-1, keepdim=True) / 8)
+    scale = scale.to(dtype).float()
+    if not bool(torch.isfinite(scale).all()):
+        raise ValueError(f"quantize4: a group's range is beyond {dtype}")
+    step = torch.where(scale > 0, scale, 1.0)
+    zero = (-low / step).round().clamp(0, 15) if zeros else torch.full_like(scale, 8.0)
+    codes = ((w / step).round() + zero).clamp(0, 15).to(torch.uint8).flatten(1)
+    return Weight4(codes[:, 0::2] | codes[:, 1::2] << 4, scale.squeeze(-1).to(dtype),
+                   zero.squeeze(-1).to(torch.uint8) if zeros else None)
+
+
+def linear4_supported(x: torch.Tensor, weight: Weight4) -> bool:
+    """Whether ``linear4(x, weight)`` takes these operands: 1 to ``LINEAR_MAX_ROWS`` rows of K
+    bfloat16 or float16 values on the weight's ROCm device, no autograd, and no autocast that would
+    compute in another dtype."""
+    return (x.dim() == 2 and x.shape[1] == weight.shape[1] and 0 < x.shape[0] <= LINEAR_MAX_ROWS
+            and x.device.type == "cuda" and x.device == weight.device
+            and x.dtype in (torch.bfloat16, torch.float16)
+            and not (torch.is_autocast_enabled("cuda")
+                     and torch.get_autocast_dtype("cuda") != x.dtype)
+            and not (torch.is_grad_enabled() and x.requires_grad))
+
+
+def _aligned16(t: torch.Tensor) -> torch.Tensor:
+    """``t`` with 16-byte aligned rows of unit inner stride (itself if it has them)."""
+    if t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and (t.dim() == 1 or t.stride(0) % 8 == 0):
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
+
+
+def linear4(x: torch.Tensor, weight: Weight4, residual: torch.Tensor | None = None, *,
+            out: torch.Tensor | None = None, norm_weight: torch.Tensor | None = None,
+            norm_eps: float = NORM_EPS) -> torch.Tensor:
+    """``linear`` with a 4-bit weight (``m3_linear4``): ``x @ W.T (+ residual)`` for the few rows
+    of a decode step, ``W = (code - zero) * scale`` a ``Weight4``.
+
+    ``x [M, K]`` (``M <= 256``) bfloat16 or float16; ``residual`` and ``out`` ``[M, N]`` of that
+    dtype. Sums are FP32, the residual is added to them and the result rounded once. With
+    ``norm_weight [K]`` ``x`` is first RMS-normalised, as ``F.rms_norm(x, (K,), norm_weight,
+    norm_eps)``. No backward.
+    """
+    device = _require_device(x, residual, out, norm_weight)
+    _require_inference(x, residual, norm_weight)
+    if not linear4_supported(x, weight):
+        raise ValueError(f"linear4: unsupported operands x {tuple(x.shape)} {x.dtype} on "
+                         f"{x.device}, weight {weight.shape} on {weight.device}")
+    m, (n, k) = x.shape[0], weight.shape
+    for name, t in (("residual", residual), ("out", out)):
+        if t is not None and (tuple(t.shape) != (m, n) or t.dtype != x.dtype):
+            raise ValueError(f"linear4: {name} must be [{m}, {n}] {x.dtype}, got "
+                             f"{tuple(t.shape)} {t.dtype}")
+    x = _aligned16(x)
+    code, tensor = _hip.dtype_code(x.dtype), _hip.Tensor
+    args = _hip.Linear4Args(m, n, k, code, _hip.dtype_code(weight.dtype), weight.group, norm_eps,
+                            weight.codes.data_ptr(), weight.scales.data_ptr(),
+                            None if weight.zeros is None else weight.zeros.data_ptr(),
+                            tensor(x.data_ptr(), code, 0, x.stride()))
+    if norm_weight is not None:
+        if norm_weight.shape != (k,):
+            raise ValueError(f"linear4: norm_weight must be [{k}]")
+        norm_weight = _aligned16(norm_weight.detach().to(x.dtype))
+        args.norm_weight = tensor(norm_weight.data_ptr(), code, 0, (1,))
+    if residual is not None:
+        residual = _inner(residual)
+        args.residual = tensor(residual.data_ptr(), code, 0, residual.stride())
+    if out is None:
+        out = torch.empty(m, n, dtype=x.dtype, device=device)
+    elif n > 1 and out.stride(1) != 1:
+        raise ValueError("linear4: out needs a unit inner stride")
+    args.out = tensor(out.data_ptr(), code, 0, out.stride())
+    _hip.launch("m3_linear4", args, device)
+    return out
+
+
 # --------------------------------------------------------------------------- gated recurrence
 
 
@@ -855,4 +1018,5 @@ def gated_step(x: torch.Tensor, decay: torch.Tensor, state: torch.Tensor,
 
 __all__ = ["heavy_tail_activation", "mamba3_scan", "mamba3_step", "fused_step", "chunk_state",
            "ScanCall", "scan_projection", "step_projection", "split_projection", "linear",
-           "linear_supported", "rms_norm", "rms_norm_supported", "gated_scan", "gated_step"]
+           "linear_supported", "rms_norm", "rms_norm_supported", "gated_scan", "gated_step",
+           "Weight4", "quantize4", "linear4", "linear4_supported"]
