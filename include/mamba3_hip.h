@@ -277,7 +277,7 @@ int m3_rms_norm(const m3_rms_norm_args* args, hipStream_t stream);
  * an empty state (what came before it, NaN and infinities too, is dropped).
  * rate >= 0; a negative one gives NaN.
  */
-#define M3_GATED_TILE 128 /* tokens between two of the states that carry holds */
+#define M3_GATED_TILE 64 /* tokens between two of the states that carry holds */
 typedef struct {
   int32_t batch, length, width;
   int32_t dtype;           /* of x, decay, gate and out */

@@ -127,7 +127,7 @@ ENTRY_POINTS = ("m3_scan_fwd", "m3_scan_workspace_size", "m3_scan_segments", "m3
                 "m3_rms_norm", "m3_gated_scan", "m3_gated_scan_workspace_size",
                 "m3_gated_scan_bwd", "m3_gated_scan_bwd_workspace_size", "m3_linear4",
                 "m3_last_error", "m3_abi_version")
-GATED_TILE = 128  # M3_GATED_TILE: tokens between two of the states a gated scan's carry holds
+GATED_TILE = 64  # M3_GATED_TILE: tokens between two of the states a gated scan's carry holds
 SCRATCH_BYTES = 64 << 20  # M3_SCRATCH_BYTES: the no-alloc scan's per-GPU scratch
 
 _lib: ctypes.CDLL | None = None

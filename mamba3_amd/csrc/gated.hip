@@ -11,8 +11,8 @@
 // again from there with one fma each. Tiles of one row are chained through memory: a tile publishes its own
 // map, then looks back for the nearest state that is already known.
 //
-// The backward pass walks a channel's tokens from the end, tile by tile, recomputing each tile's
-// states from the carry the forward pass left.
+// Backward: tiles of 64 tokens, chained from the last, each with its states run again from the carry
+// that the forward pass left.
 #include <hip/hip_runtime.h>
 
 #include "m3_common.hpp"
@@ -21,7 +21,9 @@
 namespace m3 {
 namespace {
 
-constexpr int kTile = M3_GATED_TILE;
+constexpr int kTile = 128;             // tokens of a forward tile
+constexpr int kLeap = M3_GATED_TILE;   // tokens between carried states; a backward tile
+static_assert(kTile % kLeap == 0, "a forward tile leaves whole carries");
 constexpr float kLog2e = 1.44269504088896340736f;
 
 struct GatedGeom {
@@ -42,8 +44,7 @@ struct GatedGeom {
   char *dx, *dr, *dg;
   float* dinit;                // or null
   float* drate;                // [C]
-  float* part;                 // partial sums of drate, [rows, C]
-  float* scratch;              // [B, kTile, C]
+  float* part;                 // the tiles' shares of drate, [tiles, B, C]
   int64_t dy_b, dx_b, dr_b, dg_b, dfin_b, dinit_b;
   int64_t dy_t, dx_t, dr_t, dg_t;
 };
@@ -97,13 +98,6 @@ struct Span {
   }
 };
 
-// One token of one channel: its factor a and input b = w x, and what the gradients need.
-struct Coef {
-  float a, b, w;      // w = s q (1 in the given form)
-  float p, q, pp, qq; // gates' sigmoids, p (1 - p), q (1 - q)
-  float s, inv;       // sqrt(1 - a^2) and its reciprocal (0 where s is)
-};
-
 // 1 - exp(u) for u <= 0: the series of -expm1 near 0, where the difference would lose its digits
 // (at -0.125 the first term left out is 4e-8 of the sum, the difference's error 5e-7).
 __device__ __forceinline__ float one_minus_exp(float u, float e) {
@@ -112,48 +106,41 @@ __device__ __forceinline__ float one_minus_exp(float u, float e) {
   return u > -0.125f ? series : 1.f - e;
 }
 
-template <bool GATE>
-__device__ __forceinline__ Coef coef(float x, float r, float g, float rate) {
-  Coef c;
-  if constexpr (!GATE) {
-    c.a = __builtin_amdgcn_exp2f(r * kLog2e);
-    c.b = x;
-    c.w = 1.f;
-  } else {
-    // from exp(-|r|): both sigmoid and its complement keep their digits
-    const float er = __builtin_amdgcn_exp2f(-fabsf(r) * kLog2e);
-    const float hr = __builtin_amdgcn_rcpf(1.f + er);
-    const float eg = __builtin_amdgcn_exp2f(-fabsf(g) * kLog2e);
-    const float hg = __builtin_amdgcn_rcpf(1.f + eg);
-    c.p = r < 0.f ? er * hr : hr;
-    c.q = g < 0.f ? eg * hg : hg;
-    c.pp = er * hr * hr;
-    c.qq = eg * hg * hg;
-    const float la = -rate * c.p;
-    c.a = __builtin_amdgcn_exp2f(la * kLog2e);
-    const float v = one_minus_exp(2.f * la, c.a * c.a);
-    c.inv = fabsf(v) < 1e-37f ? 0.f : __builtin_amdgcn_rsqf(v);
-    c.s = v * c.inv;
-    c.w = c.s * c.q;
-    c.b = c.w * x;
-  }
-  return c;
+__device__ __forceinline__ float sigmoid2(float x) {
+  return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(x * -kLog2e));
 }
 
-// The forward pass's share of it: the factor and the input.
+// A sigmoid and its complement, both with all their digits: from exp(-|x|).
+struct Gate {
+  float open, shut;
+  __device__ __forceinline__ explicit Gate(float x) {
+    const float e = __builtin_amdgcn_exp2f(-fabsf(x) * kLog2e);
+    const float big = __builtin_amdgcn_rcpf(1.f + e), small = e * big;
+    open = x < 0.f ? small : big;
+    shut = x < 0.f ? big : small;
+  }
+};
+
+// The factor a of one token and channel, and s = sqrt(1 - a^2) (gate form).
+template <bool GATE>
+__device__ __forceinline__ void factor_root(float r, float rate, float& a, float& root) {
+  if constexpr (!GATE) {
+    a = __builtin_amdgcn_exp2f(r * kLog2e);
+    root = 1.f;
+  } else {
+    const float p = sigmoid2(r);
+    a = __builtin_amdgcn_exp2f(rate * -kLog2e * p);
+    root = __builtin_amdgcn_sqrtf(one_minus_exp(rate * -2.f * p, a * a));
+  }
+}
+
+// The factor and the input.
 template <bool GATE>
 __device__ __forceinline__ void factor_input(float x, float r, float g, float rate, float& a,
                                              float& b) {
-  if constexpr (!GATE) {
-    a = __builtin_amdgcn_exp2f(r * kLog2e);
-    b = x;
-  } else {
-    const float p = __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(r * -kLog2e));
-    const float q = __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(g * -kLog2e));
-    a = __builtin_amdgcn_exp2f(rate * -kLog2e * p);
-    const float v = one_minus_exp(rate * -2.f * p, a * a);
-    b = __builtin_amdgcn_sqrtf(v) * q * x;
-  }
+  float root;
+  factor_root<GATE>(r, rate, a, root);
+  b = GATE ? root * sigmoid2(g) * x : x;
 }
 
 __device__ __forceinline__ int row_length(const GatedGeom& g, int b) {
@@ -415,7 +402,7 @@ __global__ __launch_bounds__(64 * kWaves, 4) void gated_tile_kernel(const GatedG
         s_in[lane * VEC + e] = v[e];
       }
       if (live) {
-        if (s < g.tiles - 1 || g.carry != nullptr) write_states<VEC>(ch.states + at + s * step, out);
+        if (s < g.tiles - 1) write_states<VEC>(ch.states + at + s * step, out);
         if (s == g.tiles - 1) {
 #pragma unroll
           for (int e = 0; e < VEC; ++e) g.fin[b * g.fin_b + c + e] = out[e];
@@ -460,10 +447,13 @@ __global__ __launch_bounds__(64 * kWaves, 4) void gated_tile_kernel(const GatedG
   }
   if (!CHAIN && w == kWaves - 1 && live) {
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) {
-      g.fin[b * g.fin_b + c + e] = v[e];
-      if (g.carry != nullptr) g.carry[at + e] = v[e];
-    }
+    for (int e = 0; e < VEC; ++e) g.fin[b * g.fin_b + c + e] = v[e];
+  }
+  constexpr int kPer = kLeap / kSpan;  // waves between carries
+  const int leap = (s * kWaves + w) / kPer;
+  if (g.carry != nullptr && live && w % kPer == kPer - 1 && leap * kLeap < g.length) {
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) g.carry[at + leap * step + e] = v[e];
   }
 }
 
@@ -492,8 +482,9 @@ __global__ __launch_bounds__(256) void gated_walk_kernel(const GatedGeom g) {
       const bool fresh = g.reset != nullptr && g.reset[b * g.reset_b + t] != 0;
 #pragma unroll
       for (int e = 0; e < VEC; ++e) {
-        const Coef k = coef<GATE>(x[e], r[e], q[e], rate[e]);
-        h[e] = fresh ? k.b : fmaf(k.a, h[e], k.b);
+        float a, in;
+        factor_input<GATE>(x[e], r[e], q[e], rate[e], a, in);
+        h[e] = fresh ? in : fmaf(a, h[e], in);
         y[e] = h[e];
       }
     } else {
@@ -501,10 +492,10 @@ __global__ __launch_bounds__(256) void gated_walk_kernel(const GatedGeom g) {
       for (int e = 0; e < VEC; ++e) y[e] = 0.f;
     }
     store_vec<T, VEC>(g.y, b * g.y_b + t * g.y_t + c, y);
-    if (g.carry != nullptr && (t % kTile == kTile - 1 || t == g.length - 1)) {
+    if (g.carry != nullptr && (t % kLeap == kLeap - 1 || t == g.length - 1)) {
 #pragma unroll
       for (int e = 0; e < VEC; ++e) {
-        g.carry[(static_cast<int64_t>(t / kTile) * g.batch + b) * g.width + c + e] = h[e];
+        g.carry[(static_cast<int64_t>(t / kLeap) * g.batch + b) * g.width + c + e] = h[e];
       }
     }
   }
@@ -512,71 +503,284 @@ __global__ __launch_bounds__(256) void gated_walk_kernel(const GatedGeom g) {
   for (int e = 0; e < VEC; ++e) g.fin[b * g.fin_b + c + e] = h[e];
 }
 
-template <typename T, bool GATE>
-__global__ __launch_bounds__(256) void gated_walk_bwd_kernel(const GatedGeom g) {
-  const int64_t id = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-  const int b = static_cast<int>(id / g.width), c = static_cast<int>(id % g.width);
-  if (b >= g.batch) return;
-  const int len = row_length(g, b);
-  const float rate = GATE ? g.rate[c] : 0.f;
-  float grad = g.dfin != nullptr ? g.dfin[b * g.dfin_b + c] : 0.f;  // a_{t+1} D_{t+1}
-  float sum = 0.f;
-  float x[1], r[1], q[1] = {0.f}, dy[1];
-  for (int s = g.tiles - 1; s >= 0; --s) {
-    const int t0 = s * kTile, t1 = min(g.length, t0 + kTile);
-    float h = s > 0 ? g.carry[(static_cast<int64_t>(s - 1) * g.batch + b) * g.width + c]
-                    : (g.init != nullptr ? g.init[b * g.init_b + c] : 0.f);
-    for (int t = t0; t < t1; ++t) {
-      const bool fresh = g.reset != nullptr && g.reset[b * g.reset_b + t] != 0;
-      if (fresh && t < len) h = 0.f;
-      g.scratch[(static_cast<int64_t>(b) * kTile + t - t0) * g.width + c] = h;
-      if (t < len) {
-        load_vec<T, 1>(g.x, b * g.x_b + t * g.x_t + c, x);
-        load_vec<T, 1>(g.r, b * g.r_b + t * g.r_t + c, r);
-        if constexpr (GATE) load_vec<T, 1>(g.g, b * g.g_b + t * g.g_t + c, q);
-        const Coef k = coef<GATE>(x[0], r[0], q[0], rate);
-        h = fmaf(k.a, h, k.b);
+// ----------------------------------------------------------------------------- backward
+
+constexpr int kBack = kLeap / kWaves;  // a wave's tokens
+
+// A tile of kLeap tokens x 64 VEC channels. The states before its tokens are run again from the
+// carry the forward pass left, as a wave's map behind those of the waves before; the gradients
+// e_{t-1} = a_t (dy_t + e_t) run the other way, their maps joined from the last wave to the first
+// and from tile to tile in a chain that begins at the last. Both kinds of map are formed from one read
+// of the inputs, kept as they came; the factor and s are kept too, the sigmoids formed again.
+template <typename T, bool GATE, int VEC, bool CHAIN>
+__global__ __launch_bounds__(64 * kWaves, 4) void gated_back_kernel(const GatedGeom g,
+                                                                    const Chain ch) {
+  constexpr int kCols = 64 * VEC;
+  __shared__ float s_a[kWaves][kCols], s_h[kWaves][kCols], s_e[kWaves][kCols], s_in[kCols];
+  __shared__ unsigned s_ticket;
+  typedef T tv __attribute__((ext_vector_type(VEC)));
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  unsigned id = blockIdx.x;
+  if constexpr (CHAIN) {
+    if (tid == 0) s_ticket = atomicAdd(ch.ticket, 1u);
+    __syncthreads();
+    id = __builtin_amdgcn_readfirstlane(s_ticket);
+  }
+  const unsigned groups = (g.width + kCols - 1) / kCols, cells = g.batch * groups;
+  const int link = id / cells, s = g.tiles - 1 - link, b = id % cells / groups;
+  const int c0 = (id % groups) * kCols + lane * VEC;
+  const bool live = c0 < g.width;
+  const int c = min(c0, g.width - VEC);
+  const int t0 = s * kLeap + w * kBack;
+  const int n = max(0, min(row_length(g, b) - t0, kBack));
+  const int64_t step = static_cast<int64_t>(g.batch) * g.width;
+  const int64_t at = static_cast<int64_t>(b) * g.width + c;
+
+  uint32_t early[VEC];
+  if constexpr (CHAIN) {
+    if (w == 0 && link > 0) read_states<VEC>(ch.states + at + (link - 1) * step, early);
+  }
+  float rate[VEC], v[VEC];  // v: the state before the wave's tokens
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) {
+    rate[e] = GATE ? g.rate[c + e] : 0.f;
+    v[e] = s > 0 ? g.carry[at + (s - 1) * step + e]
+                 : (g.init != nullptr ? g.init[b * g.init_b + c + e] : 0.f);
+  }
+  uint64_t cut = 0;
+  if (g.reset != nullptr) {
+    cut = __ballot(lane < n && g.reset[b * g.reset_b + t0 + min(lane, max(n - 1, 0))] != 0);
+  }
+
+  tv xv[kBack], rv[kBack], qv[kBack], dv[kBack];
+  float a[kBack][VEC], root[kBack][VEC], h[kBack][VEC];
+  float span_a[VEC], span_h[VEC], span_e[VEC];
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) span_a[e] = 1.f, span_h[e] = 0.f, span_e[e] = 0.f;
+  if (n > 0) {
+    const Span<T, VEC> x(g.x, b * g.x_b + t0 * g.x_t, g.x_t, c);
+    const Span<T, VEC> r(g.r, b * g.r_b + t0 * g.r_t, g.r_t, c);
+    const Span<T, VEC> q(GATE ? g.g : g.x, b * g.g_b + t0 * g.g_t, g.g_t, c);
+    const Span<T, VEC> d(g.dy, b * g.dy_b + t0 * g.dy_t, g.dy_t, c);
+#pragma unroll
+    for (int i = 0; i < kBack; ++i) {
+      const int t = min(i, n - 1);
+      xv[i] = __builtin_bit_cast(tv, x.load(t));
+      rv[i] = __builtin_bit_cast(tv, r.load(t));
+      if constexpr (GATE) qv[i] = __builtin_bit_cast(tv, q.load(t));
+      dv[i] = __builtin_bit_cast(tv, d.load(t));
+    }
+#pragma unroll
+    for (int i = 0; i < kBack; ++i) {
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        factor_root<GATE>(to_f(rv[i][e]), rate[e], a[i][e], root[i][e]);
+        h[i][e] = to_f(xv[i][e]);
+        if constexpr (GATE) h[i][e] *= root[i][e] * sigmoid2(to_f(qv[i][e]));
       }
     }
-    for (int t = t1 - 1; t >= t0; --t) {
-      float dx[1] = {0.f}, dr[1] = {0.f}, dg[1] = {0.f};
-      if (t < len) {
-        load_vec<T, 1>(g.x, b * g.x_b + t * g.x_t + c, x);
-        load_vec<T, 1>(g.r, b * g.r_b + t * g.r_t + c, r);
-        if constexpr (GATE) load_vec<T, 1>(g.g, b * g.g_b + t * g.g_t + c, q);
-        load_vec<T, 1>(g.dy, b * g.dy_b + t * g.dy_t + c, dy);
-        const Coef k = coef<GATE>(x[0], r[0], q[0], rate);
-        const float before = g.scratch[(static_cast<int64_t>(b) * kTile + t - t0) * g.width + c];
-        const float d = dy[0] + grad;
-        dx[0] = d * k.w;
-        if constexpr (GATE) {
-          const float dlog = d * (k.a * before - k.q * x[0] * (k.a * k.a * k.inv));
-          dr[0] = -rate * k.pp * dlog;
-          dg[0] = d * x[0] * k.s * k.qq;
-          sum -= k.p * dlog;
-        } else {
-          dr[0] = d * (k.a * before);
+    if (n < kBack) {
+#pragma unroll
+      for (int i = 0; i < kBack; ++i) {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+          a[i][e] = i >= n ? 1.f : a[i][e];
+          h[i][e] = i >= n ? 0.f : h[i][e];
+          if (i >= n) dv[i][e] = from_f<T>(0.f);
         }
-        const bool fresh = g.reset != nullptr && g.reset[b * g.reset_b + t] != 0;
-        grad = fresh ? 0.f : k.a * d;
       }
-      store_vec<T, 1>(g.dx, b * g.dx_b + t * g.dx_t + c, dx);
-      store_vec<T, 1>(g.dr, b * g.dr_b + t * g.dr_t + c, dr);
-      if constexpr (GATE) store_vec<T, 1>(g.dg, b * g.dg_b + t * g.dg_t + c, dg);
+    }
+    if (cut == 0) {
+#pragma unroll
+      for (int i = 0; i < kBack; ++i) {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+          span_h[e] = fmaf(a[i][e], span_h[e], h[i][e]);
+          span_a[e] *= a[i][e];
+          const int k = kBack - 1 - i;
+          span_e[e] = a[k][e] * (span_e[e] + to_f(dv[k][e]));
+        }
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < kBack; ++i) {
+        const int k = kBack - 1 - i;
+        const bool fresh = (cut >> i) & 1, last = (cut >> k) & 1;
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+          span_h[e] = fresh ? h[i][e] : fmaf(a[i][e], span_h[e], h[i][e]);
+          span_a[e] = -1.f;
+          span_e[e] = last ? 0.f : a[k][e] * (span_e[e] + to_f(dv[k][e]));
+        }
+      }
     }
   }
-  if (g.dinit != nullptr) g.dinit[b * g.dinit_b + c] = grad;
-  if constexpr (GATE) g.part[static_cast<int64_t>(b) * g.width + c] = sum;
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) {
+    s_a[w][lane * VEC + e] = span_a[e];
+    s_h[w][lane * VEC + e] = span_h[e];
+    s_e[w][lane * VEC + e] = span_e[e];
+  }
+  __syncthreads();
+  float u[VEC];  // the gradient that enters the tile from behind, then the wave
+  if (!CHAIN || link == 0) {
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) u[e] = g.dfin != nullptr ? g.dfin[b * g.dfin_b + c + e] : 0.f;
+  }
+  if (w == 0) {
+    float ta[VEC], te[VEC];
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+      ta[e] = 1.f, te[e] = 0.f;
+#pragma unroll
+      for (int k = kWaves - 1; k >= 0; --k) {
+        const float ka = s_a[k][lane * VEC + e];
+        te[e] = fold(ka, s_e[k][lane * VEC + e], te[e]);
+        ta[e] = join(ta[e], ka);
+      }
+    }
+    if (CHAIN && link > 0) {
+      bool known = true;
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        known = known && early[e] != kNotYet;
+        u[e] = __uint_as_float(early[e]);
+      }
+      if (!__all(known || !live)) {
+        if (live) {
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) {
+            const uint64_t m = static_cast<uint64_t>(word(ta[e])) << 32 | __float_as_uint(te[e]);
+            __hip_atomic_store(ch.maps + at + link * step + e, m, __ATOMIC_RELAXED,
+                               __HIP_MEMORY_SCOPE_AGENT);
+          }
+        }
+        look_back<VEC>(ch, link, at, step, live, u);
+      }
+    }
+    float out[VEC];
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+      out[e] = fold(ta[e], te[e], u[e]);
+      if constexpr (CHAIN) s_in[lane * VEC + e] = u[e];
+    }
+    if (live) {
+      if constexpr (CHAIN) {
+        if (s > 0) write_states<VEC>(ch.states + at + link * step, out);
+      }
+      if (s == 0 && g.dinit != nullptr) {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) g.dinit[b * g.dinit_b + c + e] = out[e];
+      }
+    }
+  }
+  // meanwhile the states before each token
+#pragma unroll
+  for (int k = 0; k < kWaves; ++k) {
+    if (k < w) {
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        v[e] = fold(s_a[k][lane * VEC + e], s_h[k][lane * VEC + e], v[e]);
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < kBack; ++i) {
+    const bool fresh = (cut >> i) & 1;
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+      const float before = fresh ? 0.f : v[e];
+      v[e] = fmaf(a[i][e], before, h[i][e]);
+      h[i][e] = before;
+    }
+  }
+  if constexpr (CHAIN) {
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) u[e] = s_in[lane * VEC + e];
+  }
+#pragma unroll
+  for (int k = kWaves - 1; k >= 0; --k) {
+    if (k > w) {
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        u[e] = fold(s_a[k][lane * VEC + e], s_e[k][lane * VEC + e], u[e]);
+      }
+    }
+  }
+  float sum[VEC];
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) sum[e] = 0.f;
+  const int rows = max(0, min(g.length - t0, kBack));
+#pragma unroll
+  for (int k = 0; k < kBack; ++k) {
+    const int i = kBack - 1 - k;
+    float dx[VEC], dr[VEC], dg[VEC];
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) dx[e] = 0.f, dr[e] = 0.f, dg[e] = 0.f;
+    if (i < n) {
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        const float d = to_f(dv[i][e]) + u[e];
+        if constexpr (GATE) {
+          const float x = to_f(xv[i][e]);
+          const Gate p(to_f(rv[i][e])), q(to_f(qv[i][e]));
+          // a h - q x a^2 / s, with 1 / s = 0 where s is (its factor rate p vanishes faster)
+          const float inv = root[i][e] == 0.f ? 0.f : __builtin_amdgcn_rcpf(root[i][e]);
+          const float dlog = d * a[i][e] * (h[i][e] - q.open * x * (a[i][e] * inv));
+          dx[e] = d * (root[i][e] * q.open);
+          dg[e] = dx[e] * x * q.shut;
+          dr[e] = -rate[e] * (p.open * p.shut) * dlog;
+          sum[e] = fmaf(-p.open, dlog, sum[e]);
+        } else {
+          dx[e] = d;
+          dr[e] = d * (a[i][e] * h[i][e]);
+        }
+        u[e] = (cut >> i) & 1 ? 0.f : a[i][e] * d;
+      }
+    }
+    if (live && i < rows) {
+      const int64_t t = t0 + i;
+      store_vec<T, VEC>(g.dx, b * g.dx_b + t * g.dx_t + c, dx);
+      store_vec<T, VEC>(g.dr, b * g.dr_b + t * g.dr_t + c, dr);
+      if constexpr (GATE) store_vec<T, VEC>(g.dg, b * g.dg_b + t * g.dg_t + c, dg);
+    }
+  }
+  if constexpr (GATE) {
+    __syncthreads();  // every wave is done with the maps
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) s_a[w][lane * VEC + e] = sum[e];
+    __syncthreads();
+    if (w == 0 && live) {
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        float total = 0.f;
+#pragma unroll
+        for (int k = 0; k < kWaves; ++k) total += s_a[k][lane * VEC + e];
+        g.part[at + s * step + e] = total;
+      }
+    }
+  }
 }
 
-// drate[c] = the sum of rows of partial sums, in 64 bits (a cancelling sum over all tokens).
-__global__ __launch_bounds__(256) void gated_rate_kernel(const float* part, float* drate, int rows,
-                                                         int width) {
-  const int c = blockIdx.x * 256 + threadIdx.x;
-  if (c >= width) return;
+// drate[c] = the sum of the tiles' shares, in 64 bits (a sum over all tokens that cancels), in a
+// fixed order: 16 waves take every 16th row each.
+__global__ __launch_bounds__(1024) void gated_rate_kernel(const float* part, float* drate,
+                                                          int64_t rows, int width) {
+  __shared__ double s_sum[16][64];
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const int c = blockIdx.x * 64 + lane, at = min(c, width - 1);
   double sum = 0.0;
-  for (int i = 0; i < rows; ++i) sum += part[static_cast<int64_t>(i) * width + c];
-  drate[c] = static_cast<float>(sum);
+#pragma unroll 8
+  for (int64_t i = w; i < rows; i += 16) sum += part[i * width + at];
+  s_sum[w][lane] = sum;
+  __syncthreads();
+  if (w == 0 && c < width) {
+#pragma unroll
+    for (int k = 1; k < 16; ++k) sum += s_sum[k][lane];
+    drate[c] = static_cast<float>(sum);
+  }
 }
 
 // ----------------------------------------------------------------------------- host
@@ -661,13 +865,19 @@ bool paired(const m3_tensor& t, int dims) {
   return true;
 }
 
-// Workspace of a chained call: the ticket, the maps, and the states where no carry is asked for.
+// Workspace of a chained call: the ticket, the maps and the states.
 constexpr size_t kTicketBytes = 64;
 
 size_t fwd_need(const m3_gated_scan_args& a) {
   if (a.length <= kTile || a.batch == 0 || a.width == 0) return 0;
   const size_t cells = static_cast<size_t>((a.length + kTile - 1) / kTile) * a.batch * a.width;
-  return kTicketBytes + cells * (present(a.carry) ? 8 : 12);
+  return kTicketBytes + cells * 12;
+}
+
+Chain chain(void* workspace, int64_t cells) {
+  char* ws = static_cast<char*>(workspace);
+  uint64_t* maps = reinterpret_cast<uint64_t*>(ws + kTicketBytes);
+  return Chain{reinterpret_cast<uint32_t*>(ws), maps, reinterpret_cast<uint32_t*>(maps + cells)};
 }
 
 template <typename T, bool GATE, int VEC>
@@ -676,17 +886,13 @@ int launch_tiles(const m3_gated_scan_args& a, const GatedGeom& g, hipStream_t st
   const int64_t count = static_cast<int64_t>((g.width + cols - 1) / cols) * g.batch * g.tiles;
   if (count > INT32_MAX) return fail(M3_EUNSUPPORTED, "m3_gated_scan: over 2^31 tiles");
   const dim3 grid(static_cast<unsigned>(count)), block(64 * kWaves);
-  Chain ch{};
   if (g.tiles == 1) {
-    hipLaunchKernelGGL((gated_tile_kernel<T, GATE, VEC, false>), grid, block, 0, stream, g, ch);
+    hipLaunchKernelGGL((gated_tile_kernel<T, GATE, VEC, false>), grid, block, 0, stream, g,
+                       Chain{});
     return check_launch("m3_gated_scan");
   }
   const int64_t cells = static_cast<int64_t>(g.tiles) * g.batch * g.width;
-  char* ws = static_cast<char*>(a.workspace);
-  ch.ticket = reinterpret_cast<uint32_t*>(ws);
-  ch.maps = reinterpret_cast<uint64_t*>(ws + kTicketBytes);
-  ch.states = g.carry != nullptr ? reinterpret_cast<uint32_t*>(g.carry)
-                                 : reinterpret_cast<uint32_t*>(ch.maps + cells);
+  const Chain ch = chain(a.workspace, cells);
   hipLaunchKernelGGL(gated_chain_kernel, dim3(static_cast<unsigned>((cells + 255) / 256)), dim3(256),
                      0, stream, ch, cells);
   const int rc = check_launch("m3_gated_scan");
@@ -700,7 +906,7 @@ int launch_fwd(const m3_gated_scan_args& a, hipStream_t stream) {
   const GatedGeom g = geom(a);
   const bool gate = present(a.gate);
   const bool two = a.width % 2 == 0 && paired(a.x, 3) && paired(a.decay, 3) && paired(a.gate, 3) &&
-                   paired(a.out, 3) && paired(a.carry, 1);
+                   paired(a.out, 3);
   if (a.length > 1) {
     if (gate) return two ? launch_tiles<T, true, 2>(a, g, stream) : launch_tiles<T, true, 1>(a, g, stream);
     return two ? launch_tiles<T, false, 2>(a, g, stream) : launch_tiles<T, false, 1>(a, g, stream);
@@ -715,6 +921,30 @@ int launch_fwd(const m3_gated_scan_args& a, hipStream_t stream) {
     else hipLaunchKernelGGL((gated_walk_kernel<T, false, 1>), grid, block, 0, stream, g);
   }
   return check_launch("m3_gated_scan");
+}
+
+template <typename T, bool GATE, int VEC>
+int launch_back(const m3_gated_scan_bwd_args& a, GatedGeom& g, hipStream_t stream) {
+  const int cols = 64 * VEC;
+  const int64_t count = static_cast<int64_t>((g.width + cols - 1) / cols) * g.batch * g.tiles;
+  if (count > INT32_MAX) return fail(M3_EUNSUPPORTED, "m3_gated_scan_bwd: over 2^31 tiles");
+  const dim3 grid(static_cast<unsigned>(count)), block(64 * kWaves);
+  const int64_t cells = static_cast<int64_t>(g.tiles) * g.batch * g.width;
+  const Chain ch = chain(a.fwd.workspace, cells);
+  g.part = reinterpret_cast<float*>(ch.states + cells);
+  int rc;
+  if (g.tiles == 1) {
+    hipLaunchKernelGGL((gated_back_kernel<T, GATE, VEC, false>), grid, block, 0, stream, g, ch);
+  } else {
+    hipLaunchKernelGGL(gated_chain_kernel, dim3(static_cast<unsigned>((cells + 255) / 256)),
+                       dim3(256), 0, stream, ch, cells);
+    if ((rc = check_launch("m3_gated_scan_bwd"))) return rc;
+    hipLaunchKernelGGL((gated_back_kernel<T, GATE, VEC, true>), grid, block, 0, stream, g, ch);
+  }
+  if ((rc = check_launch("m3_gated_scan_bwd")) || !GATE) return rc;
+  hipLaunchKernelGGL(gated_rate_kernel, dim3((g.width + 63) / 64), dim3(1024), 0, stream, g.part,
+                     g.drate, static_cast<int64_t>(g.tiles) * g.batch, g.width);
+  return check_launch("m3_gated_scan_bwd");
 }
 
 template <typename T>
@@ -733,26 +963,25 @@ int launch_bwd(const m3_gated_scan_bwd_args& a, hipStream_t stream) {
   g.dg_b = a.dgate.stride[0], g.dg_t = a.dgate.stride[1];
   g.dfin_b = a.dfinal.stride[0];
   g.dinit_b = a.dinitial.stride[0];
-  g.part = static_cast<float*>(a.fwd.workspace);
-  g.scratch = g.part + static_cast<int64_t>(g.batch) * g.width;
-  const int64_t lanes = static_cast<int64_t>(g.batch) * g.width;
-  const dim3 grid(static_cast<unsigned>((lanes + 255) / 256)), block(256);
-  if (present(a.fwd.gate)) {
-    hipLaunchKernelGGL((gated_walk_bwd_kernel<T, true>), grid, block, 0, stream, g);
-    const int rc = check_launch("m3_gated_scan_bwd");
-    if (rc != M3_OK) return rc;
-    hipLaunchKernelGGL(gated_rate_kernel, dim3((g.width + 255) / 256), block, 0, stream, g.part,
-                       g.drate, g.batch, g.width);
-  } else {
-    hipLaunchKernelGGL((gated_walk_bwd_kernel<T, false>), grid, block, 0, stream, g);
+  g.tiles = (g.length + kLeap - 1) / kLeap;
+  // 16-bit channels in pairs; FP32 ones singly, whose rows a wave reads as widely
+  if constexpr (sizeof(T) == 2) {
+    if (g.width % 2 == 0 && paired(a.fwd.x, 3) && paired(a.fwd.decay, 3) && paired(a.fwd.gate, 3) &&
+        paired(a.dout, 3) && paired(a.dx, 3) && paired(a.ddecay, 3) && paired(a.dgate, 3)) {
+      return present(a.fwd.gate) ? launch_back<T, true, 2>(a, g, stream)
+                                 : launch_back<T, false, 2>(a, g, stream);
+    }
   }
-  return check_launch("m3_gated_scan_bwd");
+  return present(a.fwd.gate) ? launch_back<T, true, 1>(a, g, stream)
+                             : launch_back<T, false, 1>(a, g, stream);
 }
 
 bool nothing(const m3_gated_scan_args& a) { return a.batch == 0 || a.length == 0 || a.width == 0; }
 
 size_t bwd_need(const m3_gated_scan_args& a) {
-  return nothing(a) ? 0 : static_cast<size_t>(a.batch) * a.width * (1 + kTile) * 4;
+  if (nothing(a)) return 0;
+  const size_t cells = static_cast<size_t>((a.length + kLeap - 1) / kLeap) * a.batch * a.width;
+  return kTicketBytes + cells * 16;  // maps, states, shares of drate
 }
 
 int validate_bwd(const m3_gated_scan_bwd_args& a) {
@@ -769,8 +998,11 @@ int validate_bwd(const m3_gated_scan_bwd_args& a) {
       (rc = check_rows(a.dinitial, "dinitial", 2, f.width, false, M3_F32))) {
     return rc;
   }
-  if (f.length > kTile && !present(f.carry) && live) {
-    return fail(M3_EINVAL, "m3_gated_scan_bwd: more than %d tokens need the forward's carry", kTile);
+  if (present(a.dout) && a.dout.stride[1] > (1 << 24)) {
+    return fail(M3_EUNSUPPORTED, "m3_gated_scan_bwd: tokens over 2^24 elements apart");
+  }
+  if (f.length > kLeap && !present(f.carry) && live) {
+    return fail(M3_EINVAL, "m3_gated_scan_bwd: more than %d tokens need the forward's carry", kLeap);
   }
   return M3_OK;
 }
@@ -824,8 +1056,9 @@ extern "C" int m3_gated_scan_bwd(const m3_gated_scan_bwd_args* args, hipStream_t
   const int rc = validate_bwd(*args);
   if (rc != M3_OK) return rc;
   if (nothing(args->fwd)) return M3_OK;
-  if (args->fwd.workspace == nullptr || args->fwd.workspace_bytes < bwd_need(args->fwd)) {
-    return fail(M3_EWORKSPACE, "m3_gated_scan_bwd: workspace of %zu bytes, %zu needed",
+  if (args->fwd.workspace == nullptr || args->fwd.workspace_bytes < bwd_need(args->fwd) ||
+      reinterpret_cast<uintptr_t>(args->fwd.workspace) % 8 != 0) {
+    return fail(M3_EWORKSPACE, "m3_gated_scan_bwd: workspace of %zu bytes, %zu needed (8-byte aligned)",
                 args->fwd.workspace_bytes, bwd_need(args->fwd));
   }
   switch (args->fwd.dtype) {
