@@ -44,14 +44,15 @@ template <> struct Code<_Float16> {
   }
 };
 
+// `sixteens` is Code<T>::kOne in a vector register (and-or takes one scalar, which the mask is).
 template <typename T>
-__device__ __forceinline__ typename Code<T>::v8 expand(uint32_t w) {
+__device__ __forceinline__ typename Code<T>::v8 expand(uint32_t w, uint32_t sixteens) {
   u32x4 v;
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     constexpr int up = Code<T>::kUp;
     const uint32_t at = 4 * j > up ? w >> (4 * j - up) : w << (up - 4 * j);
-    v[j] = (at & Code<T>::kMask) | Code<T>::kOne;
+    v[j] = (at & Code<T>::kMask) | sixteens;
   }
   return __builtin_bit_cast(typename Code<T>::v8, v);
 }
@@ -67,6 +68,7 @@ struct Lin4Geom {
   int64_t x_ld, r_ld, o_ld;
   int m, n, k, tk;     // tk: tiles of 128 columns
   int tiles;           // of 16 weight rows
+  bool four;           // rows of out are 8-byte aligned
   float eps;
 };
 
@@ -86,9 +88,38 @@ __device__ __forceinline__ f4 scales4(u32x2 v) {
   return s;
 }
 
+// -scale (16 + z) of four zeros in bytes.
+__device__ __forceinline__ f4 shifts4(uint32_t z, f4 scale) {
+  f4 v;
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    v[r] = -(16.f + static_cast<float>((z >> (8 * r)) & 0xffu)) * scale[r];
+  }
+  return v;
+}
+
+// An offset past every extent (all below 2^30 bytes), also with another added: the load gives 0. Offsets
+// go into a load whole, none as the scalar offset, which the range check does not add.
+constexpr unsigned kNowhere = 0x7fff0000u;
+
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t rsrc4(const void* base, int64_t bytes) {
   return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), static_cast<short>(0),
                                            static_cast<int>(bytes), 0x00020000);
+}
+
+// Eight x values times the norm's weights, rounded once; their squares go to sq.
+template <typename T>
+__device__ __forceinline__ u32x4 normed(u32x4 x, u32x4 weight, float& sq) {
+  using V8 = typename Code<T>::v8;
+  V8 b = __builtin_bit_cast(V8, x);
+  const V8 n = __builtin_bit_cast(V8, weight);
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const float xf = static_cast<float>(b[e]);
+    sq = fmaf(xf, xf, sq);
+    b[e] = static_cast<T>(xf * static_cast<float>(n[e]));
+  }
+  return __builtin_bit_cast(u32x4, b);
 }
 
 // Between a wave's writes of its own LDS region and its lanes' reads of one another's, and back: LDS
@@ -99,7 +130,12 @@ __device__ __forceinline__ void stage_turn() {
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 
-constexpr int kRowBytes = 256 + 16;  // an x row of a tile in LDS: 16 rows start in 16 bank groups
+// A barrier for what lies in LDS: global loads stay in flight across it.
+__device__ __forceinline__ void lds_barrier() {
+  asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+}
+
+constexpr int kRowBytes = 256;  // an x row of a tile in LDS; chunk c of 16 bytes lies at c ^ (row & 15)
 
 template <typename T, typename S, int GPT, int MT, int TN, int WAVES, bool NORM>
 __global__ __launch_bounds__(64 * WAVES) void linear4_kernel(const Lin4Geom g) {
@@ -113,7 +149,6 @@ __global__ __launch_bounds__(64 * WAVES) void linear4_kernel(const Lin4Geom g) {
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int l16 = lane & 15, lg = lane >> 4;
   const int tn = blockIdx.x * TN, m0 = blockIdx.y * (16 * MT);
-  const int loads = (min(g.m - m0, 16 * MT) + 3) / 4;  // four x rows of 256 bytes each
   char* const stage = lds + w * kStage;
 
   // what a tile of columns needs: codes, scales and zeros of TN tile rows, x rows 4 j + lg.
@@ -124,46 +159,41 @@ __global__ __launch_bounds__(64 * WAVES) void linear4_kernel(const Lin4Geom g) {
   const int64_t tile0 = static_cast<int64_t>(tn) * g.tk, left = min(g.tiles - tn, TN) * g.tk;
   const __amdgpu_buffer_rsrc_t rc = rsrc4(g.codes + tile0 * 1024, left * 1024);
   const __amdgpu_buffer_rsrc_t rs = rsrc4(g.scales + tile0 * (GPT * 32), left * (GPT * 32));
-  const __amdgpu_buffer_rsrc_t rz =
-      rsrc4(g.zeros + (g.zeros != nullptr ? tile0 * (GPT * 16) : 0), left * (GPT * 16));
+  const bool has_zeros = g.zeros != nullptr;  // else 0 is read, and 8 meant
+  const __amdgpu_buffer_rsrc_t rz = rsrc4(has_zeros ? g.zeros + tile0 * (GPT * 16) : g.codes,
+                                          has_zeros ? left * (GPT * 16) : 0);
+  const uint32_t eights = has_zeros ? 0u : 0x08080808u;
   const __amdgpu_buffer_rsrc_t rx = rsrc4(g.x, ((g.m - 1) * g.x_ld + g.k) * 2);
   const __amdgpu_buffer_rsrc_t rn = rsrc4(g.nw, NORM ? 2 * g.k : 0);
-  const int x_row = static_cast<int>(g.x_ld) * 2;
+  const unsigned x_row = static_cast<unsigned>(g.x_ld) * 2;
   auto fetch = [&](int t) __attribute__((always_inline)) {
 #pragma unroll
     for (int j = 0; j < TN; ++j) {
       const int tile = j * g.tk + t;
       // non-temporal (aux bit 1): the codes are read once a call
       code[j] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(
-                                              rc, 16 * lane, 1024 * tile, 2));
+                                              rc, 1024 * tile + 16 * lane, 0, 2));
 #pragma unroll
       for (int gi = 0; gi < GPT; ++gi) {
         const int at = (tile * GPT + gi) * 16;
         sc[j][gi] = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(
-                                                  rs, 8 * lg, 2 * at, 0));
-        if (g.zeros != nullptr) {
-          zr[j][gi] = __builtin_amdgcn_raw_buffer_load_b32(rz, 4 * lg, at, 0);
-        }
+                                                  rs, 2 * at + 8 * lg, 0, 0));
+        zr[j][gi] = __builtin_amdgcn_raw_buffer_load_b32(rz, at + 4 * lg, 0, 0);
       }
     }
-    const int k = 2 * (128 * t + 8 * l16);  // columns past K: read, not used
+    const int k = 128 * t + 8 * l16;
+    const unsigned at = k < g.k ? (m0 + lg) * x_row + 2 * k : kNowhere;
 #pragma unroll
     for (int j = 0; j < 4 * MT; ++j) {
-      if (j < loads) {
+      if (MT > 1 || j == 0 || 4 * j < g.m - m0) {
         xv[j] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(
-                                              rx, lg * x_row + k, (m0 + 4 * j) * x_row, 0));
+                                              rx, at + 4 * j * x_row, 0, 0));
       }
     }
     if constexpr (NORM) {
-      nv = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rn, k, 0, 0));
+      nv = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rn, 2 * k, 0, 0));
     }
   };
-#pragma unroll
-  for (int j = 0; j < TN; ++j) {
-#pragma unroll
-    for (int gi = 0; gi < GPT; ++gi) zr[j][gi] = 0x08080808u;
-  }
-
   f4 total[TN][MT];
 #pragma unroll
   for (int j = 0; j < TN; ++j) {
@@ -174,6 +204,8 @@ __global__ __launch_bounds__(64 * WAVES) void linear4_kernel(const Lin4Geom g) {
 #pragma unroll
   for (int j = 0; j < 4 * MT; ++j) sq[j] = 0.f;
   const V8 ones = __builtin_bit_cast(V8, u32x4{C::kUnit, C::kUnit, C::kUnit, C::kUnit});
+  uint32_t sixteens = C::kOne;
+  asm("" : "+v"(sixteens));
 
   if (w < g.tk) fetch(w);
   for (int t = w; t < g.tk; t += WAVES) {
@@ -185,67 +217,51 @@ __global__ __launch_bounds__(64 * WAVES) void linear4_kernel(const Lin4Geom g) {
 #pragma unroll
       for (int gi = 0; gi < GPT; ++gi) {
         s[j][gi] = scales4<S>(sc[j][gi]);
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          z[j][gi][r] = -(16.f + static_cast<float>((zr[j][gi] >> (8 * r)) & 0xffu)) * s[j][gi][r];
-        }
+        z[j][gi] = shifts4(zr[j][gi] | eights, s[j][gi]);
       }
     }
 #pragma unroll
     for (int j = 0; j < 4 * MT; ++j) {
-      if (j < loads) {
-        u32x4 v = xv[j];
-        if constexpr (NORM) {
-          V8 b = __builtin_bit_cast(V8, v);
-          const V8 n = __builtin_bit_cast(V8, nv);
-          const bool in = 128 * t + 8 * l16 < g.k;
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const float xf = static_cast<float>(b[e]), xk = in ? xf : 0.f;
-            sq[j] = fmaf(xk, xk, sq[j]);
-            b[e] = static_cast<T>(xf * static_cast<float>(n[e]));
-          }
-          v = __builtin_bit_cast(u32x4, b);
-        }
-        *reinterpret_cast<u32x4*>(stage + (4 * j + lg) * kRowBytes + 16 * l16) = v;
-      }
+      if (MT == 1 && j > 0 && 4 * j >= g.m - m0) break;  // rows that are not there
+      if constexpr (NORM) xv[j] = normed<T>(xv[j], nv, sq[j]);
+      *reinterpret_cast<u32x4*>(stage + (4 * j + lg) * kRowBytes +
+                                16 * (l16 ^ ((4 * j + lg) & 15))) = xv[j];
     }
     if (t + WAVES < g.tk) fetch(t + WAVES);
     stage_turn();
 #pragma unroll
     for (int gi = 0; gi < GPT; ++gi) {
-      if (128 * t + gi * (128 / GPT) < g.k) {
-        f4 acc[TN][MT], sum[MT];
+      f4 acc[TN][MT], sum[MT];
+#pragma unroll
+      for (int m = 0; m < MT; ++m) {
+        sum[m] = f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int j = 0; j < TN; ++j) acc[j][m] = f4{0.f, 0.f, 0.f, 0.f};
+      }
+#pragma unroll
+      for (int i = gi * (4 / GPT); i < (gi + 1) * (4 / GPT); ++i) {
+        V8 b[MT];
 #pragma unroll
         for (int m = 0; m < MT; ++m) {
-          sum[m] = f4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-          for (int j = 0; j < TN; ++j) acc[j][m] = f4{0.f, 0.f, 0.f, 0.f};
-        }
-#pragma unroll
-        for (int i = gi * (4 / GPT); i < (gi + 1) * (4 / GPT); ++i) {
-          V8 b[MT];
-#pragma unroll
-          for (int m = 0; m < MT; ++m) {
-            b[m] = *reinterpret_cast<const V8*>(stage + (16 * m + l16) * kRowBytes + 64 * i + 16 * lg);
-            sum[m] = C::mma(ones, b[m], sum[m]);
-          }
-#pragma unroll
-          for (int j = 0; j < TN; ++j) {
-            const V8 a = expand<T>(q[j][i]);
-#pragma unroll
-            for (int m = 0; m < MT; ++m) acc[j][m] = C::mma(a, b[m], acc[j][m]);
-          }
+          b[m] = *reinterpret_cast<const V8*>(stage + (16 * m + l16) * kRowBytes +
+                                              16 * ((4 * i + lg) ^ l16));
+          sum[m] = C::mma(ones, b[m], sum[m]);
         }
 #pragma unroll
         for (int j = 0; j < TN; ++j) {
+          const V8 a = expand<T>(q[j][i], sixteens);
 #pragma unroll
-          for (int m = 0; m < MT; ++m) {
+          for (int m = 0; m < MT; ++m) acc[j][m] = C::mma(a, b[m], acc[j][m]);
+        }
+      }
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-              total[j][m][r] = fmaf(z[j][gi][r], sum[m][r],
-                                    fmaf(s[j][gi][r], acc[j][m][r], total[j][m][r]));
-            }
+      for (int j = 0; j < TN; ++j) {
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            total[j][m][r] = fmaf(z[j][gi][r], sum[m][r],
+                                  fmaf(s[j][gi][r], acc[j][m][r], total[j][m][r]));
           }
         }
       }
@@ -296,6 +312,268 @@ __global__ __launch_bounds__(64 * WAVES) void linear4_kernel(const Lin4Geom g) {
       y += static_cast<float>(static_cast<const T*>(g.res)[m * g.r_ld + n]);
     }
     static_cast<T*>(g.out)[m * g.o_ld + n] = static_cast<T>(y);
+  }
+}
+
+// Many rows of x and many of W: a workgroup of four waves takes 64 x rows and 4 TN tiles of weight
+// rows, TN for each wave, over all of K. A tile of x columns is staged once for the workgroup, in two
+// LDS buffers; x is three tiles ahead of its use (two of them in registers), the codes two to
+// four. Wave
+// w forms X for x block w and leaves it to the others, who apply it a tile later.
+template <typename T, typename S, int GPT, int TN, int KS, bool NORM>
+__global__ __launch_bounds__(256 * KS, 2) void linear4_wide_kernel(const Lin4Geom g) {
+  using C = Code<T>;
+  using V8 = typename C::v8;
+  constexpr int MT = 4, kStage = MT * 16 * 256;  // an x block for each wave
+  constexpr int kAhead = 2;
+  static_assert(KS <= 2 && 3 * kStage >= TN * MT * 4096, "the second team's sums fit its stages");
+  __shared__ __attribute__((aligned(16))) char lds_all[KS][3 * kStage];
+  __shared__ float s_x_all[KS][2][GPT][16 * MT], s_sq[NORM ? KS : 1][16 * MT];
+  const int team = __builtin_amdgcn_readfirstlane(threadIdx.x >> 8), tid = threadIdx.x & 255;
+  const int lane = tid & 63;
+  const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  char* const lds = lds_all[team];
+  auto& s_x = s_x_all[team];
+  const int l16 = lane & 15, lg = lane >> 4;
+  const int tn = (blockIdx.x * 4 + w) * TN, m0 = blockIdx.y * (16 * MT);
+
+  // reads past an extent give 0: tile rows past the last, x rows past M
+  const int64_t tile0 = static_cast<int64_t>(min(tn, g.tiles)) * g.tk;
+  const int64_t left = max(0, min(g.tiles - tn, TN)) * g.tk;
+  const __amdgpu_buffer_rsrc_t rc = rsrc4(g.codes + tile0 * 1024, left * 1024);
+  const __amdgpu_buffer_rsrc_t rs = rsrc4(g.scales + tile0 * (GPT * 32), left * (GPT * 32));
+  const bool has_zeros = g.zeros != nullptr;  // else 0 is read, and 8 meant
+  const __amdgpu_buffer_rsrc_t rz = rsrc4(has_zeros ? g.zeros + tile0 * (GPT * 16) : g.codes,
+                                          has_zeros ? left * (GPT * 16) : 0);
+  const uint32_t eights = has_zeros ? 0u : 0x08080808u;
+  const __amdgpu_buffer_rsrc_t rx = rsrc4(g.x, ((g.m - 1) * g.x_ld + g.k) * 2);
+  const __amdgpu_buffer_rsrc_t rn = rsrc4(g.nw, NORM ? 2 * g.k : 0);
+  const unsigned x_row = static_cast<unsigned>(g.x_ld) * 2;
+  const int row = tid >> 4, chunk = tid & 15;  // what this thread stages: rows 16 u + row
+
+  u32x4 code[kAhead][TN], xv[MT], nv;
+  u32x2 sc[kAhead][TN][GPT];
+  uint32_t zr[kAhead][TN][GPT];
+  auto fetch_w = [&](int d, int t) __attribute__((always_inline)) {
+#pragma unroll
+    for (int j = 0; j < TN; ++j) {
+      // tiles past K: nothing, which makes every product 0
+      const unsigned tile = j * g.tk + t, none = t < g.tk ? 0u : kNowhere;
+      code[d][j] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(
+                                                 rc, (none + 1024 * tile) + 16 * lane, 0, 2));
+#pragma unroll
+      for (int gi = 0; gi < GPT; ++gi) {
+        const unsigned at = (tile * GPT + gi) * 16;
+        sc[d][j][gi] = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(
+                                                     rs, (none + 2 * at) + 8 * lg, 0, 0));
+        zr[d][j][gi] = __builtin_amdgcn_raw_buffer_load_b32(rz, (none + at) + 4 * lg, 0, 0);
+      }
+    }
+  };
+  auto fetch_x = [&](int t) __attribute__((always_inline)) {
+    const int k = 128 * t + 8 * chunk;
+    const unsigned at = k < g.k ? (m0 + row) * x_row + 2 * k : kNowhere;
+#pragma unroll
+    for (int u = 0; u < MT; ++u) {
+      xv[u] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(
+                                            rx, at + 16 * u * x_row, 0, 0));
+    }
+    if constexpr (NORM) {
+      nv = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rn, 2 * k, 0, 0));
+    }
+  };
+  float sq[MT];
+  auto put_x = [&](int buffer) __attribute__((always_inline)) {
+#pragma unroll
+    for (int u = 0; u < MT; ++u) {
+      if constexpr (NORM) xv[u] = normed<T>(xv[u], nv, sq[u]);
+      *reinterpret_cast<u32x4*>(lds + buffer + (16 * u + row) * 256 + 16 * (chunk ^ row)) = xv[u];
+    }
+  };
+
+  f4 total[TN][MT], acc[2][TN][MT], z[TN][GPT], last[TN];
+#pragma unroll
+  for (int j = 0; j < TN; ++j) {
+    last[j] = f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int gi = 0; gi < GPT; ++gi) z[j][gi] = last[j];
+#pragma unroll
+    for (int m = 0; m < MT; ++m) total[j][m] = acc[0][j][m] = acc[1][j][m] = last[j];
+  }
+#pragma unroll
+  for (int u = 0; u < MT; ++u) sq[u] = 0.f;
+  const V8 ones = __builtin_bit_cast(V8, u32x4{C::kUnit, C::kUnit, C::kUnit, C::kUnit});
+  uint32_t sixteens = C::kOne;
+  asm("" : "+v"(sixteens));
+  // total -= scale (16 + z) X of a group of the tile before, whose X lies in s_x[b]
+  auto shift = [&](int b, int gi) __attribute__((always_inline)) {
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+      const float x = s_x[b][gi][16 * m + l16];
+#pragma unroll
+      for (int j = 0; j < TN; ++j) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) total[j][m][r] = fmaf(z[j][gi][r], x, total[j][m][r]);
+      }
+    }
+  };
+  // total += scale A of the group before
+  auto settle = [&](int p) __attribute__((always_inline)) {
+#pragma unroll
+    for (int j = 0; j < TN; ++j) {
+#pragma unroll
+      for (int m = 0; m < MT; ++m) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          total[j][m][r] = fmaf(last[j][r], acc[p][j][m][r], total[j][m][r]);
+        }
+        asm volatile("" : "+v"(total[j][m]));  // here, not all after the loop
+      }
+    }
+  };
+  V8 b[2][MT + 1];
+  auto read = [&](int p, int buffer, int i) __attribute__((always_inline)) {
+    // chunk c of a row lies at c ^ (row & 15): a read of 16 rows meets 16 bank groups
+    const char* at = lds + buffer + l16 * 256 + 16 * ((4 * i + lg) ^ l16);
+#pragma unroll
+    for (int m = 0; m < MT; ++m) b[p][m] = *reinterpret_cast<const V8*>(at + 16 * m * 256);
+    b[p][MT] = *reinterpret_cast<const V8*>(at + 16 * w * 256);
+  };
+
+  fetch_x(team);
+#pragma unroll
+  for (int d = 0; d < kAhead; ++d) fetch_w(d, team + KS * d);
+  put_x(0);
+  fetch_x(team + KS);
+  put_x(kStage);
+  fetch_x(team + 2 * KS);
+  if (tid < 16 * MT) {  // no tile is before the first
+#pragma unroll
+    for (int gi = 0; gi < GPT; ++gi) s_x[1][gi][tid] = 0.f;
+  }
+  lds_barrier();
+  read(0, 0, 0);
+  int here = 0, next = kStage, after = 2 * kStage;
+  // Whole groups of kAhead tiles with no way out inside, so that the compiler's counts of loads in
+  // flight stay exact; tiles past K add 0. A tile's x is put in place two tiles early, so its
+  // operands can be read a step ahead also across a barrier. A group's sums are scaled while the next group's form.
+  for (int t0 = team; t0 - team < g.tk; t0 += KS * kAhead) {
+#pragma unroll
+    for (int d = 0; d < kAhead; ++d) {
+      const int t = t0 + KS * d;
+      put_x(after);
+      fetch_x(t + 3 * KS);
+      constexpr int kPer = 4 / GPT;  // steps of a group
+      f4 sum;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int gi = i / kPer, p = (GPT * d + gi) & 1;
+        read((i + 1) & 1, i < 3 ? here : next, (i + 1) & 3);
+        if (i % kPer == 0) {
+          sum = f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int j = 0; j < TN; ++j) {
+#pragma unroll
+            for (int m = 0; m < MT; ++m) acc[p][j][m] = sum;
+          }
+        }
+        sum = C::mma(ones, b[i & 1][MT], sum);
+#pragma unroll
+        for (int j = 0; j < TN; ++j) {
+          const V8 a = expand<T>(code[d][j][i], sixteens);
+#pragma unroll
+          for (int m = 0; m < MT; ++m) acc[p][j][m] = C::mma(a, b[i & 1][m], acc[p][j][m]);
+        }
+        if (i % kPer == 0) {
+          settle(p ^ 1);
+          shift((d + 1) & 1, gi);
+#pragma unroll
+          for (int j = 0; j < TN; ++j) {
+            last[j] = scales4<S>(sc[d][j][gi]);
+            z[j][gi] = shifts4(zr[d][j][gi] | eights, last[j]);
+          }
+        }
+        if (i % kPer == kPer - 1) s_x[d & 1][gi][16 * w + l16] = sum[0];  // the same from four lanes
+        // one matrix product at a time and a few vector instructions under it
+#pragma unroll
+        for (int u = 0; u < TN * MT + 1; ++u) {
+          __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+          __builtin_amdgcn_sched_group_barrier(0x002, 5, 0);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      fetch_w(d, t + KS * kAhead);
+      lds_barrier();
+      const int free = here;
+      here = next, next = after, after = free;
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  }
+  settle((GPT * kAhead - 1) & 1);
+#pragma unroll
+  for (int gi = 0; gi < GPT; ++gi) shift((kAhead - 1) & 1, gi);
+  if constexpr (NORM) {
+#pragma unroll
+    for (int u = 0; u < MT; ++u) {
+      float v = sq[u];
+#pragma unroll
+      for (int o = 8; o > 0; o >>= 1) v += __shfl_xor(v, o);
+      if (chunk == 0) s_sq[team][16 * u + row] = v;
+    }
+  }
+  if constexpr (KS == 2) {  // the second team's sums, through its own stages
+    __syncthreads();
+    f4* const sums = reinterpret_cast<f4*>(lds_all[KS - 1]);
+    if (team == 1) {
+#pragma unroll
+      for (int j = 0; j < TN; ++j) {
+#pragma unroll
+        for (int m = 0; m < MT; ++m) sums[(j * MT + m) * 256 + tid] = total[j][m];
+      }
+    }
+    __syncthreads();
+    if (team == 1) return;
+#pragma unroll
+    for (int j = 0; j < TN; ++j) {
+#pragma unroll
+      for (int m = 0; m < MT; ++m) total[j][m] += sums[(j * MT + m) * 256 + tid];
+    }
+  } else if constexpr (NORM) {
+    __syncthreads();
+  }
+  // lane holds weight rows 16 j + 4 lg + r of the wave's, x rows 16 m + l16
+#pragma unroll
+  for (int m = 0; m < MT; ++m) {
+    const int xr = m0 + 16 * m + l16;
+    if (xr >= g.m) continue;
+    float scale = 1.f;
+    if constexpr (NORM) {
+      float total_sq = s_sq[0][16 * m + l16];
+      if constexpr (KS == 2) total_sq += s_sq[1][16 * m + l16];
+      scale = rsqrtf(total_sq / static_cast<float>(g.k) + g.eps);
+    }
+#pragma unroll
+    for (int j = 0; j < TN; ++j) {
+      const int n = 16 * (tn + j) + 4 * lg;
+      const T* res = g.res != nullptr ? static_cast<const T*>(g.res) + xr * g.r_ld + n : nullptr;
+      T* out = static_cast<T*>(g.out) + xr * g.o_ld + n;
+      typedef T t4 __attribute__((ext_vector_type(4)));
+      t4 y;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        float v = total[j][m][r] * scale;
+        if (res != nullptr && n + r < g.n) v += static_cast<float>(res[r]);
+        y[r] = static_cast<T>(v);
+      }
+      if (g.four && n + 4 <= g.n) {
+        *reinterpret_cast<t4*>(out) = y;
+      } else {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          if (n + r < g.n) out[r] = y[r];
+        }
+      }
+    }
   }
 }
 
@@ -369,19 +647,36 @@ int launch_kernel(const Lin4Geom& g, hipStream_t stream) {
   return check_launch("m3_linear4");
 }
 
+template <typename T, typename S, int GPT, int TN, int KS>
+int launch_wide(const Lin4Geom& g, hipStream_t stream) {
+  const dim3 grid((g.tiles + 4 * TN - 1) / (4 * TN), (g.m + 63) / 64), block(256 * KS);
+  if (g.nw != nullptr) {
+    hipLaunchKernelGGL((linear4_wide_kernel<T, S, GPT, TN, KS, true>), grid, block, 0, stream, g);
+  } else {
+    hipLaunchKernelGGL((linear4_wide_kernel<T, S, GPT, TN, KS, false>), grid, block, 0, stream, g);
+  }
+  return check_launch("m3_linear4");
+}
+
 template <typename T, typename S, int GPT>
 int launch_rows(const Lin4Geom& g, hipStream_t stream) {
   if (g.m <= 16) {
-    if (g.tiles < 256 && g.tk >= 32) return launch_kernel<T, S, GPT, 1, 1, 16>(g, stream);
-    if (g.tiles < 1024) return launch_kernel<T, S, GPT, 1, 1, 8>(g, stream);
-    return launch_kernel<T, S, GPT, 1, 2, 8>(g, stream);
+    if (g.tiles < 384) return launch_kernel<T, S, GPT, 1, 1, 8>(g, stream);
+    if constexpr (GPT < 4) {
+      if (g.tiles >= 1024) return launch_kernel<T, S, GPT, 1, 4, 4>(g, stream);
+      if (g.nw != nullptr) return launch_kernel<T, S, GPT, 1, 2, 4>(g, stream);
+    }
+    return launch_kernel<T, S, GPT, 1, 1, 4>(g, stream);
   }
-  if (g.m <= 32) {
-    return g.tiles < 512 ? launch_kernel<T, S, GPT, 2, 1, 8>(g, stream)
-                         : launch_kernel<T, S, GPT, 2, 2, 8>(g, stream);
+  const int blocks = (g.m + 63) / 64;
+  if (g.tiles < 384 && g.tiles * blocks < 512) return launch_kernel<T, S, GPT, 2, 1, 8>(g, stream);
+  const int w1 = (g.tiles + 3) / 4 * blocks, w2 = (g.tiles + 7) / 8 * blocks;
+  const int two = (w2 + 255) / 256 * 65, one = (w1 + 255) / 256 * 44, half = max(w1, 512) * 87 / 512;
+  if constexpr (GPT < 4) {
+    if (two <= one && two <= half) return launch_wide<T, S, GPT, 2, 2>(g, stream);
   }
-  return g.tiles < 512 ? launch_kernel<T, S, GPT, 4, 1, 8>(g, stream)
-                       : launch_kernel<T, S, GPT, 4, 2, 8>(g, stream);
+  return one <= half ? launch_wide<T, S, GPT, 1, 2>(g, stream)
+                     : launch_wide<T, S, GPT, 1, 1>(g, stream);
 }
 
 template <typename T, typename S>
@@ -415,7 +710,9 @@ extern "C" int m3_linear4(const m3_linear4_args* args, hipStream_t stream) {
                    static_cast<const char*>(a.norm_weight.ptr), a.residual.ptr, a.out.ptr,
                    a.x.stride[0], a.residual.stride[0], a.out.stride[0],
                    static_cast<int>(a.m), static_cast<int>(a.n), static_cast<int>(a.k),
-                   static_cast<int>((a.k + 127) / 128), static_cast<int>((a.n + 15) / 16), a.norm_eps};
+                   static_cast<int>((a.k + 127) / 128), static_cast<int>((a.n + 15) / 16),
+                   reinterpret_cast<uintptr_t>(a.out.ptr) % 8 == 0 && a.out.stride[0] % 4 == 0,
+                   a.norm_eps};
   return a.dtype == M3_BF16 ? launch<__bf16>(g, a.scale_dtype, a.group, stream)
                             : launch<_Float16>(g, a.scale_dtype, a.group, stream);
 }
