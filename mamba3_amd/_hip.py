@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 
 import torch
 
@@ -122,6 +123,15 @@ class Linear4Args(ctypes.Structure):
     ]
 
 
+# The same blocks as formats of `struct`: a decode call takes its host about as long as its kernels the
+# GPU, and packing a block whole costs a third of filling a Structure field by field. A block is bytes:
+# no two calls share one.
+_TENSOR = "Pii5q"
+GATED_SCAN = struct.Struct("@4i" + 5 * _TENSOR + "PPq" + 3 * _TENSOR + "PN")
+GATED_SCAN_BWD = struct.Struct(GATED_SCAN.format + 7 * _TENSOR)
+LINEAR4 = struct.Struct("@3q3ifPPP" + 4 * _TENSOR)
+NO_TENSOR = (0,) * 8
+
 ENTRY_POINTS = ("m3_scan_fwd", "m3_scan_workspace_size", "m3_scan_segments", "m3_scan_fwd_noalloc",
                 "m3_chunk_state", "m3_step", "m3_linear", "m3_linear_workspace_size",
                 "m3_rms_norm", "m3_gated_scan", "m3_gated_scan_workspace_size",
@@ -179,12 +189,6 @@ def tensor(t: torch.Tensor | None) -> Tensor:
     return out
 
 
-def row_tensor(t: torch.Tensor) -> Tensor:
-    """``tensor`` for an operand that is present, in one construction (the decode calls' host time
-    is as long as their kernels')."""
-    return Tensor(t.data_ptr() if t.numel() else None, _DTYPE[t.dtype], 0, t.stride())
-
-
 def dtype_code(dtype: torch.dtype) -> int:
     try:
         return _DTYPE[dtype]
@@ -207,10 +211,11 @@ def scan_workspace(args: ctypes.Structure, device: torch.device,
     return ws
 
 
-def workspace_query(name: str, args: ctypes.Structure, nbytes: ctypes.c_size_t) -> None:
+def workspace_query(name: str, args: ctypes.Structure | bytes, nbytes: ctypes.c_size_t) -> None:
     """A workspace query into ``nbytes``; raise on failure."""
     lib = load()
-    rc = getattr(lib, name)(ctypes.byref(args), ctypes.byref(nbytes))
+    rc = getattr(lib, name)(args if isinstance(args, bytes) else ctypes.byref(args),
+                            ctypes.byref(nbytes))
     if rc != 0:
         raise HipError(name, rc, lib.m3_last_error().decode(errors="replace"))
 
@@ -226,17 +231,23 @@ def scan_segments(args: ctypes.Structure, concurrent: int) -> int:
     return g.value
 
 
-def launch(name: str, args: ctypes.Structure, device: torch.device) -> None:
-    """``call`` on ``device``'s current torch stream, with that device made current if it is not,
-    and without a stream object."""
-    index = device.index
-    if index != torch.cuda.current_device():
-        with torch.cuda.device(device):
-            return call(name, args, device)
-    lib = load()
-    rc = getattr(lib, name)(ctypes.byref(args), torch._C._cuda_getCurrentRawStream(index))
+def launch(name: str, block: bytes, index: int) -> None:
+    """``call`` with a packed argument block on device ``index``'s current torch stream, with that
+    device made current if it is not."""
+    if index != torch._C._cuda_getDevice():
+        with torch.cuda.device(index):
+            return launch(name, block, index)
+    lib = _lib or load()
+    rc = getattr(lib, name)(block, torch._C._cuda_getCurrentRawStream(index))
     if rc != 0:
         raise HipError(name, rc, lib.m3_last_error().decode(errors="replace"))
+
+
+def need(name: str, block: bytes) -> int:
+    """The workspace bytes that the query ``name`` gives for a packed argument block."""
+    nbytes = ctypes.c_size_t(0)
+    workspace_query(name, block, nbytes)
+    return nbytes.value
 
 
 def call(name: str, args: ctypes.Structure, device: torch.device) -> None:

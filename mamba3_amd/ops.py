@@ -15,8 +15,6 @@ step / scan ran on the HIP path (the reference's ``_TRITON_LAST_DISPATCH`` /
 
 from __future__ import annotations
 
-import ctypes
-
 import torch
 
 from . import _hip
@@ -800,36 +798,41 @@ def linear4(x: torch.Tensor, weight: Weight4, residual: torch.Tensor | None = No
     ``norm_weight [K]`` ``x`` is first RMS-normalised, as ``F.rms_norm(x, (K,), norm_weight,
     norm_eps)``. No backward.
     """
-    device = _require_device(x, residual, out, norm_weight)
+    index = x.get_device()
+    if index < 0 or any(t is not None and t.get_device() != index
+                        for t in (residual, out, norm_weight)):
+        _require_device(x, residual, out, norm_weight)
     _require_inference(x, residual, norm_weight)
     if not linear4_supported(x, weight):
         raise ValueError(f"linear4: unsupported operands x {tuple(x.shape)} {x.dtype} on "
                          f"{x.device}, weight {weight.shape} on {weight.device}")
-    m, (n, k) = x.shape[0], weight.shape
+    m, (n, k), dtype = x.shape[0], weight.shape, x.dtype
     for name, t in (("residual", residual), ("out", out)):
-        if t is not None and (tuple(t.shape) != (m, n) or t.dtype != x.dtype):
-            raise ValueError(f"linear4: {name} must be [{m}, {n}] {x.dtype}, got "
+        if t is not None and (t.shape != (m, n) or t.dtype != dtype):
+            raise ValueError(f"linear4: {name} must be [{m}, {n}] {dtype}, got "
                              f"{tuple(t.shape)} {t.dtype}")
-    x = _aligned16(x)
-    code, tensor = _hip.dtype_code(x.dtype), _hip.Tensor
-    args = _hip.Linear4Args(m, n, k, code, _hip.dtype_code(weight.dtype), weight.group, norm_eps,
-                            weight.codes.data_ptr(), weight.scales.data_ptr(),
-                            None if weight.zeros is None else weight.zeros.data_ptr(),
-                            tensor(x.data_ptr(), code, 0, x.stride()))
     if norm_weight is not None:
         if norm_weight.shape != (k,):
             raise ValueError(f"linear4: norm_weight must be [{k}]")
-        norm_weight = _aligned16(norm_weight.detach().to(x.dtype))
-        args.norm_weight = tensor(norm_weight.data_ptr(), code, 0, (1,))
-    if residual is not None:
-        residual = _inner(residual)
-        args.residual = tensor(residual.data_ptr(), code, 0, residual.stride())
+        if norm_weight.dtype != dtype:
+            norm_weight = norm_weight.detach().to(dtype)
+        norm_weight = _aligned16(norm_weight)
+    x = _aligned16(x)
+    residual = _inner(residual)
     if out is None:
-        out = torch.empty(m, n, dtype=x.dtype, device=device)
+        out = x.new_empty((m, n))
     elif n > 1 and out.stride(1) != 1:
         raise ValueError("linear4: out needs a unit inner stride")
-    args.out = tensor(out.data_ptr(), code, 0, out.stride())
-    _hip.launch("m3_linear4", args, device)
+    code = _hip.dtype_code(dtype)
+    none = _hip.NO_TENSOR
+    _hip.launch("m3_linear4", _hip.LINEAR4.pack(
+        m, n, k, code, _hip.dtype_code(weight.dtype), weight.group, norm_eps,
+        weight.codes.data_ptr(), weight.scales.data_ptr(),
+        0 if weight.zeros is None else weight.zeros.data_ptr(),
+        x.data_ptr(), code, 0, *x.stride(), 0, 0, 0,
+        *(none if norm_weight is None else (norm_weight.data_ptr(), code, 0, 1, 0, 0, 0, 0)),
+        *(none if residual is None else (residual.data_ptr(), code, 0, *residual.stride(), 0, 0, 0)),
+        out.data_ptr(), code, 0, *out.stride(), 0, 0, 0), index)
     return out
 
 
@@ -857,35 +860,36 @@ def _rate32(rate: torch.Tensor | None) -> torch.Tensor | None:
     return rate.float().contiguous()
 
 
-def _gated_args(x, decay, gate, rate, state, lengths, reset) -> _hip.GatedScanArgs:
-    """The inputs of a gated scan [B, L, C] as an argument block; the caller keeps the tensors."""
-    batch, length, width = x.shape
-    args = _hip.GatedScanArgs(batch, length, width, _hip.dtype_code(x.dtype), _hip.row_tensor(x),
-                              _hip.row_tensor(decay))
-    if gate is not None:
-        args.gate, args.rate = _hip.row_tensor(gate), _hip.row_tensor(rate)
-    if state is not None:
-        args.initial_state = _hip.row_tensor(state)
-    if lengths is not None:
-        args.lengths = lengths.data_ptr()
-    if reset is not None:
-        args.reset, args.reset_stride = reset.data_ptr(), reset.stride(0)
-    return args
+def _packed(t: torch.Tensor | None, code: int = 0):
+    """A tensor of 1 to 3 axes as the values of its descriptor."""
+    if t is None:
+        return _hip.NO_TENSOR
+    strides = t.stride()
+    return (t.data_ptr(), code, 0, *strides, *(0,) * (5 - len(strides)))
+
+
+def _gated_inputs(x, decay, gate, rate, state, lengths, reset):
+    """The inputs of a gated scan [B, L, C] as the first values of its argument block."""
+    code = _hip.dtype_code(x.dtype)
+    return (*x.shape, code, *_packed(x, code), *_packed(decay, code), *_packed(gate, code),
+            *_packed(rate), *_packed(state), 0 if lengths is None else lengths.data_ptr(),
+            *((0, 0) if reset is None else (reset.data_ptr(), reset.stride(0))))
 
 
 def _gated_forward(x, decay, gate, rate, state, lengths, reset, want_carry):
     batch, length, width = x.shape
-    args = _gated_args(x, decay, gate, rate, state, lengths, reset)
-    out = torch.empty(batch, length, width, dtype=x.dtype, device=x.device)
-    final = torch.empty(batch, width, dtype=torch.float32, device=x.device)
-    carry = None
-    args.out, args.final_state = _hip.row_tensor(out), _hip.row_tensor(final)
-    if want_carry:
-        carry = torch.empty(-(-length // _hip.GATED_TILE), batch, width, dtype=torch.float32,
-                            device=x.device)
-        args.carry = _hip.row_tensor(carry)
-    ws = _hip.scan_workspace(args, x.device, "m3_gated_scan_workspace_size")
-    _hip.launch("m3_gated_scan", args, x.device)
+    out = x.new_empty(x.shape)
+    final = torch.empty((batch, width), dtype=torch.float32, device=x.device)
+    carry = torch.empty((-(-length // _hip.GATED_TILE), batch, width), dtype=torch.float32,
+                        device=x.device) if want_carry else None
+    values = (*_gated_inputs(x, decay, gate, rate, state, lengths, reset),
+              *_packed(out, _hip.dtype_code(x.dtype)), *_packed(final), *_packed(carry))
+    block, ws = _hip.GATED_SCAN.pack(*values, 0, 0), None
+    size = _hip.need("m3_gated_scan_workspace_size", block)
+    if size:
+        ws = torch.empty(size, dtype=torch.uint8, device=x.device)
+        block = _hip.GATED_SCAN.pack(*values, ws.data_ptr(), size)
+    _hip.launch("m3_gated_scan", block, x.get_device())
     del ws
     return out, final, carry
 
@@ -907,27 +911,25 @@ class _GatedScan(torch.autograd.Function):
         x, decay, gate, rate, state, lengths, reset, carry = ctx.saved_tensors
         if dout is None and dfinal is None:
             return (None,) * 7
-        dout = torch.zeros(x.shape, dtype=x.dtype, device=x.device) if dout is None else _inner(dout)
+        code, none = _hip.dtype_code(x.dtype), _hip.NO_TENSOR
+        dout = x.new_zeros(x.shape) if dout is None else _inner(dout)
         dfinal = _inner(dfinal)
-        args = _hip.GatedScanBwdArgs(_gated_args(x, decay, gate, rate, state, lengths, reset),
-                                     _hip.row_tensor(dout))
-        args.fwd.carry = _hip.row_tensor(carry)
-        if dfinal is not None:
-            args.dfinal = _hip.row_tensor(dfinal)
-        dx, ddecay = (torch.empty(x.shape, dtype=x.dtype, device=x.device) for _ in range(2))
-        args.dx, args.ddecay = _hip.row_tensor(dx), _hip.row_tensor(ddecay)
+        dx, ddecay = x.new_empty(x.shape), x.new_empty(x.shape)
         dgate = drate = dstate = None
         if gate is not None:
-            dgate, drate = torch.empty_like(dx), torch.empty_like(rate)
-            args.dgate, args.drate = _hip.row_tensor(dgate), _hip.row_tensor(drate)
+            dgate, drate = x.new_empty(x.shape), torch.empty_like(rate)
         if state is not None:
-            dstate = torch.empty(state.shape, dtype=torch.float32, device=x.device)
-            args.dinitial = _hip.row_tensor(dstate)
-        need = ctypes.c_size_t(0)
-        _hip.workspace_query("m3_gated_scan_bwd_workspace_size", args, need)
-        ws = torch.empty(need.value, dtype=torch.uint8, device=x.device)
-        args.fwd.workspace, args.fwd.workspace_bytes = ws.data_ptr(), need.value
-        _hip.launch("m3_gated_scan_bwd", args, x.device)
+            dstate = torch.empty_like(state, memory_format=torch.contiguous_format)
+        inputs = (*_gated_inputs(x, decay, gate, rate, state, lengths, reset), *none, *none,
+                  *_packed(carry))
+        grads = (*_packed(dout, code), *_packed(dfinal), *_packed(dx, code),
+                 *_packed(ddecay, code), *_packed(dgate, code), *_packed(drate),
+                 *_packed(dstate))
+        size = _hip.need("m3_gated_scan_bwd_workspace_size",
+                         _hip.GATED_SCAN_BWD.pack(*inputs, 0, 0, *grads))
+        ws = torch.empty(size, dtype=torch.uint8, device=x.device)
+        _hip.launch("m3_gated_scan_bwd",
+                    _hip.GATED_SCAN_BWD.pack(*inputs, ws.data_ptr(), size, *grads), x.get_device())
         return dx, ddecay, dgate, drate, dstate, None, None
 
 
@@ -966,12 +968,10 @@ def gated_scan(x: torch.Tensor, decay: torch.Tensor, gate: torch.Tensor | None =
         final = (torch.zeros(batch, width, device=device) if initial_state is None
                  else initial_state.clone())
         return torch.empty_like(x), final
-    if lengths is not None:
+    if lengths is not None and (lengths.dtype != torch.int32 or not lengths.is_contiguous()):
         lengths = lengths.clamp(0, length).to(torch.int32).contiguous()
-    if reset is not None:
-        reset = _inner(reset)
-        reset = reset.view(torch.uint8) if reset.dtype == torch.bool else reset
-    x, decay, gate, state = _inner(x), _inner(decay), _inner(gate), _inner(initial_state)
+    x, decay, gate, state, reset = (_inner(x), _inner(decay), _inner(gate), _inner(initial_state),
+                                    _inner(reset))
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad
                                        for t in (x, decay, gate, rate, state)):
         return _GatedScan.apply(x, decay, gate, rate, state, lengths, reset)
@@ -989,30 +989,35 @@ def gated_step(x: torch.Tensor, decay: torch.Tensor, state: torch.Tensor,
     if x.ndim != 2:
         raise ValueError("x must have shape [B, C]")
     _validate_gated(x, decay, gate, rate, state, "state")
-    device = _require_device(x, decay, gate, rate, state)
+    index = x.get_device()
+    if index < 0 or decay.get_device() != index or state.get_device() != index or (
+            gate is not None and not gate.get_device() == rate.get_device() == index):
+        _require_device(x, decay, gate, rate, state)
     _require_inference(x, decay, gate, rate, state)
     batch, width = x.shape
     if inplace and ((width > 1 and state.stride(1) != 1) or
                     (batch > 1 and state.stride(0) < width)):
         raise ValueError("state must have a unit innermost stride and rows of its own to be "
                          "updated in place")
-    out = torch.empty(batch, width, dtype=x.dtype, device=device)
-    new = state if inplace else torch.empty(batch, width, dtype=torch.float32, device=device)
+    out = x.new_empty((batch, width))
+    new = state if inplace else state.new_empty((batch, width))
     if batch == 0 or width == 0:
         return out, new
     x, decay, gate, state, rate = (_inner(x), _inner(decay), _inner(gate), _inner(state),
                                    _rate32(rate))
-    code, tensor = _hip.dtype_code(x.dtype), _hip.Tensor
-    args = _hip.GatedScanArgs(batch, 1, width, code,
-                              tensor(x.data_ptr(), code, 0, (x.stride(0), 0, 1)),
-                              tensor(decay.data_ptr(), code, 0, (decay.stride(0), 0, 1)))
-    if gate is not None:
-        args.gate = tensor(gate.data_ptr(), code, 0, (gate.stride(0), 0, 1))
-        args.rate = tensor(rate.data_ptr(), 0, 0, (1,))
-    args.initial_state = tensor(state.data_ptr(), 0, 0, (state.stride(0), 1))
-    args.out = tensor(out.data_ptr(), code, 0, (width, 0, 1))
-    args.final_state = tensor(new.data_ptr(), 0, 0, (new.stride(0), 1))
-    _hip.launch("m3_gated_scan", args, device)
+    code, none = _hip.dtype_code(x.dtype), _hip.NO_TENSOR
+    _hip.launch("m3_gated_scan", _hip.GATED_SCAN.pack(
+        batch, 1, width, code,
+        x.data_ptr(), code, 0, x.stride(0), 0, 1, 0, 0,
+        decay.data_ptr(), code, 0, decay.stride(0), 0, 1, 0, 0,
+        *((*none, *none) if gate is None else
+          (gate.data_ptr(), code, 0, gate.stride(0), 0, 1, 0, 0,
+           rate.data_ptr(), 0, 0, 1, 0, 0, 0, 0)),
+        state.data_ptr(), 0, 0, state.stride(0), 1, 0, 0, 0,
+        0, 0, 0,
+        out.data_ptr(), code, 0, width, 0, 1, 0, 0,
+        new.data_ptr(), 0, 0, new.stride(0), 1, 0, 0, 0,
+        *none, 0, 0), index)
     return out, new
 
 

@@ -154,6 +154,26 @@ def test_backward_validation_on_the_host(lib):
     assert query(ctypes.byref(args), ctypes.byref(size)) == 1 and b"drate" in lib.m3_last_error()
 
 
+def test_packed_blocks_put_every_value_in_its_field():
+    """A block packed from 1, 2, 3, ... reads back so, field by field, through the structure."""
+    def flat(value):
+        if isinstance(value, ctypes.Structure):
+            for name, _ in value._fields_:
+                yield from flat(getattr(value, name))
+        elif isinstance(value, ctypes.Array):
+            yield from value
+        else:
+            yield value
+
+    for packed, py in ((_hip.GATED_SCAN, _hip.GatedScanArgs),
+                       (_hip.GATED_SCAN_BWD, _hip.GatedScanBwdArgs),
+                       (_hip.LINEAR4, _hip.Linear4Args)):
+        count = len(list(flat(py())))
+        assert packed.size == ctypes.sizeof(py)
+        read = py.from_buffer_copy(packed.pack(*range(1, count + 1)))
+        assert list(flat(read)) == list(range(1, count + 1))
+
+
 def test_structs_match_the_header_layout(tmp_path):
     import shutil
     import subprocess
@@ -162,6 +182,9 @@ def test_structs_match_the_header_layout(tmp_path):
         pytest.skip("gcc not available")
     structs = {"m3_gated_scan_args": _hip.GatedScanArgs,
                "m3_gated_scan_bwd_args": _hip.GatedScanBwdArgs}
+    for packed, py in ((_hip.GATED_SCAN, _hip.GatedScanArgs),
+                       (_hip.GATED_SCAN_BWD, _hip.GatedScanBwdArgs)):
+        assert packed.size == ctypes.sizeof(py)
     lines = ['#include "mamba3_hip.h"', "#include <stdio.h>", "int main(void) {"]
     for cname, py in structs.items():
         lines.append(f'printf("{cname} - %zu\\n", sizeof({cname}));')
