@@ -174,7 +174,7 @@ struct Chain {
   uint32_t* states;  // [tiles, B, C]: the state that leaves a tile
 };
 
-constexpr int kWindow = 4;           // tiles looked back over at once
+constexpr int kWindow = 16;          // links looked back over
 constexpr int kSpins = 1 << 22;      // polls (about 1 us each) before a wait gives up with NaN
 
 template <int VEC>
@@ -200,53 +200,73 @@ __device__ __forceinline__ void write_states(uint32_t* p, const float (&v)[VEC])
   }
 }
 
-// The state that enters link s of a chain (s >= 1), for the channels at `at`; `step` elements lie between links.
-// Waits until, for every channel, one of the kWindow links before has published its state and
-// all links after that one their maps. The state is carried forward over those maps by the very
-// operation with which each link computes its own state, so it does not depend on which
-// link was found. Every wait ends: links are started in ticket order, each waits for earlier ones
-// only, and a running wave always gets to run; kSpins is there in case that is wrong.
+// The state that enters link s of a chain (s >= 1), for the channels at `at`; `step` elements lie
+// between links. First the nearest link of the last kWindow whose states are published for all of the
+// wave's channels, then the maps of the links after it, in order. A state is carried over a map by the
+// very operation with which that link computes its own state, so the result does not depend on which
+// link was found. A link that has its state at once publishes no map, so a map that is missing means
+// another look at the states, never a wait for the map. Every wait ends: every link publishes its state once the
+// links before it have; links are started in ticket order, and a running wave always gets to run. kSpins is
+// there in case that is wrong.
 template <int VEC>
 __device__ __forceinline__ void look_back(const Chain& ch, int s, int64_t at, int64_t step,
                                           bool live, float (&v)[VEC]) {
-  const int n = min(kWindow, s);
-  for (int spin = 0;; ++spin) {
-    uint32_t st[kWindow][VEC];
-    uint64_t map[kWindow][VEC];
+  constexpr int kStates = 8, kMaps = 4;  // in flight at once
+  const int far = max(0, s - kWindow);
+  for (int spin = 0; spin < kSpins; ++spin) {
+    int found = -1;
+    for (int near = s - 1; near >= far && found < 0; near -= kStates) {
+      uint32_t st[kStates][VEC];
 #pragma unroll
-    for (int j = 0; j < kWindow; ++j) {
-      const int64_t p = at + (s - 1 - min(j, n - 1)) * step;
-      read_states<VEC>(ch.states + p, st[j]);
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) {
-        map[j][e] = __hip_atomic_load(ch.maps + p + e, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      for (int j = 0; j < kStates; ++j) {
+        read_states<VEC>(ch.states + at + max(near - j, far) * step, st[j]);
       }
-    }
-    bool all = true;
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) {
-      bool have = false;
+      for (int j = 0; j < kStates; ++j) {
+        bool known = true;
 #pragma unroll
-      for (int j = kWindow - 1; j >= 0; --j) {
-        const uint32_t a = static_cast<uint32_t>(map[j][e] >> 32);
-        if (st[j][e] != kNotYet) {
-          v[e] = __uint_as_float(st[j][e]);
-          have = true;
-        } else {
-          v[e] = fold(__uint_as_float(a), __uint_as_float(static_cast<uint32_t>(map[j][e])), v[e]);
-          have = have && a != kNotYet;
+        for (int e = 0; e < VEC; ++e) known = known && st[j][e] != kNotYet;
+        if (found < 0 && near - j >= far && __all(known || !live)) {
+          found = near - j;
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) v[e] = __uint_as_float(st[j][e]);
         }
       }
-      all = all && have;
     }
-    if (__all(all || !live)) return;
-    if (spin >= kSpins) {
+    bool whole = found >= 0;
+    for (int p = found + 1; p < s && whole; p += kMaps) {
+      uint64_t map[kMaps][VEC];
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) v[e] = __uint_as_float(0x7fc00000u);
-      return;
+      for (int j = 0; j < kMaps; ++j) {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+          map[j][e] = __hip_atomic_load(ch.maps + at + min(p + j, s - 1) * step + e, __ATOMIC_RELAXED,
+                                        __HIP_MEMORY_SCOPE_AGENT);
+        }
+      }
+      bool known = true;
+#pragma unroll
+      for (int j = 0; j < kMaps; ++j) {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) known = known && (map[j][e] >> 32) != kNotYet;
+      }
+      whole = __all(known || !live);
+#pragma unroll
+      for (int j = 0; j < kMaps; ++j) {
+        if (p + j < s) {
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) {
+            v[e] = fold(__uint_as_float(static_cast<uint32_t>(map[j][e] >> 32)),
+                        __uint_as_float(static_cast<uint32_t>(map[j][e])), v[e]);
+          }
+        }
+      }
     }
+    if (whole) return;
     __builtin_amdgcn_s_sleep(2);
   }
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) v[e] = __uint_as_float(0x7fc00000u);
 }
 
 __global__ __launch_bounds__(256) void gated_chain_kernel(Chain ch, int64_t cells) {
