@@ -108,7 +108,8 @@ def test_scan_validation_on_the_host(lib):
     assert query(None, ctypes.byref(size)) == 1 and b"NULL" in lib.m3_last_error()
     assert lib.m3_gated_scan(None, None) == 1 and lib.m3_gated_scan_bwd(None, None) == 1
     for field, value, code, text in (("batch", -1, 1, b"negative"), ("dtype", 7, 1, b"dtype 7"),
-                                     ("width", 1 << 30, 2, b"above 2^30")):
+                                     ("batch", 1 << 25, 2, b"above 2^30"),
+                                     ("width", 1 << 28, 2, b"above 2^27")):
         args = _scan_args()
         setattr(args, field, value)
         assert query(ctypes.byref(args), ctypes.byref(size)) == code, field
