@@ -878,18 +878,19 @@ def _gated_inputs(x, decay, gate, rate, state, lengths, reset):
 
 def _gated_forward(x, decay, gate, rate, state, lengths, reset, want_carry):
     batch, length, width = x.shape
+    device = x.device
     out = x.new_empty(x.shape)
-    final = torch.empty((batch, width), dtype=torch.float32, device=x.device)
+    final = torch.empty((batch, width), dtype=torch.float32, device=device)
     carry = torch.empty((-(-length // _hip.GATED_TILE), batch, width), dtype=torch.float32,
-                        device=x.device) if want_carry else None
+                        device=device) if want_carry else None
     values = (*_gated_inputs(x, decay, gate, rate, state, lengths, reset),
               *_packed(out, _hip.dtype_code(x.dtype)), *_packed(final), *_packed(carry))
     block, ws = _hip.GATED_SCAN.pack(*values, 0, 0), None
     size = _hip.need("m3_gated_scan_workspace_size", block)
     if size:
-        ws = torch.empty(size, dtype=torch.uint8, device=x.device)
+        ws = torch.empty(size, dtype=torch.uint8, device=device)
         block = _hip.GATED_SCAN.pack(*values, ws.data_ptr(), size)
-    _hip.launch("m3_gated_scan", block, x.get_device())
+    _hip.launch("m3_gated_scan", block, device.index)
     del ws
     return out, final, carry
 
@@ -962,18 +963,21 @@ def gated_scan(x: torch.Tensor, decay: torch.Tensor, gate: torch.Tensor | None =
     if reset is not None and (reset.shape != (batch, length) or
                               reset.dtype not in (torch.bool, torch.uint8)):
         raise ValueError(f"reset must be bool of shape {(batch, length)}")
-    device = _require_device(x, decay, gate, rate, initial_state, lengths, reset)
+    index = x.get_device()
+    if index < 0 or any([t is not None and t.get_device() != index for t in
+                         (decay, gate, rate, initial_state, lengths, reset)]):
+        _require_device(x, decay, gate, rate, initial_state, lengths, reset)
     rate = _rate32(rate)
     if batch == 0 or length == 0 or width == 0:
-        final = (torch.zeros(batch, width, device=device) if initial_state is None
+        final = (torch.zeros(batch, width, device=x.device) if initial_state is None
                  else initial_state.clone())
         return torch.empty_like(x), final
     if lengths is not None and (lengths.dtype != torch.int32 or not lengths.is_contiguous()):
         lengths = lengths.clamp(0, length).to(torch.int32).contiguous()
     x, decay, gate, state, reset = (_inner(x), _inner(decay), _inner(gate), _inner(initial_state),
                                     _inner(reset))
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad
-                                       for t in (x, decay, gate, rate, state)):
+    if torch.is_grad_enabled() and any([t is not None and t.requires_grad
+                                        for t in (x, decay, gate, rate, state)]):
         return _GatedScan.apply(x, decay, gate, rate, state, lengths, reset)
     return _gated_forward(x, decay, gate, rate, state, lengths, reset, False)[:2]
 
