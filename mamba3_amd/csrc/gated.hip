@@ -319,7 +319,7 @@ __global__ __launch_bounds__(64 * kWaves, 4) void gated_tile_kernel(const GatedG
   const bool live = c0 < g.width;
   const int c = min(c0, g.width - VEC);  // lanes past the width read its last channels
   const int t0 = s * kTile + w * kSpan;
-  const int n = max(0, min(row_length(g, b) - t0, kSpan));  // tokens of this wave
+  const int len = row_length(g, b), n = max(0, min(len - t0, kSpan));  // tokens of this wave
   const int64_t step = static_cast<int64_t>(g.batch) * g.width;
   const int64_t at = static_cast<int64_t>(b) * g.width + c;
 
@@ -327,9 +327,14 @@ __global__ __launch_bounds__(64 * kWaves, 4) void gated_tile_kernel(const GatedG
   if constexpr (CHAIN) {
     if (w == 0 && s > 0) read_states<VEC>(ch.states + at + (s - 1) * step, early);
   }
-  float rate[VEC];
+  // v: the state that enters the tile, then the wave; read before any wave can have written fin,
+  // which may be the same memory
+  float rate[VEC], v[VEC];
 #pragma unroll
-  for (int e = 0; e < VEC; ++e) rate[e] = GATE ? g.rate[c + e] : 0.f;
+  for (int e = 0; e < VEC; ++e) {
+    rate[e] = GATE ? g.rate[c + e] : 0.f;
+    if (!CHAIN || s == 0) v[e] = g.init != nullptr ? g.init[b * g.init_b + c + e] : 0.f;
+  }
   uint64_t cut = 0;
   if (g.reset != nullptr) {
     cut = __ballot(lane < n && g.reset[b * g.reset_b + t0 + min(lane, max(n - 1, 0))] != 0);
@@ -397,11 +402,6 @@ __global__ __launch_bounds__(64 * kWaves, 4) void gated_tile_kernel(const GatedG
     s_h[w][lane * VEC + e] = span_h[e];
   }
   __syncthreads();
-  float v[VEC];  // the state that enters the tile, then the wave
-  if (!CHAIN || s == 0) {
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) v[e] = g.init != nullptr ? g.init[b * g.init_b + c + e] : 0.f;
-  }
   if constexpr (CHAIN) {
     if (w == 0) {
       float ta[VEC], th[VEC];
@@ -442,10 +442,6 @@ __global__ __launch_bounds__(64 * kWaves, 4) void gated_tile_kernel(const GatedG
       }
       if (live) {
         if (s < g.tiles - 1) write_states<VEC>(ch.states + at + s * step, out);
-        if (s == g.tiles - 1) {
-#pragma unroll
-          for (int e = 0; e < VEC; ++e) g.fin[b * g.fin_b + c + e] = out[e];
-        }
       }
     }
     __syncthreads();
@@ -483,7 +479,8 @@ __global__ __launch_bounds__(64 * kWaves, 4) void gated_tile_kernel(const GatedG
       }
     }
   }
-  if (!CHAIN && w == kWaves - 1 && live) {
+  // the final state is the last token's, as out has it before rounding
+  if (live && (n > 0 ? t0 + n == len : len == 0 && s == 0 && w == 0)) {
 #pragma unroll
     for (int e = 0; e < VEC; ++e) g.fin[b * g.fin_b + c + e] = v[e];
   }
@@ -952,11 +949,13 @@ Chain chain(void* workspace, int64_t cells, size_t tickets, int64_t links) {
                reinterpret_cast<uint32_t*>(maps + cells)};
 }
 
+constexpr int64_t kMostTiles = (int64_t{1} << 32) / (64 * kWaves) - 1;  // a grid has below 2^32 threads
+
 template <typename T, bool GATE, int VEC>
 int launch_tiles(const m3_gated_scan_args& a, const GatedGeom& g, hipStream_t stream) {
   const int cols = 64 * VEC;
   const int64_t count = static_cast<int64_t>((g.width + cols - 1) / cols) * g.batch * g.tiles;
-  if (count > INT32_MAX) return fail(M3_EUNSUPPORTED, "m3_gated_scan: over 2^31 tiles");
+  if (count > kMostTiles) return fail(M3_EUNSUPPORTED, "m3_gated_scan: over 2^23 tiles");
   const dim3 grid(static_cast<unsigned>(count)), block(64 * kWaves);
   if (g.tiles == 1) {
     hipLaunchKernelGGL((gated_tile_kernel<T, GATE, VEC, false>), grid, block, 0, stream, g,
@@ -1003,7 +1002,7 @@ template <typename T, bool GATE, int VEC>
 int launch_back(const m3_gated_scan_bwd_args& a, GatedGeom& g, hipStream_t stream) {
   const int cols = 64 * VEC;
   const int64_t count = static_cast<int64_t>((g.width + cols - 1) / cols) * g.batch * g.tiles;
-  if (count > INT32_MAX) return fail(M3_EUNSUPPORTED, "m3_gated_scan_bwd: over 2^31 tiles");
+  if (count > kMostTiles) return fail(M3_EUNSUPPORTED, "m3_gated_scan_bwd: over 2^23 tiles");
   const dim3 grid(static_cast<unsigned>(count)), block(64 * kWaves);
   const int64_t cells = static_cast<int64_t>(g.tiles) * g.batch * g.width;
   const Chain ch = chain(a.fwd.workspace, cells, ticket_bytes(g.batch, g.width), count);

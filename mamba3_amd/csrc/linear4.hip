@@ -596,9 +596,9 @@ int validate(const m3_linear4_args& a) {
     return fail(M3_EUNSUPPORTED, "m3_linear4: M = %lld > %d rows", static_cast<long long>(a.m),
                 kMaxRows);
   }
-  if (a.k % a.group != 0 || a.k > (1 << 20) || a.n > (1 << 28)) {
+  if (a.k % a.group != 0 || a.k > (1 << 20) || a.n > (1 << 27)) {
     return fail(M3_EUNSUPPORTED, "m3_linear4: N = %lld, K = %lld: K must be a multiple of the group "
-                "up to 2^20, N at most 2^28", static_cast<long long>(a.n),
+                "up to 2^20, N at most 2^27", static_cast<long long>(a.n),
                 static_cast<long long>(a.k));
   }
   if (a.m == 0 || a.n == 0) return M3_OK;
@@ -632,6 +632,11 @@ int validate(const m3_linear4_args& a) {
   if (!apart(o0, o1, x0, x0 + ((a.m - 1) * a.x.stride[0] + a.k) * 2) ||
       !apart(o0, o1, c0, c0 + tiles * 1024)) {
     return fail(M3_EINVAL, "m3_linear4: out overlaps x or the weight");
+  }
+  const char* r0 = static_cast<const char*>(a.residual.ptr);
+  const bool same = r0 == o0 && (a.m == 1 || a.residual.stride[0] == a.out.stride[0]);
+  if (r0 != nullptr && !same && !apart(o0, o1, r0, r0 + ((a.m - 1) * a.residual.stride[0] + a.n) * 2)) {
+    return fail(M3_EINVAL, "m3_linear4: out overlaps the residual without being it");
   }
   return M3_OK;
 }

@@ -444,6 +444,8 @@ class Mamba3(nn.Module):
         afterwards (``load_state_dict``, ``to``, a copy of the model) makes ``step`` raise until
         this is called again. A step's rows must have the weights' dtype, as ever, to run on it.
         """
+        if not self.causal:
+            raise ValueError("quantize_decode requires causal=True")
         for layer in self.layers:
             for name in ("in_proj", "out_proj"):
                 weight = getattr(layer.mixer, name).weight

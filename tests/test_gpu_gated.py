@@ -12,7 +12,7 @@ from __future__ import annotations
 import pytest
 import torch
 
-from mamba3_amd import ops
+from mamba3_amd import _hip, ops
 from oracle import gated as og
 
 pytestmark = pytest.mark.gpu
@@ -306,6 +306,25 @@ def test_expanded_and_transposed_inputs():
         assert torch.equal(a.grad, b.grad)
 
 
+@pytest.mark.parametrize("length", [1, 5, 20, 128, 129, 700])
+def test_the_final_state_is_the_last_token_s_and_may_lie_on_the_first(length):
+    """FP32: final_state equals out at each row's last token bit for bit, also where the C call is
+    given the initial state's memory for it."""
+    case = _to(_inputs(3, length, 70, F32, "gate", seed=16, state=True))
+    n = torch.tensor([length, max(1, length // 2), 0], device=DEV, dtype=torch.int32)
+    with torch.inference_mode():
+        y, last = _call(case | dict(lengths=n))
+        for b, k in enumerate(n.tolist()):
+            assert torch.equal(last[b], y[b, k - 1] if k else case["state"][b])
+        out, state = torch.empty_like(y), case["state"].clone()
+        values = (*ops._gated_inputs(case["x"], case["decay"], case["gate"], case["rate"], state, n,
+                                     None), *ops._packed(out), *ops._packed(state), *(0,) * 8)
+        size = _hip.need("m3_gated_scan_workspace_size", _hip.GATED_SCAN.pack(*values, 0, 0))
+        ws = torch.empty(size + 1, dtype=torch.uint8, device=DEV)
+        _hip.launch("m3_gated_scan", _hip.GATED_SCAN.pack(*values, ws.data_ptr(), size), y.device.index)
+        assert torch.equal(state, last) and torch.equal(out, y)
+
+
 def test_repeated_calls_agree_bit_for_bit():
     case = _to(_inputs(2, 3000, 130, BF16, "gate", seed=10))
     dy = torch.randn(2, 3000, 130, device=DEV).to(BF16)
@@ -363,6 +382,76 @@ def test_streams_and_graphs():
             torch.cuda.synchronize()
             assert all(torch.equal(x, y) for x, y in zip(outs, want[other]))
             assert all(torch.equal(x, y) for x, y in zip(eager, want[other]))
+
+
+@pytest.mark.parametrize("length", [1, 40, 500])
+def test_a_loss_on_one_output(length):
+    """A loss on the final state alone, or on the outputs alone: the other's gradient is zeros."""
+    case = _to(_inputs(2, length, 66, BF16, "gate", seed=13, state=True))
+    names = ("x", "decay", "gate", "rate", "state")
+    for n in names:
+        case[n].requires_grad_(True)
+    leaves = [case[n] for n in names]
+    y, last = _call(case)
+    zero_y, zero_last = torch.zeros_like(y), torch.zeros_like(last)
+    weigh_y, weigh_last = torch.randn_like(y), torch.randn_like(last)
+    alone = torch.autograd.grad((y * weigh_y).sum(), leaves, retain_graph=True)
+    both = torch.autograd.grad((y, last), leaves, (weigh_y, zero_last), retain_graph=True)
+    assert all(torch.equal(a, b) for a, b in zip(alone, both))
+    alone = torch.autograd.grad((last * weigh_last).sum(), leaves, retain_graph=True)
+    both = torch.autograd.grad((y, last), leaves, (zero_y, weigh_last))
+    assert all(torch.equal(a, b) for a, b in zip(alone, both))
+
+
+def test_a_rate_and_a_state_shared_by_broadcast():
+    """A 16-bit rate, one number for all channels, and one state for all rows: their gradients are
+    the sums over what they were broadcast to."""
+    case = _to(_inputs(3, 90, 50, F32, "gate", seed=14))
+    rate = torch.full((1,), 0.25, device=DEV, dtype=BF16, requires_grad=True)
+    state = torch.randn(1, 50, device=DEV, requires_grad=True)
+    y, last = ops.gated_scan(case["x"], case["decay"], case["gate"], rate.expand(50),
+                             initial_state=state.expand(3, 50))
+    y.sum().backward()
+    wide_rate = torch.full((50,), 0.25, device=DEV, requires_grad=True)
+    wide_state = state.detach().expand(3, 50).contiguous().requires_grad_(True)
+    y2, _ = ops.gated_scan(case["x"], case["decay"], case["gate"], wide_rate,
+                           initial_state=wide_state)
+    torch.autograd.backward(y2, torch.ones_like(y2))
+    assert torch.equal(y, y2)
+    # sums of 50 and 3 terms in FP32, the first rounded to bf16
+    total = wide_rate.grad.double().sum()
+    size = wide_rate.grad.double().abs().sum()
+    assert (rate.grad.double() - total).abs() <= 2.0 ** -8 * total.abs() + 50 * 2.0 ** -24 * size \
+        + 2.0 ** -8 * size
+    torch.testing.assert_close(state.grad, wide_state.grad.sum(0, keepdim=True), rtol=1e-6, atol=1e-6)
+
+
+def test_lengths_beyond_32_bits_and_below_zero():
+    case = _to(_inputs(4, 300, 34, F32, "given", seed=15))
+    with torch.inference_mode():
+        want = ops.gated_scan(case["x"], case["decay"],
+                              lengths=torch.tensor([300, 0, 7, 300], device=DEV))
+        for n in (torch.tensor([1 << 40, -(1 << 40), 7, 301], device=DEV),
+                  torch.tensor([2 ** 31 - 1, -2 ** 31, 7, 301], device=DEV, dtype=torch.int32)):
+            got = ops.gated_scan(case["x"], case["decay"], lengths=n)
+            assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_many_narrow_rows_and_too_many():
+    """One channel, 100,000 rows; and more tiles than a grid holds, refused."""
+    x = torch.randn(100_000, 20, 1, device=DEV)
+    decay = -torch.rand(100_000, 20, 1, device=DEV)
+    with torch.inference_mode():
+        y, last = ops.gated_scan(x, decay)
+        h = torch.zeros(100_000, 1, device=DEV, dtype=torch.float64)
+        for t in range(20):
+            h = torch.exp(decay[:, t].double()) * h + x[:, t]
+            # 20 tokens, each off by less than 2^-20 of sums of at most 20 values below 6
+            assert (y[:, t] - h).abs().max().item() <= 20 * 2.0 ** -20 * 6 * 20
+        assert torch.equal(last, y[:, -1])
+        few = torch.zeros(1, 1, 1, device=DEV, dtype=BF16)
+        with pytest.raises(RuntimeError, match="2\\^23 tiles"):
+            ops.gated_scan(few.expand(1 << 23, 17, 1), few.expand(1 << 23, 17, 1))
 
 
 def test_empty_extents():

@@ -151,6 +151,29 @@ def test_rows_do_not_touch_each_other():
         assert torch.isnan(got[:, 9]).all() and torch.equal(got[:, keep], want[:, keep])
 
 
+@pytest.mark.parametrize("m,n,k,group", [(40, 6200, 256, 128), (64, 6145, 1184, 32), (33, 9000, 448, 64),
+                                         (64, 16400, 384, 128), (200, 6144, 128, 64),
+                                         (100, 24576, 128, 32), (64, 12304, 2048, 128)])
+def test_many_rows_of_both(m, n, k, group):
+    """The shapes on which a workgroup stages x once (from 384 tile rows, above 16 rows of x): one
+    and two tile rows a wave, one and two teams, odd counts of tiles, columns that end inside a tile."""
+    g = torch.Generator().manual_seed(n)
+    packed, scales, z, wide = _weight(n, k, group, BF16, n % 2 == 0, g)
+    x = torch.randn(m, k, generator=g).to(BF16)
+    res = torch.randn(m, n, generator=g).to(BF16)
+    nw = 1 + 0.1 * torch.randn(k, generator=g)
+    weight = ops.Weight4(packed.to(DEV), scales.to(DEV), None if z is None else z.to(DEV))
+    bad = x.to(DEV).clone()
+    bad[m // 2] = float("nan")
+    with torch.inference_mode():
+        _check(ops.linear4(x.to(DEV), weight), x, wide, scales, group)
+        _check(ops.linear4(x.to(DEV), weight, res.to(DEV), norm_weight=nw.to(DEV)), x, wide, scales,
+               group, res, nw)
+        want, got = ops.linear4(x.to(DEV), weight), ops.linear4(bad, weight)
+    keep = [i for i in range(m) if i != m // 2]
+    assert torch.equal(got[keep], want[keep]) and torch.isnan(got[m // 2]).all()
+
+
 def test_streams_and_graph():
     g = torch.Generator().manual_seed(3)
     packed, scales, z, _ = _weight(200, 1024, 128, BF16, False, g)

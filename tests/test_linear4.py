@@ -128,6 +128,8 @@ def test_linear4_refusals():
 def test_quantize_decode_refusals():
     with pytest.raises(ValueError, match="16 weights"):
         Mamba3(64, depth=1).quantize_decode()
+    with pytest.raises(ValueError, match="causal"):
+        Mamba3(64, depth=1, causal=False).to(torch.bfloat16).quantize_decode(32)
     model = Mamba3(64, depth=1).to(torch.bfloat16)
     before = {k: v.clone() for k, v in model.state_dict().items()}
     for group in (128, 48):
@@ -171,6 +173,12 @@ def test_validation_on_the_host(lib):
         setattr(getattr(args, name), field, value)
         assert call(ctypes.byref(args), None) == code, (name, value)
         assert text in lib.m3_last_error(), (name, value)
+    args = _args()
+    args.residual = _hip.Tensor(0x500000 + 16, _hip.BF16, 0, (64, 1))
+    assert call(ctypes.byref(args), None) == 1 and b"residual" in lib.m3_last_error()
+    args = _args()
+    args.residual = _hip.Tensor(0x500000, _hip.BF16, 0, (72, 1))
+    assert call(ctypes.byref(args), None) == 1 and b"residual" in lib.m3_last_error()
     args = _args()
     args.out.stride[0] = 8
     assert call(ctypes.byref(args), None) == 1 and b"rows of out" in lib.m3_last_error()
