@@ -56,7 +56,7 @@ def _require_device(*tensors: torch.Tensor | None) -> torch.device:
 
 
 def _require_inference(*tensors: torch.Tensor | None) -> None:
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+    if torch.is_grad_enabled() and any([t is not None and t.requires_grad for t in tensors]):
         raise RuntimeError(
             "mamba3_amd implements the inference hot path (forward, prefill, step) and has no "
             "backward; run it under torch.no_grad() or torch.inference_mode()")
@@ -799,10 +799,11 @@ def linear4(x: torch.Tensor, weight: Weight4, residual: torch.Tensor | None = No
     norm_eps)``. No backward.
     """
     index = x.get_device()
-    if index < 0 or any(t is not None and t.get_device() != index
-                        for t in (residual, out, norm_weight)):
+    if index < 0 or any([t is not None and t.get_device() != index
+                         for t in (residual, out, norm_weight)]):
         _require_device(x, residual, out, norm_weight)
-    _require_inference(x, residual, norm_weight)
+    if torch.is_grad_enabled():
+        _require_inference(x, residual, norm_weight)
     if not linear4_supported(x, weight):
         raise ValueError(f"linear4: unsupported operands x {tuple(x.shape)} {x.dtype} on "
                          f"{x.device}, weight {weight.shape} on {weight.device}")
@@ -852,6 +853,9 @@ def _validate_gated(x, decay, gate, rate, state, state_name) -> None:
         raise ValueError(f"rate must be a floating tensor of shape {(width,)}")
     if state is not None and (state.shape != (x.shape[0], width) or state.dtype != torch.float32):
         raise ValueError(f"{state_name} must be float32 of shape {(x.shape[0], width)}")
+
+
+_NO_GATES = 2 * _hip.NO_TENSOR
 
 
 def _rate32(rate: torch.Tensor | None) -> torch.Tensor | None:
@@ -997,7 +1001,8 @@ def gated_step(x: torch.Tensor, decay: torch.Tensor, state: torch.Tensor,
     if index < 0 or decay.get_device() != index or state.get_device() != index or (
             gate is not None and not gate.get_device() == rate.get_device() == index):
         _require_device(x, decay, gate, rate, state)
-    _require_inference(x, decay, gate, rate, state)
+    if torch.is_grad_enabled():
+        _require_inference(x, decay, gate, rate, state)
     batch, width = x.shape
     if inplace and ((width > 1 and state.stride(1) != 1) or
                     (batch > 1 and state.stride(0) < width)):
@@ -1007,16 +1012,17 @@ def gated_step(x: torch.Tensor, decay: torch.Tensor, state: torch.Tensor,
     new = state if inplace else state.new_empty((batch, width))
     if batch == 0 or width == 0:
         return out, new
-    x, decay, gate, state, rate = (_inner(x), _inner(decay), _inner(gate), _inner(state),
-                                   _rate32(rate))
-    code, none = _hip.dtype_code(x.dtype), _hip.NO_TENSOR
+    x, decay, state = _inner(x), _inner(decay), _inner(state)
+    code, none, gates = _hip.dtype_code(x.dtype), _hip.NO_TENSOR, _NO_GATES
+    if gate is not None:
+        gate, rate = _inner(gate), _rate32(rate)
+        gates = (gate.data_ptr(), code, 0, gate.stride(0), 0, 1, 0, 0,
+                 rate.data_ptr(), 0, 0, 1, 0, 0, 0, 0)
     _hip.launch("m3_gated_scan", _hip.GATED_SCAN.pack(
         batch, 1, width, code,
         x.data_ptr(), code, 0, x.stride(0), 0, 1, 0, 0,
         decay.data_ptr(), code, 0, decay.stride(0), 0, 1, 0, 0,
-        *((*none, *none) if gate is None else
-          (gate.data_ptr(), code, 0, gate.stride(0), 0, 1, 0, 0,
-           rate.data_ptr(), 0, 0, 1, 0, 0, 0, 0)),
+        *gates,
         state.data_ptr(), 0, 0, state.stride(0), 1, 0, 0, 0,
         0, 0, 0,
         out.data_ptr(), code, 0, width, 0, 1, 0, 0,
