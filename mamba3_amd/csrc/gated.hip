@@ -4,15 +4,27 @@
 //   gate form:   h_t = a_t h_{t-1} + s_t q_t x_t,       a_t = exp(-rate p_t), s_t = sqrt(1 - a_t^2)
 // with p_t = sigmoid(decay_t), q_t = sigmoid(gate_t).
 //
-// Forward, one token: one lane owns a channel (two where rows allow). Forward, more tokens: a
-// workgroup takes a tile of 128 tokens x 128 channels, which stays in registers, so x, decay and
-// gate are read once. Each of its 8 waves runs 16 tokens from a zero state, which gives the span's map
-// h -> A h + H; the maps of the waves before give a wave its entry state, and the tokens are run
-// again from there with one fma each. Tiles of one row are chained through memory: a tile publishes its own
-// map, then looks back for the nearest state that is already known.
+// What bounds it: memory, closely followed by the vector unit (33 instructions a token and channel forward
+// in the gate form, 6 of them exponentials, reciprocals or roots at a quarter rate). So the inputs are read
+// once and the transcendental work is done once.
 //
-// Backward: tiles of 64 tokens, chained from the last, each with its states run again from the carry
-// that the forward pass left.
+// Forward, up to 16 tokens: one lane walks a channel's tokens (two channels where rows allow).
+//
+// Forward, more tokens: a workgroup takes a tile of 128 tokens x 128 channels (64 where rows are
+// odd), which stays in registers. Each of its 8 waves runs 16 tokens from a zero state, which gives the
+// span's map h -> A h + H; the maps of the waves before give a wave its entry state, and the tokens
+// are run again from there with one fma each. Tiles of one row are chained through memory: a tile
+// publishes its own map, then looks back for the nearest state that is already known. 16 tokens x 2
+// channels a lane fill 116 of the 128 registers that leave two workgroups a CU; reading everything twice
+// instead (maps first, outputs after) would move 14 bytes for every 8.
+//
+// Backward: tiles of 64 tokens (8 a wave: its inputs, factors and states fill the 128 registers), chained
+// from the last, each with its states run again from the carry that the forward pass left, in
+// place of 2 bytes a token and channel for the outputs, which are rounded.
+//
+// Measured in bf16, gate form (a large copy reaches 4.8 TB/s): 8 x 8192 x 2048 padded prompts 183 us
+// (4.8 TB/s of what is read and written), one row of 65536 x 1536 179 us (4.5 TB/s), 1777 x 4096 20 us; forward
+// and backward of 8 x 4096 x 2048 123 + 242 us (4.4 and 3.9 TB/s).
 #include <hip/hip_runtime.h>
 
 #include "m3_common.hpp"

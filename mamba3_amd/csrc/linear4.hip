@@ -6,10 +6,16 @@
 // the group's share is scale * A - scale * (16 + z) * X: the scale and the zero meet FP32 sums, not the
 // operands. X comes from one more matrix product, with ones.
 //
-// A workgroup takes TN tiles of 16 weight rows and up to MT blocks of 16 x rows. Its waves take every WAVES-th
-// tile of 128 columns each, so no two read the same operand and the K loop has no barrier; their
-// sums meet in LDS. A wave's next codes and x are on their way in registers while it multiplies; x goes
-// through an LDS region of the wave's own, where it is normed, and comes back as the operand's columns.
+// linear4_kernel (up to 16 rows of x; up to 32 a workgroup where there are few weight rows): a workgroup
+// takes TN tiles of 16 weight rows and MT blocks of 16 x rows. Its waves take every WAVES-th tile of 128
+// columns each, so no two read the same operand and the K loop has no barrier; their sums meet in
+// LDS. A wave's next codes and x are on their way in registers while it multiplies; x goes through
+// an LDS region of the wave's own, where it is normed, and comes back as the operand's columns. Bound by
+// the weight's stream where it is long, else by the launch and one latency of memory: in graphs with
+// cold weights 28672 x 8192 at 1 row 27.1 us (4.5 TB/s; a large copy reaches 4.8), 8672 x 2048 at 1 row 4.9
+// us, 6.8 with the norm, 2048 x 4096 at 16 rows 5.6 us (512 x 512: 2.4 us).
+//
+// linear4_wide_kernel (more rows of both): below.
 #include <hip/hip_runtime.h>
 
 #include "m3_common.hpp"
@@ -319,7 +325,13 @@ __global__ __launch_bounds__(64 * WAVES) void linear4_kernel(const Lin4Geom g) {
 // rows, TN for each wave, over all of K. A tile of x columns is staged once for the workgroup, in two
 // LDS buffers; x is three tiles ahead of its use (two of them in registers), the codes two to
 // four. Wave
-// w forms X for x block w and leaves it to the others, who apply it a tile later.
+// w forms X for x block w and leaves it to the others, who apply it a tile later. KS = 2: two such teams, every
+// other tile of columns each, for two waves a SIMD where one workgroup fills a CU.
+// Bound by issue: a wave spends 191 vector and 36 matrix instructions on a tile of columns (dequantising
+// 64, scales and zeros 64, the rest addresses and staging), and with both kinds of load left out 28672
+// x 8192 at 64 rows still takes 49 of its 55 us (2.3 TB/s of weights, 540 TFLOP/s). Tried without gain: deeper
+// rings, operands expanded or read a step earlier, other mixes of matrix and vector instructions, a conflict-free
+// LDS layout alone, 4 tile rows a wave (spills).
 template <typename T, typename S, int GPT, int TN, int KS, bool NORM>
 __global__ __launch_bounds__(256 * KS, 2) void linear4_wide_kernel(const Lin4Geom g) {
   using C = Code<T>;
@@ -663,6 +675,17 @@ int launch_wide(const Lin4Geom& g, hipStream_t stream) {
   return check_launch("m3_linear4");
 }
 
+// Up to 16 rows of x, by tile rows of W (us in graphs with cold weights; WAVES x TN):
+//   few (2048 x 4096, 16 rows): 8 x 1 5.2, 16 x 1 5.7, 4 x 1 6.9, 4 x 2 8.7
+//   542 (8672 x 2048, 1 row): 4 x 1 5.6, 4 x 2 5.7, 8 x 1 6.4; with the norm, formed once a
+//     workgroup, 4 x 2 8.0, 4 x 1 8.2, 8 x 1 8.8
+//   1792 (28672 x 8192, 16 rows): 4 x 4 28.2, 4 x 2 33.3, 8 x 1 43.2; in groups of 32, whose scales
+//     fill the registers, 4 x 1 28.2, 4 x 4 35.2
+// More rows: few tile rows keep the split over columns (2048 x 4096, 64 rows: 7.9 us in blocks of 32, 12.7 in
+// blocks of 64, 21.5 wide). Else the wide kernel in the form whose rounds of workgroups over the 256 CUs cost
+// least: 65 a round with 2 tile rows a wave, 44 with 1 (both one workgroup a CU), 87 for 512
+// workgroups of one team (two a CU): 28672 x 8192 at 64 rows 55 / 74 / 72 us, 16384 x 4096 26 / 20 / 27, 8672 x 2048
+// at 256 rows 31 / 32 / 23. Two tile rows in groups of 32 spill (90 against 51 us).
 template <typename T, typename S, int GPT>
 int launch_rows(const Lin4Geom& g, hipStream_t stream) {
   if (g.m <= 16) {
