@@ -322,17 +322,18 @@ __global__ __launch_bounds__(64 * WAVES) void linear4_kernel(const Lin4Geom g) {
 }
 
 // Many rows of x and many of W: a workgroup of four waves takes 64 x rows and 4 TN tiles of weight
-// rows, TN for each wave, over all of K. A tile of x columns is staged once for the workgroup, in two
-// LDS buffers; x is three tiles ahead of its use (two of them in registers), the codes two to
-// four. Wave
-// w forms X for x block w and leaves it to the others, who apply it a tile later. KS = 2: two such teams, every
-// other tile of columns each, for two waves a SIMD where one workgroup fills a CU.
-// Bound by issue: a wave spends 191 vector and 36 matrix instructions on a tile of columns (dequantising
-// 64, scales and zeros 64, the rest addresses and staging), and with both kinds of load left out 28672
-// x 8192 at 64 rows still takes 49 of its 55 us (2.3 TB/s of weights, 540 TFLOP/s). Tried without gain: deeper
-// rings, operands expanded or read a step earlier, other mixes of matrix and vector instructions, a conflict-free
-// LDS layout alone, 4 tile rows a wave (spills).
-template <typename T, typename S, int GPT, int TN, int KS, bool NORM>
+// rows, TN for each wave, over all of K. A tile of x columns is staged once for the workgroup, in three
+// LDS buffers; x comes from memory three tiles ahead of its use, the codes two. Wave w forms X of the next
+// tile for x block w, and a group's sums begin at -(16 + z) X. KS = 2: two such teams, every other tile of
+// columns each, for two waves a SIMD where one workgroup fills a CU.
+// Bound by latency and issue together: 28672 x 8192 at 64 rows takes 55 us (2.3 TB/s of weights, 545
+// TFLOP/s); with both kinds of load left out 49, with LDS reads, dequantising and scaling left out too 35, of which the
+// matrix instructions are 18 and the rest barriers, staging and addresses (213 vector and 36 matrix
+// instructions a tile of columns). Sums that begin at -(16 + z) X need no pass over X afterwards: 191 became
+// 213 at groups of 128, which costs nothing there, and groups of 32 no longer spill (28672 x 4096 at 64 rows:
+// 51 -> 40 us). Tried without gain: deeper rings, operands expanded or read a step earlier, set mixes of
+// matrix and vector instructions, 4 tile rows a wave.
+template <typename T, typename S, int GPT, int TN, int KS, bool NORM, bool ZEROS>
 __global__ __launch_bounds__(256 * KS, 2) void linear4_wide_kernel(const Lin4Geom g) {
   using C = Code<T>;
   using V8 = typename C::v8;
@@ -354,10 +355,8 @@ __global__ __launch_bounds__(256 * KS, 2) void linear4_wide_kernel(const Lin4Geo
   const int64_t left = max(0, min(g.tiles - tn, TN)) * g.tk;
   const __amdgpu_buffer_rsrc_t rc = rsrc4(g.codes + tile0 * 1024, left * 1024);
   const __amdgpu_buffer_rsrc_t rs = rsrc4(g.scales + tile0 * (GPT * 32), left * (GPT * 32));
-  const bool has_zeros = g.zeros != nullptr;  // else 0 is read, and 8 meant
-  const __amdgpu_buffer_rsrc_t rz = rsrc4(has_zeros ? g.zeros + tile0 * (GPT * 16) : g.codes,
-                                          has_zeros ? left * (GPT * 16) : 0);
-  const uint32_t eights = has_zeros ? 0u : 0x08080808u;
+  const __amdgpu_buffer_rsrc_t rz = rsrc4(ZEROS ? g.zeros + tile0 * (GPT * 16) : g.codes,
+                                          ZEROS ? left * (GPT * 16) : 0);
   const __amdgpu_buffer_rsrc_t rx = rsrc4(g.x, ((g.m - 1) * g.x_ld + g.k) * 2);
   const __amdgpu_buffer_rsrc_t rn = rsrc4(g.nw, NORM ? 2 * g.k : 0);
   const unsigned x_row = static_cast<unsigned>(g.x_ld) * 2;
@@ -378,7 +377,9 @@ __global__ __launch_bounds__(256 * KS, 2) void linear4_wide_kernel(const Lin4Geo
         const unsigned at = (tile * GPT + gi) * 16;
         sc[d][j][gi] = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(
                                                      rs, (none + 2 * at) + 8 * lg, 0, 0));
-        zr[d][j][gi] = __builtin_amdgcn_raw_buffer_load_b32(rz, (none + at) + 4 * lg, 0, 0);
+        if constexpr (ZEROS) {
+          zr[d][j][gi] = __builtin_amdgcn_raw_buffer_load_b32(rz, (none + at) + 4 * lg, 0, 0);
+        }
       }
     }
   };
@@ -403,12 +404,10 @@ __global__ __launch_bounds__(256 * KS, 2) void linear4_wide_kernel(const Lin4Geo
     }
   };
 
-  f4 total[TN][MT], acc[2][TN][MT], z[TN][GPT], last[TN];
+  f4 total[TN][MT], acc[2][TN][MT], last[TN];
 #pragma unroll
   for (int j = 0; j < TN; ++j) {
     last[j] = f4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int gi = 0; gi < GPT; ++gi) z[j][gi] = last[j];
 #pragma unroll
     for (int m = 0; m < MT; ++m) total[j][m] = acc[0][j][m] = acc[1][j][m] = last[j];
   }
@@ -417,19 +416,7 @@ __global__ __launch_bounds__(256 * KS, 2) void linear4_wide_kernel(const Lin4Geo
   const V8 ones = __builtin_bit_cast(V8, u32x4{C::kUnit, C::kUnit, C::kUnit, C::kUnit});
   uint32_t sixteens = C::kOne;
   asm("" : "+v"(sixteens));
-  // total -= scale (16 + z) X of a group of the tile before, whose X lies in s_x[b]
-  auto shift = [&](int b, int gi) __attribute__((always_inline)) {
-#pragma unroll
-    for (int m = 0; m < MT; ++m) {
-      const float x = s_x[b][gi][16 * m + l16];
-#pragma unroll
-      for (int j = 0; j < TN; ++j) {
-#pragma unroll
-        for (int r = 0; r < 4; ++r) total[j][m][r] = fmaf(z[j][gi][r], x, total[j][m][r]);
-      }
-    }
-  };
-  // total += scale A of the group before
+  // total += scale (A - (16 + z) X) of the group before
   auto settle = [&](int p) __attribute__((always_inline)) {
 #pragma unroll
     for (int j = 0; j < TN; ++j) {
@@ -443,13 +430,16 @@ __global__ __launch_bounds__(256 * KS, 2) void linear4_wide_kernel(const Lin4Geo
       }
     }
   };
-  V8 b[2][MT + 1];
+  V8 b[2][MT];
   auto read = [&](int p, int buffer, int i) __attribute__((always_inline)) {
     // chunk c of a row lies at c ^ (row & 15): a read of 16 rows meets 16 bank groups
     const char* at = lds + buffer + l16 * 256 + 16 * ((4 * i + lg) ^ l16);
 #pragma unroll
     for (int m = 0; m < MT; ++m) b[p][m] = *reinterpret_cast<const V8*>(at + 16 * m * 256);
-    b[p][MT] = *reinterpret_cast<const V8*>(at + 16 * w * 256);
+  };
+  // x block w of a step: the wave's share of X
+  auto own = [&](int buffer, int i) __attribute__((always_inline)) {
+    return *reinterpret_cast<const V8*>(lds + buffer + (16 * w + l16) * 256 + 16 * ((4 * i + lg) ^ l16));
   };
 
   fetch_x(team);
@@ -459,9 +449,14 @@ __global__ __launch_bounds__(256 * KS, 2) void linear4_wide_kernel(const Lin4Geo
   fetch_x(team + KS);
   put_x(kStage);
   fetch_x(team + 2 * KS);
-  if (tid < 16 * MT) {  // no tile is before the first
+  lds_barrier();
+  constexpr int kPer = 4 / GPT;  // steps of a group
+  f4 sum;
 #pragma unroll
-    for (int gi = 0; gi < GPT; ++gi) s_x[1][gi][tid] = 0.f;
+  for (int i = 0; i < 4; ++i) {  // X of the first tile
+    if (i % kPer == 0) sum = f4{0.f, 0.f, 0.f, 0.f};
+    sum = C::mma(ones, own(0, i), sum);
+    if (i % kPer == kPer - 1) s_x[0][i / kPer][16 * w + l16] = sum[0];
   }
   lds_barrier();
   read(0, 0, 0);
@@ -475,43 +470,45 @@ __global__ __launch_bounds__(256 * KS, 2) void linear4_wide_kernel(const Lin4Geo
       const int t = t0 + KS * d;
       put_x(after);
       fetch_x(t + 3 * KS);
-      constexpr int kPer = 4 / GPT;  // steps of a group
-      f4 sum;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int gi = i / kPer, p = (GPT * d + gi) & 1;
+        float x[MT];
+        if (i % kPer == 0) {
+          // LDS answers in order, and the group's sums begin with these
+#pragma unroll
+          for (int m = 0; m < MT; ++m) x[m] = s_x[d & 1][gi][16 * m + l16];
+          __builtin_amdgcn_sched_barrier(0);
+        }
         read((i + 1) & 1, i < 3 ? here : next, (i + 1) & 3);
+        const V8 share = own(next, i);
         if (i % kPer == 0) {
           sum = f4{0.f, 0.f, 0.f, 0.f};
+          settle(p ^ 1);
+          // a group's sums begin at -(16 + z) X
 #pragma unroll
           for (int j = 0; j < TN; ++j) {
+            last[j] = scales4<S>(sc[d][j][gi]);
 #pragma unroll
-            for (int m = 0; m < MT; ++m) acc[p][j][m] = sum;
+            for (int m = 0; m < MT; ++m) {
+#pragma unroll
+              for (int r = 0; r < 4; ++r) {
+                acc[p][j][m][r] = ZEROS
+                    ? -(16.f + static_cast<float>((zr[d][j][gi] >> (8 * r)) & 0xffu)) * x[m]
+                    : -24.f * x[m];
+              }
+            }
           }
         }
-        sum = C::mma(ones, b[i & 1][MT], sum);
 #pragma unroll
         for (int j = 0; j < TN; ++j) {
           const V8 a = expand<T>(code[d][j][i], sixteens);
 #pragma unroll
           for (int m = 0; m < MT; ++m) acc[p][j][m] = C::mma(a, b[i & 1][m], acc[p][j][m]);
         }
-        if (i % kPer == 0) {
-          settle(p ^ 1);
-          shift((d + 1) & 1, gi);
-#pragma unroll
-          for (int j = 0; j < TN; ++j) {
-            last[j] = scales4<S>(sc[d][j][gi]);
-            z[j][gi] = shifts4(zr[d][j][gi] | eights, last[j]);
-          }
-        }
-        if (i % kPer == kPer - 1) s_x[d & 1][gi][16 * w + l16] = sum[0];  // the same from four lanes
-        // one matrix product at a time and a few vector instructions under it
-#pragma unroll
-        for (int u = 0; u < TN * MT + 1; ++u) {
-          __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-          __builtin_amdgcn_sched_group_barrier(0x002, 5, 0);
-        }
+        sum = C::mma(ones, share, sum);
+        // X of the next tile, the same from four lanes
+        if (i % kPer == kPer - 1) s_x[(d + 1) & 1][gi][16 * w + l16] = sum[0];
         __builtin_amdgcn_sched_barrier(0);
       }
       fetch_w(d, t + KS * kAhead);
@@ -522,8 +519,6 @@ __global__ __launch_bounds__(256 * KS, 2) void linear4_wide_kernel(const Lin4Geo
     }
   }
   settle((GPT * kAhead - 1) & 1);
-#pragma unroll
-  for (int gi = 0; gi < GPT; ++gi) shift((kAhead - 1) & 1, gi);
   if constexpr (NORM) {
 #pragma unroll
     for (int u = 0; u < MT; ++u) {
@@ -667,11 +662,12 @@ int launch_kernel(const Lin4Geom& g, hipStream_t stream) {
 template <typename T, typename S, int GPT, int TN, int KS>
 int launch_wide(const Lin4Geom& g, hipStream_t stream) {
   const dim3 grid((g.tiles + 4 * TN - 1) / (4 * TN), (g.m + 63) / 64), block(256 * KS);
-  if (g.nw != nullptr) {
-    hipLaunchKernelGGL((linear4_wide_kernel<T, S, GPT, TN, KS, true>), grid, block, 0, stream, g);
-  } else {
-    hipLaunchKernelGGL((linear4_wide_kernel<T, S, GPT, TN, KS, false>), grid, block, 0, stream, g);
-  }
+  const bool norm = g.nw != nullptr, zeros = g.zeros != nullptr;
+  const auto kernel = norm ? (zeros ? linear4_wide_kernel<T, S, GPT, TN, KS, true, true>
+                                    : linear4_wide_kernel<T, S, GPT, TN, KS, true, false>)
+                           : (zeros ? linear4_wide_kernel<T, S, GPT, TN, KS, false, true>
+                                    : linear4_wide_kernel<T, S, GPT, TN, KS, false, false>);
+  hipLaunchKernelGGL(kernel, grid, block, 0, stream, g);
   return check_launch("m3_linear4");
 }
 
@@ -684,8 +680,8 @@ int launch_wide(const Lin4Geom& g, hipStream_t stream) {
 // More rows: few tile rows keep the split over columns (2048 x 4096, 64 rows: 7.9 us in blocks of 32, 12.7 in
 // blocks of 64, 21.5 wide). Else the wide kernel in the form whose rounds of workgroups over the 256 CUs cost
 // least: 65 a round with 2 tile rows a wave, 44 with 1 (both one workgroup a CU), 87 for 512
-// workgroups of one team (two a CU): 28672 x 8192 at 64 rows 55 / 74 / 72 us, 16384 x 4096 26 / 20 / 27, 8672 x 2048
-// at 256 rows 31 / 32 / 23. Two tile rows in groups of 32 spill (90 against 51 us).
+// workgroups of one team (two a CU): 28672 x 8192 at 64 rows 55 / 71 / 68 us, 16384 x 4096 27 / 20 / 26, 8672 x 2048
+// at 256 rows 31 / 31 / 23; in groups of 32 28672 x 4096 at 64 rows 40 / 47 / 44.
 template <typename T, typename S, int GPT>
 int launch_rows(const Lin4Geom& g, hipStream_t stream) {
   if (g.m <= 16) {
@@ -700,9 +696,7 @@ int launch_rows(const Lin4Geom& g, hipStream_t stream) {
   if (g.tiles < 384 && g.tiles * blocks < 512) return launch_kernel<T, S, GPT, 2, 1, 8>(g, stream);
   const int w1 = (g.tiles + 3) / 4 * blocks, w2 = (g.tiles + 7) / 8 * blocks;
   const int two = (w2 + 255) / 256 * 65, one = (w1 + 255) / 256 * 44, half = max(w1, 512) * 87 / 512;
-  if constexpr (GPT < 4) {
-    if (two <= one && two <= half) return launch_wide<T, S, GPT, 2, 2>(g, stream);
-  }
+  if (two <= one && two <= half) return launch_wide<T, S, GPT, 2, 2>(g, stream);
   return one <= half ? launch_wide<T, S, GPT, 1, 2>(g, stream)
                      : launch_wide<T, S, GPT, 1, 1>(g, stream);
 }
