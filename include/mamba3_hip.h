@@ -335,6 +335,8 @@ int m3_gated_scan_bwd(const m3_gated_scan_bwd_args* args, hipStream_t stream);
  *     32 i + 8 (l / 16) + e of its tile, column e = 2 j in bits 4 j, e = 2 j + 1 in bits 4 j + 16
  *   scales [ceil(N / 16), TK, 128 / group, 16] bf16 or f16
  *   zeros the same in bytes; NULL: 8 everywhere
+ * A group's sum is scale (sum (16 + q) x - (16 + z) sum x): an infinity in a row of x makes the row of
+ * out NaN, and so do values whose sums times 31 pass FP32.
  */
 typedef struct {
   int64_t m, n, k;
@@ -345,7 +347,7 @@ typedef struct {
   const void* codes;    /* 16-byte aligned */
   const void* scales;   /* 8-byte aligned */
   const void* zeros;    /* 4-byte aligned, optional */
-  m3_tensor x;          /* [M, K], rows 16-byte aligned */
+  m3_tensor x;          /* [M, K], rows 16-byte aligned, 512 MB from first to last at most */
   m3_tensor norm_weight;/* [K] optional, 16-byte aligned */
   m3_tensor residual;   /* [M, N] optional */
   m3_tensor out;        /* [M, N]; may not overlap x or the weight, may equal residual */

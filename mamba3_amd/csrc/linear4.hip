@@ -104,8 +104,8 @@ __device__ __forceinline__ f4 shifts4(uint32_t z, f4 scale) {
   return v;
 }
 
-// An offset past every extent (all below 2^30 bytes), also with another added: the load gives 0. Offsets
-// go into a load whole, none as the scalar offset, which the range check does not add.
+// An offset past every extent, also with another added: the load gives 0. x spans less than 2^29 bytes, so
+// 48 rows more (of over 16) add less than 3 x 2^29 and do not come round to 0. Offsets go into a load whole, none as the scalar offset, which the range check does not add.
 constexpr unsigned kNowhere = 0x7fff0000u;
 
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t rsrc4(const void* base, int64_t bytes) {
@@ -627,8 +627,8 @@ int validate(const m3_linear4_args& a) {
                 "aligned, scales 8-byte, zeros 4-byte");
   }
   // offsets within x, and within the tile rows of a workgroup, are 32-bit, in bytes
-  if ((a.m - 1) * a.x.stride[0] + a.k >= (1 << 29)) {
-    return fail(M3_EUNSUPPORTED, "m3_linear4: x spans over 1 GB");
+  if ((a.m - 1) * a.x.stride[0] + a.k >= (1 << 28)) {
+    return fail(M3_EUNSUPPORTED, "m3_linear4: x spans over 512 MB");
   }
   if (a.m > 1 && a.out.stride[0] < a.n) return fail(M3_EINVAL, "m3_linear4: rows of out overlap");
   const int64_t tiles = (a.n + 15) / 16 * ((a.k + 127) / 128);

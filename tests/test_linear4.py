@@ -184,6 +184,15 @@ def test_validation_on_the_host(lib):
     assert call(ctypes.byref(args), None) == 1 and b"rows of out" in lib.m3_last_error()
 
 
+def test_rows_of_x_too_far_apart_are_refused(lib):
+    """Offsets within x, and of the rows of a block past the last, fit 32 bits only up to here."""
+    for m, stride in ((17, 1 << 24), (17, (1 << 25) - 64), (2, 1 << 28), (256, 1 << 21)):
+        args = _args(m=m, n=6144)
+        args.x = _hip.Tensor(1 << 40, _hip.BF16, 0, (stride, 1))
+        assert lib.m3_linear4(ctypes.byref(args), None) == 2, (m, stride)
+        assert b"512 MB" in lib.m3_last_error(), (m, stride)
+
+
 def test_struct_matches_the_header_layout(tmp_path):
     if shutil.which("gcc") is None:
         pytest.skip("gcc not available")
