@@ -973,9 +973,9 @@ def gated_scan(x: torch.Tensor, decay: torch.Tensor, gate: torch.Tensor | None =
         _require_device(x, decay, gate, rate, initial_state, lengths, reset)
     rate = _rate32(rate)
     if batch == 0 or length == 0 or width == 0:
-        final = (torch.zeros(batch, width, device=x.device) if initial_state is None
-                 else initial_state.clone())
-        return torch.empty_like(x), final
+        final = (torch.zeros(batch, width, dtype=torch.float32, device=x.device)
+                 if initial_state is None else initial_state.clone())
+        return x.clone(), final
     if lengths is not None and (lengths.dtype != torch.int32 or not lengths.is_contiguous()):
         lengths = lengths.clamp(0, length).to(torch.int32).contiguous()
     x, decay, gate, state, reset = (_inner(x), _inner(decay), _inner(gate), _inner(initial_state),

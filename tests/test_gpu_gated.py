@@ -465,6 +465,18 @@ def test_empty_extents():
     assert ops.gated_step(x, x, x)[0].shape == (0, 8)
 
 
+def test_empty_extents_under_autograd_and_another_default_type():
+    x = torch.randn(2, 0, 8, device=DEV, requires_grad=True)
+    torch.set_default_dtype(F16)
+    try:
+        y, last = ops.gated_scan(x, x)
+    finally:
+        torch.set_default_dtype(F32)
+    assert last.dtype == F32 and last.shape == (2, 8)
+    (y.sum() + last.sum()).backward()
+    assert x.grad.shape == x.shape
+
+
 def test_second_derivatives_are_refused():
     x, decay = (torch.randn(1, 4, 8, device=DEV, requires_grad=True) for _ in range(2))
     y, _ = ops.gated_scan(x, decay)
