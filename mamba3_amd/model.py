@@ -123,10 +123,9 @@ class _Mamba3Mixer(nn.Module):
         # 4-bit copies of the projections for decode steps, by name (quantize_decode)
         self._decode4: dict[str, tuple[ops.Weight4, tuple[object, ...]]] = {}
 
-    def quantize_decode(self, group: int, zeros: bool) -> None:
-        layers = {name: getattr(self, name) for name in ("in_proj", "out_proj")}
-        held = {name: ops.quantize4(layer.weight, group, zeros=zeros)
-                for name, layer in layers.items()}
+    def _hold4(self, held: dict[str, ops.Weight4]) -> None:
+        """Take 4-bit copies of the projections, and their values for the weights."""
+        layers = {name: getattr(self, name) for name in held}
         with torch.no_grad():
             for name, layer in layers.items():
                 layer.weight.copy_(held[name].dequantize(layer.weight.dtype))
@@ -454,8 +453,11 @@ class Mamba3(nn.Module):
                 if group not in ops.LINEAR4_GROUPS or weight.shape[1] % group != 0:
                     raise ValueError(f"group must be 32, 64 or 128 and divide {name}'s "
                                      f"{weight.shape[1]} columns")
-        for layer in self.layers:
-            layer.mixer.quantize_decode(group, zeros)
+        # all of them before any weight changes: one that holds NaN is refused
+        held = [{name: ops.quantize4(getattr(layer.mixer, name).weight, group, zeros=zeros)
+                 for name in ("in_proj", "out_proj")} for layer in self.layers]
+        for layer, copies in zip(self.layers, held):
+            layer.mixer._hold4(copies)
         return self
 
     def compile_layers(self, **kwargs: object) -> Mamba3:

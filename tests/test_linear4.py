@@ -145,6 +145,17 @@ def test_quantize_decode_refusals():
         mixer._weight4("in_proj")
 
 
+def test_quantize_decode_changes_every_layer_or_none():
+    model = Mamba3(64, depth=2).to(torch.bfloat16)
+    with torch.no_grad():
+        model.layers[1].mixer.out_proj.weight[3, 5] = float("nan")
+    before = model.layers[0].mixer.in_proj.weight.clone()
+    with pytest.raises(ValueError, match="NaN"):
+        model.quantize_decode(32)
+    assert torch.equal(model.layers[0].mixer.in_proj.weight, before)
+    assert all(layer.mixer._weight4("in_proj") is None for layer in model.layers)
+
+
 def _args(m=4, n=64, k=256):
     return _hip.Linear4Args(m, n, k, _hip.BF16, _hip.F16, 64, 1e-5, 0x100000, 0x200000, 0x300000,
                             _hip.Tensor(0x400000, _hip.BF16, 0, (k, 1)),
