@@ -328,7 +328,8 @@ int m3_gated_scan_bwd(const m3_gated_scan_bwd_args* args, hipStream_t stream);
  * m3_linear with a weight held in 4 bits: out[M, N] = x'[M, K] * W[N, K]^T (+ residual[M, N]),
  *   W[n, k] = (q[n, k] - z[n, k / group]) * scale[n, k / group],  q, z in 0..15,
  * x' and the residual as in m3_linear (M <= 256, FP32 accumulation, one rounding; the norm at any
- * M). group is 32, 64 or 128, K a multiple of 32 and of group. No counterpart in the reference.
+ * M). x * norm_weight is held in two bf16 values, whole for bf16 and to 2^-17 of itself for f16, in
+ * FP32's range, and 1 / rms meets the FP32 sums. group is 32, 64 or 128, K a multiple of 32 and of group. No counterpart in the reference.
  * The weight is laid out once, for reads of 1 KB by a wave, in tiles of 16 rows x 128 columns
  * (rows and columns past N and K: code 0, scale 0, zero 0), TK = ceil(K / 128) of them a tile row:
  *   codes [ceil(N / 16), TK, 64, 4] 32-bit words: word i of lane l holds row l % 16, columns

@@ -7,13 +7,16 @@
 // operands. X comes from one more matrix product, with ones.
 //
 // linear4_kernel (up to 16 rows of x; up to 32 a workgroup where there are few weight rows): a workgroup
-// takes TN tiles of 16 weight rows and MT blocks of 16 x rows. Its waves take every WAVES-th tile of 128
+// takes TN tiles of 16 weight rows and MT blocks of 16 operand rows: rows of x, or with the norm two for
+// each, for its product with the norm's weight has more bits than one holds. Its waves take every WAVES-th tile of 128
 // columns each, so no two read the same operand and the K loop has no barrier; their sums meet in
 // LDS. A wave's next codes and x are on their way in registers while it multiplies; x goes through
 // an LDS region of the wave's own, where it is normed, and comes back as the operand's columns. Bound by
 // the weight's stream where it is long, else by the launch and one latency of memory: in graphs with
 // cold weights 28672 x 8192 at 1 row 27.1 us (4.5 TB/s; a large copy reaches 4.8), 8672 x 2048 at 1 row 4.9
-// us, 6.8 with the norm, 2048 x 4096 at 16 rows 5.6 us (512 x 512: 2.4 us).
+// us, 6.7 with the norm, 2048 x 4096 at 16 rows 5.6 us (512 x 512: 2.4 us). A second row for the norm costs nothing
+// where matrix rows are idle (8672 x 2048 at 4 rows 6.9 us either way), else its instructions: 16 rows 11.8 us
+// with whole products, 9.0 with rounded ones.
 //
 // linear4_wide_kernel (more rows of both): below.
 #include <hip/hip_runtime.h>
@@ -113,20 +116,30 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t rsrc4(const void* base, int64_
                                            static_cast<int>(bytes), 0x00020000);
 }
 
-// Eight x values times the norm's weights, rounded once; their squares go to sq.
+// Eight x values times the norm's weights, as a bf16 value and the bf16 remainder; the squares go to sq.
+// The FP32 products are whole (8 + 8 or 11 + 11 bits). Two bf16 values hold those of bf16 rows whole and
+// 16 or more bits of those of f16 rows (2^-17 of a term, against 2^-11 of the rounded result), over FP32's range:
+// 1 / rms, which brings a row back into f16's, comes last.
 template <typename T>
-__device__ __forceinline__ u32x4 normed(u32x4 x, u32x4 weight, float& sq) {
+__device__ __forceinline__ void normed(u32x4 x, u32x4 weight, float& sq, u32x4& high, u32x4& low) {
   using V8 = typename Code<T>::v8;
-  V8 b = __builtin_bit_cast(V8, x);
-  const V8 n = __builtin_bit_cast(V8, weight);
+  typename Code<__bf16>::v8 h, l;
+  const V8 b = __builtin_bit_cast(V8, x), n = __builtin_bit_cast(V8, weight);
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
-    const float xf = static_cast<float>(b[e]);
+    const float xf = static_cast<float>(b[e]), p = xf * static_cast<float>(n[e]);
     sq = fmaf(xf, xf, sq);
-    b[e] = static_cast<T>(xf * static_cast<float>(n[e]));
+    h[e] = static_cast<__bf16>(p);
+    l[e] = static_cast<__bf16>(p - static_cast<float>(h[e]));
   }
-  return __builtin_bit_cast(u32x4, b);
+  high = __builtin_bit_cast(u32x4, h);
+  low = __builtin_bit_cast(u32x4, l);
 }
+
+// What feeds the matrix instructions: x itself, or with the norm two bf16 rows for each row of x, the
+// remainders in the second half of a workgroup's rows. Their two sums are added at the end.
+template <typename T, bool NORM> struct Operand { using type = T; };
+template <typename T> struct Operand<T, true> { using type = __bf16; };
 
 // Between a wave's writes of its own LDS region and its lanes' reads of one another's, and back: LDS
 // operations of one wave complete in order, so only the compiler has to keep them so.
@@ -145,20 +158,22 @@ constexpr int kRowBytes = 256;  // an x row of a tile in LDS; chunk c of 16 byte
 
 template <typename T, typename S, int GPT, int MT, int TN, int WAVES, bool NORM>
 __global__ __launch_bounds__(64 * WAVES) void linear4_kernel(const Lin4Geom g) {
-  using C = Code<T>;
+  using O = typename Operand<T, NORM>::type;
+  using C = Code<O>;
   using V8 = typename C::v8;
+  constexpr int kRows = 16 * MT / (NORM ? 2 : 1), kLoads = kRows / 4;  // rows of x
   constexpr int kStage = MT * 16 * kRowBytes, kSums = MT * TN * 256;
   constexpr int kLds = WAVES * (kStage > 4 * kSums ? kStage : 4 * kSums);
   __shared__ __attribute__((aligned(16))) char lds[kLds];
-  __shared__ float s_sq[NORM ? WAVES : 1][16 * MT];
+  __shared__ float s_sq[NORM ? WAVES : 1][kRows];
   const int tid = threadIdx.x, lane = tid & 63;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int l16 = lane & 15, lg = lane >> 4;
-  const int tn = blockIdx.x * TN, m0 = blockIdx.y * (16 * MT);
+  const int tn = blockIdx.x * TN, m0 = blockIdx.y * kRows;
   char* const stage = lds + w * kStage;
 
   // what a tile of columns needs: codes, scales and zeros of TN tile rows, x rows 4 j + lg.
-  u32x4 code[TN], xv[4 * MT], nv;
+  u32x4 code[TN], xv[kLoads], nv;
   u32x2 sc[TN][GPT];
   uint32_t zr[TN][GPT];
   // reads past an extent give 0: tile rows past the last, x rows past M
@@ -190,8 +205,8 @@ __global__ __launch_bounds__(64 * WAVES) void linear4_kernel(const Lin4Geom g) {
     const int k = 128 * t + 8 * l16;
     const unsigned at = k < g.k ? (m0 + lg) * x_row + 2 * k : kNowhere;
 #pragma unroll
-    for (int j = 0; j < 4 * MT; ++j) {
-      if (MT > 1 || j == 0 || 4 * j < g.m - m0) {
+    for (int j = 0; j < kLoads; ++j) {
+      if (kRows > 16 || j == 0 || 4 * j < g.m - m0) {
         xv[j] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(
                                               rx, at + 4 * j * x_row, 0, 0));
       }
@@ -206,9 +221,9 @@ __global__ __launch_bounds__(64 * WAVES) void linear4_kernel(const Lin4Geom g) {
 #pragma unroll
     for (int m = 0; m < MT; ++m) total[j][m] = f4{0.f, 0.f, 0.f, 0.f};
   }
-  float sq[4 * MT];
+  float sq[kLoads];
 #pragma unroll
-  for (int j = 0; j < 4 * MT; ++j) sq[j] = 0.f;
+  for (int j = 0; j < kLoads; ++j) sq[j] = 0.f;
   const V8 ones = __builtin_bit_cast(V8, u32x4{C::kUnit, C::kUnit, C::kUnit, C::kUnit});
   uint32_t sixteens = C::kOne;
   asm("" : "+v"(sixteens));
@@ -227,11 +242,19 @@ __global__ __launch_bounds__(64 * WAVES) void linear4_kernel(const Lin4Geom g) {
       }
     }
 #pragma unroll
-    for (int j = 0; j < 4 * MT; ++j) {
-      if (MT == 1 && j > 0 && 4 * j >= g.m - m0) break;  // rows that are not there
-      if constexpr (NORM) xv[j] = normed<T>(xv[j], nv, sq[j]);
-      *reinterpret_cast<u32x4*>(stage + (4 * j + lg) * kRowBytes +
-                                16 * (l16 ^ ((4 * j + lg) & 15))) = xv[j];
+    for (int j = 0; j < kLoads; ++j) {
+      if (kRows <= 16 && j > 0 && 4 * j >= g.m - m0) break;  // rows that are not there
+      const auto put = [&](int row, u32x4 v) __attribute__((always_inline)) {
+        *reinterpret_cast<u32x4*>(stage + row * kRowBytes + 16 * (l16 ^ (row & 15))) = v;
+      };
+      if constexpr (NORM) {
+        u32x4 high, low;
+        normed<T>(xv[j], nv, sq[j], high, low);
+        put(4 * j + lg, high);
+        put(kRows + 4 * j + lg, low);
+      } else {
+        put(4 * j + lg, xv[j]);
+      }
     }
     if (t + WAVES < g.tk) fetch(t + WAVES);
     stage_turn();
@@ -255,7 +278,7 @@ __global__ __launch_bounds__(64 * WAVES) void linear4_kernel(const Lin4Geom g) {
         }
 #pragma unroll
         for (int j = 0; j < TN; ++j) {
-          const V8 a = expand<T>(q[j][i], sixteens);
+          const V8 a = expand<O>(q[j][i], sixteens);
 #pragma unroll
           for (int m = 0; m < MT; ++m) acc[j][m] = C::mma(a, b[m], acc[j][m]);
         }
@@ -275,11 +298,11 @@ __global__ __launch_bounds__(64 * WAVES) void linear4_kernel(const Lin4Geom g) {
     stage_turn();
   }
 
-  // lane holds weight rows 16 j + 4 lg + r, x row 16 m + l16 (and, for the norm, the squares of x
+  // lane holds weight rows 16 j + 4 lg + r, operand row 16 m + l16 (and, for the norm, the squares of x
   // rows 4 j + lg, over its columns)
   if constexpr (NORM) {
 #pragma unroll
-    for (int j = 0; j < 4 * MT; ++j) {
+    for (int j = 0; j < kLoads; ++j) {
       float v = sq[j];
 #pragma unroll
       for (int o = 8; o > 0; o >>= 1) v += __shfl_xor(v, o);
@@ -299,7 +322,7 @@ __global__ __launch_bounds__(64 * WAVES) void linear4_kernel(const Lin4Geom g) {
     }
   }
   __syncthreads();
-  for (int e = tid; e < kSums; e += 64 * WAVES) {
+  for (int e = tid; e < kRows * 16 * TN; e += 64 * WAVES) {
     const int col = e % (16 * TN), row = e / (16 * TN);
     const int m = m0 + row, n = 16 * tn + col;
     if (m >= g.m || n >= g.n) continue;
@@ -309,6 +332,9 @@ __global__ __launch_bounds__(64 * WAVES) void linear4_kernel(const Lin4Geom g) {
 #pragma unroll
     for (int v = 0; v < WAVES; ++v) y += at[v * kSums];
     if constexpr (NORM) {
+      constexpr int kLow = MT == 1 ? 8 : MT / 2 * 256;  // from a row's sum to its remainder's
+#pragma unroll
+      for (int v = 0; v < WAVES; ++v) y += at[v * kSums + kLow];
       float total_sq = 0.f;
 #pragma unroll
       for (int v = 0; v < WAVES; ++v) total_sq += s_sq[v][row];
@@ -321,7 +347,8 @@ __global__ __launch_bounds__(64 * WAVES) void linear4_kernel(const Lin4Geom g) {
   }
 }
 
-// Many rows of x and many of W: a workgroup of four waves takes 64 x rows and 4 TN tiles of weight
+// Many rows of x and many of W: a workgroup of four waves takes 64 operand rows (64 of x, or 32 with the
+// norm: 8672 x 2048 at 64 rows then takes 19 us, 15.5 with rounded products) and 4 TN tiles of weight
 // rows, TN for each wave, over all of K. A tile of x columns is staged once for the workgroup, in three
 // LDS buffers; x comes from memory three tiles ahead of its use, the codes two. Wave w forms X of the next
 // tile for x block w, and a group's sums begin at -(16 + z) X. KS = 2: two such teams, every other tile of
@@ -335,20 +362,22 @@ __global__ __launch_bounds__(64 * WAVES) void linear4_kernel(const Lin4Geom g) {
 // matrix and vector instructions, 4 tile rows a wave.
 template <typename T, typename S, int GPT, int TN, int KS, bool NORM, bool ZEROS>
 __global__ __launch_bounds__(256 * KS, 2) void linear4_wide_kernel(const Lin4Geom g) {
-  using C = Code<T>;
+  using O = typename Operand<T, NORM>::type;
+  using C = Code<O>;
   using V8 = typename C::v8;
-  constexpr int MT = 4, kStage = MT * 16 * 256;  // an x block for each wave
+  constexpr int MT = 4, kStage = MT * 16 * 256;  // a block of operand rows for each wave
+  constexpr int kBlocks = MT / (NORM ? 2 : 1);   // of x rows
   constexpr int kAhead = 2;
   static_assert(KS <= 2 && 3 * kStage >= TN * MT * 4096, "the second team's sums fit its stages");
   __shared__ __attribute__((aligned(16))) char lds_all[KS][3 * kStage];
-  __shared__ float s_x_all[KS][2][GPT][16 * MT], s_sq[NORM ? KS : 1][16 * MT];
+  __shared__ float s_x_all[KS][2][GPT][16 * MT], s_sq[NORM ? KS : 1][16 * kBlocks];
   const int team = __builtin_amdgcn_readfirstlane(threadIdx.x >> 8), tid = threadIdx.x & 255;
   const int lane = tid & 63;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
   char* const lds = lds_all[team];
   auto& s_x = s_x_all[team];
   const int l16 = lane & 15, lg = lane >> 4;
-  const int tn = (blockIdx.x * 4 + w) * TN, m0 = blockIdx.y * (16 * MT);
+  const int tn = (blockIdx.x * 4 + w) * TN, m0 = blockIdx.y * (16 * kBlocks);
 
   // reads past an extent give 0: tile rows past the last, x rows past M
   const int64_t tile0 = static_cast<int64_t>(min(tn, g.tiles)) * g.tk;
@@ -362,7 +391,7 @@ __global__ __launch_bounds__(256 * KS, 2) void linear4_wide_kernel(const Lin4Geo
   const unsigned x_row = static_cast<unsigned>(g.x_ld) * 2;
   const int row = tid >> 4, chunk = tid & 15;  // what this thread stages: rows 16 u + row
 
-  u32x4 code[kAhead][TN], xv[MT], nv;
+  u32x4 code[kAhead][TN], xv[kBlocks], nv;
   u32x2 sc[kAhead][TN][GPT];
   uint32_t zr[kAhead][TN][GPT];
   auto fetch_w = [&](int d, int t) __attribute__((always_inline)) {
@@ -387,7 +416,7 @@ __global__ __launch_bounds__(256 * KS, 2) void linear4_wide_kernel(const Lin4Geo
     const int k = 128 * t + 8 * chunk;
     const unsigned at = k < g.k ? (m0 + row) * x_row + 2 * k : kNowhere;
 #pragma unroll
-    for (int u = 0; u < MT; ++u) {
+    for (int u = 0; u < kBlocks; ++u) {
       xv[u] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(
                                             rx, at + 16 * u * x_row, 0, 0));
     }
@@ -395,12 +424,16 @@ __global__ __launch_bounds__(256 * KS, 2) void linear4_wide_kernel(const Lin4Geo
       nv = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rn, 2 * k, 0, 0));
     }
   };
-  float sq[MT];
+  float sq[kBlocks];
   auto put_x = [&](int buffer) __attribute__((always_inline)) {
 #pragma unroll
-    for (int u = 0; u < MT; ++u) {
-      if constexpr (NORM) xv[u] = normed<T>(xv[u], nv, sq[u]);
-      *reinterpret_cast<u32x4*>(lds + buffer + (16 * u + row) * 256 + 16 * (chunk ^ row)) = xv[u];
+    for (int u = 0; u < kBlocks; ++u) {
+      u32x4* const to = reinterpret_cast<u32x4*>(lds + buffer + (16 * u + row) * 256 + 16 * (chunk ^ row));
+      if constexpr (NORM) {
+        normed<T>(xv[u], nv, sq[u], to[0], to[kBlocks * 256]);
+      } else {
+        *to = xv[u];
+      }
     }
   };
 
@@ -412,7 +445,7 @@ __global__ __launch_bounds__(256 * KS, 2) void linear4_wide_kernel(const Lin4Geo
     for (int m = 0; m < MT; ++m) total[j][m] = acc[0][j][m] = acc[1][j][m] = last[j];
   }
 #pragma unroll
-  for (int u = 0; u < MT; ++u) sq[u] = 0.f;
+  for (int u = 0; u < kBlocks; ++u) sq[u] = 0.f;
   const V8 ones = __builtin_bit_cast(V8, u32x4{C::kUnit, C::kUnit, C::kUnit, C::kUnit});
   uint32_t sixteens = C::kOne;
   asm("" : "+v"(sixteens));
@@ -437,7 +470,7 @@ __global__ __launch_bounds__(256 * KS, 2) void linear4_wide_kernel(const Lin4Geo
 #pragma unroll
     for (int m = 0; m < MT; ++m) b[p][m] = *reinterpret_cast<const V8*>(at + 16 * m * 256);
   };
-  // x block w of a step: the wave's share of X
+  // operand block w of a step: the wave's share of X
   auto own = [&](int buffer, int i) __attribute__((always_inline)) {
     return *reinterpret_cast<const V8*>(lds + buffer + (16 * w + l16) * 256 + 16 * ((4 * i + lg) ^ l16));
   };
@@ -502,7 +535,7 @@ __global__ __launch_bounds__(256 * KS, 2) void linear4_wide_kernel(const Lin4Geo
         }
 #pragma unroll
         for (int j = 0; j < TN; ++j) {
-          const V8 a = expand<T>(code[d][j][i], sixteens);
+          const V8 a = expand<O>(code[d][j][i], sixteens);
 #pragma unroll
           for (int m = 0; m < MT; ++m) acc[p][j][m] = C::mma(a, b[i & 1][m], acc[p][j][m]);
         }
@@ -521,7 +554,7 @@ __global__ __launch_bounds__(256 * KS, 2) void linear4_wide_kernel(const Lin4Geo
   settle((GPT * kAhead - 1) & 1);
   if constexpr (NORM) {
 #pragma unroll
-    for (int u = 0; u < MT; ++u) {
+    for (int u = 0; u < kBlocks; ++u) {
       float v = sq[u];
 #pragma unroll
       for (int o = 8; o > 0; o >>= 1) v += __shfl_xor(v, o);
@@ -548,9 +581,9 @@ __global__ __launch_bounds__(256 * KS, 2) void linear4_wide_kernel(const Lin4Geo
   } else if constexpr (NORM) {
     __syncthreads();
   }
-  // lane holds weight rows 16 j + 4 lg + r of the wave's, x rows 16 m + l16
+  // lane holds weight rows 16 j + 4 lg + r of the wave's, operand rows 16 m + l16
 #pragma unroll
-  for (int m = 0; m < MT; ++m) {
+  for (int m = 0; m < kBlocks; ++m) {
     const int xr = m0 + 16 * m + l16;
     if (xr >= g.m) continue;
     float scale = 1.f;
@@ -568,7 +601,7 @@ __global__ __launch_bounds__(256 * KS, 2) void linear4_wide_kernel(const Lin4Geo
       t4 y;
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        float v = total[j][m][r] * scale;
+        float v = NORM ? (total[j][m][r] + total[j][(m + kBlocks) % MT][r]) * scale : total[j][m][r];
         if (res != nullptr && n + r < g.n) v += static_cast<float>(res[r]);
         y[r] = static_cast<T>(v);
       }
@@ -648,21 +681,19 @@ int validate(const m3_linear4_args& a) {
   return M3_OK;
 }
 
-template <typename T, typename S, int GPT, int MT, int TN, int WAVES>
+template <typename T, typename S, int GPT, int MT, int TN, int WAVES, bool NORM>
 int launch_kernel(const Lin4Geom& g, hipStream_t stream) {
-  const dim3 grid((g.tiles + TN - 1) / TN, (g.m + 16 * MT - 1) / (16 * MT)), block(64 * WAVES);
-  if (g.nw != nullptr) {
-    hipLaunchKernelGGL((linear4_kernel<T, S, GPT, MT, TN, WAVES, true>), grid, block, 0, stream, g);
-  } else {
-    hipLaunchKernelGGL((linear4_kernel<T, S, GPT, MT, TN, WAVES, false>), grid, block, 0, stream, g);
-  }
+  constexpr int rows = 16 * MT / (NORM ? 2 : 1);
+  const dim3 grid((g.tiles + TN - 1) / TN, (g.m + rows - 1) / rows), block(64 * WAVES);
+  hipLaunchKernelGGL((linear4_kernel<T, S, GPT, MT, TN, WAVES, NORM>), grid, block, 0, stream, g);
   return check_launch("m3_linear4");
 }
 
 template <typename T, typename S, int GPT, int TN, int KS>
 int launch_wide(const Lin4Geom& g, hipStream_t stream) {
-  const dim3 grid((g.tiles + 4 * TN - 1) / (4 * TN), (g.m + 63) / 64), block(256 * KS);
   const bool norm = g.nw != nullptr, zeros = g.zeros != nullptr;
+  const int rows = norm ? 32 : 64;
+  const dim3 grid((g.tiles + 4 * TN - 1) / (4 * TN), (g.m + rows - 1) / rows), block(256 * KS);
   const auto kernel = norm ? (zeros ? linear4_wide_kernel<T, S, GPT, TN, KS, true, true>
                                     : linear4_wide_kernel<T, S, GPT, TN, KS, true, false>)
                            : (zeros ? linear4_wide_kernel<T, S, GPT, TN, KS, false, true>
@@ -682,18 +713,27 @@ int launch_wide(const Lin4Geom& g, hipStream_t stream) {
 // least: 65 a round with 2 tile rows a wave, 44 with 1 (both one workgroup a CU), 87 for 512
 // workgroups of one team (two a CU): 28672 x 8192 at 64 rows 55 / 71 / 68 us, 16384 x 4096 27 / 20 / 26, 8672 x 2048
 // at 256 rows 31 / 31 / 23; in groups of 32 28672 x 4096 at 64 rows 40 / 47 / 44.
+template <typename T, typename S, int GPT, int MT, bool NORM>
+int launch_few(const Lin4Geom& g, hipStream_t stream) {
+  if (g.tiles < 384) return launch_kernel<T, S, GPT, MT, 1, 8, NORM>(g, stream);
+  if constexpr (GPT < 4) {
+    if (g.tiles >= 1024) return launch_kernel<T, S, GPT, MT, 4, 4, NORM>(g, stream);
+  }
+  return launch_kernel<T, S, GPT, MT, NORM && GPT < 4 ? 2 : 1, 4, NORM>(g, stream);
+}
+
 template <typename T, typename S, int GPT>
 int launch_rows(const Lin4Geom& g, hipStream_t stream) {
+  const bool norm = g.nw != nullptr;
   if (g.m <= 16) {
-    if (g.tiles < 384) return launch_kernel<T, S, GPT, 1, 1, 8>(g, stream);
-    if constexpr (GPT < 4) {
-      if (g.tiles >= 1024) return launch_kernel<T, S, GPT, 1, 4, 4>(g, stream);
-      if (g.nw != nullptr) return launch_kernel<T, S, GPT, 1, 2, 4>(g, stream);
-    }
-    return launch_kernel<T, S, GPT, 1, 1, 4>(g, stream);
+    if (!norm) return launch_few<T, S, GPT, 1, false>(g, stream);
+    return g.m <= 8 ? launch_few<T, S, GPT, 1, true>(g, stream) : launch_few<T, S, GPT, 2, true>(g, stream);
   }
-  const int blocks = (g.m + 63) / 64;
-  if (g.tiles < 384 && g.tiles * blocks < 512) return launch_kernel<T, S, GPT, 2, 1, 8>(g, stream);
+  if (g.tiles < 384 && g.tiles * ((g.m + 63) / 64) < 512) {
+    return norm ? launch_kernel<T, S, GPT, 2, 1, 8, true>(g, stream)
+                : launch_kernel<T, S, GPT, 2, 1, 8, false>(g, stream);
+  }
+  const int blocks = norm ? (g.m + 31) / 32 : (g.m + 63) / 64;
   const int w1 = (g.tiles + 3) / 4 * blocks, w2 = (g.tiles + 7) / 8 * blocks;
   const int two = (w2 + 255) / 256 * 65, one = (w1 + 255) / 256 * 44, half = max(w1, 512) * 87 / 512;
   if (two <= one && two <= half) return launch_wide<T, S, GPT, 2, 2>(g, stream);

@@ -795,8 +795,8 @@ def linear4(x: torch.Tensor, weight: Weight4, residual: torch.Tensor | None = No
 
     ``x [M, K]`` (``M <= 256``) bfloat16 or float16; ``residual`` and ``out`` ``[M, N]`` of that
     dtype. Sums are FP32, the residual is added to them and the result rounded once. With
-    ``norm_weight [K]`` ``x`` is first RMS-normalised, as ``F.rms_norm(x, (K,), norm_weight,
-    norm_eps)``. An infinity in a row of ``x`` makes its row of the result NaN. No backward.
+    ``norm_weight [K]`` (taken in ``x``'s dtype) ``x`` is first RMS-normalised, as
+    ``F.rms_norm(x.float(), (K,), norm_weight.float(), norm_eps)``, its rows not rounded to 16 bits. An infinity in a row of ``x`` makes its row of the result NaN. No backward.
     """
     index = x.get_device()
     if index < 0 or any([t is not None and t.get_device() != index

@@ -293,3 +293,79 @@ def test_a_recurrent_layer_from_the_operators(width, length):
     for b, n in enumerate(lengths.tolist()):
         got = torch.cat([prefill[b, :n], torch.stack([s[b] for s in steps])]).double().cpu()
         assert (got - want[b, :n + 4]).abs().max().item() <= 4 * 2.0 ** -8 * 2 * scale
+
+
+def _normed(x, nw, eps=1e-5):
+    """RMSNorm rows in 64 bits, the norm's weight as the operator takes it (in x's dtype)."""
+    xd = x.double()
+    return xd * nw.to(x.dtype).double() * (xd.square().mean(-1, keepdim=True) + eps).rsqrt()
+
+
+@pytest.mark.parametrize("m,n,k,group", [(1, 64, 256, 128), (8, 100, 512, 64), (9, 8672, 256, 32),
+                                         (16, 6200, 384, 128), (20, 520, 256, 32), (40, 6200, 256, 64),
+                                         (64, 16400, 256, 128)])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_the_norm_loses_no_bits(m, n, k, group, dtype):
+    """Rows with one value each: the sum has one term, so what the norm rounds stands alone. The result
+    is as near to the 64-bit one as its own rounding to 16 bits, but for FP32 errors B: of the sums
+    62 scale |x| times 2^-24 in each of at most 8 steps, of the factor and the product 40 * 2^-24,
+    and in f16 the term's 16 held bits, 2^-17. They count twice: with v within B of w, |round(v) - w|
+    <= |round(v) - v| + B <= |round(w) - v| + B <= |round(w) - w| + 2 B."""
+    g = torch.Generator().manual_seed(m + n)
+    packed, scales, z, wide = _weight(n, k, group, BF16, True, g)
+    at = torch.randint(0, k, (m,), generator=g)
+    x = torch.zeros(m, k)
+    x[torch.arange(m), at] = torch.randn(m, generator=g)
+    x, nw = x.to(dtype), 1 + 0.1 * torch.randn(k, generator=g)
+    weight = ops.Weight4(packed.to(DEV), scales.to(DEV), z.to(DEV))
+    with torch.inference_mode():
+        got = ops.linear4(x.to(DEV), weight, norm_weight=nw.to(DEV)).double().cpu()
+    xd = _normed(x, nw)
+    want = xd @ wide.t()
+    full = scales.double().repeat_interleave(group, 1)
+    bound = 8 * 62 * 2.0 ** -24 * (xd.abs() @ full.t()) + want.abs() * (
+        40 * 2.0 ** -24 + (2.0 ** -17 if dtype == F16 else 0))
+    assert ((got - want).abs() <= (want.to(dtype).double() - want).abs() + 2 * bound).all()
+
+
+@pytest.mark.parametrize("m,n,k", [(1, 8672, 2048), (12, 2048, 1024), (64, 8672, 1024)])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_a_normed_projection_is_off_by_its_output_s_rounding(m, n, k, dtype):
+    """Over a whole projection the error's root mean square is that of rounding the 64-bit result. The
+    FP32 sums add, independently, 31 / 4.6 * 2^-24 sqrt(128) = 5e-6 of the result, against a rounding of
+    about 2e-4 (f16): 0.1%. Rounding the normed row to 16 bits as well would add 40%."""
+    g = torch.Generator().manual_seed(k)
+    packed, scales, z, wide = _weight(n, k, 128, dtype, False, g)
+    x, nw = torch.randn(m, k, generator=g).to(dtype), 1 + 0.1 * torch.randn(k, generator=g)
+    with torch.inference_mode():
+        got = ops.linear4(x.to(DEV), ops.Weight4(packed.to(DEV), scales.to(DEV)),
+                          norm_weight=nw.to(DEV)).double().cpu()
+    want = _normed(x, nw) @ wide.t()
+    rounding = (want.to(dtype).double() - want).square().mean().sqrt()
+    assert (got - want).square().mean().sqrt() <= 1.02 * rounding
+
+
+@pytest.mark.parametrize("m,n", [(1, 70), (10, 70), (40, 6200)])
+@pytest.mark.parametrize("size,weight_size", [(2e4, 15.0), (6e4, 6e4), (1e-3, 1e-3), (6e-8, 1.0)])
+def test_the_norm_in_f16_beyond_f16_s_products(m, n, size, weight_size):
+    """x times the norm's weight outside f16's range, in rows whose norm is inside it: as
+    F.rms_norm has them. Up to 2^-17 of a term (16 held bits) and FP32 errors, as in `_check`."""
+    k = 384
+    g = torch.Generator().manual_seed(m)
+    packed, scales, z, wide = _weight(n, k, 128, F16, True, g)
+    x = (size * torch.randn(m, k, generator=g).clamp(-1, 1)).to(F16)
+    nw = (weight_size * (0.5 + 0.5 * torch.rand(k, generator=g))).to(F16)
+    scales = (scales.double() / weight_size).clamp(2.0 ** -14).to(F16) if weight_size > 1 else scales
+    codes = torch.stack([packed & 15, packed >> 4], -1).flatten(1).double().view(n, -1, 128)
+    wide = ((codes - z.double().unsqueeze(-1)) * scales.double().unsqueeze(-1)).flatten(1)
+    with torch.inference_mode():
+        got = ops.linear4(x.to(DEV), ops.Weight4(packed.to(DEV), scales.to(DEV), z.to(DEV)),
+                          norm_weight=nw.to(DEV)).double().cpu()
+    xd = _normed(x, nw)
+    want = xd @ wide.t()
+    full = scales.double().repeat_interleave(128, 1)
+    bound = (128 + 3 + 41) * 2.0 ** -24 * 63 * (xd.abs() @ full.t()) + 2.0 ** -16 * (xd.abs() @ wide.abs().t())
+    limit = bound + HALF[F16] * (want.abs() + bound) + 2.0 ** -25
+    big = want.abs() + limit >= 65504
+    assert torch.isfinite(got[~big]).all() and (~big).sum() > big.sum()
+    assert ((got - want).abs() <= limit)[~big].all()
