@@ -369,3 +369,35 @@ def test_the_norm_in_f16_beyond_f16_s_products(m, n, size, weight_size):
     big = want.abs() + limit >= 65504
     assert torch.isfinite(got[~big]).all() and (~big).sum() > big.sum()
     assert ((got - want).abs() <= limit)[~big].all()
+
+
+@pytest.mark.parametrize("m,n,k,group,norm", [
+    # up to 16 rows: 1, 2 and 4 tile rows a wave, 4 waves; with the norm also 9 to 16 rows
+    (1, 8672, 384, 32, False), (1, 8672, 384, 64, False), (16, 8672, 384, 128, False),
+    (1, 8672, 384, 32, True), (1, 8672, 384, 64, True), (8, 8672, 640, 128, True),
+    (9, 8672, 384, 64, True), (16, 8672, 640, 32, True),
+    (1, 16400, 384, 32, False), (3, 16400, 640, 64, False), (16, 16400, 384, 128, False),
+    (7, 16400, 384, 64, True), (16, 16400, 384, 128, True), (16, 16400, 384, 32, True),
+    (12, 100, 384, 64, True),
+    # more rows, x staged once: one team of waves, two, one and two tile rows a wave
+    (256, 8672, 384, 128, False), (130, 12304, 384, 64, False), (250, 8672, 384, 32, False),
+    (256, 8672, 384, 64, True), (40, 8672, 384, 128, True), (33, 28700, 256, 32, True),
+    (17, 6144, 384, 128, False), (17, 6144, 384, 128, True), (200, 4000, 384, 32, True)])
+@pytest.mark.parametrize("dtype,scale_dtype", [(BF16, BF16), (F16, F16), (BF16, F16), (F16, BF16)])
+def test_every_form_of_the_kernels(m, n, k, group, norm, dtype, scale_dtype):
+    g = torch.Generator().manual_seed(m + n + group)
+    zeros = (m + n) % 2 == 0 if dtype == BF16 else (m + n) % 2 == 1
+    packed, scales, z, wide = _weight(n, k, group, scale_dtype, zeros, g)
+    x = torch.randn(m, k, generator=g).to(dtype)
+    res = torch.randn(m, n, generator=g).to(dtype)
+    nw = 1 + 0.1 * torch.randn(k, generator=g) if norm else None
+    weight = ops.Weight4(packed.to(DEV), scales.to(DEV), None if z is None else z.to(DEV))
+    bad = x.to(DEV).clone()
+    bad[m // 2] = float("nan")
+    dev = None if nw is None else nw.to(DEV)
+    with torch.inference_mode():
+        got = ops.linear4(x.to(DEV), weight, res.to(DEV), norm_weight=dev)
+        _check(got, x, wide, scales, group, res, nw)
+        spoilt = ops.linear4(bad, weight, res.to(DEV), norm_weight=dev)
+    keep = [i for i in range(m) if i != m // 2]
+    assert torch.equal(got[keep], spoilt[keep]) and torch.isnan(spoilt[m // 2]).all()
