@@ -667,6 +667,11 @@ __global__ __launch_bounds__(64 * kWaves, 4) void gated_back_kernel(const GatedG
         }
       }
     } else {
+      // a given decay at a reset token carries nothing, whatever it is (0 times infinity is NaN)
+      if constexpr (!GATE) {
+#pragma unroll
+        for (int i = 0; i < kBack; ++i) drop_at(cut, i, a[i]);
+      }
 #pragma unroll
       for (int i = 0; i < kBack; ++i) {
         const int k = kBack - 1 - i;

@@ -486,3 +486,28 @@ def test_second_derivatives_are_refused():
     state = torch.zeros(1, 8, device=DEV)
     with pytest.raises(RuntimeError, match="no backward"):
         ops.gated_step(x[:, 0], decay[:, 0], state)
+
+
+@pytest.mark.parametrize("length,width", [(1, 6), (12, 7), (60, 66), (200, 33), (300, 130)])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_a_reset_token_s_own_decay_reaches_nothing(length, width, dtype):
+    """Given form: what stands in decay at a reset token, infinite, NaN or above exp's range, changes
+    neither outputs nor gradients, and its own gradient is 0."""
+    case = _inputs(3, length, width, dtype, "given", seed=17, state=True)
+    case["reset"] = torch.zeros(3, length, dtype=torch.bool)
+    case["reset"][0, 0] = case["reset"][1, length // 2] = case["reset"][2, length - 1] = True
+    g = torch.Generator().manual_seed(6)
+    dy = torch.randn(3, length, width, generator=g).to(dtype).to(DEV)
+    dfinal = torch.randn(3, width, generator=g).to(DEV)
+    names, first = ("x", "decay", "state"), None
+    for value in (-0.5, 0.0, 100.0, float("inf"), float("nan"), float("-inf")):
+        c = _to(case)
+        c["decay"][c["reset"]] = value
+        for n in names:
+            c[n].requires_grad_(True)
+        y, last = _call(c)
+        got = (y.detach(), last.detach(),
+               *torch.autograd.grad((y, last), [c[n] for n in names], (dy, dfinal)))
+        assert not got[3][c["reset"]].any()
+        first = first or got
+        assert all(torch.equal(a, b) for a, b in zip(got, first))
