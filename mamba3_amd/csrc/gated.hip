@@ -126,9 +126,10 @@ __device__ __forceinline__ float sigmoid2(float x) {
   return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(x * -kLog2e));
 }
 
-// A sigmoid and its complement. WHOLE: both with all their digits, from exp(-|x|). Else (for 16-bit
-// gradients) the complement as a difference, off by 2^-25 at most: half a step of bf16 or f16 of
-// its value up to x = 11 or 9, where it is 2^-16 or 2^-13, and a loss of digits only beyond.
+// A sigmoid and its complement, both with all their digits: the complement is e / (1 + e), not a
+// difference. WHOLE: from exp(-|x|), down to FP32's smallest values. Else (for 16-bit gradients, two instructions
+// fewer) from e = exp(-x), whose infinity (x below -88) leaves open = 0 and shut = min(NaN, 1) = 1; a NaN
+// x stays one in open, with which every use of shut is multiplied.
 template <bool WHOLE>
 struct Gate {
   float open, shut;
@@ -139,8 +140,9 @@ struct Gate {
       open = x < 0.f ? small : big;
       shut = x < 0.f ? big : small;
     } else {
-      open = sigmoid2(x);
-      shut = 1.f - open;
+      const float e = __builtin_amdgcn_exp2f(x * -kLog2e);
+      open = __builtin_amdgcn_rcpf(1.f + e);
+      shut = fminf(e * open, 1.f);
     }
   }
 };

@@ -511,3 +511,36 @@ def test_a_reset_token_s_own_decay_reaches_nothing(length, width, dtype):
         assert not got[3][c["reset"]].any()
         first = first or got
         assert all(torch.equal(a, b) for a, b in zip(got, first))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("level", [8.0, 12.0, 17.0, 24.0])
+def test_gradients_of_saturated_gates(dtype, level):
+    """Logits far out, to both sides: the complement of a sigmoid keeps its digits (in f16 the incoming
+    gradient is large, so that the results are not below its range). The 64-bit side forms 1 - p
+    from p, whose sum 1 + e^-x rounds by up to 2^-53 and quotient by 2^-54: below 2^-52, (1 + e^|x|) 2^-52 of it."""
+    case = _inputs(2, 70, 40, dtype, "gate", seed=18, state=True)
+    g = torch.Generator().manual_seed(7)
+    for n in ("decay", "gate"):
+        side = torch.where(torch.rand(2, 70, 40, generator=g) < 0.5, -1.0, 1.0)
+        case[n] = (side * level * (1 + 0.1 * torch.rand(2, 70, 40, generator=g))).to(dtype)
+    big = 2.0 ** 12 if dtype == F16 else 1.0
+    dy = (big * torch.randn(2, 70, 40, generator=g)).to(dtype)
+    dfinal = big * torch.randn(2, 40, generator=g)
+    names = ("x", "decay", "gate", "rate", "state")
+    wide = {n: v if n not in names else v.double().requires_grad_(True) for n, v in case.items()}
+    y64, f64 = og.scan(**wide)
+    want = torch.autograd.grad((y64, f64), [wide[n] for n in names], (dy.double(), dfinal.double()))
+    bound = og.bounds(**case, dy=dy, dfinal=dfinal)
+    for n, v in zip(names, want):
+        if n in ("decay", "gate"):
+            bound["d" + n] += 2.0 ** -52 * (1 + case[n].double().abs().exp()) * v.abs()
+    c = _to(case)
+    for n in names:
+        c[n].requires_grad_(True)
+    y, last = _call(c)
+    got = torch.autograd.grad((y, last), [c[n] for n in names], (dy.to(DEV), dfinal.to(DEV)))
+    for n, a, b in zip(names, got, want):
+        inside = b.abs() < (65504 if a.dtype == F16 else 3e38)
+        _near("d" + n, torch.where(inside, a.detach().double().cpu(), 0), torch.where(inside, b, 0),
+              bound["d" + n], a.dtype)
