@@ -544,3 +544,54 @@ def test_gradients_of_saturated_gates(dtype, level):
         inside = b.abs() < (65504 if a.dtype == F16 else 3e38)
         _near("d" + n, torch.where(inside, a.detach().double().cpu(), 0), torch.where(inside, b, 0),
               bound["d" + n], a.dtype)
+
+
+# many workgroups: (batch, length, width) of over 2,048 tiles of 128 tokens (one counter for all
+# chains), over 2,048 of 64 only (the backward's alone), and few chains of over 64 links (the look-back's
+# window), with pairs of channels and single ones
+LONG = [(64, 4300, 6), (33, 8500, 7), (40, 3400, 66), (1, 8500, 130), (2, 9000, 33)]
+
+
+def _long(shape, dtype, form, **on):
+    """Channels that remember thousands of tokens, so that a wrong carry between tiles shows."""
+    case = _inputs(*shape, dtype, form, seed=19, **on)
+    if form == "gate":
+        case["rate"] = case["rate"] * 0.02
+    else:
+        case["decay"] = (case["decay"].float() * 0.02).to(dtype)
+    if case["reset"] is not None:
+        g = torch.Generator().manual_seed(8)
+        case["reset"] = torch.rand(shape[:2], generator=g) < 1e-3
+    return case
+
+
+@pytest.mark.parametrize("shape,dtype,form,options", [
+    *[(s, d, f, "all") for s in LONG for d, f in ((BF16, "gate"), (F32, "gate"), (F16, "given"))],
+    (LONG[0], BF16, "given", "plain"), (LONG[3], BF16, "gate", "plain"), (LONG[4], F32, "given", "plain")])
+def test_many_and_long_chains(shape, dtype, form, options):
+    """Outputs and gradients in 64 bits, token by token; two calls on two streams at once agree."""
+    case = _long(shape, dtype, form, **{o: options == "all" for o in ("state", "lengths", "reset")})
+    g = torch.Generator().manual_seed(9)
+    dy = torch.randn(shape, generator=g).to(dtype)
+    dfinal = torch.randn(shape[0], shape[2], generator=g)
+    names = [n for n in ("x", "decay", "gate", "rate", "state") if case[n] is not None]
+    wide = {n: v if n not in names else v.double().requires_grad_(True) for n, v in case.items()}
+    y64, f64 = og.scan(**wide)
+    want = torch.autograd.grad((y64, f64), [wide[n] for n in names], (dy.double(), dfinal.double()))
+    bound = og.bounds(**case, dy=dy, dfinal=dfinal)
+    c, dy, dfinal = _to(case), dy.to(DEV), dfinal.to(DEV)
+    torch.cuda.synchronize()
+    results = []
+    for stream in [torch.cuda.Stream() for _ in range(2)]:
+        with torch.cuda.stream(stream):
+            leaves = {n: c[n].detach().requires_grad_(True) for n in names}
+            y, last = _call(c | leaves)
+            results.append((y.detach(), last.detach(),
+                            *torch.autograd.grad((y, last), list(leaves.values()), (dy, dfinal))))
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(*results))
+    y, last, *got = results[0]
+    _near("y", y, y64.detach(), bound["y"], dtype)
+    _near("final", last, f64.detach(), bound["final"], F32)
+    for n, a, b in zip(names, got, want):
+        _near("d" + n, a, b, bound["d" + n], a.dtype)
