@@ -16,6 +16,7 @@ step / scan ran on the HIP path (the reference's ``_TRITON_LAST_DISPATCH`` /
 from __future__ import annotations
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _hip
 
@@ -60,6 +61,13 @@ def _require_inference(*tensors: torch.Tensor | None) -> None:
         raise RuntimeError(
             "mamba3_amd implements the inference hot path (forward, prefill, step) and has no "
             "backward; run it under torch.no_grad() or torch.inference_mode()")
+
+
+def _refuse_tangents(*tensors: torch.Tensor | None) -> None:
+    """Forward-mode derivatives, which need no ``requires_grad`` and outlast ``no_grad``, are refused
+    where they would be dropped (call it only inside a dual level)."""
+    if any([t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors]):
+        raise RuntimeError("mamba3_amd has no forward-mode derivatives")
 
 
 def _inner(t: torch.Tensor | None) -> torch.Tensor | None:
@@ -798,6 +806,8 @@ def linear4(x: torch.Tensor, weight: Weight4, residual: torch.Tensor | None = No
     ``norm_weight [K]`` (taken in ``x``'s dtype) ``x`` is first RMS-normalised, as
     ``F.rms_norm(x.float(), (K,), norm_weight.float(), norm_eps)``, its rows not rounded to 16 bits. An infinity in a row of ``x`` makes its row of the result NaN. No backward.
     """
+    if forward_ad._current_level >= 0:
+        _refuse_tangents(x, residual, norm_weight)
     index = x.get_device()
     if index < 0 or any([t is not None and t.get_device() != index
                          for t in (residual, out, norm_weight)]):
@@ -955,7 +965,7 @@ def gated_scan(x: torch.Tensor, decay: torch.Tensor, gate: torch.Tensor | None =
     first token of each document in a packed row does.
 
     Unlike the Mamba-3 calls of this module this one has a backward pass: gradients reach ``x``,
-    ``decay``, ``gate``, ``rate`` and ``initial_state`` (once: no second derivatives).
+    ``decay``, ``gate``, ``rate`` and ``initial_state`` (once: no second derivatives, none in forward mode).
     """
     if x.ndim != 3:
         raise ValueError("x must have shape [B, L, C]")
@@ -967,6 +977,8 @@ def gated_scan(x: torch.Tensor, decay: torch.Tensor, gate: torch.Tensor | None =
     if reset is not None and (reset.shape != (batch, length) or
                               reset.dtype not in (torch.bool, torch.uint8)):
         raise ValueError(f"reset must be bool of shape {(batch, length)}")
+    if forward_ad._current_level >= 0:
+        _refuse_tangents(x, decay, gate, rate, initial_state)
     index = x.get_device()
     if index < 0 or any([t is not None and t.get_device() != index for t in
                          (decay, gate, rate, initial_state, lengths, reset)]):
@@ -997,6 +1009,8 @@ def gated_step(x: torch.Tensor, decay: torch.Tensor, state: torch.Tensor,
     if x.ndim != 2:
         raise ValueError("x must have shape [B, C]")
     _validate_gated(x, decay, gate, rate, state, "state")
+    if forward_ad._current_level >= 0:
+        _refuse_tangents(x, decay, gate, rate, state)
     index = x.get_device()
     if index < 0 or decay.get_device() != index or state.get_device() != index or (
             gate is not None and not gate.get_device() == rate.get_device() == index):

@@ -205,3 +205,27 @@ def test_structs_match_the_header_layout(tmp_path):
             assert ctypes.sizeof(structs[cname]) == int(value)
         else:
             assert getattr(structs[cname], field).offset == int(value), (cname, field)
+
+
+def test_forward_mode_derivatives_are_refused():
+    """Not dropped: a dual tensor has no requires_grad."""
+    import torch.autograd.forward_ad as fwd
+    x, weight = _x(2, 8), _x(8)
+    with fwd.dual_level():
+        for at in range(4):
+            case = [_x(2, 4, 8), _x(2, 4, 8), _x(2, 4, 8), weight]
+            case[at] = fwd.make_dual(case[at], torch.ones_like(case[at]))
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                ops.gated_scan(*case)
+        dual = fwd.make_dual(x, x)
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            ops.gated_scan(_x(2, 4, 8), _x(2, 4, 8), initial_state=dual)
+        with torch.no_grad():
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                ops.gated_step(x, x, dual)
+            held = ops.Weight4(torch.zeros(4, 16, dtype=torch.uint8), _x(4, 1, dtype=torch.float16))
+            row = torch.zeros(1, 32, dtype=torch.float16)
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                ops.linear4(fwd.make_dual(row, row), held)
+            with pytest.raises(RuntimeError, match="ROCm devices only"):
+                ops.linear4(row, held)  # a tensor without a tangent is none of its business
