@@ -70,6 +70,13 @@ def _refuse_tangents(*tensors: torch.Tensor | None) -> None:
         raise RuntimeError("mamba3_amd has no forward-mode derivatives")
 
 
+def _written(t: torch.Tensor) -> None:
+    """Count a kernel's write into a caller's tensor, so that a backward pass that saved it (a
+    ``gated_scan``'s) is refused instead of reading the new values."""
+    if not t.is_inference():
+        torch.autograd.graph.increment_version(t)
+
+
 def _inner(t: torch.Tensor | None) -> torch.Tensor | None:
     """A view whose innermost axis has stride 1 (copy only when it does not)."""
     if t is None or t.dim() == 0 or t.shape[-1] <= 1 or t.stride(-1) == 1:
@@ -579,8 +586,8 @@ def linear(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor | None 
             raise ValueError(f"linear: norm_weight must be [{x.shape[1]}]")
         if norm_weight.data_ptr() % 16:
             norm_weight = norm_weight.clone()
-    residual = _inner(residual)
-    if out is None:
+    residual, given = _inner(residual), out is not None
+    if not given:
         out = torch.empty(m, n, dtype=x.dtype, device=device)
     elif out.stride(1) != 1:
         raise ValueError("linear: out needs a unit inner stride")
@@ -596,6 +603,8 @@ def linear(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor | None 
     ws = _hip.scan_workspace(args, device, "m3_linear_workspace_size")
     _hip.call("m3_linear", args, device)
     del ws
+    if given:
+        _written(out)
     return out
 
 
@@ -829,8 +838,8 @@ def linear4(x: torch.Tensor, weight: Weight4, residual: torch.Tensor | None = No
             norm_weight = norm_weight.detach().to(dtype)
         norm_weight = _aligned16(norm_weight)
     x = _aligned16(x)
-    residual = _inner(residual)
-    if out is None:
+    residual, given = _inner(residual), out is not None
+    if not given:
         out = x.new_empty((m, n))
     elif n > 1 and out.stride(1) != 1:
         raise ValueError("linear4: out needs a unit inner stride")
@@ -844,6 +853,8 @@ def linear4(x: torch.Tensor, weight: Weight4, residual: torch.Tensor | None = No
         *(none if norm_weight is None else (norm_weight.data_ptr(), code, 0, 1, 0, 0, 0, 0)),
         *(none if residual is None else (residual.data_ptr(), code, 0, *residual.stride(), 0, 0, 0)),
         out.data_ptr(), code, 0, *out.stride(), 0, 0, 0), index)
+    if given:
+        _written(out)
     return out
 
 
@@ -1042,6 +1053,8 @@ def gated_step(x: torch.Tensor, decay: torch.Tensor, state: torch.Tensor,
         out.data_ptr(), code, 0, width, 0, 1, 0, 0,
         new.data_ptr(), 0, 0, new.stride(0), 1, 0, 0, 0,
         *none, 0, 0), index)
+    if inplace:
+        _written(new)
     return out, new
 
 

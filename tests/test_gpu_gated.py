@@ -595,3 +595,29 @@ def test_many_and_long_chains(shape, dtype, form, options):
     _near("final", last, f64.detach(), bound["final"], F32)
     for n, a, b in zip(names, got, want):
         _near("d" + n, a, b, bound["d" + n], a.dtype)
+
+
+def test_a_state_updated_in_place_is_not_lost_on_autograd():
+    """A backward pass over an initial state that a step has since overwritten, or over an input
+    that a product has, is refused as torch refuses its own in-place writes."""
+    case = _to(_inputs(2, 30, 32, BF16, "gate", seed=20, state=True))
+    token = [case[n][:, 0].clone() for n in ("x", "decay", "gate")]
+    case["rate"].requires_grad_(True)
+    y, _ = _call(case)
+    with torch.no_grad():
+        ops.gated_step(token[0], token[1], case["state"], token[2], case["rate"].detach(), inplace=True)
+    with pytest.raises(RuntimeError, match="inplace"):
+        y.float().sum().backward()
+    wide = torch.randn(32, 32, device=DEV).to(BF16)
+    weight = ops.quantize4(wide, 32)
+    for product, w in ((ops.linear4, weight), (ops.linear, wide)):
+        x = torch.randn(2, 1, 32, device=DEV).to(BF16)
+        y, _ = ops.gated_scan(x, case["decay"][:, :1], case["gate"][:, :1], case["rate"])
+        with torch.no_grad():
+            product(token[0], w, out=x[:, 0])
+        with pytest.raises(RuntimeError, match="inplace"):
+            y.float().sum().backward()
+    with torch.inference_mode():  # tensors without versions are written all the same
+        state, out = torch.zeros(2, 32, device=DEV), torch.empty(2, 32, device=DEV, dtype=BF16)
+        assert ops.gated_step(*token[:2], state, inplace=True)[1] is state
+        assert ops.linear4(token[0], weight, out=out) is out
