@@ -879,6 +879,15 @@ def _validate_gated(x, decay, gate, rate, state, state_name) -> None:
 _NO_GATES = 2 * _hip.NO_TENSOR
 
 
+def _tokens(t: torch.Tensor | None) -> torch.Tensor | None:
+    """``[B, L, C]`` with a unit inner stride and tokens as near as the kernels' 32-bit offsets
+    ask (copied only if it has not)."""
+    t = _inner(t)
+    if t is None or t.stride(1) <= 1 << 24:
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
+
+
 def _rate32(rate: torch.Tensor | None) -> torch.Tensor | None:
     if rate is None or (rate.dtype == torch.float32 and rate.is_contiguous()):
         return rate
@@ -938,7 +947,7 @@ class _GatedScan(torch.autograd.Function):
         if dout is None and dfinal is None:
             return (None,) * 7
         code, none = _hip.dtype_code(x.dtype), _hip.NO_TENSOR
-        dout = x.new_zeros(x.shape) if dout is None else _inner(dout)
+        dout = x.new_zeros(x.shape) if dout is None else _tokens(dout)
         dfinal = _inner(dfinal)
         dx, ddecay = x.new_empty(x.shape), x.new_empty(x.shape)
         dgate = drate = dstate = None
@@ -1001,8 +1010,8 @@ def gated_scan(x: torch.Tensor, decay: torch.Tensor, gate: torch.Tensor | None =
         return x.clone(), final
     if lengths is not None and (lengths.dtype != torch.int32 or not lengths.is_contiguous()):
         lengths = lengths.clamp(0, length).to(torch.int32).contiguous()
-    x, decay, gate, state, reset = (_inner(x), _inner(decay), _inner(gate), _inner(initial_state),
-                                    _inner(reset))
+    x, decay, gate = _tokens(x), _tokens(decay), _tokens(gate)
+    state, reset = _inner(initial_state), _inner(reset)
     if torch.is_grad_enabled() and any([t is not None and t.requires_grad
                                         for t in (x, decay, gate, rate, state)]):
         return _GatedScan.apply(x, decay, gate, rate, state, lengths, reset)

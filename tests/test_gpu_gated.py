@@ -621,3 +621,28 @@ def test_a_state_updated_in_place_is_not_lost_on_autograd():
         state, out = torch.zeros(2, 32, device=DEV), torch.empty(2, 32, device=DEV, dtype=BF16)
         assert ops.gated_step(*token[:2], state, inplace=True)[1] is state
         assert ops.linear4(token[0], weight, out=out) is out
+
+
+def test_tokens_far_apart():
+    """Rows of one token far apart, and a gradient whose tokens are: as their contiguous copies."""
+    far = (1 << 24) + 8
+    case = _to(_inputs(2, 3, 32, BF16, "gate", seed=21))
+    buffer = torch.zeros(3 * far, device=DEV, dtype=BF16)
+    for n in ("x", "decay"):
+        view = buffer.as_strided((2, 3, 32), (64, far, 1), 0 if n == "x" else 128)
+        view.copy_(case[n])
+        case[n + "_far"] = view
+    x, decay = (case[n].requires_grad_(True) for n in ("x", "decay"))
+    dy = torch.randn(2, 3, 32, device=DEV).to(BF16)
+    dy_far = buffer.as_strided((2, 3, 32), (64, far, 1), 256)
+    dy_far.copy_(dy)
+    y, _ = ops.gated_scan(x, decay, case["gate"], case["rate"])
+    want = torch.autograd.grad(y, (x, decay), dy, retain_graph=True)
+    got = torch.autograd.grad(y, (x, decay), dy_far)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    with torch.inference_mode():
+        assert torch.equal(ops.gated_scan(case["x_far"], case["decay_far"], case["gate"],
+                                          case["rate"])[0], y)
+        one = ops.gated_scan(case["x_far"][:1, :1], case["decay_far"][:1, :1], case["gate"][:1, :1],
+                             case["rate"])[0]
+        assert torch.equal(one, y[:1, :1])
