@@ -914,6 +914,9 @@ def _gated_forward(x, decay, gate, rate, state, lengths, reset, want_carry):
     batch, length, width = x.shape
     device = x.device
     out = x.new_empty(x.shape)
+    if x.numel() == 0:
+        return out, (torch.zeros(batch, width, dtype=torch.float32, device=device)
+                     if state is None else state.clone()), None
     final = torch.empty((batch, width), dtype=torch.float32, device=device)
     carry = torch.empty((-(-length // _hip.GATED_TILE), batch, width), dtype=torch.float32,
                         device=device) if want_carry else None
@@ -946,6 +949,11 @@ class _GatedScan(torch.autograd.Function):
         x, decay, gate, rate, state, lengths, reset, carry = ctx.saved_tensors
         if dout is None and dfinal is None:
             return (None,) * 7
+        if x.numel() == 0:
+            if state is not None and dfinal is None:
+                dfinal = torch.zeros_like(state)
+            return (*(None if t is None else torch.zeros_like(t) for t in (x, decay, gate, rate)),
+                    None if state is None else dfinal, None, None)
         code, none = _hip.dtype_code(x.dtype), _hip.NO_TENSOR
         dout = x.new_zeros(x.shape) if dout is None else _tokens(dout)
         dfinal = _inner(dfinal)
@@ -1004,10 +1012,6 @@ def gated_scan(x: torch.Tensor, decay: torch.Tensor, gate: torch.Tensor | None =
                          (decay, gate, rate, initial_state, lengths, reset)]):
         _require_device(x, decay, gate, rate, initial_state, lengths, reset)
     rate = _rate32(rate)
-    if batch == 0 or length == 0 or width == 0:
-        final = (torch.zeros(batch, width, dtype=torch.float32, device=x.device)
-                 if initial_state is None else initial_state.clone())
-        return x.clone(), final
     if lengths is not None and (lengths.dtype != torch.int32 or not lengths.is_contiguous()):
         lengths = lengths.clamp(0, length).to(torch.int32).contiguous()
     x, decay, gate = _tokens(x), _tokens(decay), _tokens(gate)

@@ -646,3 +646,20 @@ def test_tokens_far_apart():
         one = ops.gated_scan(case["x_far"][:1, :1], case["decay_far"][:1, :1], case["gate"][:1, :1],
                              case["rate"])[0]
         assert torch.equal(one, y[:1, :1])
+
+
+@pytest.mark.parametrize("shape", [(2, 0, 8), (0, 5, 8), (2, 5, 0)])
+def test_gradients_without_tokens(shape):
+    """Every input that asks for a gradient gets one: the final state's for the initial one, else zeros."""
+    x, decay, gate = (torch.randn(shape, device=DEV, requires_grad=True) for _ in range(3))
+    rate = torch.rand(shape[2], device=DEV, requires_grad=True)
+    state = torch.randn(shape[0], shape[2], device=DEV, requires_grad=True)
+    y, last = ops.gated_scan(x, decay, gate, rate, initial_state=state)
+    assert torch.equal(last, state) and y.shape == x.shape
+    weigh = torch.randn_like(last)
+    grads = torch.autograd.grad((y, last), (x, decay, gate, rate, state), (torch.zeros_like(y), weigh))
+    for grad, t in zip(grads, (x, decay, gate, rate, state)):
+        assert grad.shape == t.shape and grad.dtype == t.dtype
+    assert not grads[3].any() and (shape[1] > 0 or torch.equal(grads[4], weigh))
+    y, _ = ops.gated_scan(x, decay, gate, rate, initial_state=state)
+    assert not torch.autograd.grad(y.sum(), state)[0].any()
