@@ -566,7 +566,8 @@ def _long(shape, dtype, form, **on):
 
 
 @pytest.mark.parametrize("shape,dtype,form,options", [
-    *[(s, d, f, "all") for s in LONG for d, f in ((BF16, "gate"), (F32, "gate"), (F16, "given"))],
+    *[(s, BF16, "gate", "all") for s in LONG],
+    *[(s, d, f, "all") for s, d, f in zip(LONG, (F32, F16, F32, F16, F32), ("gate", "given") * 3)],
     (LONG[0], BF16, "given", "plain"), (LONG[3], BF16, "gate", "plain"), (LONG[4], F32, "given", "plain")])
 def test_many_and_long_chains(shape, dtype, form, options):
     """Outputs and gradients in 64 bits, token by token; two calls on two streams at once agree."""
