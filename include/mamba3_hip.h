@@ -351,7 +351,8 @@ typedef struct {
   m3_tensor x;          /* [M, K], rows 16-byte aligned, 512 MB from first to last at most */
   m3_tensor norm_weight;/* [K] optional, 16-byte aligned */
   m3_tensor residual;   /* [M, N] optional */
-  m3_tensor out;        /* [M, N]; may not overlap x or the weight, may equal residual */
+  m3_tensor out;        /* [M, N]; may not overlap x, the weight or norm_weight, may equal
+                           residual */
 } m3_linear4_args;
 
 int m3_linear4(const m3_linear4_args* args, hipStream_t stream);

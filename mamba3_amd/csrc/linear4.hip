@@ -659,19 +659,24 @@ int validate(const m3_linear4_args& a) {
     return fail(M3_EUNSUPPORTED, "m3_linear4: x rows, norm_weight and codes must be 16-byte "
                 "aligned, scales 8-byte, zeros 4-byte");
   }
+  if (present(a.norm_weight) && !(a.norm_eps >= 0.f)) {
+    return fail(M3_EINVAL, "m3_linear4: norm_eps must be >= 0");
+  }
   // offsets within x, and within the tile rows of a workgroup, are 32-bit, in bytes
   if ((a.m - 1) * a.x.stride[0] + a.k >= (1 << 28)) {
     return fail(M3_EUNSUPPORTED, "m3_linear4: x spans over 512 MB");
   }
   if (a.m > 1 && a.out.stride[0] < a.n) return fail(M3_EINVAL, "m3_linear4: rows of out overlap");
-  const int64_t tiles = (a.n + 15) / 16 * ((a.k + 127) / 128);
+  const int64_t tiles = (a.n + 15) / 16 * ((a.k + 127) / 128), groups = tiles * (128 / a.group);
   const char* o0 = static_cast<const char*>(a.out.ptr);
   const char* o1 = o0 + ((a.m - 1) * a.out.stride[0] + a.n) * 2;
-  const char* x0 = static_cast<const char*>(a.x.ptr);
-  const char* c0 = static_cast<const char*>(a.codes);
-  if (!apart(o0, o1, x0, x0 + ((a.m - 1) * a.x.stride[0] + a.k) * 2) ||
-      !apart(o0, o1, c0, c0 + tiles * 1024)) {
-    return fail(M3_EINVAL, "m3_linear4: out overlaps x or the weight");
+  const auto meets = [&](const void* p, int64_t bytes) {
+    const char* p0 = static_cast<const char*>(p);
+    return p != nullptr && !apart(o0, o1, p0, p0 + bytes);
+  };
+  if (meets(a.x.ptr, ((a.m - 1) * a.x.stride[0] + a.k) * 2) || meets(a.codes, tiles * 1024) ||
+      meets(a.scales, groups * 32) || meets(a.zeros, groups * 16) || meets(a.norm_weight.ptr, a.k * 2)) {
+    return fail(M3_EINVAL, "m3_linear4: out overlaps x, the weight or norm_weight");
   }
   const char* r0 = static_cast<const char*>(a.residual.ptr);
   const bool same = r0 == o0 && (a.m == 1 || a.residual.stride[0] == a.out.stride[0]);

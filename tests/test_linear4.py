@@ -222,3 +222,21 @@ def test_struct_matches_the_header_layout(tmp_path):
         size = (ctypes.sizeof(_hip.Linear4Args) if field == "-"
                 else getattr(_hip.Linear4Args, field).offset)
         assert size == int(value), field
+
+
+def test_the_norm_s_epsilon_and_what_out_overlaps(lib):
+    call = lib.m3_linear4
+    for eps in (-1e-5, float("nan")):
+        args = _args()
+        args.norm_weight, args.norm_eps = _hip.Tensor(0x600000, _hip.BF16, 0, (1,)), eps
+        assert call(ctypes.byref(args), None) == 1 and b"norm_eps" in lib.m3_last_error()
+    # out [4, 64] bf16 over the last bytes of the scales (4 tile rows x 2 x 2 groups x 16, 512 bytes), the
+    # zeros (256 bytes) and the norm's weight (512)
+    for at, size in ((0x200000, 512), (0x300000, 256), (0x600000, 512)):
+        args = _args()
+        args.norm_weight = _hip.Tensor(0x600000, _hip.BF16, 0, (1,))
+        args.out.ptr = at + size - 2
+        assert call(ctypes.byref(args), None) == 1, hex(at)
+        assert b"out overlaps" in lib.m3_last_error()
+        args.out.ptr = at - (3 * 64 + 64) * 2 + 2
+        assert call(ctypes.byref(args), None) == 1, hex(at)
