@@ -275,8 +275,8 @@ int m3_rms_norm(const m3_rms_norm_args* args, hipStream_t stream);
  * lengths: row b holds max(0, min(lengths[b], L)) tokens; after them out is 0 and the state
  * stays, whatever x, decay and gate hold there. reset: a token whose byte is not 0 starts from
  * an empty state (what came before it, NaN and infinities too, is dropped).
- * rate >= 0; a negative one gives NaN. Tokens lie at most 2^24 elements apart; out overlaps nothing
- * else. With B, L or C 0 nothing is written.
+ * rate >= 0; a negative one gives NaN. L is at most 2^30, tokens lie at most 2^24 elements apart; out
+ * overlaps nothing else. With B, L or C 0 nothing is written.
  */
 #define M3_GATED_TILE 64 /* tokens between two of the states that carry holds */
 typedef struct {

@@ -878,6 +878,8 @@ int validate(const m3_gated_scan_args& a, bool backward) {
       return fail(M3_EUNSUPPORTED, "m3_gated_scan: tokens over 2^24 elements apart");
     }
   }
+  // more are over 2^23 tiles, and tiles and tokens are counted in 32 bits
+  if (a.length > (1 << 30)) return fail(M3_EUNSUPPORTED, "m3_gated_scan: length above 2^30");
   if (a.width > (1 << 27)) return fail(M3_EUNSUPPORTED, "m3_gated_scan: width above 2^27");
   // the lanes of a launch are counted in 32 bits
   if (static_cast<int64_t>(a.batch) * a.width >= INT32_MAX / 2) {

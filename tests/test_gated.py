@@ -229,3 +229,17 @@ def test_forward_mode_derivatives_are_refused():
                 ops.linear4(fwd.make_dual(row, row), held)
             with pytest.raises(RuntimeError, match="ROCm devices only"):
                 ops.linear4(row, held)  # a tensor without a tangent is none of its business
+
+
+@pytest.mark.parametrize("length", [(1 << 30) + 1, (1 << 31) - 127, (1 << 31) - 1])
+def test_a_length_beyond_the_tiles_of_a_grid(lib, length):
+    """Refused as such: rounding it up to whole tiles would leave 32 bits."""
+    size = ctypes.c_size_t(0)
+    args = _scan_args(batch=1, width=1)
+    args.length = length
+    assert lib.m3_gated_scan_workspace_size(ctypes.byref(args), ctypes.byref(size)) == 2
+    assert b"2^30" in lib.m3_last_error()
+    assert lib.m3_gated_scan(ctypes.byref(args), None) == 2
+    back = _hip.GatedScanBwdArgs(args)
+    assert lib.m3_gated_scan_bwd_workspace_size(ctypes.byref(back), ctypes.byref(size)) == 2
+    assert b"2^30" in lib.m3_last_error()
