@@ -716,6 +716,8 @@ class Weight4:
             raise ValueError("zeros must be uint8 of the scales' shape")
         if any(t is not None and t.device != packed.device for t in (scales, zeros)):
             raise ValueError("packed, scales and zeros must be on the same device")
+        if zeros is not None and bool((zeros > 15).any()):
+            raise ValueError("zeros must be codes, 0 to 15")
         self.shape, self.group, self.device = (n, k), group, packed.device
         self.dtype = scales.dtype
         tn, tk = -(-n // 16), -(-k // 128)
@@ -727,7 +729,7 @@ class Weight4:
         codes = codes.reshape(tn, tk, 64, 4, 8)
         self.codes = (codes[..., 0::2] | codes[..., 1::2] << 4).contiguous()
         self.scales = self._tiles(scales, tn, tk)
-        self.zeros = None if zeros is None else self._tiles(zeros.clamp(max=15), tn, tk)
+        self.zeros = None if zeros is None else self._tiles(zeros, tn, tk)
 
     def _tiles(self, t: torch.Tensor, tn: int, tk: int) -> torch.Tensor:
         per = 128 // self.group

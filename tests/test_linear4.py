@@ -240,3 +240,14 @@ def test_the_norm_s_epsilon_and_what_out_overlaps(lib):
         assert b"out overlaps" in lib.m3_last_error()
         args.out.ptr = at - (3 * 64 + 64) * 2 + 2
         assert call(ctypes.byref(args), None) == 1, hex(at)
+
+
+@pytest.mark.parametrize("group", [32, 64, 128])
+def test_zeros_above_a_code_are_refused(group):
+    """Not held as 15: a format whose zeros are off by one (1..16) would lose weight unnoticed."""
+    packed, scales, z = _parts(20, 256, group)
+    z[3, -1] = 16
+    with pytest.raises(ValueError, match="zeros must be .* 0 to 15"):
+        ops.Weight4(packed, scales, z)
+    z[3, -1] = 15
+    assert ops.Weight4(packed, scales, z).zeros.max() <= 15
