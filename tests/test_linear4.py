@@ -251,3 +251,14 @@ def test_zeros_above_a_code_are_refused(group):
         ops.Weight4(packed, scales, z)
     z[3, -1] = 15
     assert ops.Weight4(packed, scales, z).zeros.max() <= 15
+
+
+
+def test_quantize_decode_of_a_shared_weight():
+    model = Mamba3(64, depth=3).to(torch.bfloat16)
+    model.layers[2].mixer.in_proj.weight = model.layers[0].mixer.in_proj.weight
+    model.quantize_decode(32)
+    for layer in model.layers:
+        for name in ("in_proj", "out_proj"):
+            assert torch.equal(layer.mixer._weight4(name).dequantize(torch.bfloat16),
+                               getattr(layer.mixer, name).weight)
