@@ -124,13 +124,9 @@ class _Mamba3Mixer(nn.Module):
         self._decode4: dict[str, tuple[ops.Weight4, tuple[object, ...]]] = {}
 
     def _hold4(self, held: dict[str, ops.Weight4]) -> None:
-        """Take 4-bit copies of the projections, and their values for the weights."""
-        layers = {name: getattr(self, name) for name in held}
-        with torch.no_grad():
-            for name, layer in layers.items():
-                layer.weight.copy_(held[name].dequantize(layer.weight.dtype))
-        self._decode4 = {name: (held[name], _storage_signature(layer.weight))
-                         for name, layer in layers.items()}
+        """Take 4-bit copies of the projections, whose values the weights hold by now."""
+        self._decode4 = {name: (copy, _storage_signature(getattr(self, name).weight))
+                         for name, copy in held.items()}
 
     def _weight4(self, name: str) -> ops.Weight4 | None:
         """The projection's 4-bit copy, if there is one; refused once the weight has changed."""
@@ -459,6 +455,12 @@ class Mamba3(nn.Module):
         # all of them before any weight changes: one that holds NaN is refused
         held = [{name: ops.quantize4(getattr(layer.mixer, name).weight, group, zeros=zeros)
                  for name in ("in_proj", "out_proj")} for layer in self.layers]
+        with torch.no_grad():
+            for layer, copies in zip(self.layers, held):
+                for name, copy in copies.items():
+                    weight = getattr(layer.mixer, name).weight
+                    weight.copy_(copy.dequantize(weight.dtype))
+        # once every weight is written: layers may share one
         for layer, copies in zip(self.layers, held):
             layer.mixer._hold4(copies)
         return self

@@ -262,3 +262,15 @@ def test_quantize_decode_of_a_shared_weight():
         for name in ("in_proj", "out_proj"):
             assert torch.equal(layer.mixer._weight4(name).dequantize(torch.bfloat16),
                                getattr(layer.mixer, name).weight)
+
+
+
+def test_quantize_decode_writes_no_infinity():
+    """7 codes times the rounded scale of f16's largest value are above it."""
+    model = Mamba3(64, depth=2).half()
+    with torch.no_grad():
+        model.layers[1].mixer.out_proj.weight[0, 0] = 65504.0
+    before = {k: v.clone() for k, v in model.state_dict().items()}
+    with pytest.raises(ValueError, match="beyond"):
+        model.quantize_decode(32, zeros=False)
+    assert all(torch.equal(v, before[k]) for k, v in model.state_dict().items())
