@@ -452,9 +452,14 @@ class Mamba3(nn.Module):
                 if group not in ops.LINEAR4_GROUPS or weight.shape[1] % group != 0:
                     raise ValueError(f"group must be 32, 64 or 128 and divide {name}'s "
                                      f"{weight.shape[1]} columns")
-        # all of them before any weight changes: one that holds NaN is refused
+        # all of them before any weight changes: one that holds NaN or rounds to infinity is refused
         held = [{name: ops.quantize4(getattr(layer.mixer, name).weight, group, zeros=zeros)
                  for name in ("in_proj", "out_proj")} for layer in self.layers]
+        for layer, copies in zip(self.layers, held):
+            for name, copy in copies.items():
+                dtype = getattr(layer.mixer, name).weight.dtype
+                if not bool(torch.isfinite(copy.dequantize(dtype)).all()):
+                    raise ValueError(f"quantize_decode: {name}'s rounded values are beyond {dtype}")
         with torch.no_grad():
             for layer, copies in zip(self.layers, held):
                 for name, copy in copies.items():
