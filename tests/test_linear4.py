@@ -274,3 +274,14 @@ def test_quantize_decode_writes_no_infinity():
     with pytest.raises(ValueError, match="beyond"):
         model.quantize_decode(32, zeros=False)
     assert all(torch.equal(v, before[k]) for k, v in model.state_dict().items())
+
+
+def test_quantize_decode_without_versions_changes_nothing():
+    """Weights made under inference_mode have no version by which a later change would show."""
+    with torch.inference_mode():
+        model = Mamba3(64, depth=2).to(torch.bfloat16)
+        before = {k: v.clone() for k, v in model.state_dict().items()}
+        with pytest.raises(ValueError, match="inference_mode"):
+            model.quantize_decode(32)
+        assert all(torch.equal(v, before[k]) for k, v in model.state_dict().items())
+    assert not any(layer.mixer._decode4 for layer in model.layers)
