@@ -446,9 +446,11 @@ class Mamba3(nn.Module):
                 weight = getattr(layer.mixer, name).weight
                 if weight.dtype not in (torch.bfloat16, torch.float16):
                     raise ValueError("quantize_decode needs bfloat16 or float16 weights")
-                if weight.is_inference():
-                    raise ValueError("quantize_decode needs weights that count their changes, not ones "
-                                     "made under torch.inference_mode()")
+                try:
+                    weight._version
+                except RuntimeError as error:
+                    raise ValueError("quantize_decode needs weights that count their changes, not "
+                                     "ones made under torch.inference_mode()") from error
                 if group not in ops.LINEAR4_GROUPS or weight.shape[1] % group != 0:
                     raise ValueError(f"group must be 32, 64 or 128 and divide {name}'s "
                                      f"{weight.shape[1]} columns")
