@@ -235,7 +235,8 @@ class _Mamba3Mixer(nn.Module):
         small = rows.shape[0] <= ops.DECODE_LINEAR_ROWS
         supported = ops.linear_norm_supported if norm is not None else ops.linear_supported
         in4, out4 = self._weight4("in_proj"), self._weight4("out_proj")
-        if small and in4 is not None and ops.linear4_supported(rows, in4):
+        if (small and in4 is not None and rows.dtype == self.in_proj.weight.dtype
+                and ops.linear4_supported(rows, in4)):
             proj = ops.linear4(rows, in4, norm_weight=norm.weight if norm is not None else None,
                                norm_eps=norm.eps if norm is not None else ops.NORM_EPS)
             proj = proj.unsqueeze(1)

@@ -401,3 +401,14 @@ def test_every_form_of_the_kernels(m, n, k, group, norm, dtype, scale_dtype):
         spoilt = ops.linear4(bad, weight, res.to(DEV), norm_weight=dev)
     keep = [i for i in range(m) if i != m // 2]
     assert torch.equal(got[keep], spoilt[keep]) and torch.isnan(spoilt[m // 2]).all()
+
+
+def test_a_step_in_another_type_than_the_weights_is_refused():
+    """As without 4-bit copies: rows of the other 16-bit type do not run on them."""
+    model = Mamba3(256, d_state=128, depth=1).eval().to(DEV, F16)
+    x = torch.zeros(1, 1, 256, device=DEV, dtype=BF16)
+    with torch.inference_mode():
+        for _ in range(2):
+            with pytest.raises(RuntimeError):
+                model.step(x, None)
+            model.quantize_decode()
