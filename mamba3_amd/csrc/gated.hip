@@ -859,11 +859,6 @@ __global__ __launch_bounds__(1024) void gated_rate_kernel(const float* part, flo
 
 // ----------------------------------------------------------------------------- host
 
-int check_rows(const m3_tensor& t, const char* name, int dims, int64_t inner, bool required,
-               int dtype) {
-  return check_tensor(t, name, dims, inner, required, dtype);
-}
-
 int validate(const m3_gated_scan_args& a, bool backward) {
   if (a.batch < 0 || a.length < 0 || a.width < 0) {
     return fail(M3_EINVAL, "m3_gated_scan: negative dimensions");
@@ -888,14 +883,14 @@ int validate(const m3_gated_scan_args& a, bool backward) {
   }
   const bool live = a.batch > 0 && a.length > 0 && a.width > 0;
   int rc;
-  if ((rc = check_rows(a.x, "x", 3, a.width, live, a.dtype)) ||
-      (rc = check_rows(a.decay, "decay", 3, a.width, live, a.dtype)) ||
-      (rc = check_rows(a.gate, "gate", 3, a.width, false, a.dtype)) ||
-      (rc = check_rows(a.rate, "rate", 1, a.width, false, M3_F32)) ||
-      (rc = check_rows(a.initial_state, "initial_state", 2, a.width, false, M3_F32)) ||
-      (rc = check_rows(a.carry, "carry", 3, a.width, false, M3_F32)) ||
-      (!backward && ((rc = check_rows(a.out, "out", 3, a.width, live, a.dtype)) ||
-                     (rc = check_rows(a.final_state, "final_state", 2, a.width, live, M3_F32))))) {
+  if ((rc = check_tensor(a.x, "x", 3, a.width, live, a.dtype)) ||
+      (rc = check_tensor(a.decay, "decay", 3, a.width, live, a.dtype)) ||
+      (rc = check_tensor(a.gate, "gate", 3, a.width, false, a.dtype)) ||
+      (rc = check_tensor(a.rate, "rate", 1, a.width, false, M3_F32)) ||
+      (rc = check_tensor(a.initial_state, "initial_state", 2, a.width, false, M3_F32)) ||
+      (rc = check_tensor(a.carry, "carry", 3, a.width, false, M3_F32)) ||
+      (!backward && ((rc = check_tensor(a.out, "out", 3, a.width, live, a.dtype)) ||
+                     (rc = check_tensor(a.final_state, "final_state", 2, a.width, live, M3_F32))))) {
     return rc;
   }
   if (present(a.carry) && (a.carry.stride[1] != a.width ||
@@ -1085,13 +1080,13 @@ int validate_bwd(const m3_gated_scan_bwd_args& a) {
   int rc;
   if ((rc = validate(f, true))) return rc;
   const bool live = !nothing(f), gate = present(f.gate);
-  if ((rc = check_rows(a.dout, "dout", 3, f.width, live, f.dtype)) ||
-      (rc = check_rows(a.dfinal, "dfinal", 2, f.width, false, M3_F32)) ||
-      (rc = check_rows(a.dx, "dx", 3, f.width, live, f.dtype)) ||
-      (rc = check_rows(a.ddecay, "ddecay", 3, f.width, live, f.dtype)) ||
-      (rc = check_rows(a.dgate, "dgate", 3, f.width, live && gate, f.dtype)) ||
-      (rc = check_rows(a.drate, "drate", 1, f.width, live && gate, M3_F32)) ||
-      (rc = check_rows(a.dinitial, "dinitial", 2, f.width, false, M3_F32))) {
+  if ((rc = check_tensor(a.dout, "dout", 3, f.width, live, f.dtype)) ||
+      (rc = check_tensor(a.dfinal, "dfinal", 2, f.width, false, M3_F32)) ||
+      (rc = check_tensor(a.dx, "dx", 3, f.width, live, f.dtype)) ||
+      (rc = check_tensor(a.ddecay, "ddecay", 3, f.width, live, f.dtype)) ||
+      (rc = check_tensor(a.dgate, "dgate", 3, f.width, live && gate, f.dtype)) ||
+      (rc = check_tensor(a.drate, "drate", 1, f.width, live && gate, M3_F32)) ||
+      (rc = check_tensor(a.dinitial, "dinitial", 2, f.width, false, M3_F32))) {
     return rc;
   }
   for (const m3_tensor* t : {&a.dout, &a.dx, &a.ddecay, &a.dgate}) {
