@@ -14,8 +14,8 @@
 // an LDS region of the wave's own, where it is normed, and comes back as the operand's columns. Bound by
 // the weight's stream where it is long, else by the launch and one latency of memory: in graphs with
 // cold weights 28672 x 8192 at 1 row 27.1 us (4.5 TB/s; a large copy reaches 4.8), 8672 x 2048 at 1 row 4.9
-// us, 6.7 with the norm, 2048 x 4096 at 16 rows 5.6 us (512 x 512: 2.4 us). A second row for the norm costs nothing
-// where matrix rows are idle (8672 x 2048 at 4 rows 6.9 us either way), else its instructions: 16 rows 11.8 us
+// us, 6.7 with the norm, 2048 x 4096 at 16 rows 5.5 us (512 x 512: 2.4 us). A second row for the norm costs nothing
+// where matrix rows are idle (8672 x 2048 at 4 rows 6.9 us either way), else its instructions: 16 rows 10.6 us
 // with whole products, 9.0 with rounded ones.
 //
 // linear4_wide_kernel (more rows of both): below.
@@ -353,8 +353,8 @@ __global__ __launch_bounds__(64 * WAVES) void linear4_kernel(const Lin4Geom g) {
 // LDS buffers; x comes from memory three tiles ahead of its use, the codes two. Wave w forms X of the next
 // tile for x block w, and a group's sums begin at -(16 + z) X. KS = 2: two such teams, every other tile of
 // columns each, for two waves a SIMD where one workgroup fills a CU.
-// Bound by latency and issue together: 28672 x 8192 at 64 rows takes 55 us (2.3 TB/s of weights, 545
-// TFLOP/s); with both kinds of load left out 49, with LDS reads, dequantising and scaling left out too 35, of which the
+// Bound by latency and issue together: 28672 x 8192 at 64 rows takes 55 to 59 us with cold weights (2.1 TB/s
+// of them, 530 TFLOP/s), 50 where two of them lie in the last cache in turn; with both kinds of load left out 49, with LDS reads, dequantising and scaling left out too 35, of which the
 // matrix instructions are 18 and the rest barriers, staging and addresses (213 vector and 36 matrix
 // instructions a tile of columns). Sums that begin at -(16 + z) X need no pass over X afterwards: 191 became
 // 213 at groups of 128, which costs nothing there, and groups of 32 no longer spill (28672 x 4096 at 64 rows:
@@ -708,31 +708,39 @@ int launch_wide(const Lin4Geom& g, hipStream_t stream) {
 }
 
 // Up to 16 rows of x, by tile rows of W (us in graphs with cold weights; WAVES x TN):
-//   few (2048 x 4096, 16 rows): 8 x 1 5.2, 16 x 1 5.7, 4 x 1 6.9, 4 x 2 8.7
-//   542 (8672 x 2048, 1 row): 4 x 1 5.6, 4 x 2 5.7, 8 x 1 6.4; with the norm, formed once a
-//     workgroup, 4 x 2 8.0, 4 x 1 8.2, 8 x 1 8.8
-//   1792 (28672 x 8192, 16 rows): 4 x 4 28.2, 4 x 2 33.3, 8 x 1 43.2; in groups of 32, whose scales
-//     fill the registers, 4 x 1 28.2, 4 x 4 35.2
-// More rows: few tile rows keep the split over columns (2048 x 4096, 64 rows: 7.9 us in blocks of 32, 12.7 in
-// blocks of 64, 21.5 wide). Else the wide kernel in the form whose rounds of workgroups over the 256 CUs cost
-// least: 65 a round with 2 tile rows a wave, 44 with 1 (both one workgroup a CU), 87 for 512
-// workgroups of one team (two a CU): 28672 x 8192 at 64 rows 55 / 71 / 68 us, 16384 x 4096 27 / 20 / 26, 8672 x 2048
-// at 256 rows 31 / 31 / 23; in groups of 32 28672 x 4096 at 64 rows 40 / 47 / 44.
-template <typename T, typename S, int GPT, int MT, bool NORM>
+//   few (2048 x 4096, 16 rows): 8 x 1 5.5, 4 x 1 7.9, 4 x 2 8.8, 4 x 4 10.8
+//   542 (8672 x 2048), 1 row: 4 x 1 4.9, 4 x 2 5.4, 8 x 1 5.6; 16 rows: 6.4, 6.9, 7.6. With the norm, formed
+//     once a workgroup, 4 x 2 6.6, 4 x 1 6.6, 8 x 1 7.4 at 1 row and 10.5, 11.1, 12.3 at 16, in two
+//     workgroups of 8 rows; one of 16 rows takes 11.8
+//   1792 (28672 x 8192), 16 rows: 4 x 4 30, 4 x 2 35, 4 x 1 46, 8 x 1 44; with the norm, the weight read once
+//     for 16 rows, 49, and twice for 8 each 62. In groups of 32, whose scales fill the registers, 4 x 1 54, 8 x 1
+//     53, 4 x 2 56, 4 x 4 76
+// More rows: few tile rows keep the split over columns (2048 x 4096, 64 rows: 7.2 us in blocks of 32, 18 and
+// more wide). Else the wide kernel in the form whose rounds of workgroups over the 256 CUs cost least: 65
+// a round with 2 tile rows a wave, 44 with 1 (both one workgroup a CU), 87 for 512 workgroups of one team
+// (two a CU): 28672 x 8192 at 64 rows 57 / 68 / 65 us, 16384 x 4096 27 / 20 / 26, 8672 x 2048 at 256 rows
+// 31 / 31 / 23 and at 64 rows 16.5 / 11.8 / 14.7, with the norm 18.9 / 25.6 / 21.8; in groups of 32 28672 x 4096 at
+// 64 rows 39 / 47 / 44. Between 384 and 1,023 tile rows at up to 32 rows of x the split over columns would be
+// quicker (8672 x 2048: 8.6 at 17 rows and 9.7 at 32, against 10.8 and 11.0); it is slower with the norm (14.8 and
+// 18.3 against 13.7 and 13.9) and from 64 rows on.
+template <typename T, typename S, int GPT, bool NORM>
 int launch_few(const Lin4Geom& g, hipStream_t stream) {
-  if (g.tiles < 384) return launch_kernel<T, S, GPT, MT, 1, 8, NORM>(g, stream);
-  if constexpr (GPT < 4) {
-    if (g.tiles >= 1024) return launch_kernel<T, S, GPT, MT, 4, 4, NORM>(g, stream);
+  if (g.tiles < 384) return launch_kernel<T, S, GPT, 1, 1, 8, NORM>(g, stream);
+  if (g.tiles >= 1024) {
+    constexpr int tn = GPT < 4 ? 4 : 1;
+    if constexpr (NORM) {
+      if (g.m > 8) return launch_kernel<T, S, GPT, 2, tn, 4, true>(g, stream);
+    }
+    return launch_kernel<T, S, GPT, 1, tn, 4, NORM>(g, stream);
   }
-  return launch_kernel<T, S, GPT, MT, NORM && GPT < 4 ? 2 : 1, 4, NORM>(g, stream);
+  return launch_kernel<T, S, GPT, 1, NORM && GPT < 4 ? 2 : 1, 4, NORM>(g, stream);
 }
 
 template <typename T, typename S, int GPT>
 int launch_rows(const Lin4Geom& g, hipStream_t stream) {
   const bool norm = g.nw != nullptr;
   if (g.m <= 16) {
-    if (!norm) return launch_few<T, S, GPT, 1, false>(g, stream);
-    return g.m <= 8 ? launch_few<T, S, GPT, 1, true>(g, stream) : launch_few<T, S, GPT, 2, true>(g, stream);
+    return norm ? launch_few<T, S, GPT, true>(g, stream) : launch_few<T, S, GPT, false>(g, stream);
   }
   if (g.tiles < 384 && g.tiles * ((g.m + 63) / 64) < 512) {
     return norm ? launch_kernel<T, S, GPT, 2, 1, 8, true>(g, stream)
