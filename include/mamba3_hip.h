@@ -222,7 +222,8 @@ int m3_step(const m3_step_args* args, hipStream_t stream);
  * reference's plugin hooks: it replaces the block's RMSNorm, the in_proj / out_proj nn.Linear
  * calls and the residual add of a decode step (mamba3/model.py:441-458, 514-520), where a
  * general GEMM leaves most of the GPU idle.
- * K is a multiple of 32; x and weight rows are 16-byte aligned. The split of K over workgroups
+ * K is a multiple of 32; x and weight rows are 16-byte aligned. With the norm x * norm_weight is rounded to
+ * x's dtype before the division by the RMS: in f16 it has to stay below 65504. The split of K over workgroups
  * keeps FP32 partial sums in the caller's workspace (m3_linear_workspace_size, 0 when unsplit).
  */
 typedef struct {
@@ -270,12 +271,17 @@ int m3_rms_norm(const m3_rms_norm_args* args, hipStream_t stream);
  *   given form (no gate, no rate):  h_t = exp(decay_t) h_{t-1} + x_t
  *   gate form (gate and rate):      log a_t = -rate sigmoid(decay_t)
  *                                   h_t = a_t h_{t-1} + sqrt(1 - a_t^2) sigmoid(gate_t) x_t
+ * The gate form is the real-gated linear recurrent unit (RG-LRU; De et al., 2024) but for the tokens that
+ * begin a sequence, first ones and reset ones: its published implementation leaves the factor
+ * sqrt(1 - a_t^2) out there, this one has it at every token.
  * out_t = h_t in the activation dtype. length 1 is a decode step; final_state may then (and at
  * any length) be initial_state itself.
  * lengths: row b holds max(0, min(lengths[b], L)) tokens; after them out is 0 and the state
  * stays, whatever x, decay and gate hold there. reset: a token whose byte is not 0 starts from
  * an empty state (what came before it, NaN and infinities too, is dropped).
- * rate >= 0; a negative one gives NaN. L is at most 2^30, tokens lie at most 2^24 elements apart; out
+ * Log decays <= 0: factors of up to 128 tokens are multiplied before they meet a state, so that positive
+ * ones can give NaN where the recurrence is finite. An infinite state or input, likewise, can be NaN in the
+ * tokens after it. rate >= 0; a negative one gives NaN. L is at most 2^30, tokens lie at most 2^24 elements apart; out
  * overlaps nothing else. With B, L or C 0 nothing is written.
  */
 #define M3_GATED_TILE 64 /* tokens between two of the states that carry holds */

@@ -562,8 +562,8 @@ def linear(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor | None 
     ``out`` are ``[M, N]`` of that dtype. Products accumulate in FP32; the residual is added
     to the FP32 sum, which is rounded once. With ``norm_weight`` (``[K]``; ``M <= 32``, or
     ``M <= 64`` with K a multiple of 256) ``x`` is first RMS-normalised, as
-    ``F.rms_norm(x, (K,), norm_weight, norm_eps)``. This replaces
-    the decode step's RMSNorm, ``in_proj`` / ``out_proj`` calls and the block's residual add
+    ``F.rms_norm(x, (K,), norm_weight, norm_eps)``, with ``x * norm_weight`` rounded to ``x``'s
+    dtype before the division (in float16 it has to stay below 65504). This replaces the decode step's RMSNorm, ``in_proj`` / ``out_proj`` calls and the block's residual add
     (reference ``model.py:441-458, 514-520``).
     """
     device = _require_device(x, weight, residual, out, norm_weight)
@@ -983,8 +983,9 @@ def gated_scan(x: torch.Tensor, decay: torch.Tensor, gate: torch.Tensor | None =
                lengths: torch.Tensor | None = None, reset: torch.Tensor | None = None):
     """A gated linear recurrence over ``[B, L, C]``, one FP32 state per channel (``m3_gated_scan``).
 
-    Without ``gate`` and ``rate``, ``decay`` holds log decays: ``h_t = exp(decay_t) h_{t-1} +
-    x_t``. With them ``decay`` and ``gate`` hold logits and ``rate [C]`` (>= 0) the log decay of an
+    Without ``gate`` and ``rate``, ``decay`` holds log decays, at most 0 (factors are multiplied over
+    tiles of tokens, so positive ones can give NaN where the recurrence is finite): ``h_t =
+    exp(decay_t) h_{t-1} + x_t``. With them ``decay`` and ``gate`` hold logits and ``rate [C]`` (>= 0) the log decay of an
     open gate: ``a_t = exp(-rate sigmoid(decay_t))``, ``h_t = a_t h_{t-1} + sqrt(1 - a_t^2)
     sigmoid(gate_t) x_t``. ``x``, ``decay`` and ``gate`` share one dtype and may be slices of one
     projection. Returns ``(out [B, L, C] = h in x's dtype, final_state [B, C] FP32)``.
@@ -992,7 +993,9 @@ def gated_scan(x: torch.Tensor, decay: torch.Tensor, gate: torch.Tensor | None =
     ``initial_state [B, C]`` FP32 continues a sequence. ``lengths [B]`` (integers; clamped to 0..L)
     ends each row of a padded batch: past its end ``out`` is 0 and the state stays, whatever the
     padding holds. ``reset [B, L]`` (bool) marks tokens that start from an empty state, as the
-    first token of each document in a packed row does.
+    first token of each document in a packed row does. The gate form is the RG-LRU recurrence, except
+    that the published one drops the factor ``sqrt(1 - a_t^2)`` at tokens that begin a sequence (the
+    first and reset ones); here they have it too.
 
     Unlike the Mamba-3 calls of this module this one has a backward pass: gradients reach ``x``,
     ``decay``, ``gate``, ``rate`` and ``initial_state`` (once: no second derivatives, none in forward mode).
