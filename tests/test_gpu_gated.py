@@ -549,7 +549,7 @@ def test_gradients_of_saturated_gates(dtype, level):
 # many workgroups: (batch, length, width) of over 2,048 tiles of 128 tokens (one counter for all
 # chains), over 2,048 of 64 only (the backward's alone), and few chains of over 64 links (the look-back's
 # window), with pairs of channels and single ones
-LONG = [(64, 4300, 6), (33, 8500, 7), (40, 3400, 66), (1, 8500, 130), (2, 9000, 33)]
+LONG = [(64, 4300, 6), (33, 8500, 7), (40, 3400, 10), (1, 8500, 130), (2, 9000, 33)]
 
 
 def _long(shape, dtype, form, **on):
