@@ -24,7 +24,7 @@
 //
 // Measured in bf16, gate form (a large copy reaches 4.8 TB/s): 8 x 8192 x 2048 padded prompts 183 us
 // (4.8 TB/s of what is read and written), one row of 65536 x 1536 179 us (4.5 TB/s), 1777 x 4096 20 us; forward
-// and backward of 8 x 4096 x 2048 123 + 242 us (4.4 and 3.9 TB/s).
+// and backward of 8 x 4096 x 2048 125 + 264 us (medians of a trace: 4.3 and 3.6 TB/s).
 #include <hip/hip_runtime.h>
 
 #include "m3_common.hpp"
