@@ -314,8 +314,9 @@ int m3_gated_scan(const m3_gated_scan_args* args, hipStream_t stream);
  *   given form: dx = D, ddecay = D a h_{t-1}
  *   gate form:  dx = D s q, dgate = D s x q (1 - q), with p, q the gates' sigmoids, s = sqrt(1 - a^2);
  *               ddecay = -rate p (1 - p) dlog, drate = -sum p dlog,
- *               dlog = D (a h_{t-1} - q x a^2 / s)
- * Tokens past a row's length get gradient 0. drate is summed in a fixed order.
+ *               dlog = D (a h_{t-1} - q x a^2 / s), with 1 / s taken as 0 where s is 0
+ * At a reset token h_{t-1} is 0 and nothing passes to the token before. Tokens past a row's length get
+ * gradient 0. drate is summed in a fixed order. What is written overlaps nothing else.
  */
 typedef struct {
   m3_gated_scan_args fwd;
@@ -335,7 +336,8 @@ int m3_gated_scan_bwd(const m3_gated_scan_bwd_args* args, hipStream_t stream);
  *   W[n, k] = (q[n, k] - z[n, k / group]) * scale[n, k / group],  q, z in 0..15,
  * x' and the residual as in m3_linear (M <= 256, FP32 accumulation, one rounding; the norm at any
  * M). x * norm_weight is held in two bf16 values, whole for bf16 and to 2^-17 of itself for f16, in
- * FP32's range, and 1 / rms meets the FP32 sums. group is 32, 64 or 128, K a multiple of 32 and of group. No counterpart in the reference.
+ * FP32's range, and 1 / rms meets the FP32 sums. group is 32, 64 or 128, K a multiple of 32 and of
+ * group. No counterpart in the reference.
  * The weight is laid out once, for reads of 1 KB by a wave, in tiles of 16 rows x 128 columns
  * (rows and columns past N and K: code 0, scale 0, zero 0), TK = ceil(K / 128) of them a tile row:
  *   codes [ceil(N / 16), TK, 64, 4] 32-bit words: word i of lane l holds row l % 16, columns

@@ -354,12 +354,13 @@ __global__ __launch_bounds__(64 * WAVES) void linear4_kernel(const Lin4Geom g) {
 // tile for x block w, and a group's sums begin at -(16 + z) X. KS = 2: two such teams, every other tile of
 // columns each, for two waves a SIMD where one workgroup fills a CU.
 // Bound by latency and issue together: 28672 x 8192 at 64 rows takes 54 to 59 us in graphs, with cold and
-// with cached weights (2.1 TB/s of them, 530 TFLOP/s), and 50 timed call by call; with both kinds of load left out 49, with LDS reads, dequantising and scaling left out too 35, of which the
-// matrix instructions are 18 and the rest barriers, staging and addresses (213 vector and 36 matrix
-// instructions a tile of columns). Sums that begin at -(16 + z) X need no pass over X afterwards: 191 became
-// 213 at groups of 128, which costs nothing there, and groups of 32 no longer spill (28672 x 4096 at 64 rows:
-// 51 -> 40 us). Tried without gain: deeper rings, operands expanded or read a step earlier, set mixes of
-// matrix and vector instructions, 4 tile rows a wave.
+// with cached weights (2.1 TB/s of them, 530 TFLOP/s), and 50 timed call by call; with both kinds of load
+// left out 49, with LDS reads, dequantising and scaling left out too 35, of which the matrix instructions
+// are 18 and the rest barriers, staging and addresses (213 vector and 36 matrix instructions a tile of
+// columns). Sums that begin at -(16 + z) X need no pass over X afterwards: 191 became 213 at groups of 128,
+// which costs nothing there, and groups of 32 no longer spill (28672 x 4096 at 64 rows: 51 -> 40 us). Tried
+// without gain: deeper rings, operands expanded or read a step earlier, set mixes of matrix and vector
+// instructions, 4 tile rows a wave.
 template <typename T, typename S, int GPT, int TN, int KS, bool NORM, bool ZEROS>
 __global__ __launch_bounds__(256 * KS, 2) void linear4_wide_kernel(const Lin4Geom g) {
   using O = typename Operand<T, NORM>::type;

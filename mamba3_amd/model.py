@@ -433,11 +433,12 @@ class Mamba3(nn.Module):
         """Hold every mixer's ``in_proj`` and ``out_proj`` in 4 bits for decode steps.
 
         The 16-bit weights are rounded to 4-bit codes with a scale (and, with ``zeros``, a zero) for
-        every ``group`` columns (32, 64 or 128; ``ops.quantize4``) and overwritten, for good, with the rounded
-        values in their own dtype, so that forward, prefill and steps of more than
-        ``ops.DECODE_LINEAR_ROWS`` rows compute the same model through the general GEMMs, but for that dtype's
-        rounding of ``(code - zero) * scale``. Steps of fewer rows stream the 4-bit copies (``ops.linear4``)
-        instead of the weights. Both are held: memory grows by a quarter of the projections'. A weight that is replaced or modified
+        every ``group`` columns (32, 64 or 128; ``ops.quantize4``) and overwritten, for good, with
+        the rounded values in their own dtype, so that forward, prefill and steps of more than
+        ``ops.DECODE_LINEAR_ROWS`` rows compute the same model through the general GEMMs, but for
+        that dtype's rounding of ``(code - zero) * scale``. Steps of fewer rows stream the 4-bit
+        copies (``ops.linear4``) instead of the weights (quicker up to about 16 rows). Both are
+        held: memory grows by a quarter of the projections'. A weight that is replaced or modified
         afterwards (``load_state_dict``, ``to``, a copy of the model) makes ``step`` raise until
         this is called again. A step's rows must have the weights' dtype, as ever, to run on it.
         """

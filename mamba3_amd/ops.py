@@ -563,8 +563,9 @@ def linear(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor | None 
     to the FP32 sum, which is rounded once. With ``norm_weight`` (``[K]``; ``M <= 32``, or
     ``M <= 64`` with K a multiple of 256) ``x`` is first RMS-normalised, as
     ``F.rms_norm(x, (K,), norm_weight, norm_eps)``, with ``x * norm_weight`` rounded to ``x``'s
-    dtype before the division (in float16 it has to stay below 65504). This replaces the decode step's RMSNorm, ``in_proj`` / ``out_proj`` calls and the block's residual add
-    (reference ``model.py:441-458, 514-520``).
+    dtype before the division (in float16 it has to stay below 65504). This replaces the decode
+    step's RMSNorm, ``in_proj`` / ``out_proj`` calls and the block's residual add (reference
+    ``model.py:441-458, 514-520``).
     """
     device = _require_device(x, weight, residual, out, norm_weight)
     _require_inference(x, weight, residual, norm_weight)
@@ -815,7 +816,8 @@ def linear4(x: torch.Tensor, weight: Weight4, residual: torch.Tensor | None = No
     ``x [M, K]`` (``M <= 256``) bfloat16 or float16; ``residual`` and ``out`` ``[M, N]`` of that
     dtype. Sums are FP32, the residual is added to them and the result rounded once. With
     ``norm_weight [K]`` (taken in ``x``'s dtype) ``x`` is first RMS-normalised, as
-    ``F.rms_norm(x.float(), (K,), norm_weight.float(), norm_eps)``, its rows not rounded to 16 bits. An infinity in a row of ``x`` makes its row of the result NaN. No backward.
+    ``F.rms_norm(x.float(), (K,), norm_weight.float(), norm_eps)``, its rows not rounded to 16
+    bits. An infinity in a row of ``x`` makes its row of the result NaN. No backward.
     """
     if forward_ad._current_level >= 0:
         _refuse_tangents(x, residual, norm_weight)
@@ -985,10 +987,10 @@ def gated_scan(x: torch.Tensor, decay: torch.Tensor, gate: torch.Tensor | None =
 
     Without ``gate`` and ``rate``, ``decay`` holds log decays, at most 0 (factors are multiplied over
     tiles of tokens, so positive ones can give NaN where the recurrence is finite): ``h_t =
-    exp(decay_t) h_{t-1} + x_t``. With them ``decay`` and ``gate`` hold logits and ``rate [C]`` (>= 0) the log decay of an
-    open gate: ``a_t = exp(-rate sigmoid(decay_t))``, ``h_t = a_t h_{t-1} + sqrt(1 - a_t^2)
-    sigmoid(gate_t) x_t``. ``x``, ``decay`` and ``gate`` share one dtype and may be slices of one
-    projection. Returns ``(out [B, L, C] = h in x's dtype, final_state [B, C] FP32)``.
+    exp(decay_t) h_{t-1} + x_t``. With them ``decay`` and ``gate`` hold logits and ``rate [C]`` (>=
+    0) the log decay of an open gate: ``a_t = exp(-rate sigmoid(decay_t))``, ``h_t = a_t h_{t-1} +
+    sqrt(1 - a_t^2) sigmoid(gate_t) x_t``. ``x``, ``decay`` and ``gate`` share one dtype and may be
+    slices of one projection. Returns ``(out [B, L, C] = h in x's dtype, final_state [B, C] FP32)``.
 
     ``initial_state [B, C]`` FP32 continues a sequence. ``lengths [B]`` (integers; clamped to 0..L)
     ends each row of a padded batch: past its end ``out`` is 0 and the state stays, whatever the
@@ -998,7 +1000,8 @@ def gated_scan(x: torch.Tensor, decay: torch.Tensor, gate: torch.Tensor | None =
     first and reset ones); here they have it too.
 
     Unlike the Mamba-3 calls of this module this one has a backward pass: gradients reach ``x``,
-    ``decay``, ``gate``, ``rate`` and ``initial_state`` (once: no second derivatives, none in forward mode).
+    ``decay``, ``gate``, ``rate`` and ``initial_state`` (once: no second derivatives, none in
+    forward mode).
     """
     if x.ndim != 3:
         raise ValueError("x must have shape [B, L, C]")
