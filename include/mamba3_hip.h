@@ -29,7 +29,8 @@
  * m3_linear has no reference hook: it takes the decode step's projection GEMMs (see below).
  * m3_gated_scan and m3_gated_scan_bwd have no counterpart in the reference: an elementwise gated
  * recurrence beside the matrix-state one, with its gradients. Nor has m3_linear4, m3_linear's
- * product with a weight held in 4 bits.
+ * product with a weight held in 4 bits, nor m3_rows8 and m3_linear8, a projection of any number of rows
+ * in 8 bits.
  */
 #ifndef MAMBA3_HIP_H
 #define MAMBA3_HIP_H
@@ -364,6 +365,64 @@ typedef struct {
 } m3_linear4_args;
 
 int m3_linear4(const m3_linear4_args* args, hipStream_t stream);
+
+/*
+ * Rows rounded to 8-bit codes with one FP32 scale each, m3_linear8's operand: of x, or behind m3_rms_norm's
+ * residual add and RMSNorm. No counterpart in the reference.
+ *   s = x (+ add, summed in FP32 and rounded to x's dtype), optionally sum_out = s
+ *   p = s * weight (the weight rounded to x's dtype; without weight p = x), most = max |p| of the row
+ *   code = rint(127 p / most) of the exact quotient, ties to even
+ *   scale = most / 127, with weight times rsqrt(mean(s^2) + eps)
+ * so that code * scale is what x, or its RMSNorm, holds. A row of zeros has codes and scale 0; a row
+ * that holds an infinity or NaN has codes 0 and scale NaN. The sum of squares and p have to stay in
+ * FP32's range.
+ * x, add, sum_out as in m3_rms_norm (FP32 with an add of any dtype, or 16 bits throughout; sum_out may be x, or
+ * an add of its dtype), at any alignment, dim from 1 to M3_LINEAR8_MAX_K. What is written otherwise
+ * overlaps nothing.
+ */
+#define M3_LINEAR8_MAX_K 131071 /* 128 * 128 * K stays below 2^31 */
+typedef struct {
+  int64_t rows, dim;
+  float eps;
+  int32_t reserved;
+  m3_tensor x;          /* [rows, dim] */
+  m3_tensor add;        /* [rows, dim] optional (needs weight) */
+  m3_tensor weight;     /* [dim] optional: with it the norm */
+  m3_tensor sum_out;    /* [rows, dim] optional (needs add), x's dtype */
+  int8_t* codes;        /* [rows, codes_stride], 16-byte aligned; bytes past dim, up to the next
+                           multiple of 16, may be written */
+  int64_t codes_stride; /* bytes, a multiple of 16 */
+  float* scales;        /* [rows] */
+} m3_rows8_args;
+
+int m3_rows8(const m3_rows8_args* args, hipStream_t stream);
+
+/*
+ * The product of such rows with a weight in 8 bits:
+ *   out[m, n] = sum_k codes[m, k] q[n, k] * row_scale[m] * scale[n] (+ residual[m, n])
+ * The sum is exact, in 32-bit integers; scales and residual meet it in FP32, rounded once to out's dtype. Any
+ * M and N, K up to M3_LINEAR8_MAX_K. No counterpart in the reference.
+ * The weight is laid out once, for reads of 1 KB by a wave and outputs of 16 bytes by a lane, in tiles of 64
+ * rows x 64 columns (rows past N and columns past K: 0), TK = 2 ceil(K / 128) of them a tile row:
+ *   q [ceil(N / 64), TK, 4, 64, 16] bytes: byte e of lane l of quarter j holds column 16 (l / 16) + e of
+ *     its tile, row 32 (j / 2) + 8 (l % 16 / 4) + 4 (j % 2) + l % 4
+ *   scale [64 ceil(N / 64)] FP32, 0 past N
+ * What lies in codes between K and the row's stride has no effect.
+ */
+typedef struct {
+  int64_t m, n, k;
+  int32_t dtype;        /* of out and residual */
+  int32_t reserved;
+  const int8_t* codes;  /* [M, codes_stride], 16-byte aligned */
+  int64_t codes_stride; /* bytes, a multiple of 16, at least K */
+  const float* row_scales; /* [M] */
+  const int8_t* q;      /* 16-byte aligned */
+  const float* scales;  /* 16-byte aligned */
+  m3_tensor residual;   /* [M, N] optional */
+  m3_tensor out;        /* [M, N]; may equal residual, overlaps nothing else */
+} m3_linear8_args;
+
+int m3_linear8(const m3_linear8_args* args, hipStream_t stream);
 
 const char* m3_last_error(void);
 int m3_abi_version(void);

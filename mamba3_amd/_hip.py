@@ -123,6 +123,26 @@ class Linear4Args(ctypes.Structure):
     ]
 
 
+class Rows8Args(ctypes.Structure):
+    _fields_ = [
+        *[(n, ctypes.c_int64) for n in ("rows", "dim")],
+        ("eps", ctypes.c_float), ("reserved", ctypes.c_int32),
+        *[(n, _T) for n in ("x", "add", "weight", "sum_out")],
+        ("codes", ctypes.c_void_p), ("codes_stride", ctypes.c_int64),
+        ("scales", ctypes.c_void_p),
+    ]
+
+
+class Linear8Args(ctypes.Structure):
+    _fields_ = [
+        *[(n, ctypes.c_int64) for n in ("m", "n", "k")],
+        ("dtype", ctypes.c_int32), ("reserved", ctypes.c_int32),
+        ("codes", ctypes.c_void_p), ("codes_stride", ctypes.c_int64),
+        *[(n, ctypes.c_void_p) for n in ("row_scales", "q", "scales")],
+        *[(n, _T) for n in ("residual", "out")],
+    ]
+
+
 # The same blocks as formats of `struct`: a decode call takes its host about as long as its kernels the
 # GPU, and packing a block whole costs a third of filling a Structure field by field. A block is bytes:
 # no two calls share one.
@@ -130,13 +150,16 @@ _TENSOR = "Pii5q"
 GATED_SCAN = struct.Struct("@4i" + 5 * _TENSOR + "PPq" + 3 * _TENSOR + "PN")
 GATED_SCAN_BWD = struct.Struct(GATED_SCAN.format + 7 * _TENSOR)
 LINEAR4 = struct.Struct("@3q3ifPPP" + 4 * _TENSOR)
+ROWS8 = struct.Struct("@2qfi" + 4 * _TENSOR + "PqP")
+LINEAR8 = struct.Struct("@3q2iPqPPP" + 2 * _TENSOR)
 NO_TENSOR = (0,) * 8
 
 ENTRY_POINTS = ("m3_scan_fwd", "m3_scan_workspace_size", "m3_scan_segments", "m3_scan_fwd_noalloc",
                 "m3_chunk_state", "m3_step", "m3_linear", "m3_linear_workspace_size",
                 "m3_rms_norm", "m3_gated_scan", "m3_gated_scan_workspace_size",
                 "m3_gated_scan_bwd", "m3_gated_scan_bwd_workspace_size", "m3_linear4",
-                "m3_last_error", "m3_abi_version")
+                "m3_rows8", "m3_linear8", "m3_last_error", "m3_abi_version")
+LINEAR8_MAX_K = 131071  # M3_LINEAR8_MAX_K: sums of products of 8 bits stay in 32
 GATED_TILE = 64  # M3_GATED_TILE: tokens between two of the states a gated scan's carry holds
 SCRATCH_BYTES = 64 << 20  # M3_SCRATCH_BYTES: the no-alloc scan's per-GPU scratch
 
@@ -153,7 +176,8 @@ def load() -> ctypes.CDLL:
             f"{LIB_PATH} is not built; run `python -m mamba3_amd.build` (hipcc, gfx950)")
     lib = ctypes.CDLL(LIB_PATH)
     for name in ("m3_scan_fwd", "m3_scan_fwd_noalloc", "m3_chunk_state", "m3_step", "m3_linear",
-                 "m3_rms_norm", "m3_gated_scan", "m3_gated_scan_bwd", "m3_linear4"):
+                 "m3_rms_norm", "m3_gated_scan", "m3_gated_scan_bwd", "m3_linear4", "m3_rows8",
+                 "m3_linear8"):
         fn = getattr(lib, name)
         fn.restype = ctypes.c_int
         fn.argtypes = [ctypes.c_void_p, ctypes.c_void_p]

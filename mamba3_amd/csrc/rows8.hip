@@ -1,0 +1,385 @@
+// m3_rows8: rows rounded to 8-bit codes with one FP32 scale each, alone or behind the residual add and
+// RMSNorm of m3_rms_norm: the operand of m3_linear8.
+//
+//   s = x (+ add, rounded to x's dtype), p = s * w (or x), most = max |p|
+//   code = rint(127 p / most),  scale = most / 127 * rsqrt(mean s^2 + eps)   (no norm: most / 127)
+//
+// The norm's factor is one positive number a row, so it is no part of the codes: they need no second
+// reduction, and no rounding of the factor moves one of them.
+//
+// A code is the exact quotient's nearest integer, ties to even: half of the greatest value, 63.5 codes,
+// is a value that 16-bit rows do hold. p times 127 / most in FP32 is off by less than 1e-4 codes; a quotient
+// nearer than that to a half is settled by the sign of 254 |p| - (2 k + 1) most in FP64, which is
+// exact. One element in 5,000 is.
+//
+// Bound by memory: the row stays in registers between the two passes over it (its maximum, its codes), so
+// x, add, the sum and the codes each move once.
+#include <hip/hip_runtime.h>
+
+#include "m3_common.hpp"
+#include "m3_host.hpp"
+
+namespace m3 {
+namespace {
+
+constexpr int kChunk = 8;  // elements a lane takes at a time: 8 bytes of codes
+
+struct Rows8Geom {
+  const char* x;
+  const char* add;   // or null
+  const void* w;     // or null: no norm
+  char* sum;         // or null
+  int8_t* codes;
+  float* scales;
+  int64_t x_ld, a_ld, s_ld, c_ld;  // elements (codes: bytes)
+  int rows, dim, w_dtype;
+  float eps;
+};
+
+// Eight elements from `at` on, at any alignment.
+template <typename T>
+__device__ __forceinline__ void load8(const void* row, int at, float (&v)[kChunk]) {
+  T t[kChunk];
+  __builtin_memcpy(t, static_cast<const T*>(row) + at, sizeof(t));
+#pragma unroll
+  for (int e = 0; e < kChunk; ++e) v[e] = to_f(t[e]);
+}
+
+// What a row's values tell: the sum of squares, the bits of the greatest magnitude (as integers they
+// order infinities and NaN above all others), and for products of FP32 values, which FP32 does not hold,
+// the greatest one in FP64.
+template <bool WIDE>
+struct Seen {
+  float sq;
+  uint32_t bits;
+  double wide;
+  __device__ __forceinline__ void look(float s, float w, float p) {
+    sq = fmaf(s, s, sq);
+    bits = max(bits, __float_as_uint(p) & 0x7fffffffu);
+    if constexpr (WIDE) wide = fmax(wide, fabs(static_cast<double>(s) * static_cast<double>(w)));
+  }
+  __device__ __forceinline__ void join(const Seen& o) {
+    sq += o.sq;
+    bits = max(bits, o.bits);
+    if constexpr (WIDE) wide = fmax(wide, o.wide);
+  }
+  __device__ __forceinline__ void join_wave() {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) {
+      Seen other;
+      other.sq = __shfl_xor(sq, o);
+      other.bits = __shfl_xor(bits, o);
+      other.wide = WIDE ? __shfl_xor(wide, o) : 0.0;
+      join(other);
+    }
+  }
+};
+
+// One row of the call.
+template <typename T, typename TA, bool NORM, bool ADD>
+struct Row {
+  const T* x;
+  const TA* add;
+  T* sum;  // or null
+  const Rows8Geom& g;
+  __device__ __forceinline__ Row(const Rows8Geom& geom, int64_t row)
+      : x(reinterpret_cast<const T*>(geom.x) + row * geom.x_ld),
+        add(ADD ? reinterpret_cast<const TA*>(geom.add) + row * geom.a_ld : nullptr),
+        sum(ADD && geom.sum != nullptr ? reinterpret_cast<T*>(geom.sum) + row * geom.s_ld : nullptr),
+        g(geom) {}
+
+  // s of eight elements, and of one
+  __device__ __forceinline__ void sums(int at, float (&s)[kChunk]) const {
+    load8<T>(x, at, s);
+    if constexpr (ADD) {
+      float a[kChunk];
+      load8<TA>(add, at, a);
+#pragma unroll
+      for (int e = 0; e < kChunk; ++e) s[e] = rnd<T>(s[e] + a[e]);
+    }
+  }
+  __device__ __forceinline__ float sum_at(int at) const {
+    float s = to_f(x[at]);
+    if constexpr (ADD) s = rnd<T>(s + to_f(add[at]));
+    return s;
+  }
+  __device__ __forceinline__ void keep(int at, const float (&s)[kChunk]) const {
+    if (ADD && sum != nullptr) {
+      T t[kChunk];
+#pragma unroll
+      for (int e = 0; e < kChunk; ++e) t[e] = from_f<T>(s[e]);
+      __builtin_memcpy(sum + at, t, sizeof(t));
+    }
+  }
+  // s once more, where this lane has stored it: it may have taken x's place
+  __device__ __forceinline__ float again(int at) const {
+    return ADD && sum != nullptr ? to_f(sum[at]) : sum_at(at);
+  }
+
+  // the norm's weight, rounded to the rows' dtype
+  __device__ __forceinline__ void weights(int at, float (&w)[kChunk]) const {
+    if constexpr (NORM) {
+      if (g.w_dtype == M3_F32) {
+        load8<float>(g.w, at, w);
+      } else if (g.w_dtype == M3_BF16) {
+        load8<__bf16>(g.w, at, w);
+      } else {
+        load8<_Float16>(g.w, at, w);
+      }
+#pragma unroll
+      for (int e = 0; e < kChunk; ++e) w[e] = rnd<T>(w[e]);
+    }
+  }
+  __device__ __forceinline__ float weight_at(int at) const {
+    return NORM ? rnd<T>(ldx(g.w, g.w_dtype, at)) : 1.f;
+  }
+};
+
+// The row's own constants for its codes.
+struct Scaled {
+  float up, inv;  // q = p * up * inv; `up` lifts rows whose 127 / most would be infinite
+  double most;
+  float scale;
+};
+
+template <bool NORM, bool WIDE>
+__device__ __forceinline__ Scaled scaled(const Seen<WIDE>& seen, int dim, float eps) {
+  const float most = __uint_as_float(seen.bits);
+  const bool bad = seen.bits >= 0x7f800000u;  // an infinity or NaN
+  const float up = most < 0x1p-100f ? 0x1p100f : 1.f;
+  const float inv = bad || seen.bits == 0 ? 0.f : 127.f / (most * up);
+  const float norm = NORM ? rsqrtf(seen.sq / static_cast<float>(dim) + eps) : 1.f;
+  return Scaled{up, inv, WIDE ? seen.wide : static_cast<double>(most),
+                bad ? __uint_as_float(0x7fc00000u) : most / 127.f * norm};
+}
+
+// The code of p, and whether it is too near to a half to be told in FP32. A row that holds an infinity
+// or NaN has inv = 0, and codes of 0 (where p is NaN, too: fmaxf drops it).
+__device__ __forceinline__ int code8(float p, const Scaled& c, bool& close) {
+  const float q = p * c.up * c.inv, n = rintf(q);
+  close = fabsf(q - n) > 0.4999f;
+  return c.inv == 0.f ? 0 : static_cast<int>(n);
+}
+
+// The code of s * w by the sign of 254 |s w| - (2 k + 1) most, where k and k + 1 are in question.
+__device__ __forceinline__ int settle(float s, float w, const Scaled& c) {
+  const float q = s * w * c.up * c.inv, k = floorf(fabsf(q));
+  const double p = fabs(static_cast<double>(s) * static_cast<double>(w)), odd = 2.0 * k + 1.0;
+  const double half = odd * c.most, rest = fma(odd, c.most, -half);
+  const double over = fma(254.0, p, -half) - rest;
+  const int n = static_cast<int>(k), up = over > 0.0 || (over == 0.0 && (n & 1) != 0);
+  return q < 0.f ? -(n + up) : n + up;
+}
+
+// TPR threads take a row: a wave (four rows a workgroup) or the workgroup of 256. A lane holds the p of CH
+// chunks of eight and, for dim % 8, of one element more; CH = 0 walks longer rows twice instead.
+template <typename T, typename TA, bool NORM, bool ADD, int TPR, int CH>
+__global__ __launch_bounds__(256) void rows8_kernel(const Rows8Geom g) {
+  constexpr bool kWide = NORM && sizeof(T) == 4;
+  const int tid = threadIdx.x, lane = TPR == 64 ? tid & 63 : tid;
+  const int64_t r = TPR == 64 ? static_cast<int64_t>(blockIdx.x) * 4 + (tid >> 6) : blockIdx.x;
+  if (TPR == 64 && r >= g.rows) return;
+  const Row<T, TA, NORM, ADD> row(g, r);
+  const int whole = g.dim / kChunk, rest = g.dim % kChunk;
+  Seen<kWide> seen = {0.f, 0u, 0.0};
+  const auto look8 = [&](int at, float (&s)[kChunk]) {  // leaves p in s
+    float w[kChunk];
+    row.keep(at, s);
+    row.weights(at, w);
+#pragma unroll
+    for (int e = 0; e < kChunk; ++e) {
+      const float p = NORM ? s[e] * w[e] : s[e];
+      seen.look(s[e], NORM ? w[e] : 1.f, p);
+      s[e] = p;
+    }
+  };
+  constexpr int kHeld = CH > 0 ? CH : 1;
+  float p[kHeld][kChunk], last = 0.f;
+  if constexpr (CH > 0) {
+#pragma unroll
+    for (int j = 0; j < CH; ++j) {
+      if (lane + TPR * j < whole) row.sums(kChunk * (lane + TPR * j), p[j]);
+    }
+#pragma unroll
+    for (int j = 0; j < CH; ++j) {
+      if (lane + TPR * j < whole) look8(kChunk * (lane + TPR * j), p[j]);
+    }
+  } else {
+    for (int c = lane; c < whole; c += TPR) {
+      row.sums(kChunk * c, p[0]);
+      look8(kChunk * c, p[0]);
+    }
+  }
+  const int end = kChunk * whole + lane;
+  if (lane < rest) {
+    const float s = row.sum_at(end), w = row.weight_at(end);
+    if (ADD && row.sum != nullptr) row.sum[end] = from_f<T>(s);
+    last = s * w;
+    seen.look(s, w, last);
+  }
+  seen.join_wave();
+  if constexpr (TPR > 64) {
+    __shared__ Seen<kWide> parts[4];
+    if ((tid & 63) == 0) parts[tid >> 6] = seen;
+    __syncthreads();
+    seen = parts[0];
+#pragma unroll
+    for (int i = 1; i < 4; ++i) seen.join(parts[i]);
+  }
+  const Scaled c = scaled<NORM, kWide>(seen, g.dim, g.eps);
+  int8_t* const codes = g.codes + r * g.c_ld;
+  const auto code_chunk = [&](int at, const float (&v)[kChunk]) {
+    typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+    u32x2 words = {0u, 0u};
+    unsigned open = 0;  // the elements in question
+#pragma unroll
+    for (int e = 0; e < kChunk; ++e) {
+      bool close;
+      const int n = code8(v[e], c, close);
+      words[e / 4] |= static_cast<uint32_t>(n & 0xff) << (8 * (e % 4));
+      open |= close ? 1u << e : 0u;
+    }
+    *reinterpret_cast<u32x2*>(codes + at) = words;
+    while (open != 0) {
+      const int i = at + __builtin_ctz(open);
+      open &= open - 1;
+      codes[i] = static_cast<int8_t>(settle(row.again(i), row.weight_at(i), c));
+    }
+  };
+  if constexpr (CH > 0) {
+#pragma unroll
+    for (int j = 0; j < CH; ++j) {
+      if (lane + TPR * j < whole) code_chunk(kChunk * (lane + TPR * j), p[j]);
+    }
+  } else {
+    for (int j = lane; j < whole; j += TPR) {
+      const int at = kChunk * j;
+#pragma unroll
+      for (int e = 0; e < kChunk; ++e) p[0][e] = row.again(at + e) * row.weight_at(at + e);
+      code_chunk(at, p[0]);
+    }
+  }
+  if (lane < rest) {
+    bool close;
+    int n = code8(last, c, close);
+    if (close) n = settle(row.again(end), row.weight_at(end), c);
+    codes[end] = static_cast<int8_t>(n);
+  }
+  if (lane == 0) g.scales[r] = c.scale;
+}
+
+template <typename T, typename TA, bool NORM, bool ADD, int TPR, int CH>
+int launch_one(const Rows8Geom& g, hipStream_t stream) {
+  const unsigned blocks = TPR == 64 ? (static_cast<unsigned>(g.rows) + 3) / 4 : g.rows;
+  hipLaunchKernelGGL((rows8_kernel<T, TA, NORM, ADD, TPR, CH>), dim3(blocks), dim3(256), 0, stream, g);
+  return check_launch("m3_rows8");
+}
+
+template <typename T, typename TA, bool NORM, bool ADD>
+int launch_dim(const Rows8Geom& g, hipStream_t stream) {
+  const int chunks = (g.dim + kChunk - 1) / kChunk;
+  if (chunks <= 64) return launch_one<T, TA, NORM, ADD, 64, 1>(g, stream);
+  if (chunks <= 128) return launch_one<T, TA, NORM, ADD, 64, 2>(g, stream);
+  if (chunks <= 256) return launch_one<T, TA, NORM, ADD, 64, 4>(g, stream);
+  if (chunks <= 512) return launch_one<T, TA, NORM, ADD, 256, 2>(g, stream);
+  if (chunks <= 1024) return launch_one<T, TA, NORM, ADD, 256, 4>(g, stream);
+  return launch_one<T, TA, NORM, ADD, 256, 0>(g, stream);
+}
+
+template <typename T>
+int launch_type(const Rows8Geom& g, int add_dtype, hipStream_t stream) {
+  if (g.w == nullptr) return launch_dim<T, T, false, false>(g, stream);
+  if (g.add == nullptr) return launch_dim<T, T, true, false>(g, stream);
+  if constexpr (sizeof(T) == 4) {
+    if (add_dtype == M3_BF16) return launch_dim<T, __bf16, true, true>(g, stream);
+    if (add_dtype == M3_F16) return launch_dim<T, _Float16, true, true>(g, stream);
+  }
+  return launch_dim<T, T, true, true>(g, stream);
+}
+
+struct Range {
+  const char *from, *to;
+};
+
+Range range(const m3_tensor& t, int64_t rows, int64_t dim) {
+  const char* p = static_cast<const char*>(t.ptr);
+  return {p, p == nullptr ? p : p + ((rows - 1) * t.stride[0] + dim) * elem_size(t.dtype)};
+}
+
+bool meets(const Range& a, const Range& b) {
+  return a.from != nullptr && b.from != nullptr && a.from < b.to && b.from < a.to;
+}
+
+int validate(const m3_rows8_args& a) {
+  if (a.rows < 0 || a.dim < 0) return fail(M3_EINVAL, "m3_rows8: negative dimensions");
+  if (a.rows >= (1 << 30) || a.dim > M3_LINEAR8_MAX_K) {
+    return fail(M3_EUNSUPPORTED, "m3_rows8: %lld rows of %lld: below 2^30, of at most %d",
+                static_cast<long long>(a.rows), static_cast<long long>(a.dim), M3_LINEAR8_MAX_K);
+  }
+  if (a.rows == 0) return M3_OK;
+  if (a.dim == 0) return fail(M3_EUNSUPPORTED, "m3_rows8: dim 0");
+  int rc;
+  if ((rc = check_tensor(a.x, "x", 2, a.dim, true, -1)) ||
+      (rc = check_tensor(a.weight, "weight", 1, a.dim, false, -1)) ||
+      (rc = check_tensor(a.add, "add", 2, a.dim, false, a.x.dtype == M3_F32 ? -1 : a.x.dtype)) ||
+      (rc = check_tensor(a.sum_out, "sum_out", 2, a.dim, false, a.x.dtype))) {
+    return rc;
+  }
+  if (present(a.add) && !present(a.weight)) return fail(M3_EINVAL, "m3_rows8: add needs weight");
+  if (present(a.sum_out) && !present(a.add)) return fail(M3_EINVAL, "m3_rows8: sum_out needs add");
+  if (present(a.weight) && !(a.eps >= 0.f)) return fail(M3_EINVAL, "m3_rows8: eps must be >= 0");
+  if (a.codes == nullptr || a.scales == nullptr) {
+    return fail(M3_EINVAL, "m3_rows8: codes or scales are NULL");
+  }
+  if (reinterpret_cast<uintptr_t>(a.codes) % 16 != 0 || a.codes_stride % 16 != 0 ||
+      reinterpret_cast<uintptr_t>(a.scales) % 4 != 0) {
+    return fail(M3_EUNSUPPORTED, "m3_rows8: rows of codes must be 16-byte aligned, scales 4-byte");
+  }
+  const int64_t whole = (a.dim + 15) / 16 * 16;
+  if (a.codes_stride < whole) return fail(M3_EINVAL, "m3_rows8: rows of codes overlap");
+  if (a.rows > 1 && present(a.sum_out) && a.sum_out.stride[0] < a.dim) {
+    return fail(M3_EINVAL, "m3_rows8: rows of sum_out overlap");
+  }
+  const char* c = reinterpret_cast<const char*>(a.codes);
+  const char* f = reinterpret_cast<const char*>(a.scales);
+  const Range x = range(a.x, a.rows, a.dim), add = range(a.add, a.rows, a.dim),
+              w = range(a.weight, 1, a.dim), sum = range(a.sum_out, a.rows, a.dim),
+              codes = {c, c + (a.rows - 1) * a.codes_stride + whole}, scales = {f, f + a.rows * 4};
+  for (const Range* r : {&x, &add, &w, &sum}) {
+    if (meets(*r, codes) || meets(*r, scales)) {
+      return fail(M3_EINVAL, "m3_rows8: codes or scales overlap another tensor");
+    }
+  }
+  if (meets(codes, scales)) return fail(M3_EINVAL, "m3_rows8: codes overlap scales");
+  // s may take the place of x or of an add of its dtype: each element is read before it is written
+  const auto in_place = [&](const m3_tensor& t) {
+    return t.ptr == a.sum_out.ptr && t.dtype == a.sum_out.dtype &&
+           (a.rows == 1 || t.stride[0] == a.sum_out.stride[0]);
+  };
+  if ((meets(sum, x) && !in_place(a.x)) || (meets(sum, add) && !in_place(a.add)) || meets(sum, w)) {
+    return fail(M3_EINVAL, "m3_rows8: sum_out overlaps an input without being it");
+  }
+  return M3_OK;
+}
+
+}  // namespace
+}  // namespace m3
+
+extern "C" int m3_rows8(const m3_rows8_args* args, hipStream_t stream) {
+  using namespace m3;
+  clear_error();
+  if (args == nullptr) return fail(M3_EINVAL, "m3_rows8: NULL args");
+  const m3_rows8_args& a = *args;
+  const int rc = validate(a);
+  if (rc != M3_OK) return rc;
+  if (a.rows == 0) return M3_OK;
+  const Rows8Geom g{static_cast<const char*>(a.x.ptr), static_cast<const char*>(a.add.ptr), a.weight.ptr,
+                    static_cast<char*>(a.sum_out.ptr), a.codes, a.scales,
+                    a.x.stride[0], a.add.stride[0], a.sum_out.stride[0], a.codes_stride,
+                    static_cast<int>(a.rows), static_cast<int>(a.dim), a.weight.dtype, a.eps};
+  switch (a.x.dtype) {
+    case M3_F32: return launch_type<float>(g, a.add.dtype, stream);
+    case M3_BF16: return launch_type<__bf16>(g, a.add.dtype, stream);
+    default: return launch_type<_Float16>(g, a.add.dtype, stream);
+  }
+}

@@ -862,6 +862,234 @@ def linear4(x: torch.Tensor, weight: Weight4, residual: torch.Tensor | None = No
     return out
 
 
+# --------------------------------------------------------------------------- 8-bit projections
+
+
+def _device_index(*tensors: torch.Tensor | None) -> int:
+    """The one ROCm device that all of them are on; else a ``RuntimeError`` says which is not."""
+    index = next(t for t in tensors if t is not None).get_device()
+    if index < 0 or any([t is not None and t.get_device() != index for t in tensors]):
+        _require_device(*tensors)
+    return index
+
+
+class Rows8:
+    """Rows ``[..., K]`` in 8 bits: ``codes`` int8, -128 to 127, with one FP32 scale each (``scales
+    [...]``); a row is ``code * scale``. ``quantize8_rows`` and ``rms_norm8`` make them, ``linear8`` multiplies
+    them. Codes from elsewhere are taken as they are, copied where their rows are not 16-byte aligned.
+    """
+
+    __slots__ = ("codes", "scales", "shape", "device", "_ld")
+
+    def __init__(self, codes: torch.Tensor, scales: torch.Tensor) -> None:
+        if codes.ndim < 1 or codes.dtype != torch.int8 or codes.shape[-1] == 0:
+            raise ValueError("codes must be int8 of shape [..., K]")
+        if scales.shape != codes.shape[:-1] or scales.dtype != torch.float32:
+            raise ValueError(f"scales must be float32 of shape {tuple(codes.shape[:-1])}")
+        if scales.device != codes.device:
+            raise ValueError("codes and scales must be on the same device")
+        width = codes.shape[-1]
+        if width > _hip.LINEAR8_MAX_K:
+            raise ValueError(f"rows of {width}: at most {_hip.LINEAR8_MAX_K}")
+        self.shape, self.device = codes.shape, codes.device
+        rows = codes.flatten(0, -2) if codes.ndim > 2 else codes.view(-1, width)
+        ld = rows.stride(0) if rows.shape[0] > 1 else -(-width // 16) * 16
+        end = codes.storage_offset() + (rows.shape[0] - 1) * ld + -(-width // 16) * 16
+        if (rows.stride(1) != 1 and width > 1) or rows.data_ptr() % 16 or ld % 16 or ld < width or (
+                end > rows.untyped_storage().nbytes()):
+            held, ld = _codes8(codes, rows.shape[0], width)
+            held.copy_(rows)
+            codes = held.view(self.shape) if codes.ndim > 2 else held.reshape(self.shape)
+        self.codes, self.scales, self._ld = codes, scales.contiguous(), ld
+
+    @classmethod
+    def _of(cls, codes: torch.Tensor, scales: torch.Tensor, ld: int, shape: torch.Size) -> Rows8:
+        rows = object.__new__(cls)
+        rows.codes, rows.scales, rows._ld = codes.unflatten(0, shape[:-1]) if len(shape) > 2 else (
+            codes if len(shape) == 2 else codes[0]), scales.view(shape[:-1]), ld
+        rows.shape, rows.device = shape, codes.device
+        return rows
+
+    def dequantize(self, dtype: torch.dtype = torch.float32) -> torch.Tensor:
+        """The rows ``[..., K]`` as ``code * scale``, one product in FP32 rounded to ``dtype``."""
+        return torch.mul(self.codes, self.scales.unsqueeze(-1)).to(dtype)
+
+
+def _codes8(like: torch.Tensor, rows: int, width: int) -> tuple[torch.Tensor, int]:
+    """Uninitialised codes ``[rows, width]`` in rows of whole 64 bytes, and that stride."""
+    ld = -(-width // 64) * 64
+    return like.new_empty((rows, ld), dtype=torch.int8)[:, :width], ld
+
+
+class Weight8:
+    """An ``nn.Linear`` weight ``[N, K]`` held in 8 bits, laid out for ``linear8``: ``codes [N, K]`` int8 with
+    one FP32 scale a row (an output channel); the weight is ``code * scale``. Both are copied into the kernel's
+    tiles once, here (``m3_linear8``'s layout); later changes to them are not seen.
+    """
+
+    def __init__(self, codes: torch.Tensor, scales: torch.Tensor) -> None:
+        if codes.ndim != 2 or codes.dtype != torch.int8 or codes.numel() == 0:
+            raise ValueError("codes must be int8 of shape [N, K]")
+        n, k = codes.shape
+        if scales.shape != (n,) or scales.dtype != torch.float32:
+            raise ValueError(f"scales must be float32 of shape {(n,)}")
+        if scales.device != codes.device:
+            raise ValueError("codes and scales must be on the same device")
+        if k > _hip.LINEAR8_MAX_K:
+            raise ValueError(f"rows of {k}: at most {_hip.LINEAR8_MAX_K}")
+        self.shape, self.device = (n, k), codes.device
+        tn, tk = -(-n // 64), 2 * -(-k // 128)
+        q = torch.nn.functional.pad(codes.detach(), (0, 64 * tk - k, 0, 64 * tn - n))
+        # rows of a tile: [quarter's high bit, 4, quarter's low bit, 4]; columns: [lane group, byte]
+        q = q.view(tn, 2, 4, 2, 4, tk, 4, 16).permute(0, 5, 1, 3, 6, 2, 4, 7)
+        self.q = q.reshape(tn, tk, 4, 64, 16).contiguous()
+        self.scales = torch.nn.functional.pad(scales.detach(), (0, 64 * tn - n))
+
+    def dequantize(self, dtype: torch.dtype = torch.float32) -> torch.Tensor:
+        """The weight ``[N, K]`` as ``code * scale``, one product in FP32 rounded to ``dtype``."""
+        n, k = self.shape
+        tn, tk = self.q.shape[:2]
+        q = self.q.view(tn, tk, 2, 2, 4, 4, 4, 16).permute(0, 2, 5, 3, 6, 1, 4, 7)
+        q = q.reshape(64 * tn, 64 * tk)[:n, :k]
+        return torch.mul(q, self.scales[:n].unsqueeze(1)).to(dtype)
+
+
+def quantize8(weight: torch.Tensor) -> Weight8:
+    """``weight [N, K]`` rounded to 8 bits, each row as ``quantize8_rows`` does one: its greatest
+    magnitude has code 127 or -127, and codes are the exact quotients' nearest, ties to even."""
+    if weight.ndim != 2 or weight.dtype not in _FLOAT_DTYPES or weight.numel() == 0:
+        raise ValueError("weight must be a floating [N, K] tensor")
+    weight = weight.detach()
+    most = weight.abs().amax(1, keepdim=True).double()
+    if not bool(torch.isfinite(most).all()):
+        raise ValueError("quantize8: the weight holds NaN or infinities")
+    # in 64 bits the product is exact and the quotient on the right side of half a code
+    codes = (127 * weight.double() / torch.where(most > 0, most, 1.0)).round().to(torch.int8)
+    return Weight8(codes, most.squeeze(1).float() / 127)
+
+
+def _rows8(x, weight, eps, add, keep_sum) -> tuple[Rows8, torch.Tensor | None]:
+    width = x.shape[-1]
+    lead = x.shape[:-1]
+
+    def rows_of(t):
+        return None if t is None else _inner(t.reshape(-1, width))
+
+    index = x.get_device()
+    flat, add = rows_of(x), rows_of(add)
+    rows = flat.shape[0]
+    codes, ld = _codes8(flat, rows, width)
+    scales = flat.new_empty(rows, dtype=torch.float32)
+    total = torch.empty(x.shape, dtype=x.dtype, device=x.device) if keep_sum else None
+    if rows:
+        _hip.launch("m3_rows8", _hip.ROWS8.pack(
+            rows, width, eps, 0, *_packed(flat, _hip.dtype_code(x.dtype)),
+            *(_hip.NO_TENSOR if add is None else _packed(add, _hip.dtype_code(add.dtype))),
+            *(_hip.NO_TENSOR if weight is None else _packed(weight, _hip.dtype_code(weight.dtype))),
+            *(_hip.NO_TENSOR if total is None else
+              (total.data_ptr(), _hip.dtype_code(x.dtype), 0, width, 1, 0, 0, 0)),
+            codes.data_ptr(), ld, scales.data_ptr()), index)
+    return Rows8._of(codes, scales, ld, x.shape), total
+
+
+def _check_rows8(name: str, x: torch.Tensor) -> None:
+    if x.ndim < 1 or x.dtype not in _FLOAT_DTYPES:
+        raise ValueError(f"{name}: x must be float32, bfloat16 or float16 of shape [..., K]")
+    if not 0 < x.shape[-1] <= _hip.LINEAR8_MAX_K:
+        raise ValueError(f"{name}: rows of {x.shape[-1]}: 1 to {_hip.LINEAR8_MAX_K}")
+
+
+def quantize8_rows(x: torch.Tensor) -> Rows8:
+    """Rows ``[..., K]`` rounded to 8 bits with a scale each (``m3_rows8``): ``scale = max|x| / 127``,
+    ``code = rint(127 x / max|x|)`` of the exact quotient, ties to even.
+
+    FP32, bfloat16 or float16, any strides. A row of zeros has codes and scale 0; one that holds an
+    infinity or NaN has codes 0 and scale NaN. No backward.
+    """
+    _check_rows8("quantize8_rows", x)
+    if forward_ad._current_level >= 0:
+        _refuse_tangents(x)
+    _device_index(x)
+    if torch.is_grad_enabled():
+        _require_inference(x)
+    return _rows8(x, None, 0.0, None, False)[0]
+
+
+def rms_norm8(x: torch.Tensor, weight: torch.Tensor, eps: float = NORM_EPS, *,
+              add: torch.Tensor | None = None, keep_sum: bool = False):
+    """``rms_norm`` with its output in 8 bits (``m3_rows8``): ``s = x + add`` (or ``x``), then
+    ``quantize8_rows(F.rms_norm(s, (K,), weight.to(s.dtype), eps))`` with the norm's rows not rounded in
+    between. Returns ``(Rows8, s)`` with ``s`` only when ``keep_sum`` (``add`` given).
+
+    Rows of any K and strides: an FP32 ``x`` with an ``add`` of any dtype, or a 16-bit ``x`` with one of its
+    own. The norm's factor is in the scale, not in the codes: ``code = rint(127 p / max|p|)`` with ``p = s *
+    weight``. Rows of zeros, infinities and NaN as in ``quantize8_rows``. No backward.
+    """
+    _check_rows8("rms_norm8", x)
+    if weight.shape != x.shape[-1:] or weight.dtype not in _FLOAT_DTYPES:
+        raise ValueError(f"rms_norm8: weight must be floating of shape {tuple(x.shape[-1:])}")
+    if add is not None and (add.shape != x.shape or add.dtype not in _FLOAT_DTYPES or (
+            x.dtype != torch.float32 and add.dtype != x.dtype)):
+        raise ValueError(f"rms_norm8: add must have x's shape {tuple(x.shape)}, and x's dtype unless "
+                         "x is float32")
+    if keep_sum and add is None:
+        raise ValueError("rms_norm8: keep_sum needs add")
+    if not eps >= 0:
+        raise ValueError("rms_norm8: eps must be >= 0")
+    if forward_ad._current_level >= 0:
+        _refuse_tangents(x, weight, add)
+    _device_index(x, weight, add)
+    if torch.is_grad_enabled():
+        _require_inference(x, weight, add)
+    return _rows8(x, _inner(weight), eps, add, keep_sum)
+
+
+def linear8(rows: Rows8, weight: Weight8, residual: torch.Tensor | None = None, *,
+            out: torch.Tensor | None = None, dtype: torch.dtype | None = None) -> torch.Tensor:
+    """The product of rows and a weight in 8 bits, ``rows @ W.T (+ residual)`` (``m3_linear8``).
+
+    ``rows [..., K]`` any number of them, one token's or a prompt's; the result ``[..., N]`` has ``dtype``
+    FP32, bfloat16 or float16 (default: that of ``out`` or ``residual``, else bfloat16), which
+    ``residual`` and ``out`` share. Sums are exact in 32-bit integers; scales and residual meet them in FP32, which
+    is rounded once. ``out`` may be ``residual``. No backward.
+    """
+    if dtype is None:
+        given = out if out is not None else residual
+        dtype = torch.bfloat16 if given is None else given.dtype
+    if dtype not in _FLOAT_DTYPES:
+        raise ValueError("linear8: dtype must be float32, bfloat16 or float16")
+    n, k = weight.shape
+    if rows.shape[-1] != k:
+        raise ValueError(f"linear8: rows {tuple(rows.shape)} do not fit weight {weight.shape}")
+    shape = (*rows.shape[:-1], n)
+    for name, t in (("residual", residual), ("out", out)):
+        if t is not None and (t.shape != shape or t.dtype != dtype):
+            raise ValueError(f"linear8: {name} must be {shape} {dtype}, got {tuple(t.shape)} {t.dtype}")
+    if forward_ad._current_level >= 0:
+        _refuse_tangents(residual)
+    index = _device_index(rows.codes, weight.q, residual, out)
+    if torch.is_grad_enabled():
+        _require_inference(residual)
+    given = out
+    if out is None:
+        out = rows.scales.new_empty(shape, dtype=dtype)
+    m = rows.scales.numel()
+    flat = out.view(-1, n)
+    if m > 1 and flat.stride(0) < n or n > 1 and flat.stride(1) != 1:
+        raise ValueError("linear8: out needs a unit inner stride and rows of its own")
+    code = _hip.dtype_code(dtype)
+    if m:
+        res = None if residual is None else _inner(residual.reshape(-1, n))
+        _hip.launch("m3_linear8", _hip.LINEAR8.pack(
+            m, n, k, code, 0, rows.codes.data_ptr(), rows._ld, rows.scales.data_ptr(),
+            weight.q.data_ptr(), weight.scales.data_ptr(),
+            *(_hip.NO_TENSOR if res is None else _packed(res, code)),
+            flat.data_ptr(), code, 0, *flat.stride(), 0, 0, 0), index)
+    if given is not None:
+        _written(given)
+    return out
+
+
 # --------------------------------------------------------------------------- gated recurrence
 
 
@@ -1082,4 +1310,5 @@ def gated_step(x: torch.Tensor, decay: torch.Tensor, state: torch.Tensor,
 __all__ = ["heavy_tail_activation", "mamba3_scan", "mamba3_step", "fused_step", "chunk_state",
            "ScanCall", "scan_projection", "step_projection", "split_projection", "linear",
            "linear_supported", "rms_norm", "rms_norm_supported", "gated_scan", "gated_step",
-           "Weight4", "quantize4", "linear4", "linear4_supported"]
+           "Weight4", "quantize4", "linear4", "linear4_supported", "Rows8", "Weight8", "quantize8",
+           "quantize8_rows", "rms_norm8", "linear8"]

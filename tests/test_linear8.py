@@ -1,0 +1,249 @@
+"""8-bit rows and weights without a GPU: layouts, rounding, refusals, the C entry points' checks."""
+
+from __future__ import annotations
+
+import ctypes
+import os
+import shutil
+import subprocess
+
+import pytest
+import torch
+
+from conftest import ROOT
+from mamba3_amd import _hip, ops
+
+F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
+
+
+@pytest.fixture(scope="module")
+def lib():
+    if not os.path.exists(_hip.LIB_PATH):
+        pytest.skip("libmamba3_hip.so is not built (run __graft_entry__.build())")
+    return _hip.load()
+
+
+def _parts(n, k, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    return torch.randint(-128, 128, (n, k), generator=g, dtype=torch.int8), torch.rand(n, generator=g)
+
+
+@pytest.mark.parametrize("n,k", [(1, 1), (64, 128), (65, 129), (150, 200), (63, 64)])
+def test_layout_is_the_header_s(n, k):
+    codes, scales = _parts(n, k)
+    weight = ops.Weight8(codes, scales)
+    tn, tk = -(-n // 64), 2 * -(-k // 128)
+    assert weight.q.shape == (tn, tk, 4, 64, 16) and weight.scales.shape == (64 * tn,)
+    wide = torch.zeros(64 * tn, 64 * tk, dtype=torch.int8)
+    wide[:n, :k] = codes
+    wide = wide.view(tn, 64, tk, 64)
+    for j in range(4):
+        for lane in range(64):
+            row = 32 * (j // 2) + 8 * (lane % 16 // 4) + 4 * (j % 2) + lane % 4
+            col = 16 * (lane // 16)
+            assert torch.equal(weight.q[:, :, j, lane], wide[:, row, :, col:col + 16])
+    assert torch.equal(weight.scales[:n], scales) and not weight.scales[n:].any()
+    assert torch.equal(weight.dequantize(), codes.float() * scales.unsqueeze(1))
+    assert torch.equal(weight.dequantize(BF16), (codes.float() * scales.unsqueeze(1)).to(BF16))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+def test_quantize8(dtype):
+    """Within half a code, and the ends of the range are codes 127; ties go to even."""
+    weight = torch.randn(20, 300, generator=torch.Generator().manual_seed(1)).to(dtype)
+    weight[3] = 0
+    weight[4, :4] = torch.tensor([127.0, 2.5, -3.5, 63.5]).to(dtype)
+    weight[4, 4:] = 0
+    held = ops.quantize8(weight)
+    most = weight.double().abs().amax(1)
+    q = held.q.view(1, 6, 2, 2, 4, 4, 4, 16).permute(0, 2, 5, 3, 6, 1, 4, 7).reshape(64, 384)
+    error = (q[:20, :300].double() * most.unsqueeze(1) / 127 - weight.double()).abs()
+    assert (error <= most.unsqueeze(1) / 254 * (1 + 1e-12)).all()
+    assert q.abs().amax(1)[:20].tolist() == [0 if i == 3 else 127 for i in range(20)]
+    assert q[4, :4].tolist() == [127, 2, -4, 64] and not held.dequantize()[3].any()
+
+
+def test_rows8_takes_aligned_codes_as_they_are():
+    codes, scales = _parts(6, 64)
+    rows = ops.Rows8(codes, scales)
+    assert rows.codes.data_ptr() == codes.data_ptr() and rows.shape == (6, 64)
+    wide, _ = _parts(6, 96)
+    view = ops.Rows8(wide[:, :50], scales)
+    assert view.codes.data_ptr() == wide.data_ptr() and view._ld == 96
+    for given in (wide[:, 3:53], wide[:, ::2], wide[:, :48].t().contiguous().t(), _parts(6, 33)[0],
+                  wide.flatten()[:5 * 96 + 90].as_strided((6, 90), (96, 1))):
+        held = ops.Rows8(given, scales)
+        assert torch.equal(held.codes, given) and held._ld % 16 == 0
+        assert held.codes.data_ptr() % 16 == 0 and held.codes.stride(-1) == 1
+        end = held.codes.storage_offset() + 5 * held._ld + -(-given.shape[1] // 16) * 16
+        assert end <= held.codes.untyped_storage().nbytes()
+    cube = ops.Rows8(codes.view(2, 3, 64).transpose(0, 1), scales.view(2, 3).t())
+    assert torch.equal(cube.codes, codes.view(2, 3, 64).transpose(0, 1)) and cube.shape == (3, 2, 64)
+    assert torch.equal(cube.dequantize(), cube.codes.float() * scales.view(2, 3).t().unsqueeze(-1))
+    one = ops.Rows8(codes[2], scales[2])
+    assert one.shape == (64,) and torch.equal(one.dequantize(BF16), (codes[2] * scales[2]).to(BF16))
+    none = ops.Rows8(codes[:0], scales[:0])
+    assert none.shape == (0, 64)
+
+
+@pytest.mark.parametrize("make,message", [
+    (lambda c, s: ops.Rows8(c.int(), s), "codes must"),
+    (lambda c, s: ops.Rows8(c[:, :0], s), "codes must"),
+    (lambda c, s: ops.Rows8(c, s[:3]), "scales must"),
+    (lambda c, s: ops.Rows8(c, s.double()), "scales must"),
+    (lambda c, s: ops.Rows8(torch.zeros(1, 131072, dtype=torch.int8), s[:1]), "at most 131071"),
+    (lambda c, s: ops.Rows8(c, s.to("meta")), "same device"),
+    (lambda c, s: ops.Weight8(c[0], s), "codes must"),
+    (lambda c, s: ops.Weight8(c[:0], s[:0]), "codes must"),
+    (lambda c, s: ops.Weight8(c.short(), s), "codes must"),
+    (lambda c, s: ops.Weight8(c, s.half()), "scales must"),
+    (lambda c, s: ops.Weight8(c, s[:2]), "scales must"),
+    (lambda c, s: ops.Weight8(c, s.to("meta")), "same device"),
+    (lambda c, s: ops.Weight8(torch.zeros(1, 131072, dtype=torch.int8), s[:1]), "at most 131071"),
+    (lambda c, s: ops.quantize8(c), "floating"),
+    (lambda c, s: ops.quantize8(s), "floating"),
+    (lambda c, s: ops.quantize8(torch.full((2, 3), float("nan"))), "NaN"),
+    (lambda c, s: ops.quantize8(torch.full((2, 3), float("inf"))), "infinities"),
+    (lambda c, s: ops.quantize8_rows(c), "x must"),
+    (lambda c, s: ops.quantize8_rows(s[0]), "x must"),
+    (lambda c, s: ops.quantize8_rows(s.double()), "x must"),
+    (lambda c, s: ops.quantize8_rows(s[:0]), "rows of 0"),
+    (lambda c, s: ops.quantize8_rows(torch.zeros(131072)), "rows of 131072"),
+    (lambda c, s: ops.rms_norm8(s, s[:3]), "weight must"),
+    (lambda c, s: ops.rms_norm8(s, s.double()), "weight must"),
+    (lambda c, s: ops.rms_norm8(s, s, add=s[:1]), "add must"),
+    (lambda c, s: ops.rms_norm8(s.half(), s, add=s), "add must"),
+    (lambda c, s: ops.rms_norm8(s, s, keep_sum=True), "needs add"),
+    (lambda c, s: ops.rms_norm8(s, s, -1.0), "eps"),
+    (lambda c, s: ops.rms_norm8(s, s, float("nan")), "eps"),
+    (lambda c, s: ops.linear8(ops.Rows8(c, s), ops.Weight8(c[:, :60], s)), "do not fit"),
+    (lambda c, s: ops.linear8(ops.Rows8(c, s), ops.Weight8(c, s), dtype=torch.float64), "dtype must"),
+    (lambda c, s: ops.linear8(ops.Rows8(c, s), ops.Weight8(c, s), torch.zeros(8, 7)), "residual must"),
+    (lambda c, s: ops.linear8(ops.Rows8(c, s), ops.Weight8(c, s), out=torch.zeros(7, 8)), "out must"),
+    (lambda c, s: ops.linear8(ops.Rows8(c, s), ops.Weight8(c, s), torch.zeros(8, 8), dtype=BF16),
+     "residual must"),
+])
+def test_refusals(make, message):
+    with pytest.raises(ValueError, match=message):
+        make(*_parts(8, 64))
+
+
+def test_off_the_gpu_and_under_autograd():
+    codes, scales = _parts(8, 64)
+    x, weight = torch.zeros(8, 64), ops.Weight8(codes, scales)
+    for call in (lambda: ops.quantize8_rows(x), lambda: ops.rms_norm8(x, x[0]),
+                 lambda: ops.linear8(ops.Rows8(codes, scales), weight)):
+        with pytest.raises(RuntimeError, match="ROCm devices only"):
+            call()
+    with torch.autograd.forward_ad.dual_level():
+        dual = torch.autograd.forward_ad.make_dual(x, x)
+        for call in (lambda: ops.quantize8_rows(dual), lambda: ops.rms_norm8(x, x[0], add=dual),
+                     lambda: ops.linear8(ops.Rows8(codes, scales), weight, dual[:, :8])):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                call()
+
+
+def _rows_args(rows=4, dim=100, stride=112):
+    return _hip.Rows8Args(rows, dim, 1e-5, 0, _hip.Tensor(0x100000, _hip.F32, 0, (dim, 1)),
+                          codes=0x200000, codes_stride=stride, scales=0x300000)
+
+
+def test_rows8_is_checked_on_the_host(lib):
+    call = lib.m3_rows8
+    assert call(None, None) == 1 and b"NULL" in lib.m3_last_error()
+    assert call(ctypes.byref(_rows_args(rows=0)), None) == 0
+    weight = _hip.Tensor(0x400000, _hip.BF16, 0, (1,))
+    add = _hip.Tensor(0x500000, _hip.F16, 0, (100, 1))
+    for changes, code, text in (
+            (dict(rows=-1), 1, b"negative"), (dict(rows=1 << 30), 2, b"below 2^30"),
+            (dict(dim=131072), 2, b"at most 131071"), (dict(dim=0), 2, b"dim 0"),
+            (dict(x=_hip.Tensor()), 1, b"x: required"),
+            (dict(x=_hip.Tensor(0x100000, 7, 0, (100, 1))), 1, b"x: invalid dtype"),
+            (dict(x=_hip.Tensor(0x100002, _hip.F32, 0, (100, 1))), 1, b"x: pointer"),
+            (dict(x=_hip.Tensor(0x100000, _hip.F32, 0, (200, 2))), 2, b"x: innermost"),
+            (dict(x=_hip.Tensor(0x100000, _hip.F32, 0, (-100, 1))), 2, b"x: negative"),
+            (dict(codes=None), 1, b"NULL"), (dict(scales=None), 1, b"NULL"),
+            (dict(codes=0x200008), 2, b"aligned"), (dict(codes_stride=100), 2, b"aligned"),
+            (dict(scales=0x300002), 2, b"aligned"), (dict(codes_stride=96), 1, b"overlap"),
+            (dict(add=add), 1, b"add needs weight"),
+            (dict(weight=weight, sum_out=add), 2, b"sum_out: dtype"),
+            (dict(weight=weight, sum_out=_hip.Tensor(0x600000, _hip.F32, 0, (100, 1))), 1, b"needs add"),
+            (dict(weight=weight, eps=-1.0), 1, b"eps"), (dict(weight=weight, eps=float("nan")), 1, b"eps"),
+            (dict(weight=weight, add=add, sum_out=_hip.Tensor(0x600000, _hip.F32, 0, (50, 1))), 1, b"rows of"),
+            (dict(codes=0x100000 + 3 * 400 + 384), 1, b"overlap another"),
+            (dict(scales=0x100000), 1, b"overlap another"), (dict(scales=0x200000 + 3 * 112 + 108), 1, b"overlap s"),
+            (dict(weight=weight, add=add, codes=0x500000), 1, b"overlap another"),
+            (dict(weight=weight, add=add, codes=0x400000), 1, b"overlap another"),
+            (dict(weight=weight, add=add, sum_out=_hip.Tensor(0x100004, _hip.F32, 0, (100, 1))), 1, b"without being"),
+            (dict(weight=weight, add=add, sum_out=_hip.Tensor(0x100000, _hip.F32, 0, (104, 1))), 1, b"without being"),
+            (dict(weight=weight, add=add, sum_out=_hip.Tensor(0x500000, _hip.F32, 0, (100, 1))), 1, b"without being"),
+            (dict(weight=weight, add=add, sum_out=_hip.Tensor(0x3ffffc, _hip.F32, 0, (100, 1))), 1, b"without being")):
+        args = _rows_args()
+        for field, value in changes.items():
+            setattr(args, field, value)
+        assert call(ctypes.byref(args), None) == code, (changes, lib.m3_last_error())
+        assert text in lib.m3_last_error(), (changes, lib.m3_last_error())
+    args = _rows_args()
+    args.x.dtype, args.weight, args.add = _hip.BF16, weight, add
+    assert call(ctypes.byref(args), None) == 2 and b"add: dtype" in lib.m3_last_error()
+
+
+def _args(m=4, n=64, k=256):
+    return _hip.Linear8Args(m, n, k, _hip.BF16, 0, 0x100000, k, 0x200000, 0x300000, 0x400000,
+                            out=_hip.Tensor(0x500000, _hip.BF16, 0, (n, 1)))
+
+
+def test_linear8_is_checked_on_the_host(lib):
+    call = lib.m3_linear8
+    assert call(None, None) == 1 and b"NULL" in lib.m3_last_error()
+    assert call(ctypes.byref(_args(m=0)), None) == 0 and call(ctypes.byref(_args(n=0)), None) == 0
+    for changes, code, text in (
+            (dict(m=-1), 1, b"negative"), (dict(m=1 << 30), 2, b"below 2^30"),
+            (dict(n=(1 << 27) + 1), 2, b"2^27"), (dict(k=131072), 2, b"131071"), (dict(k=0), 2, b"K = 0"),
+            (dict(dtype=5), 1, b"dtype"), (dict(codes=None), 1, b"NULL"), (dict(row_scales=None), 1, b"NULL"),
+            (dict(q=None), 1, b"NULL"), (dict(scales=None), 1, b"NULL"),
+            (dict(codes=0x100008), 2, b"aligned"), (dict(codes_stride=264), 2, b"aligned"),
+            (dict(q=0x300008), 2, b"aligned"), (dict(scales=0x400004), 2, b"aligned"),
+            (dict(row_scales=0x200002), 2, b"aligned"), (dict(codes_stride=240), 2, b"codes_stride 240"),
+            (dict(codes_stride=(1 << 22) + 16), 2, b"codes_stride"),
+            (dict(out=_hip.Tensor()), 1, b"out: required"),
+            (dict(out=_hip.Tensor(0x500000, _hip.F32, 0, (64, 1))), 2, b"out: dtype"),
+            (dict(out=_hip.Tensor(0x500000, _hip.BF16, 0, (32, 1))), 1, b"rows of out"),
+            (dict(out=_hip.Tensor(0x1003fe, _hip.BF16, 0, (64, 1))), 1, b"out overlaps codes"),
+            (dict(out=_hip.Tensor(0x20000e, _hip.BF16, 0, (64, 1))), 1, b"out overlaps codes"),
+            (dict(out=_hip.Tensor(0x303ffe, _hip.BF16, 0, (64, 1))), 1, b"out overlaps codes"),
+            (dict(out=_hip.Tensor(0x4000fe, _hip.BF16, 0, (64, 1))), 1, b"out overlaps codes"),
+            (dict(residual=_hip.Tensor(0x500010, _hip.BF16, 0, (64, 1))), 1, b"residual without"),
+            (dict(residual=_hip.Tensor(0x500000, _hip.BF16, 0, (72, 1))), 1, b"residual without")):
+        args = _args()
+        for field, value in changes.items():
+            setattr(args, field, value)
+        assert call(ctypes.byref(args), None) == code, (changes, lib.m3_last_error())
+        assert text in lib.m3_last_error(), (changes, lib.m3_last_error())
+
+
+def test_structs_match_the_header_layout(tmp_path):
+    if shutil.which("gcc") is None:
+        pytest.skip("gcc not available")
+    pairs = (("m3_rows8_args", _hip.Rows8Args, _hip.ROWS8), ("m3_linear8_args", _hip.Linear8Args, _hip.LINEAR8))
+    lines = ['#include "mamba3_hip.h"', "#include <stdio.h>", "int main(void) {",
+             'printf("max - %d\\n", M3_LINEAR8_MAX_K);']
+    for name, py, _ in pairs:
+        lines.append(f'printf("{name} - %zu\\n", sizeof({name}));')
+        lines += [f'printf("{name} {f} %zu\\n", offsetof({name}, {f}));' for f, _ in py._fields_]
+    source = tmp_path / "layout.c"
+    source.write_text("\n".join(lines + ["return 0; }"]))
+    subprocess.run(["gcc", "-D__HIP_PLATFORM_AMD__", "-I/opt/rocm/include",
+                    f"-I{os.path.join(ROOT, 'include')}", str(source), "-o",
+                    str(tmp_path / "layout")], check=True)
+    out = subprocess.run([str(tmp_path / "layout")], check=True, capture_output=True, text=True)
+    structs = {name: py for name, py, _ in pairs}
+    for line in out.stdout.splitlines():
+        name, field, value = line.split()
+        if name == "max":
+            assert _hip.LINEAR8_MAX_K == int(value)
+            continue
+        size = ctypes.sizeof(structs[name]) if field == "-" else getattr(structs[name], field).offset
+        assert size == int(value), line
+    for _, py, packed in pairs:
+        assert packed.size == ctypes.sizeof(py)
