@@ -29,7 +29,7 @@
  * m3_linear has no reference hook: it takes the decode step's projection GEMMs (see below).
  * m3_gated_scan and m3_gated_scan_bwd have no counterpart in the reference: an elementwise gated
  * recurrence beside the matrix-state one, with its gradients. Nor has m3_linear4, m3_linear's
- * product with a weight held in 4 bits, nor m3_rows8 and m3_linear8, a projection of any number of rows
+ * product with a weight held in 4 bits, nor m3_rows8, m3_rows8_values and m3_linear8, a projection of any number of rows
  * in 8 bits.
  */
 #ifndef MAMBA3_HIP_H
@@ -397,6 +397,17 @@ typedef struct {
 
 int m3_rows8(const m3_rows8_args* args, hipStream_t stream);
 
+/* What such rows stand for: out[r, d] = codes[r, d] * scales[r], one FP32 product rounded to out's dtype. */
+typedef struct {
+  int64_t rows, dim;
+  const int8_t* codes;  /* [rows, codes_stride], 16-byte aligned, readable to the next multiple of 16 */
+  int64_t codes_stride; /* bytes, a multiple of 16 */
+  const float* scales;  /* [rows] */
+  m3_tensor out;        /* [rows, dim]; overlaps nothing */
+} m3_rows8_values_args;
+
+int m3_rows8_values(const m3_rows8_values_args* args, hipStream_t stream);
+
 /*
  * The product of such rows with a weight in 8 bits:
  *   out[m, n] = sum_k codes[m, k] q[n, k] * row_scale[m] * scale[n] (+ residual[m, n])
@@ -413,7 +424,7 @@ typedef struct {
   int64_t m, n, k;
   int32_t dtype;        /* of out and residual */
   int32_t reserved;
-  const int8_t* codes;  /* [M, codes_stride], 16-byte aligned */
+  const int8_t* codes;  /* [M, codes_stride], 16-byte aligned, readable to the next multiple of 16 */
   int64_t codes_stride; /* bytes, a multiple of 16, at least K */
   const float* row_scales; /* [M] */
   const int8_t* q;      /* 16-byte aligned */

@@ -3,20 +3,17 @@
 // of rows.
 //
 // The sums are exact in 32 bits (K < 2^17), so their order is free and every kernel gives the same bits; each
-// output then has three FP32 roundings and its own.
+// output then has three FP32 roundings (of the sum and of two products, the second one with the residual) and its own.
 //
 // The weight is an instruction's first operand: a lane of its result holds four consecutive columns n of one
 // row m. The weight's tiles order their 64 rows so that two results side by side are eight columns, 16 bytes of
 // a 16-bit output, and four lanes 64 bytes.
 //
-// linear8_rows_kernel (few rows): a workgroup takes 16 weight rows and 16 MT rows of codes; its waves
-// take every WAVES-th tile of 64 columns, straight into registers, and their sums meet in LDS. Bound by the
-// weight's stream, or the launch and one latency of memory.
+// linear8_rows_kernel (few rows, or little work): a workgroup's waves take every WAVES-th tile of 64
+// columns, both operands straight into registers, and their sums meet in LDS. Bound by the weight's stream, or
+// the launch and a few latencies of memory.
 //
-// linear8_tile_kernel: a workgroup takes BM rows by BN columns and walks K in steps of 128. A step's
-// codes and tiles go from memory into one of two LDS stages without passing through registers, while the other
-// is multiplied; one barrier a step. Codes lie in LDS in rows of 128 bytes, whose eight pieces of 16 are
-// exchanged by the row's low bits: eight lanes reading one column's pieces of eight rows meet all banks.
+// linear8_tile_kernel (the rest): below.
 #include <hip/hip_runtime.h>
 
 #include "m3_common.hpp"
@@ -28,6 +25,7 @@ namespace {
 typedef int i4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
+constexpr int kCus = 256;
 constexpr int kTileBytes = 4096;  // 64 weight rows x 64 columns
 
 struct Lin8Geom {
@@ -41,6 +39,7 @@ struct Lin8Geom {
   int64_t m;
   int n, k, tk;     // tk: tiles of 64 columns in a tile row of the weight
   int tiles;        // tile rows
+  bool whole;       // 16 bytes of out at a time: aligned, N a multiple, a tile's offsets 32-bit
 };
 
 // An offset past every extent, also with a whole row of tiles added.
@@ -61,88 +60,120 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t codes_rsrc(const Lin8Geom& g, 
   return rsrc8(g.codes + m0 * g.c_ld, (left - 1) * g.c_ld + (g.k + 15) / 16 * 16);
 }
 
-// COUNT (4 or 8) consecutive outputs of one row from column n on.
+// COUNT values of a row of the residual from column n on; past its end 0.
+template <typename T, int COUNT>
+__device__ __forceinline__ void load_res(const T* row, int n, int end, float (&v)[COUNT]) {
+  if (n + COUNT <= end) {
+    T t[COUNT];
+    __builtin_memcpy(t, row + n, sizeof(t));
+#pragma unroll
+    for (int e = 0; e < COUNT; ++e) v[e] = to_f(t[e]);
+  } else {
+#pragma unroll
+    for (int e = 0; e < COUNT; ++e) v[e] = n + e < end ? to_f(row[n + e]) : 0.f;
+  }
+}
+
+// An output before its rounding to T, the same operations in every kernel.
+template <bool RES>
+__device__ __forceinline__ float scaled(int sum, float rs, float sc, float res) {
+  const float v = static_cast<float>(sum) * rs;
+  return RES ? fmaf(v, sc, res) : v * sc;
+}
+
+// COUNT (4 or 8) consecutive outputs of one row from column n on, at any alignment.
 template <typename T, int COUNT>
 __device__ __forceinline__ void put(const Lin8Geom& g, int64_t m, int n, float rs, const i4* sums) {
-  float v[COUNT];
+  float res[COUNT];
+  T y[COUNT];
+  if (g.res != nullptr) load_res(static_cast<const T*>(g.res) + m * g.r_ld, n, g.n, res);
 #pragma unroll
   for (int e = 0; e < COUNT; e += 4) {
     const f4 sc = *reinterpret_cast<const f4*>(g.scales + n + e);
 #pragma unroll
-    for (int r = 0; r < 4; ++r) v[e + r] = static_cast<float>(sums[e / 4][r]) * rs * sc[r];
-  }
-  const T* res = static_cast<const T*>(g.res) + m * g.r_ld + n;
-  T* out = static_cast<T*>(g.out) + m * g.o_ld + n;
-  T y[COUNT];
-  if (n + COUNT <= g.n) {
-    if (g.res != nullptr) {
-      T t[COUNT];
-      __builtin_memcpy(t, res, sizeof(t));
-#pragma unroll
-      for (int e = 0; e < COUNT; ++e) v[e] += to_f(t[e]);
+    for (int r = 0; r < 4; ++r) {
+      const int sum = sums[e / 4][r];
+      y[e + r] = from_f32<T>(g.res != nullptr ? scaled<true>(sum, rs, sc[r], res[e + r])
+                                              : scaled<false>(sum, rs, sc[r], 0.f));
     }
-#pragma unroll
-    for (int e = 0; e < COUNT; ++e) y[e] = from_f<T>(v[e]);
+  }
+  T* const out = static_cast<T*>(g.out) + m * g.o_ld + n;
+  if (n + COUNT <= g.n) {
     __builtin_memcpy(out, y, sizeof(y));
   } else {
 #pragma unroll
     for (int e = 0; e < COUNT; ++e) {
-      if (n + e < g.n) out[e] = from_f<T>(g.res != nullptr ? v[e] + to_f(res[e]) : v[e]);
+      if (n + e < g.n) out[e] = y[e];
     }
   }
 }
 
-template <typename T, int MT, int WAVES>
+// MT blocks of 16 rows by TN quarters of a tile's 64 columns of out (1 or 4); AHEAD tiles of K on their way at
+// a time. Rows past M read 0.
+template <typename T, int MT, int TN, int WAVES, int AHEAD>
 __global__ __launch_bounds__(64 * WAVES) void linear8_rows_kernel(const Lin8Geom g) {
-  constexpr int kAhead = 4;  // tiles on their way at a time
-  __shared__ i4 parts[WAVES][MT][64];
+  __shared__ i4 parts[WAVES][MT * TN][64];
   const int tid = threadIdx.x, lane = tid & 63, l16 = lane & 15, lg = lane >> 4;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int tile = blockIdx.x >> 2, quarter = blockIdx.x & 3;
+  const int tile = blockIdx.x * TN >> 2, quarter = blockIdx.x * TN & 3;
   const int64_t m0 = static_cast<int64_t>(blockIdx.y) * (16 * MT);
   const __amdgpu_buffer_rsrc_t rc = codes_rsrc(g, m0, 16 * MT);
   const __amdgpu_buffer_rsrc_t rq =
       rsrc8(g.q + static_cast<int64_t>(tile) * g.tk * kTileBytes, static_cast<int64_t>(g.tk) * kTileBytes);
-  i4 acc[MT];
+  i4 acc[TN][MT];
 #pragma unroll
-  for (int i = 0; i < MT; ++i) acc[i] = i4{0, 0, 0, 0};
-  unsigned xoff[MT];
+  for (int j = 0; j < TN; ++j) {
 #pragma unroll
-  for (int i = 0; i < MT; ++i) {
-    xoff[i] = m0 + 16 * i + l16 < g.m ? (16 * i + l16) * static_cast<unsigned>(g.c_ld) + 16 * lg : kNowhere;
+    for (int i = 0; i < MT; ++i) acc[j][i] = i4{0, 0, 0, 0};
   }
+  const unsigned xoff = l16 * static_cast<unsigned>(g.c_ld) + 16 * lg, xrow = 16 * static_cast<unsigned>(g.c_ld);
   const unsigned qoff = quarter * 1024 + lane * 16;
   const int tiles = (g.k + 63) / 64;
-  for (int t0 = w; t0 < tiles; t0 += WAVES * kAhead) {
-    i4 a[kAhead], b[kAhead][MT];
+  for (int t0 = w; t0 < tiles; t0 += WAVES * AHEAD) {
+    i4 a[AHEAD][TN], b[AHEAD][MT];
 #pragma unroll
-    for (int u = 0; u < kAhead; ++u) {
+    for (int u = 0; u < AHEAD; ++u) {
       const int t = t0 + u * WAVES;
       const bool live = t < tiles;
-      a[u] = __builtin_bit_cast(i4, __builtin_amdgcn_raw_buffer_load_b128(
-          rq, live ? qoff + t * kTileBytes : kNowhere, 0, 2));
+#pragma unroll
+      for (int j = 0; j < TN; ++j) {
+        a[u][j] = __builtin_bit_cast(i4, __builtin_amdgcn_raw_buffer_load_b128(
+            rq, live ? qoff + j * 1024 + t * kTileBytes : kNowhere, 0, 2));
+      }
 #pragma unroll
       for (int i = 0; i < MT; ++i) {
         b[u][i] = __builtin_bit_cast(i4, __builtin_amdgcn_raw_buffer_load_b128(
-            rc, live ? xoff[i] + t * 64 : kNowhere, 0, 0));
+            rc, live ? xoff + i * xrow + t * 64 : kNowhere, 0, 0));
       }
     }
 #pragma unroll
-    for (int u = 0; u < kAhead; ++u) {
+    for (int u = 0; u < AHEAD; ++u) {
 #pragma unroll
-      for (int i = 0; i < MT; ++i) acc[i] = mma(a[u], b[u][i], acc[i]);
+      for (int i = 0; i < MT; ++i) {
+#pragma unroll
+        for (int j = 0; j < TN; ++j) acc[j][i] = mma(a[u][j], b[u][i], acc[j][i]);
+      }
     }
   }
 #pragma unroll
-  for (int i = 0; i < MT; ++i) parts[w][i][lane] = acc[i];
-  __syncthreads();
-  for (int i = w; i < MT; i += WAVES) {
-    i4 sum = parts[0][i][lane];
+  for (int j = 0; j < TN; ++j) {
 #pragma unroll
-    for (int v = 1; v < WAVES; ++v) sum += parts[v][i][lane];
+    for (int i = 0; i < MT; ++i) parts[w][i * TN + j][lane] = acc[j][i];
+  }
+  __syncthreads();
+  constexpr int kWide = TN > 1 ? 2 : 1;
+  for (int p = w; p < MT * TN / kWide; p += WAVES) {
+    i4 sum[kWide];
+#pragma unroll
+    for (int e = 0; e < kWide; ++e) {
+      sum[e] = parts[0][p * kWide + e][lane];
+#pragma unroll
+      for (int v = 1; v < WAVES; ++v) sum[e] += parts[v][p * kWide + e][lane];
+    }
+    const int i = p * kWide / TN, j = quarter + p * kWide % TN;
     const int64_t m = m0 + 16 * i + l16;
-    const int n = 64 * tile + 32 * (quarter >> 1) + 4 * (quarter & 1) + 8 * lg;
-    if (m < g.m && n < g.n) put<T, 4>(g, m, n, g.row_scales[m], &sum);
+    const int n = 64 * tile + 32 * (j >> 1) + 4 * (j & 1) + 8 * lg;
+    if (m < g.m && n < g.n) put<T, 4 * kWide>(g, m, n, g.row_scales[m], sum);
   }
 }
 
@@ -161,9 +192,11 @@ __device__ __forceinline__ Place place(unsigned id, unsigned tiles_m, unsigned t
   return Place{first + rest % high, static_cast<int>(rest / high)};
 }
 
-// Everything that is on its way into LDS has arrived, for all waves, and what they read was read.
+// Of what is on its way from memory all but the last LATER have arrived, for all waves, and what they read from
+// LDS was read.
+template <int LATER>
 __device__ __forceinline__ void stage_barrier() {
-  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(LATER) : "memory");
 }
 
 __device__ __forceinline__ void load_lds(__amdgpu_buffer_rsrc_t r, char* dst, unsigned off) {
@@ -171,119 +204,266 @@ __device__ __forceinline__ void load_lds(__amdgpu_buffer_rsrc_t r, char* dst, un
                                            static_cast<int>(off), 0, 0, 0);
 }
 
-// WM x WN waves, each 16 XI rows by 64 columns.
-template <typename T, int WM, int WN, int XI>
-__global__ __launch_bounds__(64 * WM * WN) void linear8_tile_kernel(const Lin8Geom g, unsigned tiles_m,
-                                                                    unsigned tiles_n, unsigned band) {
-  constexpr int kWaves = WM * WN, BM = 16 * XI * WM, BN = 64 * WN;
-  constexpr int kStage = (BM + BN) * 128, kUnits = (BM + BN) / 8 / kWaves;
-  static_assert((BM / 8) % kWaves == 0 && (BN / 8) % kWaves == 0, "units of one kind for all waves");
-  __shared__ __attribute__((aligned(128))) char stages[2 * kStage];
-  const int tid = threadIdx.x, lane = tid & 63, l16 = lane & 15, lg = lane >> 4;
-  const int w = __builtin_amdgcn_readfirstlane(tid >> 6), wm = w / WN, wn = w % WN;
-  const Place at = place(blockIdx.x, tiles_m, tiles_n, band);
-  const int64_t m0 = at.m * BM;
-  const int tile0 = at.n * WN;  // the first of the workgroup's tile rows of the weight
-  const int64_t row_bytes = static_cast<int64_t>(g.tk) * kTileBytes;
-  const __amdgpu_buffer_rsrc_t rc = codes_rsrc(g, m0, BM);
-  const __amdgpu_buffer_rsrc_t rq = rsrc8(g.q + tile0 * row_bytes, min(WN, g.tiles - tile0) * row_bytes);
-  // unit u of the workgroup's loads is 1 KB: 8 rows of codes, or a quarter of a tile
-  constexpr int kOfCodes = BM / 8 / kWaves;
-  unsigned off[kUnits];
+// Neighbouring lanes hold rows 2 t (even lane) and 2 t + 1, two pieces of 16 bytes each that lie next to one another
+// over four lanes. After the exchange `first` of both lanes is row 2 t and `second` row 2 t + 1, the even
+// lane's their first pieces: a store then writes whole lines of 128 bytes. Stores of half lines reach 2.1 TB/s here,
+// these 4 and more.
+__device__ __forceinline__ void exchange(bool odd, u32x4& first, u32x4& second) {
 #pragma unroll
-  for (int v = 0; v < kUnits; ++v) {
-    if (v < kOfCodes) {
-      const int r = 8 * (v * kWaves + w) + (lane >> 3);
-      off[v] = m0 + r < g.m ? r * static_cast<unsigned>(g.c_ld) + 16 * ((lane & 7) ^ (lane >> 3)) : kNowhere;
-    } else {
-      const int u = (v - kOfCodes) * kWaves + w, tile = u >> 3;
-      off[v] = tile0 + tile < g.tiles ? tile * static_cast<unsigned>(row_bytes) + (u & 7) * 1024 + lane * 16
-                                      : kNowhere;
-    }
+  for (int e = 0; e < 4; ++e) {
+    const uint32_t got = __builtin_amdgcn_mov_dpp(odd ? first[e] : second[e], 0xb1, 0xf, 0xf, true);
+    first[e] = odd ? got : first[e];
+    second[e] = odd ? second[e] : got;
   }
-  const auto fetch = [&](char* stage) {
+}
+
+// A piece of a row's outputs, at any alignment; the row ends at column `end`.
+template <typename T>
+__device__ __forceinline__ void store_piece(T* row, int n, int end, const u32x4& piece) {
+  constexpr int kPiece = 16 / static_cast<int>(sizeof(T));
+  if (n + kPiece <= end) {
+    __builtin_memcpy(row + n, &piece, sizeof(piece));
+  } else {
+    T t[kPiece];
+    __builtin_memcpy(t, &piece, sizeof(t));
 #pragma unroll
-    for (int v = 0; v < kUnits; ++v) {
-      char* const dst = stage + (v < kOfCodes ? v * kWaves + w : BM / 8 + (v - kOfCodes) * kWaves + w) * 1024;
-      load_lds(v < kOfCodes ? rc : rq, dst, off[v]);
-      off[v] += v < kOfCodes ? 128 : 2 * kTileBytes;
-    }
-  };
-  i4 acc[4][XI];
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-#pragma unroll
-    for (int i = 0; i < XI; ++i) acc[j][i] = i4{0, 0, 0, 0};
-  }
-  const auto multiply = [&](const char* stage) {
-    const char* const rows = stage + (16 * XI * wm + l16) * 128;
-    const char* const tiles = stage + BM * 128 + wn * (2 * kTileBytes) + lane * 16;
-#pragma unroll
-    for (int kk = 0; kk < 2; ++kk) {
-      i4 a[4], b[XI];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) a[j] = *reinterpret_cast<const i4*>(tiles + kk * kTileBytes + j * 1024);
-#pragma unroll
-      for (int i = 0; i < XI; ++i) {
-        b[i] = *reinterpret_cast<const i4*>(rows + i * 2048 + 16 * ((4 * kk + lg) ^ (l16 & 7)));
-      }
-#pragma unroll
-      for (int i = 0; i < XI; ++i) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) acc[j][i] = mma(a[j], b[i], acc[j][i]);
-      }
-    }
-  };
-  const int steps = g.tk / 2;
-  fetch(stages);
-  int now = 0;
-#pragma unroll 1
-  for (int s = 1; s < steps; ++s) {
-    stage_barrier();
-    fetch(stages + (kStage - now));
-    multiply(stages + now);
-    now = kStage - now;
-  }
-  stage_barrier();
-  multiply(stages + now);
-#pragma unroll
-  for (int i = 0; i < XI; ++i) {
-    const int64_t m = m0 + 16 * XI * wm + 16 * i + l16;
-    if (m >= g.m) continue;
-    const float rs = g.row_scales[m];
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int n = 64 * (tile0 + wn) + 32 * h + 8 * lg;
-      const i4 pair[2] = {acc[2 * h][i], acc[2 * h + 1][i]};
-      if (n < g.n) put<T, 8>(g, m, n, rs, pair);
+    for (int e = 0; e < kPiece; ++e) {
+      if (n + e < end) row[n + e] = t[e];
     }
   }
 }
 
-template <typename T, int MT, int WAVES>
-int launch_few(const Lin8Geom& g, hipStream_t stream) {
-  const dim3 grid(4 * g.tiles, static_cast<unsigned>((g.m + 16 * MT - 1) / (16 * MT)));
-  hipLaunchKernelGGL((linear8_rows_kernel<T, MT, WAVES>), grid, dim3(64 * WAVES), 0, stream, g);
+// A workgroup of WM x WN waves, each 16 XI rows by 64 columns, takes tile after tile and walks K in steps of 128.
+// A step's codes go from memory into one of two LDS stages without passing through registers, rows of 128
+// bytes whose eight pieces of 16 are exchanged by the row's low bits: eight lanes that read one column's
+// pieces of eight rows meet all banks. The weight's operands, which few waves share, come straight into
+// registers: LDS then moves half as much. In each half of a step the products of one half are under way while
+// the codes of the next are read and each operand of the weight is followed by the next step's; one barrier a
+// step. The next tile's first step is on its way while a tile is written.
+//
+// WHOLE: out is written by every lane in 16 bytes at a time, what lies outside past the extent, so that the number
+// of stores is known. Else rows may lie at any alignment and end within a piece.
+template <typename T, int WM, int WN, int XI, bool WHOLE, bool RES>
+__global__ __launch_bounds__(64 * WM * WN, 2) void linear8_tile_kernel(const Lin8Geom g, unsigned tiles_m,
+                                                                    unsigned tiles_n, unsigned band) {
+  constexpr int kWaves = WM * WN, BM = 16 * XI * WM, kStage = BM * 128, kUnits = BM / 8 / kWaves;
+  static_assert(BM / 8 % kWaves == 0 && XI % 4 == 0, "whole units and reads for each wave");
+  __shared__ __attribute__((aligned(128))) char stages[2 * kStage];
+  const int tid = threadIdx.x, lane = tid & 63, l16 = lane & 15, lg = lane >> 4;
+  const int w = __builtin_amdgcn_readfirstlane(tid >> 6), wm = w / WN, wn = w % WN;
+  const unsigned all = tiles_m * tiles_n;
+  const int64_t row_bytes = static_cast<int64_t>(g.tk) * kTileBytes;
+  const int steps = g.tk / 2;
+
+  // The codes' loads, units of 8 rows (1 KB), and where they have come to. Rows past M lie past the extent,
+  // and so does everything after the last tile.
+  __amdgpu_buffer_rsrc_t rc;
+  unsigned coff, c_id = blockIdx.x;
+  int c_step = 0;
+  const unsigned unit = 8 * kWaves * static_cast<unsigned>(g.c_ld);
+  const auto aim_codes = [&]() {
+    const int64_t m0 = place(min(c_id, all - 1), tiles_m, tiles_n, band).m * BM;
+    const int64_t left = g.m - m0 < BM ? g.m - m0 : BM;
+    rc = rsrc8(g.codes + m0 * g.c_ld, c_id < all ? (left - 1) * g.c_ld + (g.k + 15) / 16 * 16 : 0);
+    coff = (8 * w + (lane >> 3)) * static_cast<unsigned>(g.c_ld) + 16 * ((lane & 7) ^ (lane >> 3));
+  };
+  const auto fetch = [&](int stage) {
+#pragma unroll
+    for (int v = 0; v < kUnits; ++v) load_lds(rc, stages + stage + (v * kWaves + w) * 1024, coff + v * unit);
+    coff += 128;
+    if (++c_step == steps) {
+      c_step = 0;
+      c_id += gridDim.x;
+      aim_codes();
+    }
+  };
+
+  // The same of the weight's operands; tile rows past N lie past the extent.
+  __amdgpu_buffer_rsrc_t rq;
+  unsigned qoff, q_id = blockIdx.x;
+  int q_step = 0;
+  const auto aim_weight = [&]() {
+    const int tile0 = place(min(q_id, all - 1), tiles_m, tiles_n, band).n * WN;
+    rq = rsrc8(g.q + tile0 * row_bytes, q_id < all ? min(WN, g.tiles - tile0) * row_bytes : 0);
+    qoff = wn * static_cast<unsigned>(row_bytes) + lane * 16;
+  };
+  const auto step_weight = [&]() {
+    qoff += 2 * kTileBytes;
+    if (++q_step == steps) {
+      q_step = 0;
+      q_id += gridDim.x;
+      aim_weight();
+    }
+  };
+
+  i4 acc[4][XI], a[2][4], b[2][XI];
+  const auto weight = [&](int kk, int j) {
+    a[kk][j] = __builtin_bit_cast(
+        i4, __builtin_amdgcn_raw_buffer_load_b128(rq, qoff + (4 * kk + j) * 1024, 0, 0));
+  };
+  const char* const rows = stages + (16 * XI * wm + l16) * 128;
+  const int piece[2] = {16 * (lg ^ (l16 & 7)), 16 * ((4 + lg) ^ (l16 & 7))};
+  const auto read = [&](int stage, int kk, int i) {
+    b[kk][i] = *reinterpret_cast<const i4*>(rows + stage + piece[kk] + i * 2048);
+  };
+  // half kk of a step; `stage` holds the half after it
+  const auto half = [&](int kk, int stage) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+#pragma unroll
+      for (int i = 0; i < XI; ++i) acc[j][i] = mma(a[kk][j], b[kk][i], acc[j][i]);
+      weight(kk, j);
+#pragma unroll
+      for (int i = 0; i < XI / 4; ++i) read(stage, 1 - kk, j * (XI / 4) + i);
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+#pragma unroll
+      for (int i = 0; i < XI / 4; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);  // a read from LDS
+        __builtin_amdgcn_sched_group_barrier(0x008, 4, 0);  // products
+      }
+      __builtin_amdgcn_sched_group_barrier(0x020, 1, 0);  // a load
+    }
+    __builtin_amdgcn_sched_barrier(0);
+  };
+
+  aim_codes();
+  aim_weight();
+  fetch(0);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) weight(0, j);
+  stage_barrier<0>();
+  int now = 0;
+  fetch(kStage);
+  __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) weight(1, j);
+  step_weight();
+#pragma unroll
+  for (int i = 0; i < XI; ++i) read(0, 0, i);
+  // loads and stores count down in the order of their issue: after a stage's fetch come the weight's 8 loads
+  // in the two halves until it is needed, and at a tile's first step the stores of the tile before
+  constexpr int kStores = (sizeof(T) == 4 ? 4 : 2) * XI;
+  bool stored = false;
+  for (unsigned id = blockIdx.x; id < all; id += gridDim.x) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+#pragma unroll
+      for (int i = 0; i < XI; ++i) acc[j][i] = i4{0, 0, 0, 0};
+    }
+#pragma unroll 1
+    for (int s = 0; s < steps; ++s) {
+      half(0, now);
+      if (stored) {
+        stored = false;
+        stage_barrier<8 + kStores>();
+      } else {
+        stage_barrier<8>();
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      fetch(now);
+      __builtin_amdgcn_sched_barrier(0);
+      now = kStage - now;
+      half(1, now);
+      step_weight();
+    }
+    const Place at = place(id, tiles_m, tiles_n, band);
+    const int64_t m0 = at.m * BM;
+    const int left = static_cast<int>(g.m - m0 < BM ? g.m - m0 : BM);  // rows
+    const int m1 = 16 * XI * wm + l16, n0 = 64 * (at.n * WN + wn) + 8 * lg;
+    // the scales before the first store: a wait for them waits for every store before them
+    f4 sc[4];
+    float rs[XI];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int n = n0 + 32 * (j >> 1) + 4 * (j & 1);
+      sc[j] = n < g.n ? *reinterpret_cast<const f4*>(g.scales + n) : f4{0.f, 0.f, 0.f, 0.f};
+    }
+#pragma unroll
+    for (int i = 0; i < XI; ++i) rs[i] = g.row_scales[m0 + min(m1 + 16 * i, left - 1)];
+    T* const out = static_cast<T*>(g.out);
+    __amdgpu_buffer_rsrc_t ro;
+    if constexpr (WHOLE) {
+      ro = rsrc8(out + m0 * g.o_ld, ((left - 1) * g.o_ld + g.n) * static_cast<int64_t>(sizeof(T)));
+    }
+    constexpr int kPiece = 16 / static_cast<int>(sizeof(T));  // elements
+    const bool odd = (lane & 1) != 0;
+#pragma unroll
+    for (int i = 0; i < XI; ++i) {
+      const int m = m1 + 16 * i;
+      u32x4 y[2][8 / kPiece];  // [half of the 64 columns][pieces of 16 bytes]
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        float v[8];
+        T t[8];
+        if constexpr (RES) {
+          load_res(static_cast<const T*>(g.res) + (m0 + min(m, left - 1)) * g.r_ld, n0 + 32 * h, g.n, v);
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          t[e] = from_f32<T>(scaled<RES>(acc[2 * h + e / 4][i][e % 4], rs[i], sc[2 * h + e / 4][e % 4],
+                                         RES ? v[e] : 0.f));
+        }
+        __builtin_memcpy(y[h], t, sizeof(t));
+      }
+#pragma unroll
+      for (int p = 0; p < 8 / kPiece; ++p) {
+        // 16 bits: the halves' pieces; FP32: the two of a half
+        u32x4 first = y[kPiece == 4 ? p : 0][0], second = y[kPiece == 4 ? p : 1][8 / kPiece - 1];
+        exchange(odd, first, second);
+        const int n = kPiece == 4 ? n0 + 32 * p + (odd ? 4 : 0) : n0 + (odd ? 32 : 0), m2 = m - odd;
+        if constexpr (WHOLE) {
+          const unsigned pitch = static_cast<unsigned>(g.o_ld) * static_cast<unsigned>(sizeof(T));
+          const unsigned to = m2 * pitch + n * static_cast<unsigned>(sizeof(T));
+          __builtin_amdgcn_raw_buffer_store_b128(first, ro, n < g.n && m2 < left ? to : kNowhere, 0, 0);
+          __builtin_amdgcn_raw_buffer_store_b128(second, ro, n < g.n && m2 + 1 < left ? to + pitch : kNowhere, 0,
+                                                 0);
+        } else {
+          T* const to = out + (m0 + m2) * g.o_ld;
+          if (m2 < left) store_piece(to, n, g.n, first);
+          if (m2 + 1 < left) store_piece(to + g.o_ld, n, g.n, second);
+        }
+      }
+      // one row block's residual and addresses at a time: more would not fit the registers
+      if constexpr (RES || !WHOLE) __builtin_amdgcn_sched_barrier(0);
+    }
+    stored = WHOLE;
+  }
+}
+
+template <typename T, int MT, int TN, int WAVES, int AHEAD>
+int launch_rows(const Lin8Geom& g, hipStream_t stream) {
+  const dim3 grid(4 / TN * g.tiles, static_cast<unsigned>((g.m + 16 * MT - 1) / (16 * MT)));
+  hipLaunchKernelGGL((linear8_rows_kernel<T, MT, TN, WAVES, AHEAD>), grid, dim3(64 * WAVES), 0, stream, g);
   return check_launch("m3_linear8");
 }
 
 template <typename T, int WM, int WN, int XI>
-int launch_tile(const Lin8Geom& g, hipStream_t stream) {
+int launch_tile(const Lin8Geom& g, int a_cu, hipStream_t stream) {
   constexpr int BM = 16 * XI * WM;
-  const int64_t tm = (g.m + BM - 1) / BM, tn = (g.tiles + WN - 1) / WN;
-  if (tm * tn >= INT32_MAX) return fail(M3_EUNSUPPORTED, "m3_linear8: too many tiles");
-  hipLaunchKernelGGL((linear8_tile_kernel<T, WM, WN, XI>), dim3(static_cast<unsigned>(tm * tn)),
-                     dim3(64 * WM * WN), 0, stream, g, static_cast<unsigned>(tm), static_cast<unsigned>(tn),
-                     8u);
+  const int64_t tm = (g.m + BM - 1) / BM, tn = (g.tiles + WN - 1) / WN, all = tm * tn;
+  if (all >= 1 << 30) return fail(M3_EUNSUPPORTED, "m3_linear8: over 2^30 tiles of out");
+  const unsigned grid = static_cast<unsigned>(all < a_cu * kCus ? all : a_cu * kCus);
+  const bool res = g.res != nullptr;
+  const auto kernel = g.whole ? (res ? linear8_tile_kernel<T, WM, WN, XI, true, true>
+                                     : linear8_tile_kernel<T, WM, WN, XI, true, false>)
+                              : (res ? linear8_tile_kernel<T, WM, WN, XI, false, true>
+                                     : linear8_tile_kernel<T, WM, WN, XI, false, false>);
+  hipLaunchKernelGGL(kernel, dim3(grid), dim3(64 * WM * WN), 0, stream, g, static_cast<unsigned>(tm),
+                     static_cast<unsigned>(tn), 8u);
   return check_launch("m3_linear8");
 }
 
 template <typename T>
 int launch8(const Lin8Geom& g, hipStream_t stream) {
-  if (g.m <= 16) return launch_few<T, 1, 8>(g, stream);
-  if (g.m <= 64) return launch_few<T, 4, 8>(g, stream);
-  if ((g.m + 255) / 256 * ((g.tiles + 3) / 4) >= 256) return launch_tile<T, 2, 4, 8>(g, stream);
-  return launch_tile<T, 2, 2, 4>(g, stream);
+  if (g.m <= 16) return launch_rows<T, 1, 1, 8, 4>(g, stream);
+  if (g.tiles * ((g.m + 31) / 32) <= 2 * kCus) return launch_rows<T, 2, 4, 8, 2>(g, stream);
+  const int64_t tm = (g.m + 127) / 128, large = tm * ((g.tiles + 7) / 8), small = tm * ((g.tiles + 1) / 2);
+  if (3 * ((large + kCus - 1) / kCus) <= 2 * ((small + 2 * kCus - 1) / (2 * kCus))) {
+    return launch_tile<T, 1, 8, 8>(g, 1, stream);
+  }
+  return launch_tile<T, 2, 2, 4>(g, 2, stream);
 }
 
 int validate(const m3_linear8_args& a) {
@@ -345,11 +525,14 @@ extern "C" int m3_linear8(const m3_linear8_args* args, hipStream_t stream) {
   const int rc = validate(a);
   if (rc != M3_OK) return rc;
   if (a.m == 0 || a.n == 0) return M3_OK;
+  const int64_t es = elem_size(a.dtype), pitch = a.out.stride[0] * es;
+  const bool whole = reinterpret_cast<uintptr_t>(a.out.ptr) % 16 == 0 && a.n * es % 16 == 0 &&
+                     (a.m == 1 || (pitch % 16 == 0 && pitch < (1 << 23)));
   const Lin8Geom g{reinterpret_cast<const char*>(a.codes), a.row_scales,
                    reinterpret_cast<const char*>(a.q), a.scales, a.residual.ptr, a.out.ptr,
                    a.codes_stride, a.residual.stride[0], a.out.stride[0], a.m, static_cast<int>(a.n),
                    static_cast<int>(a.k), static_cast<int>((a.k + 127) / 128 * 2),
-                   static_cast<int>((a.n + 63) / 64)};
+                   static_cast<int>((a.n + 63) / 64), whole};
   switch (a.dtype) {
     case M3_F32: return launch8<float>(g, stream);
     case M3_BF16: return launch8<__bf16>(g, stream);

@@ -24,6 +24,14 @@ __device__ __forceinline__ float to_f(_Float16 x) { return static_cast<float>(x)
 template <typename T>
 __device__ __forceinline__ T from_f(float x) { return static_cast<T>(x); }
 
+// The same of an FP32 value that is rounded to FP32 first: to f16 the compiler may otherwise take a product
+// and its rounding as one instruction, which rounds once.
+template <typename T>
+__device__ __forceinline__ T from_f32(float x) {
+  if constexpr (__is_same(T, _Float16)) asm("" : "+v"(x));
+  return static_cast<T>(x);
+}
+
 // Round an FP32 value to the activation type and back (the cast points of the reference).
 template <typename T>
 __device__ __forceinline__ float rnd(float x) { return to_f(from_f<T>(x)); }

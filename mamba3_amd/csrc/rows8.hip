@@ -268,6 +268,47 @@ __global__ __launch_bounds__(256) void rows8_kernel(const Rows8Geom g) {
   if (lane == 0) g.scales[r] = c.scale;
 }
 
+// code * scale in FP32, rounded to T: what the rows stand for. A lane writes 16 bytes; LANES lanes take a row.
+template <typename T>
+__global__ __launch_bounds__(256) void values8_kernel(const int8_t* codes, int64_t c_ld, const float* scales,
+                                                      T* out, int64_t o_ld, int rows, int dim, int lanes_log2) {
+  constexpr int kPiece = 16 / static_cast<int>(sizeof(T));
+  const int lanes = 1 << lanes_log2, lane = threadIdx.x & (lanes - 1);
+  const int64_t row = (static_cast<int64_t>(blockIdx.x) << (8 - lanes_log2)) + (threadIdx.x >> lanes_log2);
+  if (row >= rows) return;
+  const float scale = scales[row];
+  const int8_t* const from = codes + row * c_ld;
+  T* const to = out + row * o_ld;
+#pragma unroll 4
+  for (int at = kPiece * lane; at < dim; at += kPiece * lanes) {
+    int8_t c[kPiece];  // rows of codes reach to a multiple of 16
+    __builtin_memcpy(c, __builtin_assume_aligned(from + at, kPiece), sizeof(c));
+    T t[kPiece];
+#pragma unroll
+    for (int e = 0; e < kPiece; ++e) t[e] = from_f32<T>(static_cast<float>(c[e]) * scale);
+    if (at + kPiece <= dim) {
+      __builtin_memcpy(to + at, t, sizeof(t));
+    } else {
+#pragma unroll
+      for (int e = 0; e < kPiece; ++e) {
+        if (at + e < dim) to[at + e] = t[e];
+      }
+    }
+  }
+}
+
+template <typename T>
+int launch_values(const m3_rows8_values_args& a, hipStream_t stream) {
+  constexpr int kPiece = 16 / static_cast<int>(sizeof(T));
+  int log2 = 0;
+  while (log2 < 8 && (kPiece << log2) < a.dim) ++log2;
+  const int64_t per = 256 >> log2;
+  hipLaunchKernelGGL(values8_kernel<T>, dim3(static_cast<unsigned>((a.rows + per - 1) / per)), dim3(256), 0,
+                     stream, a.codes, a.codes_stride, a.scales, static_cast<T*>(a.out.ptr), a.out.stride[0],
+                     static_cast<int>(a.rows), static_cast<int>(a.dim), log2);
+  return check_launch("m3_rows8_values");
+}
+
 template <typename T, typename TA, bool NORM, bool ADD, int TPR, int CH>
 int launch_one(const Rows8Geom& g, hipStream_t stream) {
   const unsigned blocks = TPR == 64 ? (static_cast<unsigned>(g.rows) + 3) / 4 : g.rows;
@@ -310,15 +351,29 @@ bool meets(const Range& a, const Range& b) {
   return a.from != nullptr && b.from != nullptr && a.from < b.to && b.from < a.to;
 }
 
-int validate(const m3_rows8_args& a) {
-  if (a.rows < 0 || a.dim < 0) return fail(M3_EINVAL, "m3_rows8: negative dimensions");
-  if (a.rows >= (1 << 30) || a.dim > M3_LINEAR8_MAX_K) {
-    return fail(M3_EUNSUPPORTED, "m3_rows8: %lld rows of %lld: below 2^30, of at most %d",
-                static_cast<long long>(a.rows), static_cast<long long>(a.dim), M3_LINEAR8_MAX_K);
+int check_sizes(const char* name, int64_t rows, int64_t dim) {
+  if (rows < 0 || dim < 0) return fail(M3_EINVAL, "%s: negative dimensions", name);
+  if (rows >= (1 << 30) || dim > M3_LINEAR8_MAX_K) {
+    return fail(M3_EUNSUPPORTED, "%s: %lld rows of %lld: below 2^30, of at most %d", name,
+                static_cast<long long>(rows), static_cast<long long>(dim), M3_LINEAR8_MAX_K);
   }
-  if (a.rows == 0) return M3_OK;
-  if (a.dim == 0) return fail(M3_EUNSUPPORTED, "m3_rows8: dim 0");
+  if (rows != 0 && dim == 0) return fail(M3_EUNSUPPORTED, "%s: dim 0", name);
+  return M3_OK;
+}
+
+int check_codes(const char* name, const int8_t* codes, int64_t stride, const float* scales, int64_t dim) {
+  if (codes == nullptr || scales == nullptr) return fail(M3_EINVAL, "%s: codes or scales are NULL", name);
+  if (reinterpret_cast<uintptr_t>(codes) % 16 != 0 || stride % 16 != 0 ||
+      reinterpret_cast<uintptr_t>(scales) % 4 != 0) {
+    return fail(M3_EUNSUPPORTED, "%s: rows of codes must be 16-byte aligned, scales 4-byte", name);
+  }
+  if (stride < dim) return fail(M3_EINVAL, "%s: rows of codes overlap", name);
+  return M3_OK;
+}
+
+int validate(const m3_rows8_args& a) {
   int rc;
+  if ((rc = check_sizes("m3_rows8", a.rows, a.dim)) || a.rows == 0) return rc;
   if ((rc = check_tensor(a.x, "x", 2, a.dim, true, -1)) ||
       (rc = check_tensor(a.weight, "weight", 1, a.dim, false, -1)) ||
       (rc = check_tensor(a.add, "add", 2, a.dim, false, a.x.dtype == M3_F32 ? -1 : a.x.dtype)) ||
@@ -328,15 +383,8 @@ int validate(const m3_rows8_args& a) {
   if (present(a.add) && !present(a.weight)) return fail(M3_EINVAL, "m3_rows8: add needs weight");
   if (present(a.sum_out) && !present(a.add)) return fail(M3_EINVAL, "m3_rows8: sum_out needs add");
   if (present(a.weight) && !(a.eps >= 0.f)) return fail(M3_EINVAL, "m3_rows8: eps must be >= 0");
-  if (a.codes == nullptr || a.scales == nullptr) {
-    return fail(M3_EINVAL, "m3_rows8: codes or scales are NULL");
-  }
-  if (reinterpret_cast<uintptr_t>(a.codes) % 16 != 0 || a.codes_stride % 16 != 0 ||
-      reinterpret_cast<uintptr_t>(a.scales) % 4 != 0) {
-    return fail(M3_EUNSUPPORTED, "m3_rows8: rows of codes must be 16-byte aligned, scales 4-byte");
-  }
+  if ((rc = check_codes("m3_rows8", a.codes, a.codes_stride, a.scales, a.dim))) return rc;
   const int64_t whole = (a.dim + 15) / 16 * 16;
-  if (a.codes_stride < whole) return fail(M3_EINVAL, "m3_rows8: rows of codes overlap");
   if (a.rows > 1 && present(a.sum_out) && a.sum_out.stride[0] < a.dim) {
     return fail(M3_EINVAL, "m3_rows8: rows of sum_out overlap");
   }
@@ -362,8 +410,39 @@ int validate(const m3_rows8_args& a) {
   return M3_OK;
 }
 
+int validate(const m3_rows8_values_args& a) {
+  int rc;
+  if ((rc = check_sizes("m3_rows8_values", a.rows, a.dim)) || a.rows == 0) return rc;
+  if ((rc = check_codes("m3_rows8_values", a.codes, a.codes_stride, a.scales, a.dim)) ||
+      (rc = check_tensor(a.out, "out", 2, a.dim, true, -1))) {
+    return rc;
+  }
+  if (a.rows > 1 && a.out.stride[0] < a.dim) return fail(M3_EINVAL, "m3_rows8_values: rows of out overlap");
+  const char* c = reinterpret_cast<const char*>(a.codes);
+  const char* f = reinterpret_cast<const char*>(a.scales);
+  const Range out = range(a.out, a.rows, a.dim);
+  if (meets(out, {c, c + (a.rows - 1) * a.codes_stride + a.dim}) || meets(out, {f, f + a.rows * 4})) {
+    return fail(M3_EINVAL, "m3_rows8_values: out overlaps codes or scales");
+  }
+  return M3_OK;
+}
+
 }  // namespace
 }  // namespace m3
+
+extern "C" int m3_rows8_values(const m3_rows8_values_args* args, hipStream_t stream) {
+  using namespace m3;
+  clear_error();
+  if (args == nullptr) return fail(M3_EINVAL, "m3_rows8_values: NULL args");
+  const int rc = validate(*args);
+  if (rc != M3_OK) return rc;
+  if (args->rows == 0) return M3_OK;
+  switch (args->out.dtype) {
+    case M3_F32: return launch_values<float>(*args, stream);
+    case M3_BF16: return launch_values<__bf16>(*args, stream);
+    default: return launch_values<_Float16>(*args, stream);
+  }
+}
 
 extern "C" int m3_rows8(const m3_rows8_args* args, hipStream_t stream) {
   using namespace m3;

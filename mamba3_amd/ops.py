@@ -911,8 +911,17 @@ class Rows8:
         return rows
 
     def dequantize(self, dtype: torch.dtype = torch.float32) -> torch.Tensor:
-        """The rows ``[..., K]`` as ``code * scale``, one product in FP32 rounded to ``dtype``."""
-        return torch.mul(self.codes, self.scales.unsqueeze(-1)).to(dtype)
+        """The rows ``[..., K]`` as ``code * scale``, one product in FP32 rounded to ``dtype``
+        (``m3_rows8_values``; rows off the GPU in torch)."""
+        if dtype not in _FLOAT_DTYPES or self.device.type != "cuda":
+            return torch.mul(self.codes, self.scales.unsqueeze(-1)).to(dtype)
+        width, rows = self.shape[-1], self.scales.numel()
+        out = torch.empty(self.shape, dtype=dtype, device=self.device)
+        if rows:
+            _hip.launch("m3_rows8_values", _hip.ROWS8_VALUES.pack(
+                rows, width, self.codes.data_ptr(), self._ld, self.scales.data_ptr(),
+                out.data_ptr(), _hip.dtype_code(dtype), 0, width, 1, 0, 0, 0), self.codes.get_device())
+        return out
 
 
 def _codes8(like: torch.Tensor, rows: int, width: int) -> tuple[torch.Tensor, int]:

@@ -166,15 +166,22 @@ def test_offsets_past_32_bits():
     assert got.numel() > 1 << 31 and (got[-3:] == 30).all() and not got[-2000:-3].any() and not got[:2000].any()
 
 
-def test_every_kernel_gives_the_same_bits():
-    """Sums are exact: a row's result does not depend on how many rows come with it."""
+@pytest.mark.parametrize("residual", [False, True])
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("n", [5000, 5003])
+def test_every_kernel_gives_the_same_bits(n, dtype, residual):
+    """Sums are exact, and an output's operations the same in all kernels: a row's result does not depend
+    on how many rows come with it."""
     g = torch.Generator().manual_seed(8)
-    codes, q, rs, s = _operands(3000, 5000, 333, g)
+    codes, q, rs, s = _operands(3000, n, 333, g)
     weight = ops.Weight8(q.to(DEV), s.to(DEV))
+    res = torch.randn(3000, n, generator=g).to(dtype).to(DEV) if residual else None
     with torch.inference_mode():
-        whole = ops.linear8(ops.Rows8(codes.to(DEV), rs.to(DEV)), weight)
+        whole = ops.linear8(ops.Rows8(codes.to(DEV), rs.to(DEV)), weight, res, dtype=dtype)
+        _check(whole, codes, q, rs, s, res)
         for m in (1, 2, 16, 17, 40, 64, 65, 128, 200, 500, 1500):
-            part = ops.linear8(ops.Rows8(codes[:m].to(DEV), rs[:m].to(DEV)), weight)
+            part = ops.linear8(ops.Rows8(codes[:m].to(DEV), rs[:m].to(DEV)), weight,
+                               None if res is None else res[:m], dtype=dtype)
             assert torch.equal(part, whole[:m]), m
 
 

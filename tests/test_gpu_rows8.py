@@ -200,6 +200,21 @@ def test_strides_and_shapes():
             assert none[0].shape == (0, 9, 200) and none[1].shape == (0, 9, 200)
 
 
+@pytest.mark.parametrize("k", [1, 3, 4, 5, 8, 31, 100, 1024, 1111, 2049, 8200])
+@pytest.mark.parametrize("dtype", [F32, BF16, F16, torch.float64])
+def test_values(k, dtype):
+    """What the rows stand for, the same FP32 product and rounding as torch's; a NaN scale's row is NaN."""
+    g = torch.Generator().manual_seed(k)
+    for m in (1, 7, 300):
+        codes = torch.randint(-128, 128, (m, k), generator=g, dtype=torch.int8)
+        scales = torch.rand(m, generator=g) / 100
+        scales[m // 2] = float("nan")
+        got = ops.Rows8(codes.to(DEV), scales.to(DEV)).dequantize(dtype)
+        want = (codes.float() * scales.unsqueeze(1)).to(dtype)
+        assert got.dtype == dtype and torch.equal(got.cpu().nan_to_num(9.0), want.nan_to_num(9.0))
+        assert torch.isnan(got[m // 2]).all()
+
+
 def test_what_is_written():
     """The C entry point: codes and scales of the rows and nothing else; the sum in x's place, or the add's."""
     g = torch.Generator().manual_seed(3)

@@ -222,10 +222,37 @@ def test_linear8_is_checked_on_the_host(lib):
         assert text in lib.m3_last_error(), (changes, lib.m3_last_error())
 
 
+def test_rows8_values_is_checked_on_the_host(lib):
+    call = lib.m3_rows8_values
+
+    def block(rows=4):
+        return _hip.Rows8ValuesArgs(rows, 100, 0x100000, 112, 0x200000, _hip.Tensor(0x300000, _hip.BF16, 0, (100, 1)))
+
+    assert call(None, None) == 1 and b"NULL" in lib.m3_last_error()
+    assert call(ctypes.byref(block(0)), None) == 0
+    for changes, code, text in (
+            (dict(rows=-1), 1, b"negative"), (dict(rows=1 << 30), 2, b"below 2^30"),
+            (dict(dim=131072), 2, b"at most 131071"), (dict(dim=0), 2, b"dim 0"),
+            (dict(codes=None), 1, b"NULL"), (dict(scales=None), 1, b"NULL"),
+            (dict(codes=0x100004), 2, b"aligned"), (dict(codes_stride=120), 2, b"aligned"),
+            (dict(scales=0x200001), 2, b"aligned"), (dict(codes_stride=96), 1, b"overlap"),
+            (dict(out=_hip.Tensor()), 1, b"out: required"),
+            (dict(out=_hip.Tensor(0x300000, _hip.BF16, 0, (200, 2))), 2, b"out: innermost"),
+            (dict(out=_hip.Tensor(0x300000, _hip.BF16, 0, (99, 1))), 1, b"rows of out"),
+            (dict(out=_hip.Tensor(0x100000 + 3 * 112 + 98, _hip.BF16, 0, (100, 1))), 1, b"out overlaps"),
+            (dict(out=_hip.Tensor(0x20000e, _hip.BF16, 0, (100, 1))), 1, b"out overlaps")):
+        args = block()
+        for field, value in changes.items():
+            setattr(args, field, value)
+        assert call(ctypes.byref(args), None) == code, (changes, lib.m3_last_error())
+        assert text in lib.m3_last_error(), (changes, lib.m3_last_error())
+
+
 def test_structs_match_the_header_layout(tmp_path):
     if shutil.which("gcc") is None:
         pytest.skip("gcc not available")
-    pairs = (("m3_rows8_args", _hip.Rows8Args, _hip.ROWS8), ("m3_linear8_args", _hip.Linear8Args, _hip.LINEAR8))
+    pairs = (("m3_rows8_args", _hip.Rows8Args, _hip.ROWS8), ("m3_linear8_args", _hip.Linear8Args, _hip.LINEAR8),
+             ("m3_rows8_values_args", _hip.Rows8ValuesArgs, _hip.ROWS8_VALUES))
     lines = ['#include "mamba3_hip.h"', "#include <stdio.h>", "int main(void) {",
              'printf("max - %d\\n", M3_LINEAR8_MAX_K);']
     for name, py, _ in pairs:
