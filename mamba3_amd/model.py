@@ -9,7 +9,8 @@ decode step. ``in_proj`` / ``out_proj`` and the residual RMSNorm stay in torch
 (hipBLASLt), except in a decode step of a small batch with 16-bit weights: there both
 projections run on ``ops.linear`` (``m3_linear``), the block's RMSNorm fused into
 ``in_proj`` and its residual add into ``out_proj`` (``ops.linear4`` after
-``Mamba3.quantize_decode``, with the weights in 4 bits).
+``Mamba3.quantize_decode``, with the weights in 4 bits). After ``Mamba3.quantize_prefill`` the
+other calls' projections run in 8 bits: ``ops.rms_norm8`` / ``ops.quantize8_rows`` and ``ops.linear8``.
 
 Scope: inference (``forward``, ``prefill``, ``step``, ``cuda_graph``) on ROCm devices.
 Autograd through the mixer and CPU execution raise ``RuntimeError``. ``compile`` and
@@ -122,20 +123,47 @@ class _Mamba3Mixer(nn.Module):
             self.direction_logit = nn.Parameter(torch.zeros(d_model))
         # 4-bit copies of the projections for decode steps, by name (quantize_decode)
         self._decode4: dict[str, tuple[ops.Weight4, tuple[object, ...]]] = {}
+        # 8-bit copies for the other calls (quantize_prefill)
+        self._prefill8: dict[str, tuple[ops.Weight8, tuple[object, ...]]] = {}
+
+    def _signed(self, held: dict[str, object]) -> dict[str, tuple]:
+        """Copies of the projections by name, each with what its weight is now."""
+        return {name: (copy, _storage_signature(getattr(self, name).weight))
+                for name, copy in held.items()}
 
     def _hold4(self, held: dict[str, ops.Weight4]) -> None:
         """Take 4-bit copies of the projections, whose values the weights hold by now."""
-        self._decode4 = {name: (copy, _storage_signature(getattr(self, name).weight))
-                         for name, copy in held.items()}
+        self._decode4 = self._signed(held)
+
+    def _held(self, copies: dict[str, tuple], name: str, maker: str):
+        """The projection's copy, if there is one; refused once the weight has changed."""
+        if name not in copies:
+            return None
+        held, then = copies[name]
+        if not _same_storage(_storage_signature(getattr(self, name).weight), then):
+            raise RuntimeError(f"{name}.weight changed since {maker}; call it again")
+        return held
 
     def _weight4(self, name: str) -> ops.Weight4 | None:
-        """The projection's 4-bit copy, if there is one; refused once the weight has changed."""
-        if name not in self._decode4:
-            return None
-        held, then = self._decode4[name]
-        if not _same_storage(_storage_signature(getattr(self, name).weight), then):
-            raise RuntimeError(f"{name}.weight changed since quantize_decode; call it again")
-        return held
+        return self._held(self._decode4, name, "quantize_decode")
+
+    def _weight8(self, name: str) -> ops.Weight8 | None:
+        return self._held(self._prefill8, name, "quantize_prefill")
+
+    def _project(self, name: str, x: torch.Tensor | ops.Rows8,
+                 dtype: torch.dtype | None = None) -> torch.Tensor:
+        """``in_proj`` or ``out_proj`` of ``x``, in 8 bits if there is such a copy. Rows already in
+        8 bits (from ``ops.rms_norm8``) give ``dtype``; others what the projection itself gives."""
+        weight = self._weight8(name)
+        if isinstance(x, ops.Rows8):
+            return ops.linear8(x, weight, dtype=dtype)
+        module = getattr(self, name)
+        if weight is None:
+            return module(x)
+        dtype = _compute_dtype(x)
+        if dtype != module.weight.dtype and not torch.is_autocast_enabled(x.device.type):
+            return module(x)  # refuses rows of another type than its weight's
+        return ops.linear8(ops.quantize8_rows(x), weight, dtype=dtype)
 
     def _chunk(self) -> int:
         return (self.chunk_size if self.training and torch.is_grad_enabled()
@@ -150,13 +178,14 @@ class _Mamba3Mixer(nn.Module):
 
     # ---- forward / prefill
 
-    def forward(self, hidden_states: torch.Tensor, cache: _LayerCache | None = None, *,
-                return_cache: bool = False):
+    def forward(self, hidden_states: torch.Tensor | ops.Rows8, cache: _LayerCache | None = None, *,
+                return_cache: bool = False, dtype: torch.dtype | None = None):
+        """``dtype``: what ``in_proj`` gives where ``hidden_states`` are rows in 8 bits."""
         if not self.causal and (cache is not None or return_cache):
             raise ValueError("bidirectional Mamba3 does not support caches; "
                              "prefill and step require causal=True")
-        self._check_inference(hidden_states)
-        proj = self.in_proj(hidden_states)
+        self._check_inference(*(() if isinstance(hidden_states, ops.Rows8) else (hidden_states,)))
+        proj = self._project("in_proj", hidden_states, dtype)
         if not self.causal:
             # the reverse scan on a side stream, concurrent with the forward one: each direction
             # alone may leave CUs idle in its last round of workgroups
@@ -170,7 +199,7 @@ class _Mamba3Mixer(nn.Module):
         mixed, state, final_phase, final_k = ops.scan_projection(
             proj, self, cache=cache, want_cache=return_cache and self.causal,
             chunk_size=self._chunk(), concurrent=1 if self.causal else 2)
-        output = self.out_proj(mixed.flatten(-2))
+        output = self._project("out_proj", mixed.flatten(-2))
         if self.causal:
             if not return_cache:
                 return output
@@ -183,7 +212,7 @@ class _Mamba3Mixer(nn.Module):
         # order (no flip, no second projection).
         main.wait_stream(side)
         mixed_r.record_stream(main)
-        backward = self.out_proj(mixed_r.flatten(-2))
+        backward = self._project("out_proj", mixed_r.flatten(-2))
         blend = torch.sigmoid(self.direction_logit).to(dtype=output.dtype)
         return output * blend + backward * (1.0 - blend)
 
@@ -221,20 +250,25 @@ class _Mamba3Mixer(nn.Module):
 
     def step(self, hidden_states: torch.Tensor, cache: _LayerCache | None, *,
              inplace: bool = False, residual: torch.Tensor | None = None,
-             norm: _RMSNorm | None = None):
+             norm: _RMSNorm | None = None, dtype: torch.dtype | None = None):
         """One decode token. ``norm`` (the block's RMSNorm) is applied to ``hidden_states``
         first; with ``residual`` (``[batch, 1, d_model]``) the result is
         ``residual + out_proj(...)``. With 16-bit weights, ``in_proj`` runs on ``ops.linear``
         with the norm fused up to ``ops.DECODE_LINEAR_ROWS`` rows, and ``out_proj`` with the
-        residual add fused up to ``ops.DECODE_LINEAR_OUT_ROWS``."""
-        if hidden_states.ndim != 3 or hidden_states.shape[1:] != (1, self.d_model):
+        residual add fused up to ``ops.DECODE_LINEAR_OUT_ROWS``. Rows in 8 bits are normed already, and
+        ``dtype`` is what ``in_proj`` gives of them."""
+        if len(hidden_states.shape) != 3 or hidden_states.shape[1:] != (1, self.d_model):
             raise ValueError(
                 f"expected [batch, 1, {self.d_model}], got {tuple(hidden_states.shape)}")
+        if isinstance(hidden_states, ops.Rows8):
+            self._check_inference()
+            return self._step_from(self._project("in_proj", hidden_states, dtype), cache, inplace,
+                                   residual)
         self._check_inference(hidden_states)
         rows = hidden_states[:, 0]
         small = rows.shape[0] <= ops.DECODE_LINEAR_ROWS
         supported = ops.linear_norm_supported if norm is not None else ops.linear_supported
-        in4, out4 = self._weight4("in_proj"), self._weight4("out_proj")
+        in4 = self._weight4("in_proj")
         if (small and in4 is not None and rows.dtype == self.in_proj.weight.dtype
                 and ops.linear4_supported(rows, in4)):
             proj = ops.linear4(rows, in4, norm_weight=norm.weight if norm is not None else None,
@@ -246,24 +280,32 @@ class _Mamba3Mixer(nn.Module):
                               norm_eps=norm.eps if norm is not None else ops.NORM_EPS)
             proj = proj.unsqueeze(1)
         else:
-            proj = self.in_proj(norm(hidden_states) if norm is not None else hidden_states)
+            normed = norm(hidden_states) if norm is not None else hidden_states
+            # few rows keep to the weights that their neighbours' kernels read
+            proj = self.in_proj(normed) if small else self._project("in_proj", normed)
+        return self._step_from(proj, cache, inplace, residual)
+
+    def _step_from(self, proj: torch.Tensor, cache: _LayerCache | None, inplace: bool,
+                   residual: torch.Tensor | None):
+        """The rest of a step, from ``in_proj``'s output."""
+        batch, out4 = proj.shape[0], self._weight4("out_proj")
         if cache is None:
-            cache = self.allocate_cache(hidden_states.shape[0], device=hidden_states.device,
-                                        dtype=proj.dtype)
+            cache = self.allocate_cache(batch, device=proj.device, dtype=proj.dtype)
         else:
-            self._validate_cache(cache, hidden_states.shape[0])
+            self._validate_cache(cache, batch)
         mixed, next_cache = ops.step_projection(proj, self, cache, inplace=inplace)
         mixed = mixed.flatten(-2)
-        if (rows.shape[0] <= ops.DECODE_LINEAR_OUT_ROWS and out4 is not None
+        if (batch <= ops.DECODE_LINEAR_OUT_ROWS and out4 is not None
                 and ops.linear4_supported(mixed, out4)
                 and (residual is None or residual.dtype == mixed.dtype)):
             res = residual[:, 0] if residual is not None else None
             return ops.linear4(mixed, out4, res).unsqueeze(1), next_cache
-        if rows.shape[0] <= ops.DECODE_LINEAR_OUT_ROWS and ops.linear_supported(
+        if batch <= ops.DECODE_LINEAR_OUT_ROWS and ops.linear_supported(
                 mixed, self.out_proj.weight) and (residual is None or residual.dtype == mixed.dtype):
             res = residual[:, 0] if residual is not None else None
             return ops.linear(mixed, self.out_proj.weight, res).unsqueeze(1), next_cache
-        output = self.out_proj(mixed).unsqueeze(1)
+        small = batch <= ops.DECODE_LINEAR_OUT_ROWS
+        output = (self.out_proj(mixed) if small else self._project("out_proj", mixed)).unsqueeze(1)
         if residual is not None:
             output = residual + output
         return output, next_cache
@@ -330,8 +372,8 @@ class Mamba3(nn.Module):
 
     def _norm_dtype(self, h: torch.Tensor) -> torch.dtype:
         """The dtype the next in_proj computes in: autocast's for FP32 rows, else the rows'."""
-        if h.dtype == torch.float32 and torch.is_autocast_enabled(h.device.type):
-            return torch.get_autocast_dtype(h.device.type)
+        if h.dtype == torch.float32:
+            return _compute_dtype(h)
         return h.dtype
 
     def _add_norm(self, h: torch.Tensor, mixed: torch.Tensor | None, norm: _RMSNorm,
@@ -346,17 +388,31 @@ class Mamba3(nn.Module):
         s = h if mixed is None else h + mixed
         return norm(s), s
 
+    def _next_rows(self, h: torch.Tensor, mixed: torch.Tensor | None, layer: _Mamba3Block):
+        """``(the next mixer's rows, the dtype its in_proj gives, h + mixed)``: normed rows, in 8 bits
+        where the mixer has a copy of its in_proj in them."""
+        if (layer.mixer._weight8("in_proj") is None
+                or _compute_dtype(h) != layer.mixer.in_proj.weight.dtype
+                and not torch.is_autocast_enabled(h.device.type)):
+            normed, h = self._add_norm(h, mixed, layer.norm, self._norm_dtype(h), keep_sum=True)
+            return normed, None, h
+        if mixed is not None and torch.promote_types(h.dtype, mixed.dtype) != h.dtype:
+            h, mixed = h + mixed, None
+        rows, s = ops.rms_norm8(h, layer.norm.weight, layer.norm.eps, add=mixed,
+                                keep_sum=mixed is not None)
+        return rows, _compute_dtype(h), h if mixed is None else s
+
     def _run_layers(self, x: torch.Tensor, *, return_cache: bool):
         """The layer loop of forward / prefill (reference ``model.py:585-607``): each block's
         residual add runs fused with the RMSNorm after it (the next block's, or norm_f)."""
         h, mixed, cache = x, None, []
         for layer in self.layers:
-            normed, h = self._add_norm(h, mixed, layer.norm, self._norm_dtype(h), keep_sum=True)
+            rows, dtype, h = self._next_rows(h, mixed, layer)
             if return_cache:
-                mixed, layer_cache = layer.mixer(normed, return_cache=True)
+                mixed, layer_cache = layer.mixer(rows, return_cache=True, dtype=dtype)
                 cache.append(layer_cache)
             else:
-                mixed = layer.mixer(normed)
+                mixed = layer.mixer(rows, dtype=dtype)
         out, _ = self._add_norm(h, mixed, self.norm_f, h.dtype if mixed is None else
                                 torch.promote_types(h.dtype, mixed.dtype), keep_sum=False)
         return out, cache
@@ -406,8 +462,8 @@ class Mamba3(nn.Module):
         h, mixed = x, None
         for i, layer in enumerate(self.layers):
             layer_cache = None if cache is None else cache[i]
-            normed, h = self._add_norm(h, mixed, layer.norm, self._norm_dtype(h), keep_sum=True)
-            mixed, layer_cache = layer.mixer.step(normed, layer_cache,
+            rows, dtype, h = self._next_rows(h, mixed, layer)
+            mixed, layer_cache = layer.mixer.step(rows, layer_cache, dtype=dtype,
                                                   inplace=inplace and layer_cache is not None)
             updated.append(layer_cache)
         out, _ = self._add_norm(h, mixed, self.norm_f, torch.promote_types(h.dtype, mixed.dtype),
@@ -475,6 +531,32 @@ class Mamba3(nn.Module):
             layer.mixer._hold4(copies)
         return self
 
+    def quantize_prefill(self) -> Mamba3:
+        """Hold every mixer's ``in_proj`` and ``out_proj`` in 8 bits for the calls over many rows.
+
+        ``forward``, ``prefill`` and steps of more than ``ops.DECODE_LINEAR_ROWS`` rows then run both
+        projections in 8 bits: rows are rounded with a scale each behind the norm or the mixer
+        (``ops.rms_norm8``, ``ops.quantize8_rows``), weights with a scale for each output channel
+        (``ops.quantize8``), and multiplied in integers (``ops.linear8``). Steps of fewer rows and the
+        weights themselves stay as they are, so that decoding continues such a prefill with projections that are
+        not rounded to 8 bits. Weights of any floating type; memory grows by a byte for each of the projections'
+        values. A weight that is replaced or modified afterwards (``load_state_dict``, ``to``,
+        ``quantize_decode``, a copy of the model) makes these calls raise until this is called again.
+        """
+        for layer in self.layers:
+            for name in ("in_proj", "out_proj"):
+                try:
+                    getattr(layer.mixer, name).weight._version
+                except RuntimeError as error:
+                    raise ValueError("quantize_prefill needs weights that count their changes, not "
+                                     "ones made under torch.inference_mode()") from error
+        # all of them before any is held: one that holds NaN or infinities is refused
+        held = [{name: ops.quantize8(getattr(layer.mixer, name).weight)
+                 for name in ("in_proj", "out_proj")} for layer in self.layers]
+        for layer, copies in zip(self.layers, held):
+            layer.mixer._prefill8 = layer.mixer._signed(copies)
+        return self
+
     def compile_layers(self, **kwargs: object) -> Mamba3:
         """Accepted for API compatibility; the HIP kernels are already fused."""
         return self
@@ -486,6 +568,13 @@ class Mamba3(nn.Module):
     def cuda_graph(self, batch_size: int = 1) -> _HipGraphDecoder:
         """Capture the complete stateful decode step in a hipGraph."""
         return _HipGraphDecoder(self, batch_size)
+
+
+def _compute_dtype(x: torch.Tensor) -> torch.dtype:
+    """The dtype a linear layer computes ``x`` in: autocast's, else its own."""
+    if torch.is_autocast_enabled(x.device.type):
+        return torch.get_autocast_dtype(x.device.type)
+    return x.dtype
 
 
 def _storage_signature(w: torch.Tensor) -> tuple[object, ...]:
@@ -524,8 +613,9 @@ class _HipGraphDecoder:
         # storage it read (address, device, dtype, shape): `Module.to`, `.half()` or
         # `p.data = ...` keep the object and its version but move the storage
         self._captured = [_storage_signature(w) for w in weights]
-        # the 4-bit copies that the graph reads live as long as it does
-        self._weights4 = [dict(layer.mixer._decode4) for layer in model.layers]
+        # the 4-bit and 8-bit copies that the graph reads live as long as it does
+        self._copies = [(dict(layer.mixer._decode4), dict(layer.mixer._prefill8))
+                        for layer in model.layers]
         self.input = torch.zeros(batch_size, 1, model.d_model, device=device, dtype=dtype)
         self.cache = [layer.mixer.allocate_cache(batch_size, device=device, dtype=dtype)
                       for layer in model.layers]

@@ -9,7 +9,7 @@ from __future__ import annotations
 import pytest
 import torch
 
-from mamba3_amd import _hip, ops
+from mamba3_amd import Mamba3, _hip, ops
 
 pytestmark = pytest.mark.gpu
 DEV = torch.device("cuda")
@@ -248,3 +248,91 @@ def test_a_block_s_projections(m, width, inner, dtype):
     want = part + s.to(DEV).double()
     slack = 8 * 2.0 ** -24 * part.abs() + 2.0 ** -24 * want.abs()
     assert ((y.double() - want).abs() <= slack + HALF[dtype] * (want.abs() + slack) + tiny).all()
+
+
+def _layer8(model, h, mixed, layer, dtype, cache):
+    """One layer of a model whose projections are in 8 bits, by the operators."""
+    rows, s = ops.rms_norm8(h, layer.norm.weight, layer.norm.eps, add=mixed, keep_sum=mixed is not None)
+    mixer = layer.mixer
+    in8, out8 = (ops.quantize8(getattr(mixer, name).weight) for name in ("in_proj", "out_proj"))
+    proj = ops.linear8(rows, in8, dtype=dtype)
+    y, state, phase, k = ops.scan_projection(proj, mixer, want_cache=True, chunk_size=mixer._chunk())
+    return ops.linear8(ops.quantize8_rows(y.flatten(-2)), out8, dtype=dtype), h if mixed is None else s, state
+
+
+@pytest.mark.parametrize("width,dtype,autocast", [(256, F32, BF16), (96, BF16, None), (512, F16, None),
+                                                  (160, F32, None)])
+def test_quantize_prefill(width, dtype, autocast):
+    """forward and prefill are the operators' composition, bit for bit, and stay within the rounding of
+    8 bits of the model that is not rounded: each of a layer's two projections has operands off by up to half a
+    code of 127 on either side, about 2 / 254 of the greatest value of rows of some 4 standard deviations, that is
+    2 * 4 / 254 / sqrt(3) = 2% of the result's size in the mean; 4 layers' sums of both at most 4 * 2 * 2%."""
+    torch.manual_seed(width)
+    model = Mamba3(width, d_state=64, depth=2).eval().to(DEV, dtype)
+    x = torch.randn(3, 70, width, device=DEV, dtype=dtype)
+    with torch.inference_mode(), torch.autocast("cuda", dtype=autocast or BF16, enabled=autocast is not None):
+        plain = model(x)
+        cache0 = model.prefill(x)[1]
+        model.quantize_prefill()
+        got, (y, cache) = model(x), model.prefill(x)
+        h, mixed = x, None
+        for i, layer in enumerate(model.layers):
+            mixed, h, state = _layer8(model, h, mixed, layer, autocast or dtype, cache)
+            assert torch.equal(state, cache[i][1])
+        want = model._add_norm(h, mixed, model.norm_f, torch.promote_types(h.dtype, mixed.dtype), False)[0]
+    assert torch.equal(got, y) and torch.equal(got, want) and got.dtype == plain.dtype
+    assert not torch.equal(got, plain)
+    assert (got.double() - plain.double()).norm() <= 4 * 2 * 0.02 * plain.double().norm()
+    assert [[t.dtype for t in c] for c in cache] == [[t.dtype for t in c] for c in cache0]
+
+
+def test_quantize_prefill_steps_and_graphs():
+    """Steps of up to 64 rows are as they were, those of more run in 8 bits, eager and captured; the
+    prefill's cache continues in either."""
+    torch.manual_seed(0)
+    model = Mamba3(256, d_state=64, depth=2).eval().to(DEV, BF16)
+    x = torch.randn(80, 6, 256, device=DEV, dtype=BF16)
+    with torch.inference_mode():
+        few, _ = model.step(x[:5, :1])
+        many, _ = model.step(x[:, :1])
+        model.quantize_prefill()
+        assert torch.equal(model.step(x[:5, :1])[0], few)
+        y, cache = model.prefill(x[:, :4])
+        steps = []
+        for t in (4, 5):
+            out, cache = model.step(x[:, t:t + 1], cache)
+            steps.append(out)
+        first, _ = model.step(x[:, :1])
+        assert not torch.equal(first, many)
+        # a step and a prefill of one token differ by roundings alone: the step kernel's, and codes beside them
+        one, _ = model.prefill(x[:, :1])
+        assert (first.float() - one.float()).norm() <= 0.05 * one.float().norm()
+        graph = model.cuda_graph(80)
+        for _ in range(2):
+            graph.load_cache(model.prefill(x[:, :4])[1])
+            for t, want in zip((4, 5), steps):
+                assert torch.equal(graph(x[:, t:t + 1]), want)
+
+
+def test_quantize_prefill_both_directions():
+    torch.manual_seed(1)
+    model = Mamba3(192, d_state=32, depth=2, causal=False).eval().to(DEV, F16)
+    x = torch.randn(2, 90, 192, device=DEV, dtype=F16)
+    with torch.inference_mode():
+        plain = model(x)
+        got = model.quantize_prefill()(x)
+        assert torch.equal(got, model(x))
+    assert not torch.equal(got, plain) and (got.float() - plain.float()).norm() <= 0.16 * plain.float().norm()
+
+
+def test_a_changed_weight_is_refused():
+    model = Mamba3(128, depth=1).eval().to(DEV, BF16).quantize_prefill()
+    x = torch.randn(2, 5, 128, device=DEV, dtype=BF16)
+    with torch.inference_mode():
+        model(x)
+        with pytest.raises(RuntimeError):  # rows of another type than the weights', as without copies
+            model(x.half())
+    with torch.no_grad():
+        model.layers[0].mixer.out_proj.weight.mul_(2)
+    with torch.inference_mode(), pytest.raises(RuntimeError, match="call it again"):
+        model(x)

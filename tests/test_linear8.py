@@ -11,7 +11,7 @@ import pytest
 import torch
 
 from conftest import ROOT
-from mamba3_amd import _hip, ops
+from mamba3_amd import Mamba3, _hip, ops
 
 F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
 
@@ -274,3 +274,47 @@ def test_structs_match_the_header_layout(tmp_path):
         assert size == int(value), line
     for _, py, packed in pairs:
         assert packed.size == ctypes.sizeof(py)
+
+
+def test_quantize_prefill_holds_copies_and_changes_nothing():
+    model = Mamba3(64, depth=2).to(BF16)
+    before = {k: v.clone() for k, v in model.state_dict().items()}
+    assert model.quantize_prefill() is model
+    assert all(torch.equal(v, before[k]) for k, v in model.state_dict().items())
+    assert list(model.state_dict()) == list(before)
+    mixer = model.layers[1].mixer
+    for name in ("in_proj", "out_proj"):
+        weight = getattr(mixer, name).weight
+        want = ops.quantize8(weight)
+        assert torch.equal(mixer._weight8(name).q, want.q)
+        assert torch.equal(mixer._weight8(name).scales, want.scales)
+    with pytest.raises(RuntimeError, match="ROCm devices only"), torch.no_grad():
+        model(torch.zeros(1, 2, 64, dtype=BF16))
+    model.load_state_dict(before)
+    with pytest.raises(RuntimeError, match="quantize_prefill; call it again"):
+        mixer._weight8("in_proj")
+    with pytest.raises(RuntimeError, match="quantize_prefill; call it again"), torch.no_grad():
+        model(torch.zeros(1, 2, 64, dtype=BF16))
+
+
+def test_quantize_prefill_and_quantize_decode():
+    """The 4-bit copies' rounding changes the weights: the 8-bit ones are made after it."""
+    model = Mamba3(64, depth=1).to(BF16).quantize_prefill().quantize_decode(32)
+    mixer = model.layers[0].mixer
+    with pytest.raises(RuntimeError, match="call it again"):
+        mixer._weight8("out_proj")
+    model.quantize_prefill()
+    assert mixer._weight8("out_proj") is not None and mixer._weight4("out_proj") is not None
+
+
+def test_quantize_prefill_holds_every_layer_or_none():
+    model = Mamba3(64, depth=2)
+    with torch.no_grad():
+        model.layers[1].mixer.out_proj.weight[3, 5] = float("inf")
+    with pytest.raises(ValueError, match="infinities"):
+        model.quantize_prefill()
+    assert not any(layer.mixer._prefill8 for layer in model.layers)
+    with torch.inference_mode():
+        unversioned = Mamba3(64, depth=1)
+        with pytest.raises(ValueError, match="inference_mode"):
+            unversioned.quantize_prefill()
