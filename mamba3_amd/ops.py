@@ -865,11 +865,11 @@ def linear4(x: torch.Tensor, weight: Weight4, residual: torch.Tensor | None = No
 # --------------------------------------------------------------------------- 8-bit projections
 
 
-def _device_index(*tensors: torch.Tensor | None) -> int:
+def _device_index(first: torch.Tensor, *others: torch.Tensor | None) -> int:
     """The one ROCm device that all of them are on; else a ``RuntimeError`` says which is not."""
-    index = next(t for t in tensors if t is not None).get_device()
-    if index < 0 or any([t is not None and t.get_device() != index for t in tensors]):
-        _require_device(*tensors)
+    index = first.get_device()
+    if index < 0 or any([t is not None and t.get_device() != index for t in others]):
+        _require_device(first, *others)
     return index
 
 
@@ -879,55 +879,64 @@ class Rows8:
     them. Codes from elsewhere are taken as they are, copied where their rows are not 16-byte aligned.
     """
 
-    __slots__ = ("codes", "scales", "shape", "device", "_ld")
+    __slots__ = ("scales", "shape", "device", "_held", "_ld")
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor) -> None:
-        if codes.ndim < 1 or codes.dtype != torch.int8 or codes.shape[-1] == 0:
+        shape = codes.shape
+        if len(shape) < 1 or codes.dtype != torch.int8 or shape[-1] == 0:
             raise ValueError("codes must be int8 of shape [..., K]")
-        if scales.shape != codes.shape[:-1] or scales.dtype != torch.float32:
-            raise ValueError(f"scales must be float32 of shape {tuple(codes.shape[:-1])}")
+        if scales.shape != shape[:-1] or scales.dtype != torch.float32:
+            raise ValueError(f"scales must be float32 of shape {tuple(shape[:-1])}")
         if scales.device != codes.device:
             raise ValueError("codes and scales must be on the same device")
-        width = codes.shape[-1]
+        width = shape[-1]
         if width > _hip.LINEAR8_MAX_K:
             raise ValueError(f"rows of {width}: at most {_hip.LINEAR8_MAX_K}")
-        self.shape, self.device = codes.shape, codes.device
+        self.shape, self.device, self.scales = shape, codes.device, scales.contiguous()
+        if width % 16 == 0 and codes.is_contiguous() and codes.data_ptr() % 16 == 0:
+            self._held, self._ld = codes, width
+            return
         rows = codes.flatten(0, -2) if codes.ndim > 2 else codes.view(-1, width)
-        ld = rows.stride(0) if rows.shape[0] > 1 else -(-width // 16) * 16
-        end = codes.storage_offset() + (rows.shape[0] - 1) * ld + -(-width // 16) * 16
+        whole = -(-width // 16) * 16
+        ld = rows.stride(0) if rows.shape[0] > 1 else whole
+        end = rows.storage_offset() + (rows.shape[0] - 1) * ld + whole
         if (rows.stride(1) != 1 and width > 1) or rows.data_ptr() % 16 or ld % 16 or ld < width or (
-                end > rows.untyped_storage().nbytes()):
-            held, ld = _codes8(codes, rows.shape[0], width)
-            held.copy_(rows)
-            codes = held.view(self.shape) if codes.ndim > 2 else held.reshape(self.shape)
-        self.codes, self.scales, self._ld = codes, scales.contiguous(), ld
+                ld > 1 << 22 or end > rows.untyped_storage().nbytes()):
+            given, ld = rows, -(-width // 64) * 64
+            rows = given.new_empty((given.shape[0], ld))[:, :width]
+            rows.copy_(given)
+        self._held, self._ld = rows, ld
 
     @classmethod
-    def _of(cls, codes: torch.Tensor, scales: torch.Tensor, ld: int, shape: torch.Size) -> Rows8:
+    def _of(cls, held: torch.Tensor, scales: torch.Tensor, shape: torch.Size) -> Rows8:
+        """Of ``held`` ``[rows, whole 16 bytes]``, what a kernel writes."""
         rows = object.__new__(cls)
-        rows.codes, rows.scales, rows._ld = codes.unflatten(0, shape[:-1]) if len(shape) > 2 else (
-            codes if len(shape) == 2 else codes[0]), scales.view(shape[:-1]), ld
-        rows.shape, rows.device = shape, codes.device
+        rows.scales, rows.shape, rows.device = scales, shape, held.device
+        rows._held, rows._ld = held, held.shape[1]
         return rows
+
+    @property
+    def codes(self) -> torch.Tensor:
+        """The codes, int8 ``[..., K]``."""
+        held, shape = self._held, self.shape
+        if held.shape == shape:
+            return held
+        return held[:, :shape[-1]].unflatten(0, shape[:-1]) if len(shape) > 1 else held[0, :shape[0]]
 
     def dequantize(self, dtype: torch.dtype = torch.float32) -> torch.Tensor:
         """The rows ``[..., K]`` as ``code * scale``, one product in FP32 rounded to ``dtype``
         (``m3_rows8_values``; rows off the GPU in torch)."""
-        if dtype not in _FLOAT_DTYPES or self.device.type != "cuda":
-            return torch.mul(self.codes, self.scales.unsqueeze(-1)).to(dtype)
-        width, rows = self.shape[-1], self.scales.numel()
-        out = torch.empty(self.shape, dtype=dtype, device=self.device)
+        scales, shape = self.scales, self.shape
+        index = scales.get_device()
+        if dtype not in _FLOAT_DTYPES or index < 0:
+            return torch.mul(self.codes, scales.unsqueeze(-1)).to(dtype)
+        width, rows = shape[-1], scales.numel()
+        out = scales.new_empty(shape) if dtype == torch.float32 else scales.new_empty(shape, dtype=dtype)
         if rows:
             _hip.launch("m3_rows8_values", _hip.ROWS8_VALUES.pack(
-                rows, width, self.codes.data_ptr(), self._ld, self.scales.data_ptr(),
-                out.data_ptr(), _hip.dtype_code(dtype), 0, width, 1, 0, 0, 0), self.codes.get_device())
+                rows, width, self._held.data_ptr(), self._ld, scales.data_ptr(),
+                out.data_ptr(), _hip.dtype_code(dtype), 0, width, 1, 0, 0, 0), index)
         return out
-
-
-def _codes8(like: torch.Tensor, rows: int, width: int) -> tuple[torch.Tensor, int]:
-    """Uninitialised codes ``[rows, width]`` in rows of whole 64 bytes, and that stride."""
-    ld = -(-width // 64) * 64
-    return like.new_empty((rows, ld), dtype=torch.int8)[:, :width], ld
 
 
 class Weight8:
@@ -977,28 +986,29 @@ def quantize8(weight: torch.Tensor) -> Weight8:
     return Weight8(codes, most.squeeze(1).float() / 127)
 
 
-def _rows8(x, weight, eps, add, keep_sum) -> tuple[Rows8, torch.Tensor | None]:
-    width = x.shape[-1]
-    lead = x.shape[:-1]
-
-    def rows_of(t):
-        return None if t is None else _inner(t.reshape(-1, width))
-
-    index = x.get_device()
-    flat, add = rows_of(x), rows_of(add)
+def _rows8(x, weight, eps, add, keep_sum, index) -> tuple[Rows8, torch.Tensor | None]:
+    shape, flat = x.shape, x
+    width = shape[-1]
+    if len(shape) != 2:
+        flat = x.reshape(-1, width)
+        add = None if add is None else add.reshape(-1, width)
+    flat, add = _inner(flat), _inner(add)
     rows = flat.shape[0]
-    codes, ld = _codes8(flat, rows, width)
-    scales = flat.new_empty(rows, dtype=torch.float32)
-    total = torch.empty(x.shape, dtype=x.dtype, device=x.device) if keep_sum else None
+    ld = -(-width // 64) * 64
+    codes = x.new_empty((rows, ld), dtype=torch.int8)
+    scales = x.new_empty(shape[:-1], dtype=torch.float32)
+    total = x.new_empty(shape) if keep_sum else None
     if rows:
+        code, none = _hip.dtype_code(x.dtype), _hip.NO_TENSOR
         _hip.launch("m3_rows8", _hip.ROWS8.pack(
-            rows, width, eps, 0, *_packed(flat, _hip.dtype_code(x.dtype)),
-            *(_hip.NO_TENSOR if add is None else _packed(add, _hip.dtype_code(add.dtype))),
-            *(_hip.NO_TENSOR if weight is None else _packed(weight, _hip.dtype_code(weight.dtype))),
-            *(_hip.NO_TENSOR if total is None else
-              (total.data_ptr(), _hip.dtype_code(x.dtype), 0, width, 1, 0, 0, 0)),
+            rows, width, eps, 0, flat.data_ptr(), code, 0, *flat.stride(), 0, 0, 0,
+            *(none if add is None else
+              (add.data_ptr(), _hip.dtype_code(add.dtype), 0, *add.stride(), 0, 0, 0)),
+            *(none if weight is None else
+              (weight.data_ptr(), _hip.dtype_code(weight.dtype), 0, 1, 0, 0, 0, 0)),
+            *(none if total is None else (total.data_ptr(), code, 0, width, 1, 0, 0, 0)),
             codes.data_ptr(), ld, scales.data_ptr()), index)
-    return Rows8._of(codes, scales, ld, x.shape), total
+    return Rows8._of(codes, scales, shape), total
 
 
 def _check_rows8(name: str, x: torch.Tensor) -> None:
@@ -1018,10 +1028,10 @@ def quantize8_rows(x: torch.Tensor) -> Rows8:
     _check_rows8("quantize8_rows", x)
     if forward_ad._current_level >= 0:
         _refuse_tangents(x)
-    _device_index(x)
+    index = _device_index(x)
     if torch.is_grad_enabled():
         _require_inference(x)
-    return _rows8(x, None, 0.0, None, False)[0]
+    return _rows8(x, None, 0.0, None, False, index)[0]
 
 
 def rms_norm8(x: torch.Tensor, weight: torch.Tensor, eps: float = NORM_EPS, *,
@@ -1047,10 +1057,10 @@ def rms_norm8(x: torch.Tensor, weight: torch.Tensor, eps: float = NORM_EPS, *,
         raise ValueError("rms_norm8: eps must be >= 0")
     if forward_ad._current_level >= 0:
         _refuse_tangents(x, weight, add)
-    _device_index(x, weight, add)
+    index = _device_index(x, weight, add)
     if torch.is_grad_enabled():
         _require_inference(x, weight, add)
-    return _rows8(x, _inner(weight), eps, add, keep_sum)
+    return _rows8(x, _inner(weight), eps, add, keep_sum, index)
 
 
 def linear8(rows: Rows8, weight: Weight8, residual: torch.Tensor | None = None, *,
@@ -1076,26 +1086,28 @@ def linear8(rows: Rows8, weight: Weight8, residual: torch.Tensor | None = None, 
             raise ValueError(f"linear8: {name} must be {shape} {dtype}, got {tuple(t.shape)} {t.dtype}")
     if forward_ad._current_level >= 0:
         _refuse_tangents(residual)
-    index = _device_index(rows.codes, weight.q, residual, out)
-    if torch.is_grad_enabled():
+    index = _device_index(rows.scales, weight.q, residual, out)
+    if residual is not None and torch.is_grad_enabled():
         _require_inference(residual)
-    given = out
-    if out is None:
+    given, m = out is not None, rows.scales.numel()
+    if not given:
         out = rows.scales.new_empty(shape, dtype=dtype)
-    m = rows.scales.numel()
-    flat = out.view(-1, n)
-    if m > 1 and flat.stride(0) < n or n > 1 and flat.stride(1) != 1:
+    flat = out
+    if len(shape) != 2:
+        residual = None if residual is None else residual.reshape(-1, n)
+        flat = out.view(-1, n)
+    if given and (m > 1 and flat.stride(0) < n or n > 1 and flat.stride(1) != 1):
         raise ValueError("linear8: out needs a unit inner stride and rows of its own")
-    code = _hip.dtype_code(dtype)
     if m:
-        res = None if residual is None else _inner(residual.reshape(-1, n))
+        code, residual = _hip.dtype_code(dtype), _inner(residual)
         _hip.launch("m3_linear8", _hip.LINEAR8.pack(
-            m, n, k, code, 0, rows.codes.data_ptr(), rows._ld, rows.scales.data_ptr(),
+            m, n, k, code, 0, rows._held.data_ptr(), rows._ld, rows.scales.data_ptr(),
             weight.q.data_ptr(), weight.scales.data_ptr(),
-            *(_hip.NO_TENSOR if res is None else _packed(res, code)),
+            *(_hip.NO_TENSOR if residual is None else
+              (residual.data_ptr(), code, 0, *residual.stride(), 0, 0, 0)),
             flat.data_ptr(), code, 0, *flat.stride(), 0, 0, 0), index)
-    if given is not None:
-        _written(given)
+    if given:
+        _written(out)
     return out
 
 
