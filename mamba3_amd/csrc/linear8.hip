@@ -39,7 +39,7 @@ struct Lin8Geom {
   int64_t m;
   int n, k, tk;     // tk: tiles of 64 columns in a tile row of the weight
   int tiles;        // tile rows
-  bool whole;       // 16 bytes of out at a time: aligned, N a multiple, a tile's offsets 32-bit
+  bool whole;       // out and residual in 16 bytes at a time: aligned, N a multiple, a tile's offsets 32-bit
 };
 
 // An offset past every extent, also with a whole row of tiles added.
@@ -109,8 +109,9 @@ __device__ __forceinline__ void put(const Lin8Geom& g, int64_t m, int n, float r
 }
 
 // MT blocks of 16 rows by TN quarters of a tile's 64 columns of out (1 or 4); AHEAD tiles of K on their way at
-// a time. Rows past M read 0.
-template <typename T, int MT, int TN, int WAVES, int AHEAD>
+// a time. Rows past M read 0. ONCE: no other workgroup reads these of the weight's rows, and they need not stay in
+// the L2.
+template <typename T, int MT, int TN, int WAVES, int AHEAD, bool ONCE>
 __global__ __launch_bounds__(64 * WAVES) void linear8_rows_kernel(const Lin8Geom g) {
   __shared__ i4 parts[WAVES][MT * TN][64];
   const int tid = threadIdx.x, lane = tid & 63, l16 = lane & 15, lg = lane >> 4;
@@ -138,7 +139,7 @@ __global__ __launch_bounds__(64 * WAVES) void linear8_rows_kernel(const Lin8Geom
 #pragma unroll
       for (int j = 0; j < TN; ++j) {
         a[u][j] = __builtin_bit_cast(i4, __builtin_amdgcn_raw_buffer_load_b128(
-            rq, live ? qoff + j * 1024 + t * kTileBytes : kNowhere, 0, 2));
+            rq, live ? qoff + j * 1024 + t * kTileBytes : kNowhere, 0, ONCE ? 2 : 0));
       }
 #pragma unroll
       for (int i = 0; i < MT; ++i) {
@@ -340,8 +341,6 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void linear8_tile_kernel(const Lin
 #pragma unroll
   for (int j = 0; j < 4; ++j) weight(1, j);
   step_weight();
-#pragma unroll
-  for (int i = 0; i < XI; ++i) read(0, 0, i);
   // loads and stores count down in the order of their issue: after a stage's fetch come the weight's 8 loads
   // in the two halves until it is needed, and at a tile's first step the stores of the tile before
   constexpr int kStores = (sizeof(T) == 4 ? 4 : 2) * XI;
@@ -352,6 +351,9 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void linear8_tile_kernel(const Lin
 #pragma unroll
       for (int i = 0; i < XI; ++i) acc[j][i] = i4{0, 0, 0, 0};
     }
+    // (once more after a tile before, whose last half has read them: they are not kept while it is written)
+#pragma unroll
+    for (int i = 0; i < XI; ++i) read(now, 0, i);
 #pragma unroll 1
     for (int s = 0; s < steps; ++s) {
       half(0, now);
@@ -389,15 +391,48 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void linear8_tile_kernel(const Lin
     }
     constexpr int kPiece = 16 / static_cast<int>(sizeof(T));  // elements
     const bool odd = (lane & 1) != 0;
+    // the residual, as many blocks of rows at a time as the registers hold, before the stores of these
+    constexpr int kBatch = RES && WHOLE ? 2 * XI / (8 / kPiece) / 4 : 1;
+    u32x4 held[kBatch][2][8 / kPiece];
+    __amdgpu_buffer_rsrc_t rr;
+    unsigned from = 0, pitch_r = 0;
+    if constexpr (RES && WHOLE) {
+      rr = rsrc8(static_cast<const T*>(g.res) + m0 * g.r_ld,
+                 ((left - 1) * g.r_ld + g.n) * static_cast<int64_t>(sizeof(T)));
+      pitch_r = static_cast<unsigned>(g.r_ld) * static_cast<unsigned>(sizeof(T));
+      from = m1 * pitch_r + n0 * static_cast<unsigned>(sizeof(T));
+    }
 #pragma unroll
     for (int i = 0; i < XI; ++i) {
       const int m = m1 + 16 * i;
+      if constexpr (RES && WHOLE) {
+        if (i % kBatch == 0) {
+          __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+          for (int u = 0; u < kBatch; ++u) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+#pragma unroll
+              for (int p = 0; p < 8 / kPiece; ++p) {
+                held[u][h][p] = __builtin_amdgcn_raw_buffer_load_b128(
+                    rr, from + 16 * (i + u) * pitch_r + 32 * h * static_cast<unsigned>(sizeof(T)) + 16 * p, 0, 0);
+              }
+            }
+          }
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      }
       u32x4 y[2][8 / kPiece];  // [half of the 64 columns][pieces of 16 bytes]
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         float v[8];
         T t[8];
-        if constexpr (RES) {
+        if constexpr (RES && WHOLE) {
+          T r[8];
+          __builtin_memcpy(r, held[i % kBatch][h], sizeof(r));
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[e] = to_f(r[e]);
+        } else if constexpr (RES) {
           load_res(static_cast<const T*>(g.res) + (m0 + min(m, left - 1)) * g.r_ld, n0 + 32 * h, g.n, v);
         }
 #pragma unroll
@@ -425,8 +460,8 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void linear8_tile_kernel(const Lin
           if (m2 + 1 < left) store_piece(to + g.o_ld, n, g.n, second);
         }
       }
-      // one row block's residual and addresses at a time: more would not fit the registers
-      if constexpr (RES || !WHOLE) __builtin_amdgcn_sched_barrier(0);
+      // one block's addresses (and residual) at a time: more would not fit the registers
+      if constexpr (!WHOLE) __builtin_amdgcn_sched_barrier(0);
     }
     stored = WHOLE;
   }
@@ -435,7 +470,9 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void linear8_tile_kernel(const Lin
 template <typename T, int MT, int TN, int WAVES, int AHEAD>
 int launch_rows(const Lin8Geom& g, hipStream_t stream) {
   const dim3 grid(4 / TN * g.tiles, static_cast<unsigned>((g.m + 16 * MT - 1) / (16 * MT)));
-  hipLaunchKernelGGL((linear8_rows_kernel<T, MT, TN, WAVES, AHEAD>), grid, dim3(64 * WAVES), 0, stream, g);
+  const auto kernel = grid.y == 1 ? linear8_rows_kernel<T, MT, TN, WAVES, AHEAD, true>
+                                  : linear8_rows_kernel<T, MT, TN, WAVES, AHEAD, false>;
+  hipLaunchKernelGGL(kernel, grid, dim3(64 * WAVES), 0, stream, g);
   return check_launch("m3_linear8");
 }
 
@@ -458,12 +495,13 @@ int launch_tile(const Lin8Geom& g, int a_cu, hipStream_t stream) {
 template <typename T>
 int launch8(const Lin8Geom& g, hipStream_t stream) {
   if (g.m <= 16) return launch_rows<T, 1, 1, 8, 4>(g, stream);
-  if (g.tiles * ((g.m + 31) / 32) <= 2 * kCus) return launch_rows<T, 2, 4, 8, 2>(g, stream);
-  const int64_t tm = (g.m + 127) / 128, large = tm * ((g.tiles + 7) / 8), small = tm * ((g.tiles + 1) / 2);
-  if (3 * ((large + kCus - 1) / kCus) <= 2 * ((small + 2 * kCus - 1) / (2 * kCus))) {
-    return launch_tile<T, 1, 8, 8>(g, 1, stream);
-  }
-  return launch_tile<T, 2, 2, 4>(g, 2, stream);
+  if (g.tiles * ((g.m + 31) / 32) <= 3 * kCus) return launch_rows<T, 2, 4, 8, 2>(g, stream);
+  const int64_t tm = (g.m + 127) / 128, medium = tm * ((g.tiles + 3) / 4);
+  if (medium < 3 * kCus / 4) return launch_tile<T, 2, 2, 4>(g, 2, stream);
+  const int64_t large = tm * ((g.tiles + 7) / 8), rest = medium % (2 * kCus);
+  const int64_t one = (large + kCus - 1) / kCus * 16;
+  const int64_t two = medium / (2 * kCus) * 17 + (rest == 0 ? 0 : rest <= kCus ? 12 : 17);
+  return one <= two ? launch_tile<T, 1, 8, 8>(g, 1, stream) : launch_tile<T, 1, 4, 8>(g, 2, stream);
 }
 
 int validate(const m3_linear8_args& a) {
@@ -526,8 +564,11 @@ extern "C" int m3_linear8(const m3_linear8_args* args, hipStream_t stream) {
   if (rc != M3_OK) return rc;
   if (a.m == 0 || a.n == 0) return M3_OK;
   const int64_t es = elem_size(a.dtype), pitch = a.out.stride[0] * es;
-  const bool whole = reinterpret_cast<uintptr_t>(a.out.ptr) % 16 == 0 && a.n * es % 16 == 0 &&
-                     (a.m == 1 || (pitch % 16 == 0 && pitch < (1 << 23)));
+  const int64_t pitch_r = a.residual.stride[0] * es;
+  const bool whole = reinterpret_cast<uintptr_t>(a.out.ptr) % 16 == 0 &&
+                     reinterpret_cast<uintptr_t>(a.residual.ptr) % 16 == 0 && a.n * es % 16 == 0 &&
+                     (a.m == 1 || (pitch % 16 == 0 && pitch < (1 << 23) && pitch_r % 16 == 0 &&
+                                   pitch_r < (1 << 23)));
   const Lin8Geom g{reinterpret_cast<const char*>(a.codes), a.row_scales,
                    reinterpret_cast<const char*>(a.q), a.scales, a.residual.ptr, a.out.ptr,
                    a.codes_stride, a.residual.stride[0], a.out.stride[0], a.m, static_cast<int>(a.n),
