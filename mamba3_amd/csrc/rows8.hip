@@ -63,9 +63,10 @@ struct Seen {
     bits = max(bits, o.bits);
     if constexpr (WIDE) wide = fmax(wide, o.wide);
   }
-  __device__ __forceinline__ void join_wave() {
+  template <int LANES>
+  __device__ __forceinline__ void join_lanes() {
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) {
+    for (int o = LANES / 2; o > 0; o >>= 1) {
       Seen other;
       other.sq = __shfl_xor(sq, o);
       other.bits = __shfl_xor(bits, o);
@@ -88,15 +89,14 @@ struct Row {
         sum(ADD && geom.sum != nullptr ? reinterpret_cast<T*>(geom.sum) + row * geom.s_ld : nullptr),
         g(geom) {}
 
-  // s of eight elements, and of one
-  __device__ __forceinline__ void sums(int at, float (&s)[kChunk]) const {
-    load8<T>(x, at, s);
-    if constexpr (ADD) {
-      float a[kChunk];
-      load8<TA>(add, at, a);
+  // s of eight elements, from x's and add's, and of one
+  __device__ __forceinline__ void sums(const T (&v)[kChunk], const TA (&a)[kChunk], float (&s)[kChunk]) const {
 #pragma unroll
-      for (int e = 0; e < kChunk; ++e) s[e] = rnd<T>(s[e] + a[e]);
-    }
+    for (int e = 0; e < kChunk; ++e) s[e] = ADD ? rnd<T>(to_f(v[e]) + to_f(a[e])) : to_f(v[e]);
+  }
+  __device__ __forceinline__ void load(int at, T (&v)[kChunk], TA (&a)[kChunk]) const {
+    __builtin_memcpy(v, x + at, sizeof(v));
+    if constexpr (ADD) __builtin_memcpy(a, add + at, sizeof(a));
   }
   __device__ __forceinline__ float sum_at(int at) const {
     float s = to_f(x[at]);
@@ -114,6 +114,16 @@ struct Row {
   // s once more, where this lane has stored it: it may have taken x's place
   __device__ __forceinline__ float again(int at) const {
     return ADD && sum != nullptr ? to_f(sum[at]) : sum_at(at);
+  }
+  __device__ __forceinline__ void again8(int at, float (&s)[kChunk]) const {
+    if (ADD && sum != nullptr) {
+      load8<T>(sum, at, s);
+    } else {
+      T v[kChunk];
+      TA a[kChunk];
+      load(at, v, a);
+      sums(v, a, s);
+    }
   }
 
   // the norm's weight, rounded to the rows' dtype
@@ -154,7 +164,7 @@ __device__ __forceinline__ Scaled scaled(const Seen<WIDE>& seen, int dim, float 
 }
 
 // The code of p, and whether it is too near to a half to be told in FP32. A row that holds an infinity
-// or NaN has inv = 0, and codes of 0 (where p is NaN, too: fmaxf drops it).
+// or NaN has inv = 0, and codes of 0.
 __device__ __forceinline__ int code8(float p, const Scaled& c, bool& close) {
   const float q = p * c.up * c.inv, n = rintf(q);
   close = fabsf(q - n) > 0.4999f;
@@ -171,53 +181,79 @@ __device__ __forceinline__ int settle(float s, float w, const Scaled& c) {
   return q < 0.f ? -(n + up) : n + up;
 }
 
-// TPR threads take a row: a wave (four rows a workgroup) or the workgroup of 256. A lane holds the p of CH
-// chunks of eight and, for dim % 8, of one element more; CH = 0 walks longer rows twice instead.
+// TPR threads (16, a wave or the workgroup of 256) take a row. A lane holds the p of CH chunks of eight and, for
+// dim % 8, of one element more; CH = 0 walks longer rows twice instead. All loads of a lane's row are issued
+// before the first is used, those of chunks past its end from its last one; the norm's weight is rounded once a
+// workgroup, in LDS (each row on its own took 56 in place of 48 us for 16384 x 2048).
 template <typename T, typename TA, bool NORM, bool ADD, int TPR, int CH>
 __global__ __launch_bounds__(256) void rows8_kernel(const Rows8Geom g) {
   constexpr bool kWide = NORM && sizeof(T) == 4;
-  const int tid = threadIdx.x, lane = TPR == 64 ? tid & 63 : tid;
-  const int64_t r = TPR == 64 ? static_cast<int64_t>(blockIdx.x) * 4 + (tid >> 6) : blockIdx.x;
-  if (TPR == 64 && r >= g.rows) return;
-  const Row<T, TA, NORM, ADD> row(g, r);
-  const int whole = g.dim / kChunk, rest = g.dim % kChunk;
+  const int tid = threadIdx.x, lane = tid % TPR;
+  const int64_t r = static_cast<int64_t>(blockIdx.x) * (256 / TPR) + tid / TPR;
+  const bool live = TPR == 256 || r < g.rows;
+  const Row<T, TA, NORM, ADD> row(g, live ? r : g.rows - 1);
+  const int whole = g.dim / kChunk, rest = g.dim % kChunk, end = kChunk * whole + lane;
   Seen<kWide> seen = {0.f, 0u, 0.0};
-  const auto look8 = [&](int at, float (&s)[kChunk]) {  // leaves p in s
-    float w[kChunk];
-    row.keep(at, s);
-    row.weights(at, w);
+  float p[CH > 0 ? CH : 1][kChunk], last = 0.f;
+  const auto look8 = [&](const float (&w)[kChunk], float (&s)[kChunk]) {  // leaves p in s
 #pragma unroll
     for (int e = 0; e < kChunk; ++e) {
-      const float p = NORM ? s[e] * w[e] : s[e];
-      seen.look(s[e], NORM ? w[e] : 1.f, p);
-      s[e] = p;
+      const float v = NORM ? s[e] * w[e] : s[e];
+      seen.look(s[e], NORM ? w[e] : 1.f, v);
+      s[e] = v;
     }
   };
-  constexpr int kHeld = CH > 0 ? CH : 1;
-  float p[kHeld][kChunk], last = 0.f;
   if constexpr (CH > 0) {
+    __shared__ __attribute__((aligned(16))) float weight[NORM ? TPR * CH * kChunk : 4];
+    T v[CH][kChunk];
+    TA a[CH][kChunk];
+    if (whole > 0) {
 #pragma unroll
-    for (int j = 0; j < CH; ++j) {
-      if (lane + TPR * j < whole) row.sums(kChunk * (lane + TPR * j), p[j]);
+      for (int j = 0; j < CH; ++j) row.load(kChunk * min(lane + TPR * j, whole - 1), v[j], a[j]);
+    }
+    if constexpr (NORM) {
+      if (whole > 0) {
+        constexpr int kEach = (TPR * CH + 255) / 256;  // chunks of the weight a lane
+        float w[kEach][kChunk];
+#pragma unroll
+        for (int u = 0; u < kEach; ++u) row.weights(kChunk * min(tid + 256 * u, whole - 1), w[u]);
+#pragma unroll
+        for (int u = 0; u < kEach; ++u) {
+          if (tid + 256 * u < whole) __builtin_memcpy(weight + kChunk * (tid + 256 * u), w[u], sizeof(w[u]));
+        }
+      }
+      __syncthreads();
     }
 #pragma unroll
     for (int j = 0; j < CH; ++j) {
-      if (lane + TPR * j < whole) look8(kChunk * (lane + TPR * j), p[j]);
+      const int at = kChunk * (lane + TPR * j);
+      if (at < kChunk * whole) {
+        float w[kChunk];
+        if constexpr (NORM) __builtin_memcpy(w, weight + at, sizeof(w));
+        row.sums(v[j], a[j], p[j]);
+        if (live) row.keep(at, p[j]);
+        look8(w, p[j]);
+      }
     }
   } else {
     for (int c = lane; c < whole; c += TPR) {
-      row.sums(kChunk * c, p[0]);
-      look8(kChunk * c, p[0]);
+      T v[kChunk];
+      TA a[kChunk];
+      float w[kChunk];
+      row.load(kChunk * c, v, a);
+      row.weights(kChunk * c, w);
+      row.sums(v, a, p[0]);
+      row.keep(kChunk * c, p[0]);
+      look8(w, p[0]);
     }
   }
-  const int end = kChunk * whole + lane;
   if (lane < rest) {
     const float s = row.sum_at(end), w = row.weight_at(end);
-    if (ADD && row.sum != nullptr) row.sum[end] = from_f<T>(s);
+    if (ADD && row.sum != nullptr && live) row.sum[end] = from_f<T>(s);
     last = s * w;
     seen.look(s, w, last);
   }
-  seen.join_wave();
+  seen.template join_lanes<TPR < 64 ? TPR : 64>();
   if constexpr (TPR > 64) {
     __shared__ Seen<kWide> parts[4];
     if ((tid & 63) == 0) parts[tid >> 6] = seen;
@@ -226,6 +262,7 @@ __global__ __launch_bounds__(256) void rows8_kernel(const Rows8Geom g) {
 #pragma unroll
     for (int i = 1; i < 4; ++i) seen.join(parts[i]);
   }
+  if (!live) return;
   const Scaled c = scaled<NORM, kWide>(seen, g.dim, g.eps);
   int8_t* const codes = g.codes + r * g.c_ld;
   const auto code_chunk = [&](int at, const float (&v)[kChunk]) {
@@ -241,9 +278,9 @@ __global__ __launch_bounds__(256) void rows8_kernel(const Rows8Geom g) {
     }
     *reinterpret_cast<u32x2*>(codes + at) = words;
     while (open != 0) {
-      const int i = at + __builtin_ctz(open);
+      const int k = at + __builtin_ctz(open);
       open &= open - 1;
-      codes[i] = static_cast<int8_t>(settle(row.again(i), row.weight_at(i), c));
+      codes[k] = static_cast<int8_t>(settle(row.again(k), row.weight_at(k), c));
     }
   };
   if constexpr (CH > 0) {
@@ -253,10 +290,12 @@ __global__ __launch_bounds__(256) void rows8_kernel(const Rows8Geom g) {
     }
   } else {
     for (int j = lane; j < whole; j += TPR) {
-      const int at = kChunk * j;
+      float w[kChunk];
+      row.again8(kChunk * j, p[0]);
+      row.weights(kChunk * j, w);
 #pragma unroll
-      for (int e = 0; e < kChunk; ++e) p[0][e] = row.again(at + e) * row.weight_at(at + e);
-      code_chunk(at, p[0]);
+      for (int e = 0; e < kChunk; ++e) p[0][e] = NORM ? p[0][e] * w[e] : p[0][e];
+      code_chunk(kChunk * j, p[0]);
     }
   }
   if (lane < rest) {
@@ -311,14 +350,17 @@ int launch_values(const m3_rows8_values_args& a, hipStream_t stream) {
 
 template <typename T, typename TA, bool NORM, bool ADD, int TPR, int CH>
 int launch_one(const Rows8Geom& g, hipStream_t stream) {
-  const unsigned blocks = TPR == 64 ? (static_cast<unsigned>(g.rows) + 3) / 4 : g.rows;
-  hipLaunchKernelGGL((rows8_kernel<T, TA, NORM, ADD, TPR, CH>), dim3(blocks), dim3(256), 0, stream, g);
+  constexpr unsigned rows = 256 / TPR;
+  const dim3 grid((static_cast<unsigned>(g.rows) + rows - 1) / rows);
+  hipLaunchKernelGGL((rows8_kernel<T, TA, NORM, ADD, TPR, CH>), grid, dim3(256), 0, stream, g);
   return check_launch("m3_rows8");
 }
 
 template <typename T, typename TA, bool NORM, bool ADD>
 int launch_dim(const Rows8Geom& g, hipStream_t stream) {
   const int chunks = (g.dim + kChunk - 1) / kChunk;
+  if (chunks <= 16) return launch_one<T, TA, NORM, ADD, 16, 1>(g, stream);
+  if (chunks <= 32) return launch_one<T, TA, NORM, ADD, 16, 2>(g, stream);
   if (chunks <= 64) return launch_one<T, TA, NORM, ADD, 64, 1>(g, stream);
   if (chunks <= 128) return launch_one<T, TA, NORM, ADD, 64, 2>(g, stream);
   if (chunks <= 256) return launch_one<T, TA, NORM, ADD, 64, 4>(g, stream);

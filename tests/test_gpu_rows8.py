@@ -52,7 +52,7 @@ def _check(got, x, weight=None, add=None, eps=EPS):
         assert torch.equal(total.cpu(), s)
 
 
-DIMS = [1, 2, 7, 8, 9, 64, 65, 511, 512, 513, 1000, 1024, 1111, 2048, 2049, 4096, 5003, 8192, 8199, 16400]
+DIMS = [1, 2, 7, 8, 9, 64, 65, 120, 128, 129, 250, 256, 257, 511, 512, 513, 1000, 1024, 1111, 2048, 2049, 4096, 5003, 8192, 8199, 16400]
 
 
 def _inputs(m, k, dtype, g):
@@ -65,7 +65,7 @@ def _inputs(m, k, dtype, g):
 @pytest.mark.parametrize("dtype", [F32, BF16, F16])
 def test_rows(k, dtype):
     g = torch.Generator().manual_seed(k)
-    for m in (1, 5):
+    for m in (1, 5, 37):
         x = _inputs(m, k, dtype, g)
         with torch.inference_mode():
             _check((ops.quantize8_rows(x.to(DEV)), None), x)
@@ -77,7 +77,7 @@ def test_rows(k, dtype):
 def test_normed_rows(k, dtype, add_dtype):
     g = torch.Generator().manual_seed(k + 1)
     weight = (1 + 0.2 * torch.randn(k, generator=g)).to([F32, BF16, F16][k % 3])
-    for m in (1, 6):
+    for m in (1, 38):
         x = _inputs(m, k, dtype, g)
         add = None if add_dtype is None else torch.randn(m, k, generator=g).to(add_dtype)
         dev = [None if t is None else t.to(DEV) for t in (x, weight, add)]
