@@ -24,6 +24,15 @@ namespace {
 
 constexpr int kChunk = 8;  // elements a lane takes at a time: 8 bytes of codes
 
+// Workgroups of 256 for so many: a launch has below 2^32 work-items along x.
+inline dim3 grid_of(int64_t blocks) {
+  constexpr int64_t most = 1 << 23;
+  return dim3(static_cast<unsigned>(blocks < most ? blocks : most), static_cast<unsigned>((blocks + most - 1) / most));
+}
+__device__ __forceinline__ int64_t block_index() {
+  return static_cast<int64_t>(blockIdx.y) * gridDim.x + blockIdx.x;
+}
+
 struct Rows8Geom {
   const char* x;
   const char* add;   // or null
@@ -189,8 +198,8 @@ template <typename T, typename TA, bool NORM, bool ADD, int TPR, int CH>
 __global__ __launch_bounds__(256) void rows8_kernel(const Rows8Geom g) {
   constexpr bool kWide = NORM && sizeof(T) == 4;
   const int tid = threadIdx.x, lane = tid % TPR;
-  const int64_t r = static_cast<int64_t>(blockIdx.x) * (256 / TPR) + tid / TPR;
-  const bool live = TPR == 256 || r < g.rows;
+  const int64_t r = block_index() * (256 / TPR) + tid / TPR;
+  const bool live = r < g.rows;
   const Row<T, TA, NORM, ADD> row(g, live ? r : g.rows - 1);
   const int whole = g.dim / kChunk, rest = g.dim % kChunk, end = kChunk * whole + lane;
   Seen<kWide> seen = {0.f, 0u, 0.0};
@@ -243,7 +252,7 @@ __global__ __launch_bounds__(256) void rows8_kernel(const Rows8Geom g) {
       row.load(kChunk * c, v, a);
       row.weights(kChunk * c, w);
       row.sums(v, a, p[0]);
-      row.keep(kChunk * c, p[0]);
+      if (live) row.keep(kChunk * c, p[0]);
       look8(w, p[0]);
     }
   }
@@ -313,7 +322,7 @@ __global__ __launch_bounds__(256) void values8_kernel(const int8_t* codes, int64
                                                       T* out, int64_t o_ld, int rows, int dim, int lanes_log2) {
   constexpr int kPiece = 16 / static_cast<int>(sizeof(T));
   const int lanes = 1 << lanes_log2, lane = threadIdx.x & (lanes - 1);
-  const int64_t row = (static_cast<int64_t>(blockIdx.x) << (8 - lanes_log2)) + (threadIdx.x >> lanes_log2);
+  const int64_t row = (block_index() << (8 - lanes_log2)) + (threadIdx.x >> lanes_log2);
   if (row >= rows) return;
   const float scale = scales[row];
   const int8_t* const from = codes + row * c_ld;
@@ -342,17 +351,17 @@ int launch_values(const m3_rows8_values_args& a, hipStream_t stream) {
   int log2 = 0;
   while (log2 < 8 && (kPiece << log2) < a.dim) ++log2;
   const int64_t per = 256 >> log2;
-  hipLaunchKernelGGL(values8_kernel<T>, dim3(static_cast<unsigned>((a.rows + per - 1) / per)), dim3(256), 0,
-                     stream, a.codes, a.codes_stride, a.scales, static_cast<T*>(a.out.ptr), a.out.stride[0],
+  hipLaunchKernelGGL(values8_kernel<T>, grid_of((a.rows + per - 1) / per), dim3(256), 0, stream, a.codes,
+                     a.codes_stride, a.scales, static_cast<T*>(a.out.ptr), a.out.stride[0],
                      static_cast<int>(a.rows), static_cast<int>(a.dim), log2);
   return check_launch("m3_rows8_values");
 }
 
 template <typename T, typename TA, bool NORM, bool ADD, int TPR, int CH>
 int launch_one(const Rows8Geom& g, hipStream_t stream) {
-  constexpr unsigned rows = 256 / TPR;
-  const dim3 grid((static_cast<unsigned>(g.rows) + rows - 1) / rows);
-  hipLaunchKernelGGL((rows8_kernel<T, TA, NORM, ADD, TPR, CH>), grid, dim3(256), 0, stream, g);
+  constexpr int64_t rows = 256 / TPR;
+  hipLaunchKernelGGL((rows8_kernel<T, TA, NORM, ADD, TPR, CH>), grid_of((g.rows + rows - 1) / rows), dim3(256), 0,
+                     stream, g);
   return check_launch("m3_rows8");
 }
 

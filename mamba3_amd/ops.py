@@ -928,6 +928,10 @@ class Rows8:
         (``m3_rows8_values``; rows off the GPU in torch)."""
         scales, shape = self.scales, self.shape
         index = scales.get_device()
+        if forward_ad._current_level >= 0:
+            _refuse_tangents(scales)
+        if torch.is_grad_enabled():
+            _require_inference(scales)
         if dtype not in _FLOAT_DTYPES or index < 0:
             return torch.mul(self.codes, scales.unsqueeze(-1)).to(dtype)
         width, rows = shape[-1], scales.numel()
@@ -1070,7 +1074,7 @@ def linear8(rows: Rows8, weight: Weight8, residual: torch.Tensor | None = None, 
     ``rows [..., K]`` any number of them, one token's or a prompt's; the result ``[..., N]`` has ``dtype``
     FP32, bfloat16 or float16 (default: that of ``out`` or ``residual``, else bfloat16), which
     ``residual`` and ``out`` share. Sums are exact in 32-bit integers; scales and residual meet them in FP32, which
-    is rounded once. ``out`` may be ``residual``. No backward.
+    is rounded once. ``out`` may be ``residual``. A row whose scale is NaN gives NaN. No backward.
     """
     if dtype is None:
         given = out if out is not None else residual
@@ -1085,10 +1089,10 @@ def linear8(rows: Rows8, weight: Weight8, residual: torch.Tensor | None = None, 
         if t is not None and (t.shape != shape or t.dtype != dtype):
             raise ValueError(f"linear8: {name} must be {shape} {dtype}, got {tuple(t.shape)} {t.dtype}")
     if forward_ad._current_level >= 0:
-        _refuse_tangents(residual)
+        _refuse_tangents(residual, rows.scales)
     index = _device_index(rows.scales, weight.q, residual, out)
-    if residual is not None and torch.is_grad_enabled():
-        _require_inference(residual)
+    if torch.is_grad_enabled():
+        _require_inference(residual, rows.scales)
     given, m = out is not None, rows.scales.numel()
     if not given:
         out = rows.scales.new_empty(shape, dtype=dtype)

@@ -240,6 +240,48 @@ def test_what_is_written():
                 assert name == place or torch.equal(dev[name].cpu(), given)
 
 
+def test_gradients_are_refused_not_dropped():
+    x = torch.randn(4, 40, device=DEV, requires_grad=True)
+    weight = torch.ones(40, device=DEV)
+    for call in (lambda: ops.quantize8_rows(x), lambda: ops.rms_norm8(weight.expand(4, 40), weight, add=x),
+                 lambda: ops.rms_norm8(x.detach(), x[0]),
+                 lambda: ops.linear8(ops.quantize8_rows(x.detach()), ops.quantize8(x.detach()), x[:, :4],
+                                     dtype=F32),
+                 lambda: ops.linear8(ops.Rows8(torch.zeros(4, 40, dtype=torch.int8, device=DEV), x[:, 0]),
+                                     ops.quantize8(x.detach()))):
+        with pytest.raises(RuntimeError, match="no backward"):
+            call()
+    with torch.no_grad():
+        ops.rms_norm8(x, weight, add=x, keep_sum=True)
+
+
+def test_rows_that_are_one_row():
+    """Expanded inputs: rows with a stride of 0."""
+    g = torch.Generator().manual_seed(11)
+    x, add = torch.randn(1, 300, generator=g).to(F16), torch.randn(1, 300, generator=g).to(F16)
+    weight = torch.tensor([0.5])
+    with torch.inference_mode():
+        got = ops.rms_norm8(x.to(DEV).expand(9, 300), weight.to(DEV).expand(300), add=add.to(DEV).expand(9, 300),
+                            keep_sum=True)
+        _check(got, x.expand(9, 300), weight.expand(300), add.expand(9, 300))
+
+
+def test_more_rows_than_a_launch_has_threads():
+    """2^28 rows of 16 lanes each, and what they stand for by one lane each: the last rows are the last."""
+    rows = (1 << 28) + 37
+    x = torch.ones(rows, 2, dtype=BF16, device=DEV)
+    x[:, 1] = 0.25
+    x[-5:] = torch.tensor([[1.0, -3.0]], dtype=BF16)
+    with torch.inference_mode():
+        got = ops.quantize8_rows(x)
+        assert (got.codes[:1000] == torch.tensor([127, 32], device=DEV)).all()
+        assert (got.codes[-1000:-5] == torch.tensor([127, 32], device=DEV)).all()
+        assert (got.codes[-5:] == torch.tensor([42, -127], device=DEV)).all()
+        tail = ops.Rows8(got.codes, got.scales).dequantize(BF16)[-6:].float()
+    want = torch.tensor([[1.0, 32 / 127]] + [[42 * 3 / 127, -3.0]] * 5)
+    assert ((tail.cpu() - want).abs() <= 2.0 ** -8 * want.abs()).all()
+
+
 def test_streams_and_graphs():
     """On a stream of its own, and captured and replayed with new inputs between eager calls."""
     g = torch.Generator().manual_seed(4)

@@ -135,6 +135,9 @@ def test_off_the_gpu_and_under_autograd():
                  lambda: ops.linear8(ops.Rows8(codes, scales), weight)):
         with pytest.raises(RuntimeError, match="ROCm devices only"):
             call()
+    trained = ops.Rows8(codes, torch.rand(8, requires_grad=True))
+    with pytest.raises(RuntimeError, match="no backward"):
+        trained.dequantize()
     with torch.autograd.forward_ad.dual_level():
         dual = torch.autograd.forward_ad.make_dual(x, x)
         for call in (lambda: ops.quantize8_rows(dual), lambda: ops.rms_norm8(x, x[0], add=dual),
