@@ -879,7 +879,9 @@ class Rows8:
     them. Codes from elsewhere are taken as they are, copied where their rows are not 16-byte aligned.
     """
 
-    __slots__ = ("scales", "shape", "device", "_held", "_ld")
+    # _ld: bytes between rows; _memory: the int8 tensor of both (codes, then scales), or of given codes
+    # with _given, their scales
+    __slots__ = ("shape", "_rows", "_ld", "_memory", "_given")
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor) -> None:
         shape = codes.shape
@@ -889,58 +891,82 @@ class Rows8:
             raise ValueError(f"scales must be float32 of shape {tuple(shape[:-1])}")
         if scales.device != codes.device:
             raise ValueError("codes and scales must be on the same device")
-        width = shape[-1]
+        width, rows = shape[-1], scales.numel()
         if width > _hip.LINEAR8_MAX_K:
             raise ValueError(f"rows of {width}: at most {_hip.LINEAR8_MAX_K}")
-        self.shape, self.device, self.scales = shape, codes.device, scales.contiguous()
-        if width % 16 == 0 and codes.is_contiguous() and codes.data_ptr() % 16 == 0:
-            self._held, self._ld = codes, width
-            return
-        rows = codes.flatten(0, -2) if codes.ndim > 2 else codes.view(-1, width)
-        whole = -(-width // 16) * 16
-        ld = rows.stride(0) if rows.shape[0] > 1 else whole
-        end = rows.storage_offset() + (rows.shape[0] - 1) * ld + whole
-        if (rows.stride(1) != 1 and width > 1) or rows.data_ptr() % 16 or ld % 16 or ld < width or (
-                ld > 1 << 22 or end > rows.untyped_storage().nbytes()):
-            given, ld = rows, -(-width // 64) * 64
-            rows = given.new_empty((given.shape[0], ld))[:, :width]
-            rows.copy_(given)
-        self._held, self._ld = rows, ld
+        scales, ld = scales.contiguous(), width
+        if width % 16 or not codes.is_contiguous() or codes.data_ptr() % 16:
+            codes, ld = _whole_rows(codes if len(shape) == 2 else codes.reshape(-1, width))
+        self.shape, self._rows, self._ld, self._memory, self._given = shape, rows, ld, codes, scales
 
     @classmethod
-    def _of(cls, held: torch.Tensor, scales: torch.Tensor, shape: torch.Size) -> Rows8:
-        """Of ``held`` ``[rows, whole 16 bytes]``, what a kernel writes."""
-        rows = object.__new__(cls)
-        rows.scales, rows.shape, rows.device = scales, shape, held.device
-        rows._held, rows._ld = held, held.shape[1]
-        return rows
+    def _of(cls, memory: torch.Tensor, shape: torch.Size, rows: int, ld: int) -> Rows8:
+        """Of ``memory``, what a kernel writes: ``[rows, ld]`` bytes of codes, then the scales."""
+        self = object.__new__(cls)
+        self.shape, self._rows, self._ld, self._memory, self._given = shape, rows, ld, memory, None
+        return self
+
+    def _block(self) -> tuple[int, int, int]:
+        """Where the codes lie, the bytes between rows, where the scales lie."""
+        at = self._memory.data_ptr()
+        return (at, self._ld, at + self._rows * self._ld if self._given is None
+                else self._given.data_ptr())
+
+    @property
+    def device(self) -> torch.device:
+        return self._memory.device
 
     @property
     def codes(self) -> torch.Tensor:
         """The codes, int8 ``[..., K]``."""
-        held, shape = self._held, self.shape
+        held, shape = self._memory, self.shape
+        if self._given is None:
+            held = held[:self._rows * self._ld].view(self._rows, self._ld)
         if held.shape == shape:
             return held
-        return held[:, :shape[-1]].unflatten(0, shape[:-1]) if len(shape) > 1 else held[0, :shape[0]]
+        held = held[:, :shape[-1]]
+        return held[0] if len(shape) == 1 else held.unflatten(0, shape[:-1])
+
+    @property
+    def scales(self) -> torch.Tensor:
+        """The scales, FP32 ``[...]``."""
+        if self._given is not None:
+            return self._given
+        return self._memory[self._rows * self._ld:].view(torch.float32).view(self.shape[:-1])
 
     def dequantize(self, dtype: torch.dtype = torch.float32) -> torch.Tensor:
         """The rows ``[..., K]`` as ``code * scale``, one product in FP32 rounded to ``dtype``
         (``m3_rows8_values``; rows off the GPU in torch)."""
-        scales, shape = self.scales, self.shape
-        index = scales.get_device()
+        given, memory, shape, rows = self._given, self._memory, self.shape, self._rows
         if forward_ad._current_level >= 0:
-            _refuse_tangents(scales)
-        if torch.is_grad_enabled():
-            _require_inference(scales)
+            _refuse_tangents(given)
+        if given is not None and torch.is_grad_enabled():
+            _require_inference(given)
+        index = memory.get_device()
         if dtype not in _FLOAT_DTYPES or index < 0:
-            return torch.mul(self.codes, scales.unsqueeze(-1)).to(dtype)
-        width, rows = shape[-1], scales.numel()
-        out = scales.new_empty(shape) if dtype == torch.float32 else scales.new_empty(shape, dtype=dtype)
+            return torch.mul(self.codes, self.scales.unsqueeze(-1)).to(dtype)
+        out = memory.new_empty(shape, dtype=dtype)
         if rows:
+            width = shape[-1]
             _hip.launch("m3_rows8_values", _hip.ROWS8_VALUES.pack(
-                rows, width, self._held.data_ptr(), self._ld, scales.data_ptr(),
+                rows, width, *self._block(),
                 out.data_ptr(), _hip.dtype_code(dtype), 0, width, 1, 0, 0, 0), index)
         return out
+
+
+def _whole_rows(codes: torch.Tensor) -> tuple[torch.Tensor, int]:
+    """Codes ``[rows, K]`` with 16-byte aligned rows that reach to a multiple of 16, and the bytes
+    between them: as they are if they have such rows, else copied."""
+    rows, width = codes.shape
+    whole = -(-width // 16) * 16
+    if not codes.is_contiguous() and codes.stride(1) == 1 and codes.data_ptr() % 16 == 0:
+        ld = codes.stride(0) if rows > 1 else whole
+        if ld % 16 == 0 and width <= ld <= 1 << 22 and (
+                codes.storage_offset() + (rows - 1) * ld + whole <= codes.untyped_storage().nbytes()):
+            return codes, ld
+    held = codes.new_empty((rows, whole))[:, :width]
+    held.copy_(codes)
+    return held, whole
 
 
 class Weight8:
@@ -999,8 +1025,8 @@ def _rows8(x, weight, eps, add, keep_sum, index) -> tuple[Rows8, torch.Tensor | 
     flat, add = _inner(flat), _inner(add)
     rows = flat.shape[0]
     ld = -(-width // 64) * 64
-    codes = x.new_empty((rows, ld), dtype=torch.int8)
-    scales = x.new_empty(shape[:-1], dtype=torch.float32)
+    memory = x.new_empty(rows * (ld + 4), dtype=torch.int8)
+    held = Rows8._of(memory, shape, rows, ld)
     total = x.new_empty(shape) if keep_sum else None
     if rows:
         code, none = _hip.dtype_code(x.dtype), _hip.NO_TENSOR
@@ -1011,8 +1037,8 @@ def _rows8(x, weight, eps, add, keep_sum, index) -> tuple[Rows8, torch.Tensor | 
             *(none if weight is None else
               (weight.data_ptr(), _hip.dtype_code(weight.dtype), 0, 1, 0, 0, 0, 0)),
             *(none if total is None else (total.data_ptr(), code, 0, width, 1, 0, 0, 0)),
-            codes.data_ptr(), ld, scales.data_ptr()), index)
-    return Rows8._of(codes, scales, shape), total
+            *held._block()), index)
+    return held, total
 
 
 def _check_rows8(name: str, x: torch.Tensor) -> None:
@@ -1089,13 +1115,13 @@ def linear8(rows: Rows8, weight: Weight8, residual: torch.Tensor | None = None, 
         if t is not None and (t.shape != shape or t.dtype != dtype):
             raise ValueError(f"linear8: {name} must be {shape} {dtype}, got {tuple(t.shape)} {t.dtype}")
     if forward_ad._current_level >= 0:
-        _refuse_tangents(residual, rows.scales)
-    index = _device_index(rows.scales, weight.q, residual, out)
+        _refuse_tangents(residual, rows._given)
+    index = _device_index(rows._memory, weight.q, residual, out)
     if torch.is_grad_enabled():
-        _require_inference(residual, rows.scales)
-    given, m = out is not None, rows.scales.numel()
+        _require_inference(residual, rows._given)
+    given, m = out is not None, rows._rows
     if not given:
-        out = rows.scales.new_empty(shape, dtype=dtype)
+        out = rows._memory.new_empty(shape, dtype=dtype)
     flat = out
     if len(shape) != 2:
         residual = None if residual is None else residual.reshape(-1, n)
@@ -1105,7 +1131,7 @@ def linear8(rows: Rows8, weight: Weight8, residual: torch.Tensor | None = None, 
     if m:
         code, residual = _hip.dtype_code(dtype), _inner(residual)
         _hip.launch("m3_linear8", _hip.LINEAR8.pack(
-            m, n, k, code, 0, rows._held.data_ptr(), rows._ld, rows.scales.data_ptr(),
+            m, n, k, code, 0, *rows._block(),
             weight.q.data_ptr(), weight.scales.data_ptr(),
             *(_hip.NO_TENSOR if residual is None else
               (residual.data_ptr(), code, 0, *residual.stride(), 0, 0, 0)),

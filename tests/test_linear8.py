@@ -2,6 +2,7 @@
 
 from __future__ import annotations
 
+import copy
 import ctypes
 import os
 import shutil
@@ -75,6 +76,7 @@ def test_rows8_takes_aligned_codes_as_they_are():
         held = ops.Rows8(given, scales)
         assert torch.equal(held.codes, given) and held._ld % 16 == 0
         assert held.codes.data_ptr() % 16 == 0 and held.codes.stride(-1) == 1
+        assert held._block() == (held.codes.data_ptr(), held.codes.stride(0), held.scales.data_ptr())
         end = held.codes.storage_offset() + 5 * held._ld + -(-given.shape[1] // 16) * 16
         assert end <= held.codes.untyped_storage().nbytes()
     cube = ops.Rows8(codes.view(2, 3, 64).transpose(0, 1), scales.view(2, 3).t())
@@ -84,6 +86,8 @@ def test_rows8_takes_aligned_codes_as_they_are():
     assert one.shape == (64,) and torch.equal(one.dequantize(BF16), (codes[2] * scales[2]).to(BF16))
     none = ops.Rows8(codes[:0], scales[:0])
     assert none.shape == (0, 64)
+    twin = copy.deepcopy(view)
+    assert torch.equal(twin.codes, view.codes) and twin._block()[0] == twin.codes.data_ptr() != view._block()[0]
 
 
 @pytest.mark.parametrize("make,message", [
