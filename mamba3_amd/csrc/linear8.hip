@@ -26,6 +26,7 @@ typedef int i4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kCus = 256;
+constexpr unsigned kBand = 8;  // tiles along M that an XCD takes before the next column
 constexpr int kTileBytes = 4096;  // 64 weight rows x 64 columns
 
 struct Lin8Geom {
@@ -244,17 +245,23 @@ __device__ __forceinline__ void store_piece(T* row, int n, int end, const u32x4&
 //
 // WHOLE: out is written by every lane in 16 bytes at a time, what lies outside past the extent, so that the number
 // of stores is known. Else rows may lie at any alignment and end within a piece.
-template <typename T, int WM, int WN, int XI, bool WHOLE, bool RES>
-__global__ __launch_bounds__(64 * WM * WN, 2) void linear8_tile_kernel(const Lin8Geom g, unsigned tiles_m,
-                                                                    unsigned tiles_n, unsigned band) {
+//
+// KS: groups of WM x WN waves that take every KS-th step of K, each with stages of its own; the others' sums
+// go to the first through LDS. Such a workgroup takes one tile.
+template <typename T, int WM, int WN, int XI, int KS, bool WHOLE, bool RES>
+__global__ __launch_bounds__(64 * WM * WN * KS, 2) void linear8_tile_kernel(const Lin8Geom g, unsigned tiles_m,
+                                                                         unsigned tiles_n, unsigned band) {
   constexpr int kWaves = WM * WN, BM = 16 * XI * WM, kStage = BM * 128, kUnits = BM / 8 / kWaves;
+  constexpr int kSums = (KS - 1) * kWaves * 4 * XI * 1024, kLds = 2 * KS * kStage > kSums ? 2 * KS * kStage : kSums;
   static_assert(BM / 8 % kWaves == 0 && XI % 4 == 0, "whole units and reads for each wave");
-  __shared__ __attribute__((aligned(128))) char stages[2 * kStage];
+  __shared__ __attribute__((aligned(128))) char lds[kLds];
   const int tid = threadIdx.x, lane = tid & 63, l16 = lane & 15, lg = lane >> 4;
-  const int w = __builtin_amdgcn_readfirstlane(tid >> 6), wm = w / WN, wn = w % WN;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), part = KS == 1 ? 0 : wave / kWaves;
+  const int w = KS == 1 ? wave : wave % kWaves, wm = w / WN, wn = w % WN;
+  char* const stages = lds + part * 2 * kStage;
   const unsigned all = tiles_m * tiles_n;
   const int64_t row_bytes = static_cast<int64_t>(g.tk) * kTileBytes;
-  const int steps = g.tk / 2;
+  const int all_steps = g.tk / 2, steps = (all_steps + KS - 1) / KS;
 
   // The codes' loads, units of 8 rows (1 KB), and where they have come to. Rows past M lie past the extent,
   // and so does everything after the last tile.
@@ -266,12 +273,13 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void linear8_tile_kernel(const Lin
     const int64_t m0 = place(min(c_id, all - 1), tiles_m, tiles_n, band).m * BM;
     const int64_t left = g.m - m0 < BM ? g.m - m0 : BM;
     rc = rsrc8(g.codes + m0 * g.c_ld, c_id < all ? (left - 1) * g.c_ld + (g.k + 15) / 16 * 16 : 0);
-    coff = (8 * w + (lane >> 3)) * static_cast<unsigned>(g.c_ld) + 16 * ((lane & 7) ^ (lane >> 3));
+    coff = (8 * w + (lane >> 3)) * static_cast<unsigned>(g.c_ld) + 16 * ((lane & 7) ^ (lane >> 3)) +
+           128 * part;
   };
   const auto fetch = [&](int stage) {
 #pragma unroll
     for (int v = 0; v < kUnits; ++v) load_lds(rc, stages + stage + (v * kWaves + w) * 1024, coff + v * unit);
-    coff += 128;
+    coff += 128 * KS;
     if (++c_step == steps) {
       c_step = 0;
       c_id += gridDim.x;
@@ -279,17 +287,19 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void linear8_tile_kernel(const Lin
     }
   };
 
-  // The same of the weight's operands; tile rows past N lie past the extent.
+  // The same of the weight's operands; tile rows past N lie past the extent, and a step that a group has past
+  // the last one does too: its products are 0.
   __amdgpu_buffer_rsrc_t rq;
   unsigned qoff, q_id = blockIdx.x;
   int q_step = 0;
   const auto aim_weight = [&]() {
     const int tile0 = place(min(q_id, all - 1), tiles_m, tiles_n, band).n * WN;
     rq = rsrc8(g.q + tile0 * row_bytes, q_id < all ? min(WN, g.tiles - tile0) * row_bytes : 0);
-    qoff = wn * static_cast<unsigned>(row_bytes) + lane * 16;
+    qoff = part < all_steps ? (wn * static_cast<unsigned>(row_bytes) + 2 * kTileBytes * part) + lane * 16 : kNowhere;
   };
   const auto step_weight = [&]() {
-    qoff += 2 * kTileBytes;
+    qoff += 2 * kTileBytes * KS;
+    if (KS > 1 && (q_step + 1) * KS + part >= all_steps) qoff = kNowhere;
     if (++q_step == steps) {
       q_step = 0;
       q_id += gridDim.x;
@@ -369,6 +379,27 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void linear8_tile_kernel(const Lin
       now = kStage - now;
       half(1, now);
       step_weight();
+    }
+    if constexpr (KS > 1) {
+      i4* const sums = reinterpret_cast<i4*>(lds) + lane;
+      stage_barrier<0>();  // of the fetches past the last step, too
+      if (part > 0) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+#pragma unroll
+          for (int i = 0; i < XI; ++i) sums[(((part - 1) * kWaves + w) * 4 * XI + j * XI + i) * 64] = acc[j][i];
+        }
+      }
+      __syncthreads();
+      if (part > 0) return;
+#pragma unroll
+      for (int u = 0; u < KS - 1; ++u) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+#pragma unroll
+          for (int i = 0; i < XI; ++i) acc[j][i] += sums[((u * kWaves + w) * 4 * XI + j * XI + i) * 64];
+        }
+      }
     }
     const Place at = place(id, tiles_m, tiles_n, band);
     const int64_t m0 = at.m * BM;
@@ -476,32 +507,33 @@ int launch_rows(const Lin8Geom& g, hipStream_t stream) {
   return check_launch("m3_linear8");
 }
 
-template <typename T, int WM, int WN, int XI>
+// By a_cu workgroups on every CU, that take tile after tile; with groups of waves (KS > 1) by one a tile.
+template <typename T, int WM, int WN, int XI, int KS>
 int launch_tile(const Lin8Geom& g, int a_cu, hipStream_t stream) {
   constexpr int BM = 16 * XI * WM;
   const int64_t tm = (g.m + BM - 1) / BM, tn = (g.tiles + WN - 1) / WN, all = tm * tn;
   if (all >= 1 << 30) return fail(M3_EUNSUPPORTED, "m3_linear8: over 2^30 tiles of out");
-  const unsigned grid = static_cast<unsigned>(all < a_cu * kCus ? all : a_cu * kCus);
+  const unsigned grid = static_cast<unsigned>(KS > 1 || all < a_cu * kCus ? all : a_cu * kCus);
   const bool res = g.res != nullptr;
-  const auto kernel = g.whole ? (res ? linear8_tile_kernel<T, WM, WN, XI, true, true>
-                                     : linear8_tile_kernel<T, WM, WN, XI, true, false>)
-                              : (res ? linear8_tile_kernel<T, WM, WN, XI, false, true>
-                                     : linear8_tile_kernel<T, WM, WN, XI, false, false>);
-  hipLaunchKernelGGL(kernel, dim3(grid), dim3(64 * WM * WN), 0, stream, g, static_cast<unsigned>(tm),
-                     static_cast<unsigned>(tn), 8u);
+  const auto kernel = g.whole ? (res ? linear8_tile_kernel<T, WM, WN, XI, KS, true, true>
+                                     : linear8_tile_kernel<T, WM, WN, XI, KS, true, false>)
+                              : (res ? linear8_tile_kernel<T, WM, WN, XI, KS, false, true>
+                                     : linear8_tile_kernel<T, WM, WN, XI, KS, false, false>);
+  hipLaunchKernelGGL(kernel, dim3(grid), dim3(64 * WM * WN * KS), 0, stream, g, static_cast<unsigned>(tm),
+                     static_cast<unsigned>(tn), kBand);
   return check_launch("m3_linear8");
 }
 
 template <typename T>
 int launch8(const Lin8Geom& g, hipStream_t stream) {
   if (g.m <= 16) return launch_rows<T, 1, 1, 8, 4>(g, stream);
-  if (g.tiles * ((g.m + 31) / 32) <= 3 * kCus) return launch_rows<T, 2, 4, 8, 2>(g, stream);
+  if (g.tiles * ((g.m + 31) / 32) <= 3 * kCus / 2) return launch_rows<T, 2, 4, 8, 2>(g, stream);
   const int64_t tm = (g.m + 127) / 128, medium = tm * ((g.tiles + 3) / 4);
-  if (medium < 3 * kCus / 4) return launch_tile<T, 2, 2, 4>(g, 2, stream);
+  if (medium <= kCus / 2) return launch_tile<T, 1, 2, 4, 2>(g, 1, stream);
   const int64_t large = tm * ((g.tiles + 7) / 8), rest = medium % (2 * kCus);
   const int64_t one = (large + kCus - 1) / kCus * 16;
   const int64_t two = medium / (2 * kCus) * 17 + (rest == 0 ? 0 : rest <= kCus ? 12 : 17);
-  return one <= two ? launch_tile<T, 1, 8, 8>(g, 1, stream) : launch_tile<T, 1, 4, 8>(g, 2, stream);
+  return one <= two ? launch_tile<T, 1, 8, 8, 1>(g, 1, stream) : launch_tile<T, 1, 4, 8, 1>(g, 2, stream);
 }
 
 int validate(const m3_linear8_args& a) {

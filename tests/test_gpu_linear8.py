@@ -179,7 +179,7 @@ def test_every_kernel_gives_the_same_bits(n, dtype, residual):
     with torch.inference_mode():
         whole = ops.linear8(ops.Rows8(codes.to(DEV), rs.to(DEV)), weight, res, dtype=dtype)
         _check(whole, codes, q, rs, s, res)
-        for m in (1, 2, 16, 17, 40, 64, 65, 128, 200, 500, 1500):
+        for m in (1, 2, 16, 17, 40, 64, 65, 128, 200, 500, 700, 1500):
             part = ops.linear8(ops.Rows8(codes[:m].to(DEV), rs[:m].to(DEV)), weight,
                                None if res is None else res[:m], dtype=dtype)
             assert torch.equal(part, whole[:m]), m
