@@ -524,10 +524,20 @@ int launch_tile(const Lin8Geom& g, int a_cu, hipStream_t stream) {
   return check_launch("m3_linear8");
 }
 
+// Which kernel (us in graphs with cold weights, bf16; M x N x K):
+//   16 x 16 of out a workgroup of 8 waves, while these are at most two a CU (64 x 2048 x 4096: 7.3, the next 8.3;
+//     16 x 4480 x 1024: 3.9, 4.4), or three with up to 4 rows (4 x 8672 x 2048: 5.5, 5.9; 8 rows: 6.1, 6.0)
+//   32 x 64, for up to 32 rows or 1.5 a CU (16 x 16384 x 4096: 12.4, the one before 21; 256 x 2048 x 4096: 10.1, the
+//     next 13.9; 512 x 2048 x 4096, two a CU: 16.9, 16.0)
+//   64 x 128 with K in halves, for up to half a 128 x 256 tile a CU (1000 x 2048 x 4096: 16.6, 128 x 128 26.6;
+//     2000 x 2048 x 4096: 26.1, 128 x 256 about 30; 512 x 8672 x 2048, 136 tiles: 21.2, 18.9)
+//   128 x 256 by two workgroups a CU or 128 x 512 by one, whose rounds cost 17 and 16, half a round of the first
+//     12 (4000 x 2048 x 4096: 33.5, 45.7; 2000 x 8672 x 2048: 40.8, 50.5; 8192 x 28672 x 8192: 1,430, 1,340)
 template <typename T>
 int launch8(const Lin8Geom& g, hipStream_t stream) {
-  if (g.m <= 16) return launch_rows<T, 1, 1, 8, 4>(g, stream);
-  if (g.tiles * ((g.m + 31) / 32) <= 3 * kCus / 2) return launch_rows<T, 2, 4, 8, 2>(g, stream);
+  const int64_t cells = 4 * g.tiles * ((g.m + 15) / 16);
+  if (cells <= 2 * kCus || (g.m <= 4 && cells <= 3 * kCus)) return launch_rows<T, 1, 1, 8, 4>(g, stream);
+  if (g.m <= 32 || g.tiles * ((g.m + 31) / 32) <= 3 * kCus / 2) return launch_rows<T, 2, 4, 8, 2>(g, stream);
   const int64_t tm = (g.m + 127) / 128, medium = tm * ((g.tiles + 3) / 4);
   if (medium <= kCus / 2) return launch_tile<T, 1, 2, 4, 2>(g, 1, stream);
   const int64_t large = tm * ((g.tiles + 7) / 8), rest = medium % (2 * kCus);
