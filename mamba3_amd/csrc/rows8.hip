@@ -13,7 +13,11 @@
 // exact. One element in 5,000 is.
 //
 // Bound by memory: the row stays in registers between the two passes over it (its maximum, its codes), so
-// x, add, the sum and the codes each move once.
+// x, add, the sum and the codes each move once. Measured (a large copy reaches 5.0 to 5.5 TB/s): 65536 x 1024 FP32 with
+// a bf16 add and the sum kept 138 us (5.35 TB/s of what moves), 16384 x 2048 bf16 the same way 47.5 us (4.95),
+// 32768 x 4096 bf16 without norm 77.5 us (5.2), one row of 2048 3.5 us.
+//
+// m3_rows8_values, what the rows stand for, likewise: 32768 x 4096 to FP32 150 us (4.5 TB/s).
 #include <hip/hip_runtime.h>
 
 #include "m3_common.hpp"
