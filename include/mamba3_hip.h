@@ -400,8 +400,8 @@ int m3_rows8(const m3_rows8_args* args, hipStream_t stream);
 /* What such rows stand for: out[r, d] = codes[r, d] * scales[r], one FP32 product rounded to out's dtype. */
 typedef struct {
   int64_t rows, dim;
-  const int8_t* codes;  /* [rows, codes_stride], 16-byte aligned, readable to the next multiple of 16 */
-  int64_t codes_stride; /* bytes, a multiple of 16 */
+  const int8_t* codes;  /* [rows, codes_stride], at any alignment */
+  int64_t codes_stride; /* bytes */
   const float* scales;  /* [rows] */
   m3_tensor out;        /* [rows, dim]; overlaps nothing */
 } m3_rows8_values_args;
@@ -418,21 +418,27 @@ int m3_rows8_values(const m3_rows8_values_args* args, hipStream_t stream);
  *   q [ceil(N / 64), TK, 4, 64, 16] bytes: byte e of lane l of quarter j holds column 16 (l / 16) + e of
  *     its tile, row 32 (j / 2) + 8 (l % 16 / 4) + 4 (j % 2) + l % 4
  *   scale [64 ceil(N / 64)] FP32, 0 past N
- * What lies in codes between K and the row's stride has no effect.
+ * What lies in codes between K and the row's stride has no effect. Rows of codes that are not 16-byte aligned, or
+ * (exact) end where their memory does, are read with care by the kernels for few rows and copied into the workspace for the
+ * others (m3_linear8_workspace_size, 0 where nothing is copied).
  */
 typedef struct {
   int64_t m, n, k;
   int32_t dtype;        /* of out and residual */
-  int32_t reserved;
-  const int8_t* codes;  /* [M, codes_stride], 16-byte aligned, readable to the next multiple of 16 */
-  int64_t codes_stride; /* bytes, a multiple of 16, at least K */
+  int32_t exact;        /* not 0: nothing past a row's K codes may be read; 0: rows that are 16-byte aligned
+                           are readable to the next multiple of 16 */
+  const int8_t* codes;  /* [M, codes_stride] */
+  int64_t codes_stride; /* bytes, at least K */
   const float* row_scales; /* [M] */
   const int8_t* q;      /* 16-byte aligned */
   const float* scales;  /* 16-byte aligned */
   m3_tensor residual;   /* [M, N] optional */
   m3_tensor out;        /* [M, N]; may equal residual, overlaps nothing else */
+  void* workspace;      /* 16-byte aligned */
+  size_t workspace_bytes;
 } m3_linear8_args;
 
+int m3_linear8_workspace_size(const m3_linear8_args* args, size_t* bytes);
 int m3_linear8(const m3_linear8_args* args, hipStream_t stream);
 
 const char* m3_last_error(void);

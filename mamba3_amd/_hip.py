@@ -144,10 +144,11 @@ class Rows8ValuesArgs(ctypes.Structure):
 class Linear8Args(ctypes.Structure):
     _fields_ = [
         *[(n, ctypes.c_int64) for n in ("m", "n", "k")],
-        ("dtype", ctypes.c_int32), ("reserved", ctypes.c_int32),
+        ("dtype", ctypes.c_int32), ("exact", ctypes.c_int32),
         ("codes", ctypes.c_void_p), ("codes_stride", ctypes.c_int64),
         *[(n, ctypes.c_void_p) for n in ("row_scales", "q", "scales")],
         *[(n, _T) for n in ("residual", "out")],
+        ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_size_t),
     ]
 
 
@@ -160,14 +161,14 @@ GATED_SCAN_BWD = struct.Struct(GATED_SCAN.format + 7 * _TENSOR)
 LINEAR4 = struct.Struct("@3q3ifPPP" + 4 * _TENSOR)
 ROWS8 = struct.Struct("@2qfi" + 4 * _TENSOR + "PqP")
 ROWS8_VALUES = struct.Struct("@2qPqP" + _TENSOR)
-LINEAR8 = struct.Struct("@3q2iPqPPP" + 2 * _TENSOR)
+LINEAR8 = struct.Struct("@3q2iPqPPP" + 2 * _TENSOR + "PN")
 NO_TENSOR = (0,) * 8
 
 ENTRY_POINTS = ("m3_scan_fwd", "m3_scan_workspace_size", "m3_scan_segments", "m3_scan_fwd_noalloc",
                 "m3_chunk_state", "m3_step", "m3_linear", "m3_linear_workspace_size",
                 "m3_rms_norm", "m3_gated_scan", "m3_gated_scan_workspace_size",
                 "m3_gated_scan_bwd", "m3_gated_scan_bwd_workspace_size", "m3_linear4",
-                "m3_rows8", "m3_rows8_values", "m3_linear8", "m3_last_error", "m3_abi_version")
+                "m3_rows8", "m3_rows8_values", "m3_linear8", "m3_linear8_workspace_size", "m3_last_error", "m3_abi_version")
 LINEAR8_MAX_K = 131071  # M3_LINEAR8_MAX_K: sums of products of 8 bits stay in 32
 GATED_TILE = 64  # M3_GATED_TILE: tokens between two of the states a gated scan's carry holds
 SCRATCH_BYTES = 64 << 20  # M3_SCRATCH_BYTES: the no-alloc scan's per-GPU scratch
@@ -191,7 +192,8 @@ def load() -> ctypes.CDLL:
         fn.restype = ctypes.c_int
         fn.argtypes = [ctypes.c_void_p, ctypes.c_void_p]
     for name in ("m3_scan_workspace_size", "m3_linear_workspace_size",
-                 "m3_gated_scan_workspace_size", "m3_gated_scan_bwd_workspace_size"):
+                 "m3_gated_scan_workspace_size", "m3_gated_scan_bwd_workspace_size",
+                 "m3_linear8_workspace_size"):
         fn = getattr(lib, name)
         fn.restype = ctypes.c_int
         fn.argtypes = [ctypes.c_void_p, ctypes.POINTER(ctypes.c_size_t)]

@@ -44,6 +44,7 @@ struct Lin8Geom {
   int64_t m;
   int n, k, tk;     // tk: tiles of 64 columns in a tile row of the weight
   int tiles;        // tile rows
+  bool aligned;     // rows of codes: 16-byte aligned, readable to the next multiple of 16
   bool whole;       // out and residual in 16 bytes at a time: aligned, N a multiple, a tile's offsets 32-bit
 };
 
@@ -114,10 +115,26 @@ __device__ __forceinline__ void put(const Lin8Geom& g, int64_t m, int n, float r
   }
 }
 
+// 16 codes at column `at` of row m, at any alignment. Those past the row's end meet zeros of the weight; past the last
+// row's they are not read.
+__device__ __forceinline__ i4 load_codes(const Lin8Geom& g, int64_t m, int at) {
+  const char* p = g.codes + m * g.c_ld + at;
+  const int64_t left = (g.m - 1 - m) * g.c_ld + g.k - at;
+  i4 v = {0, 0, 0, 0};
+  if (left >= 16) {
+    __builtin_memcpy(&v, p, sizeof(v));
+  } else {
+    for (int e = 0; e < left; ++e) {
+      v[e / 4] |= static_cast<int>(static_cast<uint32_t>(static_cast<uint8_t>(p[e])) << (8 * (e % 4)));
+    }
+  }
+  return v;
+}
+
 // MT blocks of 16 rows by TN quarters of a tile's 64 columns of out (1 or 4); AHEAD tiles of K on their way at
 // a time. Rows past M read 0. ONCE: no other workgroup reads these of the weight's rows, and they need not stay in
-// the L2.
-template <typename T, int MT, int TN, int WAVES, int AHEAD, bool ONCE>
+// the L2. ALIGNED: rows of codes are 16-byte aligned and readable to the next multiple of 16.
+template <typename T, int MT, int TN, int WAVES, int AHEAD, bool ONCE, bool ALIGNED>
 __global__ __launch_bounds__(64 * WAVES) void linear8_rows_kernel(const Lin8Geom g) {
   __shared__ i4 parts[WAVES][MT * TN][64];
   const int tid = threadIdx.x, lane = tid & 63, l16 = lane & 15, lg = lane >> 4;
@@ -136,6 +153,9 @@ __global__ __launch_bounds__(64 * WAVES) void linear8_rows_kernel(const Lin8Geom
   const unsigned xoff = l16 * static_cast<unsigned>(g.c_ld) + 16 * lg, xrow = 16 * static_cast<unsigned>(g.c_ld);
   const unsigned qoff = quarter * 1024 + lane * 16;
   const int tiles = (g.k + 63) / 64;
+  // whether any lane's codes could lie past the last row's: then each asks
+  const char* const from = g.codes + (m0 + l16) * g.c_ld + 16 * lg;
+  const bool careful = (m0 + 16 * MT - 1) * g.c_ld + tiles * 64 > (g.m - 1) * g.c_ld + g.k;
   for (int t0 = w; t0 < tiles; t0 += WAVES * AHEAD) {
     i4 a[AHEAD][TN], b[AHEAD][MT];
 #pragma unroll
@@ -149,8 +169,15 @@ __global__ __launch_bounds__(64 * WAVES) void linear8_rows_kernel(const Lin8Geom
       }
 #pragma unroll
       for (int i = 0; i < MT; ++i) {
-        b[u][i] = __builtin_bit_cast(i4, __builtin_amdgcn_raw_buffer_load_b128(
-            rc, live ? xoff + i * xrow + t * 64 : kNowhere, 0, 0));
+        if constexpr (ALIGNED) {
+          b[u][i] = __builtin_bit_cast(i4, __builtin_amdgcn_raw_buffer_load_b128(
+              rc, live ? xoff + i * xrow + t * 64 : kNowhere, 0, 0));
+        } else if (careful) {
+          const int64_t m = m0 + 16 * i + l16;
+          b[u][i] = live && m < g.m ? load_codes(g, m, t * 64 + 16 * lg) : i4{0, 0, 0, 0};
+        } else {
+          __builtin_memcpy(&b[u][i], from + (16 * i) * g.c_ld + min(t, tiles - 1) * 64, sizeof(i4));
+        }
       }
     }
 #pragma unroll
@@ -506,8 +533,11 @@ __global__ __launch_bounds__(64 * WM * WN * KS, 2) void linear8_tile_kernel(cons
 template <typename T, int MT, int TN, int WAVES, int AHEAD>
 int launch_rows(const Lin8Geom& g, hipStream_t stream) {
   const dim3 grid(4 / TN * g.tiles, static_cast<unsigned>((g.m + 16 * MT - 1) / (16 * MT)));
-  const auto kernel = grid.y == 1 ? linear8_rows_kernel<T, MT, TN, WAVES, AHEAD, true>
-                                  : linear8_rows_kernel<T, MT, TN, WAVES, AHEAD, false>;
+  const auto kernel =
+      g.aligned ? (grid.y == 1 ? linear8_rows_kernel<T, MT, TN, WAVES, AHEAD, true, true>
+                               : linear8_rows_kernel<T, MT, TN, WAVES, AHEAD, false, true>)
+                : (grid.y == 1 ? linear8_rows_kernel<T, MT, TN, WAVES, AHEAD, true, false>
+                               : linear8_rows_kernel<T, MT, TN, WAVES, AHEAD, false, false>);
   hipLaunchKernelGGL(kernel, grid, dim3(64 * WAVES), 0, stream, g);
   return check_launch("m3_linear8");
 }
@@ -538,17 +568,71 @@ int launch_tile(const Lin8Geom& g, int a_cu, hipStream_t stream) {
 //     2000 x 2048 x 4096: 26.1, 128 x 256 about 30; 512 x 8672 x 2048, 136 tiles: 21.2, 18.9)
 //   128 x 256 by two workgroups a CU or 128 x 512 by one, whose rounds cost 17 and 16, half a round of the first
 //     12 (4000 x 2048 x 4096: 33.5, 45.7; 2000 x 8672 x 2048: 40.8, 50.5; 8192 x 28672 x 8192: 1,430, 1,340)
-template <typename T>
-int launch8(const Lin8Geom& g, hipStream_t stream) {
-  const int64_t cells = 4 * g.tiles * ((g.m + 15) / 16);
-  if (cells <= 2 * kCus || (g.m <= 4 && cells <= 3 * kCus)) return launch_rows<T, 1, 1, 8, 4>(g, stream);
-  if (g.m <= 32 || g.tiles * ((g.m + 31) / 32) <= 3 * kCus / 2) return launch_rows<T, 2, 4, 8, 2>(g, stream);
-  const int64_t tm = (g.m + 127) / 128, medium = tm * ((g.tiles + 3) / 4);
-  if (medium <= kCus / 2) return launch_tile<T, 1, 2, 4, 2>(g, 1, stream);
-  const int64_t large = tm * ((g.tiles + 7) / 8), rest = medium % (2 * kCus);
+enum Form { kCells, kRows, kHalves, kMedium, kLarge };
+Form form_of(int64_t m, int64_t tiles) {
+  const int64_t cells = 4 * tiles * ((m + 15) / 16);
+  if (cells <= 2 * kCus || (m <= 4 && cells <= 3 * kCus)) return kCells;
+  if (m <= 32 || tiles * ((m + 31) / 32) <= 3 * kCus / 2) return kRows;
+  const int64_t tm = (m + 127) / 128, medium = tm * ((tiles + 3) / 4);
+  if (medium <= kCus / 2) return kHalves;
+  const int64_t large = tm * ((tiles + 7) / 8), rest = medium % (2 * kCus);
   const int64_t one = (large + kCus - 1) / kCus * 16;
   const int64_t two = medium / (2 * kCus) * 17 + (rest == 0 ? 0 : rest <= kCus ? 12 : 17);
-  return one <= two ? launch_tile<T, 1, 8, 8, 1>(g, 1, stream) : launch_tile<T, 1, 4, 8, 1>(g, 2, stream);
+  return one <= two ? kLarge : kMedium;
+}
+
+template <typename T>
+int launch8(const Lin8Geom& g, Form form, hipStream_t stream) {
+  switch (form) {
+    case kCells: return launch_rows<T, 1, 1, 8, 4>(g, stream);
+    case kRows: return launch_rows<T, 2, 4, 8, 2>(g, stream);
+    case kHalves: return launch_tile<T, 1, 2, 4, 2>(g, 1, stream);
+    case kMedium: return launch_tile<T, 1, 4, 8, 1>(g, 2, stream);
+    default: return launch_tile<T, 1, 8, 8, 1>(g, 1, stream);
+  }
+}
+
+// Rows of codes at any alignment into rows of whole 16 bytes; what lies past a row's end becomes 0. A lane takes
+// 16 bytes; 2^lanes_log2 lanes take a row.
+__global__ __launch_bounds__(256) void pad8_kernel(const char* codes, int64_t c_ld, char* to, int64_t to_ld,
+                                                   int64_t rows, int k, int lanes_log2) {
+  const int lanes = 1 << lanes_log2, lane = threadIdx.x & (lanes - 1);
+  const int64_t block = static_cast<int64_t>(blockIdx.y) * gridDim.x + blockIdx.x;
+  const int64_t row = (block << (8 - lanes_log2)) + (threadIdx.x >> lanes_log2);
+  if (row >= rows) return;
+  for (int at = 16 * lane; at < k; at += 16 * lanes) {
+    const char* p = codes + row * c_ld + at;
+    u32x4 v = {0u, 0u, 0u, 0u};
+    if (at + 16 <= k) {
+      __builtin_memcpy(&v, p, sizeof(v));
+    } else {
+      for (int e = 0; e < k - at; ++e) {
+        v[e / 4] |= static_cast<uint32_t>(static_cast<uint8_t>(p[e])) << (8 * (e % 4));
+      }
+    }
+    *reinterpret_cast<u32x4*>(to + row * to_ld + at) = v;
+  }
+}
+
+int launch_pad(const Lin8Geom& g, char* to, int64_t to_ld, hipStream_t stream) {
+  int log2 = 0;
+  while (log2 < 8 && (16 << log2) < g.k) ++log2;
+  const int64_t blocks = (g.m + (256 >> log2) - 1) / (256 >> log2), most = 1 << 23;
+  const dim3 grid(static_cast<unsigned>(blocks < most ? blocks : most),
+                  static_cast<unsigned>((blocks + most - 1) / most));
+  hipLaunchKernelGGL(pad8_kernel, grid, dim3(256), 0, stream, g.codes, g.c_ld, to, to_ld, g.m, g.k, log2);
+  return check_launch("m3_linear8 (codes)");
+}
+
+bool aligned(const m3_linear8_args& a) {
+  return reinterpret_cast<uintptr_t>(a.codes) % 16 == 0 && (a.m == 1 || a.codes_stride % 16 == 0) &&
+         (a.exact == 0 || a.k % 16 == 0);
+}
+
+// Bytes of the copy of the codes that the call needs.
+size_t need(const m3_linear8_args& a) {
+  if (a.m == 0 || a.n == 0 || aligned(a) || form_of(a.m, (a.n + 63) / 64) <= kRows) return 0;
+  return static_cast<size_t>(a.m) * ((a.k + 15) / 16 * 16);
 }
 
 int validate(const m3_linear8_args& a) {
@@ -570,10 +654,8 @@ int validate(const m3_linear8_args& a) {
     return fail(M3_EINVAL, "m3_linear8: codes, q or scales are NULL");
   }
   const auto off = [](const void* p, int by) { return reinterpret_cast<uintptr_t>(p) % by != 0; };
-  if (off(a.codes, 16) || a.codes_stride % 16 != 0 || off(a.q, 16) || off(a.scales, 16) ||
-      off(a.row_scales, 4)) {
-    return fail(M3_EUNSUPPORTED, "m3_linear8: rows of codes, q and scales must be 16-byte aligned, "
-                "row_scales 4-byte");
+  if (off(a.q, 16) || off(a.scales, 16) || off(a.row_scales, 4)) {
+    return fail(M3_EUNSUPPORTED, "m3_linear8: q and scales must be 16-byte aligned, row_scales 4-byte");
   }
   // offsets within the rows of a workgroup (up to 256) are 32-bit
   if (a.codes_stride < a.k || a.codes_stride > (1 << 22)) {
@@ -592,6 +674,9 @@ int validate(const m3_linear8_args& a) {
       meets(a.q, tiles * ((a.k + 127) / 128) * 2 * kTileBytes) || meets(a.scales, tiles * 256)) {
     return fail(M3_EINVAL, "m3_linear8: out overlaps codes, the weight or scales");
   }
+  if (a.workspace != nullptr && meets(a.workspace, static_cast<int64_t>(need(a)))) {
+    return fail(M3_EINVAL, "m3_linear8: out overlaps the workspace");
+  }
   const bool same = a.residual.ptr == a.out.ptr && (a.m == 1 || a.residual.stride[0] == a.out.stride[0]);
   if (present(a.residual) && !same && meets(a.residual.ptr, ((a.m - 1) * a.residual.stride[0] + a.n) * es)) {
     return fail(M3_EINVAL, "m3_linear8: out overlaps the residual without being it");
@@ -602,12 +687,22 @@ int validate(const m3_linear8_args& a) {
 }  // namespace
 }  // namespace m3
 
+extern "C" int m3_linear8_workspace_size(const m3_linear8_args* args, size_t* bytes) {
+  using namespace m3;
+  clear_error();
+  if (args == nullptr || bytes == nullptr) return fail(M3_EINVAL, "m3_linear8_workspace_size: NULL args");
+  const int rc = validate(*args);
+  if (rc != M3_OK) return rc;
+  *bytes = need(*args);
+  return M3_OK;
+}
+
 extern "C" int m3_linear8(const m3_linear8_args* args, hipStream_t stream) {
   using namespace m3;
   clear_error();
   if (args == nullptr) return fail(M3_EINVAL, "m3_linear8: NULL args");
   const m3_linear8_args& a = *args;
-  const int rc = validate(a);
+  int rc = validate(a);
   if (rc != M3_OK) return rc;
   if (a.m == 0 || a.n == 0) return M3_OK;
   const int64_t es = elem_size(a.dtype), pitch = a.out.stride[0] * es;
@@ -616,14 +711,28 @@ extern "C" int m3_linear8(const m3_linear8_args* args, hipStream_t stream) {
                      reinterpret_cast<uintptr_t>(a.residual.ptr) % 16 == 0 && a.n * es % 16 == 0 &&
                      (a.m == 1 || (pitch % 16 == 0 && pitch < (1 << 23) && pitch_r % 16 == 0 &&
                                    pitch_r < (1 << 23)));
-  const Lin8Geom g{reinterpret_cast<const char*>(a.codes), a.row_scales,
-                   reinterpret_cast<const char*>(a.q), a.scales, a.residual.ptr, a.out.ptr,
-                   a.codes_stride, a.residual.stride[0], a.out.stride[0], a.m, static_cast<int>(a.n),
-                   static_cast<int>(a.k), static_cast<int>((a.k + 127) / 128 * 2),
-                   static_cast<int>((a.n + 63) / 64), whole};
+  Lin8Geom g{reinterpret_cast<const char*>(a.codes), a.row_scales,
+             reinterpret_cast<const char*>(a.q), a.scales, a.residual.ptr, a.out.ptr,
+             a.codes_stride, a.residual.stride[0], a.out.stride[0], a.m, static_cast<int>(a.n),
+             static_cast<int>(a.k), static_cast<int>((a.k + 127) / 128 * 2),
+             static_cast<int>((a.n + 63) / 64), aligned(a), whole};
+  if (a.m == 1) g.c_ld = (a.k + 15) / 16 * 16;  // rows past the only one lie past the extent
+  const Form form = form_of(a.m, g.tiles);
+  if (const size_t bytes = need(a); bytes != 0) {
+    if (a.workspace == nullptr || a.workspace_bytes < bytes || reinterpret_cast<uintptr_t>(a.workspace) % 16 != 0) {
+      return fail(M3_EWORKSPACE, "m3_linear8: rows of codes at this alignment need a 16-byte aligned workspace of "
+                  "%zu bytes", bytes);
+    }
+    const int64_t ld = (a.k + 15) / 16 * 16;
+    char* const to = static_cast<char*>(a.workspace);
+    if ((rc = launch_pad(g, to, ld, stream)) != M3_OK) return rc;
+    g.codes = to;
+    g.c_ld = ld;
+    g.aligned = true;
+  }
   switch (a.dtype) {
-    case M3_F32: return launch8<float>(g, stream);
-    case M3_BF16: return launch8<__bf16>(g, stream);
-    default: return launch8<_Float16>(g, stream);
+    case M3_F32: return launch8<float>(g, form, stream);
+    case M3_BF16: return launch8<__bf16>(g, form, stream);
+    default: return launch8<_Float16>(g, form, stream);
   }
 }

@@ -333,18 +333,15 @@ __global__ __launch_bounds__(256) void values8_kernel(const int8_t* codes, int64
   T* const to = out + row * o_ld;
 #pragma unroll 4
   for (int at = kPiece * lane; at < dim; at += kPiece * lanes) {
-    int8_t c[kPiece];  // rows of codes reach to a multiple of 16
-    __builtin_memcpy(c, __builtin_assume_aligned(from + at, kPiece), sizeof(c));
-    T t[kPiece];
-#pragma unroll
-    for (int e = 0; e < kPiece; ++e) t[e] = from_f32<T>(static_cast<float>(c[e]) * scale);
     if (at + kPiece <= dim) {
+      int8_t c[kPiece];
+      __builtin_memcpy(c, from + at, sizeof(c));
+      T t[kPiece];
+#pragma unroll
+      for (int e = 0; e < kPiece; ++e) t[e] = from_f32<T>(static_cast<float>(c[e]) * scale);
       __builtin_memcpy(to + at, t, sizeof(t));
     } else {
-#pragma unroll
-      for (int e = 0; e < kPiece; ++e) {
-        if (at + e < dim) to[at + e] = t[e];
-      }
+      for (int e = at; e < dim; ++e) to[e] = from_f32<T>(static_cast<float>(from[e]) * scale);
     }
   }
 }
@@ -416,11 +413,11 @@ int check_sizes(const char* name, int64_t rows, int64_t dim) {
   return M3_OK;
 }
 
-int check_codes(const char* name, const int8_t* codes, int64_t stride, const float* scales, int64_t dim) {
+int check_codes(const char* name, const int8_t* codes, int64_t stride, const float* scales, int64_t dim, int by) {
   if (codes == nullptr || scales == nullptr) return fail(M3_EINVAL, "%s: codes or scales are NULL", name);
-  if (reinterpret_cast<uintptr_t>(codes) % 16 != 0 || stride % 16 != 0 ||
+  if (reinterpret_cast<uintptr_t>(codes) % by != 0 || stride % by != 0 ||
       reinterpret_cast<uintptr_t>(scales) % 4 != 0) {
-    return fail(M3_EUNSUPPORTED, "%s: rows of codes must be 16-byte aligned, scales 4-byte", name);
+    return fail(M3_EUNSUPPORTED, "%s: rows of codes must be %d-byte aligned, scales 4-byte", name, by);
   }
   if (stride < dim) return fail(M3_EINVAL, "%s: rows of codes overlap", name);
   return M3_OK;
@@ -438,7 +435,7 @@ int validate(const m3_rows8_args& a) {
   if (present(a.add) && !present(a.weight)) return fail(M3_EINVAL, "m3_rows8: add needs weight");
   if (present(a.sum_out) && !present(a.add)) return fail(M3_EINVAL, "m3_rows8: sum_out needs add");
   if (present(a.weight) && !(a.eps >= 0.f)) return fail(M3_EINVAL, "m3_rows8: eps must be >= 0");
-  if ((rc = check_codes("m3_rows8", a.codes, a.codes_stride, a.scales, a.dim))) return rc;
+  if ((rc = check_codes("m3_rows8", a.codes, a.codes_stride, a.scales, a.dim, 16))) return rc;
   const int64_t whole = (a.dim + 15) / 16 * 16;
   if (a.rows > 1 && present(a.sum_out) && a.sum_out.stride[0] < a.dim) {
     return fail(M3_EINVAL, "m3_rows8: rows of sum_out overlap");
@@ -468,7 +465,7 @@ int validate(const m3_rows8_args& a) {
 int validate(const m3_rows8_values_args& a) {
   int rc;
   if ((rc = check_sizes("m3_rows8_values", a.rows, a.dim)) || a.rows == 0) return rc;
-  if ((rc = check_codes("m3_rows8_values", a.codes, a.codes_stride, a.scales, a.dim)) ||
+  if ((rc = check_codes("m3_rows8_values", a.codes, a.codes_stride, a.scales, a.dim, 1)) ||
       (rc = check_tensor(a.out, "out", 2, a.dim, true, -1))) {
     return rc;
   }

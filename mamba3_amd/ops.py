@@ -876,7 +876,8 @@ def _device_index(first: torch.Tensor, *others: torch.Tensor | None) -> int:
 class Rows8:
     """Rows ``[..., K]`` in 8 bits: ``codes`` int8, -128 to 127, with one FP32 scale each (``scales
     [...]``); a row is ``code * scale``. ``quantize8_rows`` and ``rms_norm8`` make them, ``linear8`` multiplies
-    them. Codes from elsewhere are taken as they are, copied where their rows are not 16-byte aligned.
+    them. Codes from elsewhere are taken as they are where their columns lie side by side and their rows
+    evenly apart, else copied.
     """
 
     # _ld: bytes between rows; _memory: the int8 tensor of both (codes, then scales), or of given codes
@@ -895,8 +896,11 @@ class Rows8:
         if width > _hip.LINEAR8_MAX_K:
             raise ValueError(f"rows of {width}: at most {_hip.LINEAR8_MAX_K}")
         scales, ld = scales.contiguous(), width
-        if width % 16 or not codes.is_contiguous() or codes.data_ptr() % 16:
-            codes, ld = _whole_rows(codes if len(shape) == 2 else codes.reshape(-1, width))
+        if not codes.is_contiguous():
+            codes = codes.reshape(-1, width)
+            if codes.stride(1) != 1 and width > 1 or not width <= codes.stride(0) <= 1 << 22:
+                codes = codes.contiguous()
+            ld = codes.stride(0)
         self.shape, self._rows, self._ld, self._memory, self._given = shape, rows, ld, codes, scales
 
     @classmethod
@@ -952,21 +956,6 @@ class Rows8:
                 rows, width, *self._block(),
                 out.data_ptr(), _hip.dtype_code(dtype), 0, width, 1, 0, 0, 0), index)
         return out
-
-
-def _whole_rows(codes: torch.Tensor) -> tuple[torch.Tensor, int]:
-    """Codes ``[rows, K]`` with 16-byte aligned rows that reach to a multiple of 16, and the bytes
-    between them: as they are if they have such rows, else copied."""
-    rows, width = codes.shape
-    whole = -(-width // 16) * 16
-    if not codes.is_contiguous() and codes.stride(1) == 1 and codes.data_ptr() % 16 == 0:
-        ld = codes.stride(0) if rows > 1 else whole
-        if ld % 16 == 0 and width <= ld <= 1 << 22 and (
-                codes.storage_offset() + (rows - 1) * ld + whole <= codes.untyped_storage().nbytes()):
-            return codes, ld
-    held = codes.new_empty((rows, whole))[:, :width]
-    held.copy_(codes)
-    return held, whole
 
 
 class Weight8:
@@ -1129,13 +1118,19 @@ def linear8(rows: Rows8, weight: Weight8, residual: torch.Tensor | None = None, 
     if given and (m > 1 and flat.stride(0) < n or n > 1 and flat.stride(1) != 1):
         raise ValueError("linear8: out needs a unit inner stride and rows of its own")
     if m:
-        code, residual = _hip.dtype_code(dtype), _inner(residual)
+        code, residual, ws = _hip.dtype_code(dtype), _inner(residual), None
+        codes, ld, scales = rows._block()
+        exact = rows._given is not None
+        values = (m, n, k, code, exact, codes, ld, scales, weight.q.data_ptr(), weight.scales.data_ptr(),
+                  *(_hip.NO_TENSOR if residual is None else
+                    (residual.data_ptr(), code, 0, *residual.stride(), 0, 0, 0)),
+                  flat.data_ptr(), code, 0, *flat.stride(), 0, 0, 0)
+        if exact and (codes % 16 or ld % 16 or k % 16):
+            size = _hip.need("m3_linear8_workspace_size", _hip.LINEAR8.pack(*values, 0, 0))
+            ws = rows._memory.new_empty(size) if size else None
         _hip.launch("m3_linear8", _hip.LINEAR8.pack(
-            m, n, k, code, 0, *rows._block(),
-            weight.q.data_ptr(), weight.scales.data_ptr(),
-            *(_hip.NO_TENSOR if residual is None else
-              (residual.data_ptr(), code, 0, *residual.stride(), 0, 0, 0)),
-            flat.data_ptr(), code, 0, *flat.stride(), 0, 0, 0), index)
+            *values, *((0, 0) if ws is None else (ws.data_ptr(), ws.numel()))), index)
+        del ws
     if given:
         _written(out)
     return out

@@ -141,6 +141,25 @@ def test_strided_operands(m, dtype):
         assert torch.equal(base_res[:, 3:3 + n], out[:m, 5:5 + n])
 
 
+@pytest.mark.parametrize("k", [1, 3, 15, 16, 17, 40, 63, 100, 129, 200, 333, 1111])
+@pytest.mark.parametrize("m,n", [(1, 70), (3, 9000), (15, 64), (16, 130), (17, 1), (33, 9000), (100, 500), (260, 1500),
+                                 (700, 5000), (3000, 2500)])
+def test_codes_at_any_alignment(m, n, k):
+    """Rows side by side of any width, at an odd address, that end where their memory does; and apart."""
+    g = torch.Generator().manual_seed(m + k)
+    codes, q, rs, s = _operands(m, n, k, g, full=True)
+    weight = ops.Weight8(q.to(DEV), s.to(DEV))
+    odd = torch.empty(m * k + 5, dtype=torch.int8, device=DEV)[5:].view(m, k)
+    odd.copy_(codes)
+    apart = torch.full((m, k + 7), 3, dtype=torch.int8, device=DEV)[:, 7:]
+    apart.copy_(codes)
+    with torch.inference_mode():
+        first = ops.linear8(ops.Rows8(odd, rs.to(DEV)), weight)
+        _check(first, codes, q, rs, s)
+        for given in (apart, codes.to(DEV)):
+            assert torch.equal(ops.linear8(ops.Rows8(given, rs.to(DEV)), weight), first)
+
+
 def test_more_axes_and_no_rows():
     g = torch.Generator().manual_seed(6)
     codes, q, rs, s = _operands(6, 40, 50, g)
