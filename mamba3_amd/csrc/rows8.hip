@@ -17,7 +17,7 @@
 // a bf16 add and the sum kept 138 us (5.35 TB/s of what moves), 16384 x 2048 bf16 the same way 47.5 us (4.95),
 // 32768 x 4096 bf16 without norm 77.5 us (5.2), one row of 2048 3.5 us.
 //
-// m3_rows8_values, what the rows stand for, likewise: 32768 x 4096 to FP32 150 us (4.5 TB/s).
+// m3_rows8_values, what the rows stand for, likewise: 32768 x 4096 to FP32 104 us (6.4 TB/s).
 #include <hip/hip_runtime.h>
 
 #include "m3_common.hpp"
