@@ -1005,29 +1005,34 @@ def quantize8(weight: torch.Tensor) -> Weight8:
     return Weight8(codes, most.squeeze(1).float() / 127)
 
 
+def _row_tensor(t: torch.Tensor | None, width: int) -> tuple[object, tuple[int, ...]]:
+    """``[..., width]`` as rows: what has to stay alive across the call, and the values of its
+    descriptor."""
+    if t is None:
+        return None, _hip.NO_TENSOR
+    if t.is_contiguous():
+        return t, (t.data_ptr(), _hip.dtype_code(t.dtype), 0, width, 1, 0, 0, 0)
+    t = _inner(t.reshape(-1, width))
+    return t, (t.data_ptr(), _hip.dtype_code(t.dtype), 0, *t.stride(), 0, 0, 0)
+
+
 def _rows8(x, weight, eps, add, keep_sum, index) -> tuple[Rows8, torch.Tensor | None]:
-    shape, flat = x.shape, x
+    shape = x.shape
     width = shape[-1]
-    if len(shape) != 2:
-        flat = x.reshape(-1, width)
-        add = None if add is None else add.reshape(-1, width)
-    flat, add = _inner(flat), _inner(add)
-    rows = flat.shape[0]
-    ld = -(-width // 64) * 64
+    rows, ld = x.numel() // width, -(-width // 64) * 64
     memory = x.new_empty(rows * (ld + 4), dtype=torch.int8)
-    held = Rows8._of(memory, shape, rows, ld)
     total = x.new_empty(shape) if keep_sum else None
     if rows:
-        code, none = _hip.dtype_code(x.dtype), _hip.NO_TENSOR
+        at = memory.data_ptr()
+        held_x, block_x = _row_tensor(x, width)
+        held_add, block_add = _row_tensor(add, width)
         _hip.launch("m3_rows8", _hip.ROWS8.pack(
-            rows, width, eps, 0, flat.data_ptr(), code, 0, *flat.stride(), 0, 0, 0,
-            *(none if add is None else
-              (add.data_ptr(), _hip.dtype_code(add.dtype), 0, *add.stride(), 0, 0, 0)),
-            *(none if weight is None else
+            rows, width, eps, 0, *block_x, *block_add,
+            *(_hip.NO_TENSOR if weight is None else
               (weight.data_ptr(), _hip.dtype_code(weight.dtype), 0, 1, 0, 0, 0, 0)),
-            *(none if total is None else (total.data_ptr(), code, 0, width, 1, 0, 0, 0)),
-            *held._block()), index)
-    return held, total
+            *_row_tensor(total, width)[1], at, ld, at + rows * ld), index)
+        del held_x, held_add
+    return Rows8._of(memory, shape, rows, ld), total
 
 
 def _check_rows8(name: str, x: torch.Tensor) -> None:
@@ -1111,26 +1116,22 @@ def linear8(rows: Rows8, weight: Weight8, residual: torch.Tensor | None = None, 
     given, m = out is not None, rows._rows
     if not given:
         out = rows._memory.new_empty(shape, dtype=dtype)
-    flat = out
-    if len(shape) != 2:
-        residual = None if residual is None else residual.reshape(-1, n)
-        flat = out.view(-1, n)
-    if given and (m > 1 and flat.stride(0) < n or n > 1 and flat.stride(1) != 1):
+    flat = out if out.is_contiguous() else out.view(-1, n)
+    if given and flat is not out and (m > 1 and flat.stride(0) < n or n > 1 and flat.stride(1) != 1):
         raise ValueError("linear8: out needs a unit inner stride and rows of its own")
     if m:
-        code, residual, ws = _hip.dtype_code(dtype), _inner(residual), None
+        ws = None
         codes, ld, scales = rows._block()
         exact = rows._given is not None
-        values = (m, n, k, code, exact, codes, ld, scales, weight.q.data_ptr(), weight.scales.data_ptr(),
-                  *(_hip.NO_TENSOR if residual is None else
-                    (residual.data_ptr(), code, 0, *residual.stride(), 0, 0, 0)),
-                  flat.data_ptr(), code, 0, *flat.stride(), 0, 0, 0)
+        residual, block = _row_tensor(residual, n)
+        values = (m, n, k, _hip.dtype_code(dtype), exact, codes, ld, scales, weight.q.data_ptr(),
+                  weight.scales.data_ptr(), *block, *_row_tensor(flat, n)[1])
         if exact and (codes % 16 or ld % 16 or k % 16):
             size = _hip.need("m3_linear8_workspace_size", _hip.LINEAR8.pack(*values, 0, 0))
             ws = rows._memory.new_empty(size) if size else None
         _hip.launch("m3_linear8", _hip.LINEAR8.pack(
             *values, *((0, 0) if ws is None else (ws.data_ptr(), ws.numel()))), index)
-        del ws
+        del ws, residual
     if given:
         _written(out)
     return out
