@@ -454,6 +454,9 @@ __global__ __launch_bounds__(64 * WM * WN * KS, 2) void linear8_tile_kernel(cons
     }
     constexpr int kPiece = 16 / static_cast<int>(sizeof(T));  // elements
     const bool odd = (lane & 1) != 0;
+    // out is not read again here: kept out of the L2 it leaves that to codes and weight (65536 x 4480 x 1024 294 -> 264
+    // us, the next kernel that reads it 10 us more); the few outputs of tiles with K in parts gain nothing by it
+    constexpr int kStream = KS == 1 ? 2 : 0;
     // the residual, as many blocks of rows at a time as the registers hold, before the stores of these
     constexpr int kBatch = RES && WHOLE ? 2 * XI / (8 / kPiece) / 4 : 1;
     u32x4 held[kBatch][2][8 / kPiece];
@@ -514,9 +517,9 @@ __global__ __launch_bounds__(64 * WM * WN * KS, 2) void linear8_tile_kernel(cons
         if constexpr (WHOLE) {
           const unsigned pitch = static_cast<unsigned>(g.o_ld) * static_cast<unsigned>(sizeof(T));
           const unsigned to = m2 * pitch + n * static_cast<unsigned>(sizeof(T));
-          __builtin_amdgcn_raw_buffer_store_b128(first, ro, n < g.n && m2 < left ? to : kNowhere, 0, 0);
+          __builtin_amdgcn_raw_buffer_store_b128(first, ro, n < g.n && m2 < left ? to : kNowhere, 0, kStream);
           __builtin_amdgcn_raw_buffer_store_b128(second, ro, n < g.n && m2 + 1 < left ? to + pitch : kNowhere, 0,
-                                                 0);
+                                                 kStream);
         } else {
           T* const to = out + (m0 + m2) * g.o_ld;
           if (m2 < left) store_piece(to, n, g.n, first);
@@ -566,15 +569,17 @@ int launch_tile(const Lin8Geom& g, int a_cu, hipStream_t stream) {
 //     next 13.9; 512 x 2048 x 4096, two a CU: 16.9, 16.0)
 //   64 x 128 with K in halves, for up to half a 128 x 256 tile a CU (1000 x 2048 x 4096: 16.6, 128 x 128 26.6;
 //     2000 x 2048 x 4096: 26.1, 128 x 256 about 30; 512 x 8672 x 2048, 136 tiles: 21.2, 18.9)
-//   128 x 256 by two workgroups a CU or 128 x 512 by one, whose rounds cost 17 and 16, half a round of the first
-//     12 (4000 x 2048 x 4096: 33.5, 45.7; 2000 x 8672 x 2048: 40.8, 50.5; 8192 x 28672 x 8192: 1,430, 1,340)
+//   128 x 256 by two workgroups a CU, whose outputs' rounding hides behind each other's products, or where K is long 128
+//     x 512 by one, whose rounds cost 17 and 16, half a round of the first 12 (65536 x 4480 x 1024: 264, 274; 16384 x
+//     8672 x 2048: 224, 237; 8192 x 28672 x 8192: 1,342, 1,300; 4000 x 2048 x 4096: 30.8, 42.8)
 enum Form { kCells, kRows, kHalves, kMedium, kLarge };
-Form form_of(int64_t m, int64_t tiles) {
+Form form_of(int64_t m, int64_t tiles, int64_t k) {
   const int64_t cells = 4 * tiles * ((m + 15) / 16);
   if (cells <= 2 * kCus || (m <= 4 && cells <= 3 * kCus)) return kCells;
   if (m <= 32 || tiles * ((m + 31) / 32) <= 3 * kCus / 2) return kRows;
   const int64_t tm = (m + 127) / 128, medium = tm * ((tiles + 3) / 4);
   if (medium <= kCus / 2) return kHalves;
+  if (k <= 2048) return kMedium;
   const int64_t large = tm * ((tiles + 7) / 8), rest = medium % (2 * kCus);
   const int64_t one = (large + kCus - 1) / kCus * 16;
   const int64_t two = medium / (2 * kCus) * 17 + (rest == 0 ? 0 : rest <= kCus ? 12 : 17);
@@ -631,7 +636,7 @@ bool aligned(const m3_linear8_args& a) {
 
 // Bytes of the copy of the codes that the call needs.
 size_t need(const m3_linear8_args& a) {
-  if (a.m == 0 || a.n == 0 || aligned(a) || form_of(a.m, (a.n + 63) / 64) <= kRows) return 0;
+  if (a.m == 0 || a.n == 0 || aligned(a) || form_of(a.m, (a.n + 63) / 64, a.k) <= kRows) return 0;
   return static_cast<size_t>(a.m) * ((a.k + 15) / 16 * 16);
 }
 
@@ -717,7 +722,7 @@ extern "C" int m3_linear8(const m3_linear8_args* args, hipStream_t stream) {
              static_cast<int>(a.k), static_cast<int>((a.k + 127) / 128 * 2),
              static_cast<int>((a.n + 63) / 64), aligned(a), whole};
   if (a.m == 1) g.c_ld = (a.k + 15) / 16 * 16;  // rows past the only one lie past the extent
-  const Form form = form_of(a.m, g.tiles);
+  const Form form = form_of(a.m, g.tiles, a.k);
   if (const size_t bytes = need(a); bytes != 0) {
     if (a.workspace == nullptr || a.workspace_bytes < bytes || reinterpret_cast<uintptr_t>(a.workspace) % 16 != 0) {
       return fail(M3_EWORKSPACE, "m3_linear8: rows of codes at this alignment need a 16-byte aligned workspace of "
