@@ -373,9 +373,9 @@ int m3_linear4(const m3_linear4_args* args, hipStream_t stream);
  *   p = s * weight (the weight rounded to x's dtype; without weight p = x), most = max |p| of the row
  *   code = rint(127 p / most) of the exact quotient, ties to even
  *   scale = most / 127, with weight times rsqrt(mean(s^2) + eps)
- * so that code * scale is what x, or its RMSNorm, holds. A row of zeros has codes and scale 0; a row
- * that holds an infinity or NaN has codes 0 and scale NaN. The sum of squares and p have to stay in
- * FP32's range.
+ * so that code * scale is what x, or its RMSNorm, holds. A row of zeros has codes and scale 0 (scale NaN
+ * behind a norm of zeros with eps = 0); a row that holds an infinity or NaN has codes 0 and scale NaN. The
+ * sum of squares and p have to stay in FP32's range.
  * x, add, sum_out as in m3_rms_norm (FP32 with an add of any dtype, or 16 bits throughout; sum_out may be x, or
  * an add of its dtype), at any alignment, dim from 1 to M3_LINEAR8_MAX_K. What is written otherwise
  * overlaps nothing.

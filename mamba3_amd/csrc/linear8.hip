@@ -531,6 +531,8 @@ __global__ __launch_bounds__(64 * WM * WN * KS, 2) void linear8_tile_kernel(cons
     }
     stored = WHOLE;
   }
+  // the fetches past the last tile write (zeros) to LDS, too: none is left behind
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 }
 
 template <typename T, int MT, int TN, int WAVES, int AHEAD>

@@ -1066,7 +1066,8 @@ def rms_norm8(x: torch.Tensor, weight: torch.Tensor, eps: float = NORM_EPS, *,
 
     Rows of any K and strides: an FP32 ``x`` with an ``add`` of any dtype, or a 16-bit ``x`` with one of its
     own. The norm's factor is in the scale, not in the codes: ``code = rint(127 p / max|p|)`` with ``p = s *
-    weight``. Rows of zeros, infinities and NaN as in ``quantize8_rows``. No backward.
+    weight``. Rows of zeros, infinities and NaN as in ``quantize8_rows``; with ``eps = 0`` zeros alone give a
+    scale of NaN, as ``F.rms_norm`` gives NaN. No backward.
     """
     _check_rows8("rms_norm8", x)
     if weight.shape != x.shape[-1:] or weight.dtype not in _FLOAT_DTYPES:

@@ -215,6 +215,22 @@ def test_values(k, dtype):
         assert torch.isnan(got[m // 2]).all()
 
 
+@pytest.mark.parametrize("k", [1, 100, 2048, 9000])
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+def test_zeros_without_eps(k, dtype):
+    """eps = 0: a row of zeros is NaN, as F.rms_norm's; the next row and any eps above 0 know nothing of it."""
+    x = torch.zeros(3, k, dtype=dtype, device=DEV)
+    x[1] = 0.5
+    weight = torch.ones(k, device=DEV)
+    rows, _ = ops.rms_norm8(x, weight, 0.0)
+    assert torch.isnan(rows.scales[::2]).all() and (rows.codes[::2] == 0).all()
+    assert torch.isnan(torch.nn.functional.rms_norm(x, (k,), weight.to(dtype), 0.0)[::2]).all()
+    # 0.5 / 127 / 0.5: a rounding of 127ths, one of the root (2 steps), one of the product
+    assert (rows.codes[1] == 127).all() and abs(rows.scales[1].item() * 127 - 1) < 5 * 2 ** -24
+    rows, _ = ops.rms_norm8(x, weight, EPS)
+    assert (rows.scales[::2] == 0).all() and (rows.codes[::2] == 0).all()
+
+
 def test_what_is_written():
     """The C entry point: codes and scales of the rows and nothing else; the sum in x's place, or the add's."""
     g = torch.Generator().manual_seed(3)
