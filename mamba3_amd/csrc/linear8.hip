@@ -568,17 +568,21 @@ int launch_tile(const Lin8Geom& g, int a_cu, hipStream_t stream) {
 //   16 x 16 of out a workgroup of 8 waves, while these are at most two a CU (64 x 2048 x 4096: 7.3, the next 8.3;
 //     16 x 4480 x 1024: 3.9, 4.4), or three with up to 4 rows (4 x 8672 x 2048: 5.5, 5.9; 8 rows: 6.1, 6.0)
 //   32 x 64, for up to 32 rows or 1.5 a CU (16 x 16384 x 4096: 12.4, the one before 21; 256 x 2048 x 4096: 10.1, the
-//     next 13.9; 512 x 2048 x 4096, two a CU: 16.9, 16.0)
+//     next 13.9; 512 x 2048 x 4096, two a CU: 16.9, 16.0); one column of tiles, too, where the codes' alignment asks the
+//     next ones for a copy of them (65536 x 64 x 1001: 31.6, 63.8; 65536 x 16 x 4095: 134, 200; two columns, 65536 x 128 x
+//     4095: 264, 204)
 //   64 x 128 with K in halves, for up to half a 128 x 256 tile a CU (1000 x 2048 x 4096: 16.6, 128 x 128 26.6;
 //     2000 x 2048 x 4096: 26.1, 128 x 256 about 30; 512 x 8672 x 2048, 136 tiles: 21.2, 18.9)
 //   128 x 256 by two workgroups a CU, whose outputs' rounding hides behind each other's products, or where K is long 128
 //     x 512 by one, whose rounds cost 17 and 16, half a round of the first 12 (65536 x 4480 x 1024: 264, 274; 16384 x
 //     8672 x 2048: 224, 237; 8192 x 28672 x 8192: 1,342, 1,300; 4000 x 2048 x 4096: 30.8, 42.8)
 enum Form { kCells, kRows, kHalves, kMedium, kLarge };
-Form form_of(int64_t m, int64_t tiles, int64_t k) {
+Form form_of(int64_t m, int64_t tiles, int64_t k, bool aligned) {
   const int64_t cells = 4 * tiles * ((m + 15) / 16);
   if (cells <= 2 * kCus || (m <= 4 && cells <= 3 * kCus)) return kCells;
   if (m <= 32 || tiles * ((m + 31) / 32) <= 3 * kCus / 2) return kRows;
+  // (a launch has 65,535 rows of workgroups)
+  if (!aligned && tiles == 1 && (m + 31) / 32 < 1 << 16) return kRows;
   const int64_t tm = (m + 127) / 128, medium = tm * ((tiles + 3) / 4);
   if (medium <= kCus / 2) return kHalves;
   if (k <= 2048) return kMedium;
@@ -638,7 +642,7 @@ bool aligned(const m3_linear8_args& a) {
 
 // Bytes of the copy of the codes that the call needs.
 size_t need(const m3_linear8_args& a) {
-  if (a.m == 0 || a.n == 0 || aligned(a) || form_of(a.m, (a.n + 63) / 64, a.k) <= kRows) return 0;
+  if (a.m == 0 || a.n == 0 || aligned(a) || form_of(a.m, (a.n + 63) / 64, a.k, false) <= kRows) return 0;
   return static_cast<size_t>(a.m) * ((a.k + 15) / 16 * 16);
 }
 
@@ -724,7 +728,7 @@ extern "C" int m3_linear8(const m3_linear8_args* args, hipStream_t stream) {
              static_cast<int>(a.k), static_cast<int>((a.k + 127) / 128 * 2),
              static_cast<int>((a.n + 63) / 64), aligned(a), whole};
   if (a.m == 1) g.c_ld = (a.k + 15) / 16 * 16;  // rows past the only one lie past the extent
-  const Form form = form_of(a.m, g.tiles, a.k);
+  const Form form = form_of(a.m, g.tiles, a.k, g.aligned);
   if (const size_t bytes = need(a); bytes != 0) {
     if (a.workspace == nullptr || a.workspace_bytes < bytes || reinterpret_cast<uintptr_t>(a.workspace) % 16 != 0) {
       return fail(M3_EWORKSPACE, "m3_linear8: rows of codes at this alignment need a 16-byte aligned workspace of "

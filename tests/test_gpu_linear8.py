@@ -160,6 +160,22 @@ def test_codes_at_any_alignment(m, n, k):
             assert torch.equal(ops.linear8(ops.Rows8(given, rs.to(DEV)), weight), first)
 
 
+@pytest.mark.parametrize("m,n,k", [(13000, 1, 17), (20000, 63, 90), (20011, 64, 333), (13000, 65, 90), (2097120, 3, 17),
+                                   (2097121, 3, 17)])
+def test_many_rows_at_any_alignment(m, n, k):
+    """Few outputs of many rows, on both sides of 64 columns and of 65,535 rows of workgroups; with a residual."""
+    g = torch.Generator().manual_seed(m + k)
+    codes, q, rs, s = _operands(m, n, k, g)
+    weight = ops.Weight8(q.to(DEV), s.to(DEV))
+    res = torch.randn(m, n, generator=g).to(F16)
+    odd = torch.empty(m * k + 3, dtype=torch.int8, device=DEV)[3:].view(m, k)
+    odd.copy_(codes)
+    with torch.inference_mode():
+        got = ops.linear8(ops.Rows8(odd, rs.to(DEV)), weight, res.to(DEV))
+        _check(got, codes, q, rs, s, res)
+        assert torch.equal(ops.linear8(ops.Rows8(codes.to(DEV), rs.to(DEV)), weight, res.to(DEV)), got)
+
+
 def test_more_axes_and_no_rows():
     g = torch.Generator().manual_seed(6)
     codes, q, rs, s = _operands(6, 40, 50, g)
