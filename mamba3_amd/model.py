@@ -136,12 +136,17 @@ class _Mamba3Mixer(nn.Module):
         self._decode4 = self._signed(held)
 
     def _held(self, copies: dict[str, tuple], name: str, maker: str):
-        """The projection's copy, if there is one; refused once the weight has changed."""
+        """The projection's copy, if there is one; refused once the weight has changed, or the
+        projection is more than its weight's product."""
         if name not in copies:
             return None
         held, then = copies[name]
-        if not _same_storage(_storage_signature(getattr(self, name).weight), then):
+        module = getattr(self, name)
+        if not _same_storage(_storage_signature(module.weight), then):
             raise RuntimeError(f"{name}.weight changed since {maker}; call it again")
+        if not _plain_linear(module):
+            raise RuntimeError(f"{name} changed since {maker}: a hook, a bias or a module around it is not "
+                               "in the copy of its weight")
         return held
 
     def _weight4(self, name: str) -> ops.Weight4 | None:
@@ -255,8 +260,9 @@ class _Mamba3Mixer(nn.Module):
         first; with ``residual`` (``[batch, 1, d_model]``) the result is
         ``residual + out_proj(...)``. With 16-bit weights, ``in_proj`` runs on ``ops.linear``
         with the norm fused up to ``ops.DECODE_LINEAR_ROWS`` rows, and ``out_proj`` with the
-        residual add fused up to ``ops.DECODE_LINEAR_OUT_ROWS``. Rows in 8 bits are normed already, and
-        ``dtype`` is what ``in_proj`` gives of them."""
+        residual add fused up to ``ops.DECODE_LINEAR_OUT_ROWS``; a projection with a bias, hooks or a
+        module around it is called as it is. Rows in 8 bits are normed already, and ``dtype`` is what
+        ``in_proj`` gives of them."""
         if len(hidden_states.shape) != 3 or hidden_states.shape[1:] != (1, self.d_model):
             raise ValueError(
                 f"expected [batch, 1, {self.d_model}], got {tuple(hidden_states.shape)}")
@@ -268,27 +274,27 @@ class _Mamba3Mixer(nn.Module):
         rows = hidden_states[:, 0]
         small = rows.shape[0] <= ops.DECODE_LINEAR_ROWS
         supported = ops.linear_norm_supported if norm is not None else ops.linear_supported
-        in4 = self._weight4("in_proj")
-        if (small and in4 is not None and rows.dtype == self.in_proj.weight.dtype
+        in_proj, in4 = self.in_proj, self._weight4("in_proj")
+        if (small and in4 is not None and rows.dtype == in_proj.weight.dtype
                 and ops.linear4_supported(rows, in4)):
             proj = ops.linear4(rows, in4, norm_weight=norm.weight if norm is not None else None,
                                norm_eps=norm.eps if norm is not None else ops.NORM_EPS)
             proj = proj.unsqueeze(1)
-        elif small and supported(rows, self.in_proj.weight):
-            proj = ops.linear(rows, self.in_proj.weight,
+        elif small and _plain_linear(in_proj) and supported(rows, in_proj.weight):
+            proj = ops.linear(rows, in_proj.weight,
                               norm_weight=norm.weight if norm is not None else None,
                               norm_eps=norm.eps if norm is not None else ops.NORM_EPS)
             proj = proj.unsqueeze(1)
         else:
             normed = norm(hidden_states) if norm is not None else hidden_states
             # few rows keep to the weights that their neighbours' kernels read
-            proj = self.in_proj(normed) if small else self._project("in_proj", normed)
+            proj = in_proj(normed) if small else self._project("in_proj", normed)
         return self._step_from(proj, cache, inplace, residual)
 
     def _step_from(self, proj: torch.Tensor, cache: _LayerCache | None, inplace: bool,
                    residual: torch.Tensor | None):
         """The rest of a step, from ``in_proj``'s output."""
-        batch, out4 = proj.shape[0], self._weight4("out_proj")
+        batch, out_proj, out4 = proj.shape[0], self.out_proj, self._weight4("out_proj")
         if cache is None:
             cache = self.allocate_cache(batch, device=proj.device, dtype=proj.dtype)
         else:
@@ -300,12 +306,12 @@ class _Mamba3Mixer(nn.Module):
                 and (residual is None or residual.dtype == mixed.dtype)):
             res = residual[:, 0] if residual is not None else None
             return ops.linear4(mixed, out4, res).unsqueeze(1), next_cache
-        if batch <= ops.DECODE_LINEAR_OUT_ROWS and ops.linear_supported(
-                mixed, self.out_proj.weight) and (residual is None or residual.dtype == mixed.dtype):
-            res = residual[:, 0] if residual is not None else None
-            return ops.linear(mixed, self.out_proj.weight, res).unsqueeze(1), next_cache
         small = batch <= ops.DECODE_LINEAR_OUT_ROWS
-        output = (self.out_proj(mixed) if small else self._project("out_proj", mixed)).unsqueeze(1)
+        if (small and _plain_linear(out_proj) and ops.linear_supported(mixed, out_proj.weight)
+                and (residual is None or residual.dtype == mixed.dtype)):
+            res = residual[:, 0] if residual is not None else None
+            return ops.linear(mixed, out_proj.weight, res).unsqueeze(1), next_cache
+        output = (out_proj(mixed) if small else self._project("out_proj", mixed)).unsqueeze(1)
         if residual is not None:
             output = residual + output
         return output, next_cache
@@ -496,12 +502,15 @@ class Mamba3(nn.Module):
         copies (``ops.linear4``) instead of the weights (quicker up to about 16 rows). Both are
         held: memory grows by a quarter of the projections'. A weight that is replaced or modified
         afterwards (``load_state_dict``, ``to``, a copy of the model) makes ``step`` raise until
-        this is called again. A step's rows must have the weights' dtype, as ever, to run on it.
+        this is called again. A step's rows must have the weights' dtype, as ever, to run on it. A
+        projection with a bias, with forward hooks or within another module (an adapter) is refused, here and by
+        ``step``: its copy would pass them by.
         """
         if not self.causal:
             raise ValueError("quantize_decode requires causal=True")
         for layer in self.layers:
             for name in ("in_proj", "out_proj"):
+                _require_plain("quantize_decode", name, getattr(layer.mixer, name))
                 weight = getattr(layer.mixer, name).weight
                 if weight.dtype not in (torch.bfloat16, torch.float16):
                     raise ValueError("quantize_decode needs bfloat16 or float16 weights")
@@ -541,12 +550,16 @@ class Mamba3(nn.Module):
         weights themselves stay as they are, so that decoding continues such a prefill with projections that are
         not rounded to 8 bits. Weights of any floating type; memory grows by a byte for each of the projections'
         values. A weight that is replaced or modified afterwards (``load_state_dict``, ``to``,
-        ``quantize_decode``, a copy of the model) makes these calls raise until this is called again.
+        ``quantize_decode``, a copy of the model) makes these calls raise until this is called again. A
+        projection with a bias, with forward hooks or within another module (an adapter) is refused, here and by
+        these calls: its copy would pass them by.
         """
         for layer in self.layers:
             for name in ("in_proj", "out_proj"):
+                module = getattr(layer.mixer, name)
+                _require_plain("quantize_prefill", name, module)
                 try:
-                    getattr(layer.mixer, name).weight._version
+                    module.weight._version
                 except RuntimeError as error:
                     raise ValueError("quantize_prefill needs weights that count their changes, not "
                                      "ones made under torch.inference_mode()") from error
@@ -575,6 +588,19 @@ def _compute_dtype(x: torch.Tensor) -> torch.dtype:
     if torch.is_autocast_enabled(x.device.type):
         return torch.get_autocast_dtype(x.device.type)
     return x.dtype
+
+
+def _plain_linear(module: nn.Module) -> bool:
+    """Whether calling ``module`` is its weight's product and nothing else, so that a kernel or a copy of the
+    weight may stand in for it: ``nn.Linear``'s own forward, without a bias or forward hooks."""
+    return (type(module).forward is nn.Linear.forward and "forward" not in module.__dict__
+            and module.bias is None and not module._forward_hooks and not module._forward_pre_hooks)
+
+
+def _require_plain(maker: str, name: str, module: nn.Module) -> None:
+    if not _plain_linear(module):
+        raise ValueError(f"{maker} needs {name} to be a plain nn.Linear, without a bias, hooks or a module "
+                         "around it")
 
 
 def _storage_signature(w: torch.Tensor) -> tuple[object, ...]:

@@ -1,0 +1,128 @@
+"""``in_proj`` and ``out_proj`` that are more than their weight's product (a hook, a bias, a module around them):
+what stands in for them elsewhere, a kernel on the weight or a copy of it in fewer bits, passes none of that by."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from mamba3_amd import Mamba3, ops
+
+BF16 = torch.bfloat16
+
+
+class _Adapter(torch.nn.Module):
+    """A projection with something beside it, under the projection's own weight."""
+
+    def __init__(self, inner):
+        super().__init__()
+        self.inner = inner
+
+    @property
+    def weight(self):
+        return self.inner.weight
+
+    def forward(self, x):
+        return self.inner(x) + 1
+
+
+def _adapted(mixer, name):
+    setattr(mixer, name, _Adapter(getattr(mixer, name)))
+
+
+def _biased(mixer, name):
+    weight = getattr(mixer, name).weight
+    setattr(mixer, name, torch.nn.Linear(weight.shape[1], weight.shape[0]))
+
+
+def _hooked(mixer, name):
+    getattr(mixer, name).register_forward_hook(lambda module, args, out: out + 1)
+
+
+def _hooked_before(mixer, name):
+    getattr(mixer, name).register_forward_pre_hook(lambda module, args: (args[0] + 1,))
+
+
+def _patched(mixer, name):
+    module = getattr(mixer, name)
+    module.forward = lambda x: torch.nn.Linear.forward(module, x) + 1
+
+
+CHANGES = [_adapted, _biased, _hooked, _hooked_before, _patched]
+
+
+@pytest.mark.parametrize("change", CHANGES)
+@pytest.mark.parametrize("name", ["in_proj", "out_proj"])
+def test_quantize_prefill_passes_nothing_by(name, change):
+    """A projection that is more than its weight's product is not replaced by its copy: neither one that is so
+    when the copies are made, nor one that becomes so afterwards."""
+    model = Mamba3(64, depth=2)
+    change(model.layers[1].mixer, name)
+    with pytest.raises(ValueError, match=f"{name} to be a plain nn.Linear"):
+        model.quantize_prefill()
+    assert not any(layer.mixer._prefill8 for layer in model.layers)
+    model = Mamba3(64, depth=2).quantize_prefill()
+    change(model.layers[0].mixer, name)
+    with pytest.raises(RuntimeError, match=f"{name}.* changed since quantize_prefill"):
+        model.layers[0].mixer._weight8(name)
+    if name == "in_proj":
+        with pytest.raises(RuntimeError, match="changed since quantize_prefill"), torch.no_grad():
+            model(torch.zeros(1, 2, 64))
+
+
+def test_quantize_prefill_takes_linears_of_another_name():
+    class Own(torch.nn.Linear):
+        pass
+
+    model = Mamba3(64, depth=1)
+    mixer = model.layers[0].mixer
+    mixer.out_proj = Own(128, 64, bias=False)
+    assert model.quantize_prefill() is model and mixer._weight8("out_proj") is not None
+
+
+@pytest.mark.parametrize("change", CHANGES)
+@pytest.mark.parametrize("name", ["in_proj", "out_proj"])
+def test_quantize_decode_passes_nothing_by(name, change):
+    model = Mamba3(64, depth=2).to(BF16)
+    change(model.layers[1].mixer, name)
+    model.to(BF16)
+    before = {k: v.clone() for k, v in model.state_dict().items()}
+    with pytest.raises(ValueError, match=f"{name} to be a plain nn.Linear"):
+        model.quantize_decode(32)
+    assert not any(layer.mixer._decode4 for layer in model.layers)
+    assert all(torch.equal(v, before[k]) for k, v in model.state_dict().items())
+    model = Mamba3(64, depth=2).to(BF16).quantize_decode(32)
+    change(model.layers[0].mixer, name)
+    with pytest.raises(RuntimeError, match=f"{name}.* changed since quantize_decode"):
+        model.layers[0].mixer._weight4(name)
+
+
+@pytest.mark.parametrize("change", [None, *CHANGES])
+@pytest.mark.parametrize("name", ["in_proj", "out_proj"])
+def test_a_step_passes_nothing_by(monkeypatch, name, change):
+    """With a decode kernel that takes all rows, in torch here, a step's projection is what calling it gives."""
+    model = Mamba3(64, depth=1)
+    mixer = model.layers[0].mixer
+    taken = []
+
+    def linear(x, weight, residual=None, **norm):
+        taken.append(weight)
+        y = torch.nn.functional.linear(x, weight)
+        return y if residual is None else residual + y
+
+    def step_projection(proj, mixer, cache, inplace):
+        return proj[:, 0, :mixer.d_inner].unflatten(-1, (mixer.nheads, mixer.headdim)), cache
+
+    monkeypatch.setattr(ops, "linear_supported", lambda x, weight: True)
+    monkeypatch.setattr(ops, "linear", linear)
+    monkeypatch.setattr(ops, "step_projection", step_projection)
+    if change is not None:
+        change(mixer, name)
+    x = torch.randn(3, 1, 64)
+    with torch.no_grad():
+        got, _ = mixer.step(x, None, residual=x)
+        mixed = step_projection(mixer.in_proj(x), mixer, None, False)[0].flatten(-2)
+        want = x + mixer.out_proj(mixed).unsqueeze(1)
+    # (the same products in other orders: a row of in_proj adds 64, one of out_proj 128 of them)
+    assert torch.allclose(got, want, rtol=0, atol=256 * 2.0 ** -24 * (want.abs().max().item() + 128))
+    assert len(taken) == (2 if change is None else 1)
