@@ -614,6 +614,14 @@ def _same_storage(now: tuple[object, ...], then: tuple[object, ...]) -> bool:
     return now[0] is then[0] and now[1:] == then[1:]
 
 
+def _layers_in8(model: Mamba3, rows: int) -> list[bool] | None:
+    """Which layers' steps of so many rows run in 8 bits; ``None`` where none do whatever copies there are. (Copies
+    of unchanged weights are equal, so which copies they are does not matter.)"""
+    if rows <= ops.DECODE_LINEAR_ROWS:
+        return None
+    return [bool(layer.mixer._prefill8) for layer in model.layers]
+
+
 class _HipGraphDecoder:
     """A decode step of the whole stack, captured once in a hipGraph and replayed.
 
@@ -622,8 +630,11 @@ class _HipGraphDecoder:
     input copy plus one graph launch. Decoding starts from zeros (``reset``) or from a
     prefill's cache (``load_cache``). The graph holds the addresses of the parameters it was
     captured with; ``validate`` refuses a model whose parameters were replaced or modified
-    since. Interface of the reference's ``cuda_graph`` decoder (``model.py:691-774``).
+    since, and one put in 8 bits since (``Mamba3.quantize_prefill``) whose steps of so many rows run so.
+    Interface of the reference's ``cuda_graph`` decoder (``model.py:691-774``).
     """
+
+    _in8: list[bool] | None = None  # the layers captured in 8 bits; None: so few rows never are
 
     def __init__(self, model: Mamba3, batch_size: int) -> None:
         if batch_size <= 0:
@@ -639,6 +650,7 @@ class _HipGraphDecoder:
         # storage it read (address, device, dtype, shape): `Module.to`, `.half()` or
         # `p.data = ...` keep the object and its version but move the storage
         self._captured = [_storage_signature(w) for w in weights]
+        self._in8 = _layers_in8(model, batch_size)
         # the 4-bit and 8-bit copies that the graph reads live as long as it does
         self._copies = [(dict(layer.mixer._decode4), dict(layer.mixer._prefill8))
                         for layer in model.layers]
@@ -683,7 +695,8 @@ class _HipGraphDecoder:
         current = [_storage_signature(w) for w in self.model.parameters()]
         same = len(current) == len(self._captured) and all(
             _same_storage(now, then) for now, then in zip(current, self._captured))
-        if not same:
+        if not same or (self._in8 is not None
+                        and self._in8 != _layers_in8(self.model, ops.DECODE_LINEAR_ROWS + 1)):
             raise RuntimeError("model state changed; recreate the CUDA graph decoder")
 
     def reset(self) -> None:

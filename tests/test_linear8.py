@@ -344,3 +344,26 @@ def test_quantize_prefill_holds_every_layer_or_none():
         unversioned = Mamba3(64, depth=1)
         with pytest.raises(ValueError, match="inference_mode"):
             unversioned.quantize_prefill()
+
+
+def test_a_graph_decoder_sees_copies_made_after_it():
+    """A graph of more rows than the decode kernels' runs on the projections that it was captured with: one from
+    before ``quantize_prefill`` is not the model's step any more. (Checked on a decoder without its capture.)"""
+    from mamba3_amd.model import _HipGraphDecoder, _layers_in8, _storage_signature
+
+    def decoder_for(model, rows):
+        dec = object.__new__(_HipGraphDecoder)
+        dec.model, dec._in8 = model, _layers_in8(model, rows)
+        dec._captured = [_storage_signature(w) for w in model.parameters()]
+        return dec
+
+    model = Mamba3(16, d_state=8, depth=2)
+    few, many = decoder_for(model, ops.DECODE_LINEAR_ROWS), decoder_for(model, ops.DECODE_LINEAR_ROWS + 1)
+    few.validate(), many.validate()
+    model.quantize_prefill()
+    few.validate()
+    with pytest.raises(RuntimeError, match="recreate"):
+        many.validate()
+    many = decoder_for(model, 200)
+    model.quantize_prefill()  # of the same weights: the same copies
+    many.validate(), few.validate()
