@@ -155,11 +155,20 @@ class _Mamba3Mixer(nn.Module):
     def _weight8(self, name: str) -> ops.Weight8 | None:
         return self._held(self._prefill8, name, "quantize_prefill")
 
-    def _project(self, name: str, x: torch.Tensor | ops.Rows8,
+    def _step_copies(self, rows: int) -> dict[str, object]:
+        """The projections' copies that a step of so many rows may run on: in 4 bits, and of more rows than the
+        decode kernels' in 8. Asked before any cache moves, since a changed weight is refused."""
+        copies: dict[str, object] = {}
+        if self._decode4:
+            copies.update(in4=self._weight4("in_proj"), out4=self._weight4("out_proj"))
+        if self._prefill8 and rows > min(ops.DECODE_LINEAR_ROWS, ops.DECODE_LINEAR_OUT_ROWS):
+            copies.update(in8=self._weight8("in_proj"), out8=self._weight8("out_proj"))
+        return copies
+
+    def _project(self, name: str, x: torch.Tensor | ops.Rows8, weight: ops.Weight8 | None,
                  dtype: torch.dtype | None = None) -> torch.Tensor:
-        """``in_proj`` or ``out_proj`` of ``x``, in 8 bits if there is such a copy. Rows already in
+        """``in_proj`` or ``out_proj`` of ``x``, in 8 bits if ``weight`` is such a copy of it. Rows already in
         8 bits (from ``ops.rms_norm8``) give ``dtype``; others what the projection itself gives."""
-        weight = self._weight8(name)
         if isinstance(x, ops.Rows8):
             return ops.linear8(x, weight, dtype=dtype)
         module = getattr(self, name)
@@ -190,7 +199,7 @@ class _Mamba3Mixer(nn.Module):
             raise ValueError("bidirectional Mamba3 does not support caches; "
                              "prefill and step require causal=True")
         self._check_inference(*(() if isinstance(hidden_states, ops.Rows8) else (hidden_states,)))
-        proj = self._project("in_proj", hidden_states, dtype)
+        proj = self._project("in_proj", hidden_states, self._weight8("in_proj"), dtype)
         if not self.causal:
             # the reverse scan on a side stream, concurrent with the forward one: each direction
             # alone may leave CUs idle in its last round of workgroups
@@ -204,7 +213,8 @@ class _Mamba3Mixer(nn.Module):
         mixed, state, final_phase, final_k = ops.scan_projection(
             proj, self, cache=cache, want_cache=return_cache and self.causal,
             chunk_size=self._chunk(), concurrent=1 if self.causal else 2)
-        output = self._project("out_proj", mixed.flatten(-2))
+        out8 = self._weight8("out_proj")
+        output = self._project("out_proj", mixed.flatten(-2), out8)
         if self.causal:
             if not return_cache:
                 return output
@@ -217,7 +227,7 @@ class _Mamba3Mixer(nn.Module):
         # order (no flip, no second projection).
         main.wait_stream(side)
         mixed_r.record_stream(main)
-        backward = self._project("out_proj", mixed_r.flatten(-2))
+        backward = self._project("out_proj", mixed_r.flatten(-2), out8)
         blend = torch.sigmoid(self.direction_logit).to(dtype=output.dtype)
         return output * blend + backward * (1.0 - blend)
 
@@ -255,26 +265,32 @@ class _Mamba3Mixer(nn.Module):
 
     def step(self, hidden_states: torch.Tensor, cache: _LayerCache | None, *,
              inplace: bool = False, residual: torch.Tensor | None = None,
-             norm: _RMSNorm | None = None, dtype: torch.dtype | None = None):
+             norm: _RMSNorm | None = None, dtype: torch.dtype | None = None,
+             copies: dict[str, object] | None = None):
         """One decode token. ``norm`` (the block's RMSNorm) is applied to ``hidden_states``
         first; with ``residual`` (``[batch, 1, d_model]``) the result is
         ``residual + out_proj(...)``. With 16-bit weights, ``in_proj`` runs on ``ops.linear``
         with the norm fused up to ``ops.DECODE_LINEAR_ROWS`` rows, and ``out_proj`` with the
         residual add fused up to ``ops.DECODE_LINEAR_OUT_ROWS``; a projection with a bias, hooks or a
         module around it is called as it is. Rows in 8 bits are normed already, and ``dtype`` is what
-        ``in_proj`` gives of them."""
+        ``in_proj`` gives of them. ``copies``: ``_step_copies``, where they have been asked."""
         if len(hidden_states.shape) != 3 or hidden_states.shape[1:] != (1, self.d_model):
             raise ValueError(
                 f"expected [batch, 1, {self.d_model}], got {tuple(hidden_states.shape)}")
         if isinstance(hidden_states, ops.Rows8):
             self._check_inference()
-            return self._step_from(self._project("in_proj", hidden_states, dtype), cache, inplace,
-                                   residual)
-        self._check_inference(hidden_states)
+        else:
+            self._check_inference(hidden_states)
+        if copies is None:
+            copies = self._step_copies(hidden_states.shape[0])
+        if isinstance(hidden_states, ops.Rows8):
+            in8 = copies["in8"] if "in8" in copies else self._weight8("in_proj")
+            proj = self._project("in_proj", hidden_states, in8, dtype)
+            return self._step_from(proj, cache, inplace, residual, copies)
         rows = hidden_states[:, 0]
         small = rows.shape[0] <= ops.DECODE_LINEAR_ROWS
         supported = ops.linear_norm_supported if norm is not None else ops.linear_supported
-        in_proj, in4 = self.in_proj, self._weight4("in_proj")
+        in_proj, in4 = self.in_proj, copies.get("in4")
         if (small and in4 is not None and rows.dtype == in_proj.weight.dtype
                 and ops.linear4_supported(rows, in4)):
             proj = ops.linear4(rows, in4, norm_weight=norm.weight if norm is not None else None,
@@ -288,13 +304,13 @@ class _Mamba3Mixer(nn.Module):
         else:
             normed = norm(hidden_states) if norm is not None else hidden_states
             # few rows keep to the weights that their neighbours' kernels read
-            proj = in_proj(normed) if small else self._project("in_proj", normed)
-        return self._step_from(proj, cache, inplace, residual)
+            proj = in_proj(normed) if small else self._project("in_proj", normed, copies.get("in8"))
+        return self._step_from(proj, cache, inplace, residual, copies)
 
     def _step_from(self, proj: torch.Tensor, cache: _LayerCache | None, inplace: bool,
-                   residual: torch.Tensor | None):
+                   residual: torch.Tensor | None, copies: dict[str, object]):
         """The rest of a step, from ``in_proj``'s output."""
-        batch, out_proj, out4 = proj.shape[0], self.out_proj, self._weight4("out_proj")
+        batch, out_proj, out4 = proj.shape[0], self.out_proj, copies.get("out4")
         if cache is None:
             cache = self.allocate_cache(batch, device=proj.device, dtype=proj.dtype)
         else:
@@ -311,7 +327,8 @@ class _Mamba3Mixer(nn.Module):
                 and (residual is None or residual.dtype == mixed.dtype)):
             res = residual[:, 0] if residual is not None else None
             return ops.linear(mixed, out_proj.weight, res).unsqueeze(1), next_cache
-        output = (out_proj(mixed) if small else self._project("out_proj", mixed)).unsqueeze(1)
+        output = (out_proj(mixed) if small
+                  else self._project("out_proj", mixed, copies.get("out8"))).unsqueeze(1)
         if residual is not None:
             output = residual + output
         return output, next_cache
@@ -330,9 +347,9 @@ class _Mamba3Block(nn.Module):
             return hidden_states + output, next_cache
         return hidden_states + mixed
 
-    def step(self, hidden_states, cache, *, inplace: bool = False):
+    def step(self, hidden_states, cache, *, inplace: bool = False, copies=None):
         return self.mixer.step(hidden_states, cache, inplace=inplace, residual=hidden_states,
-                               norm=self.norm)
+                               norm=self.norm, copies=copies)
 
 
 class Mamba3(nn.Module):
@@ -394,10 +411,11 @@ class Mamba3(nn.Module):
         s = h if mixed is None else h + mixed
         return norm(s), s
 
-    def _next_rows(self, h: torch.Tensor, mixed: torch.Tensor | None, layer: _Mamba3Block):
+    def _next_rows(self, h: torch.Tensor, mixed: torch.Tensor | None, layer: _Mamba3Block,
+                   in8: ops.Weight8 | None):
         """``(the next mixer's rows, the dtype its in_proj gives, h + mixed)``: normed rows, in 8 bits
         where the mixer has a copy of its in_proj in them."""
-        if (layer.mixer._weight8("in_proj") is None
+        if (in8 is None
                 or _compute_dtype(h) != layer.mixer.in_proj.weight.dtype
                 and not torch.is_autocast_enabled(h.device.type)):
             normed, h = self._add_norm(h, mixed, layer.norm, self._norm_dtype(h), keep_sum=True)
@@ -413,7 +431,7 @@ class Mamba3(nn.Module):
         residual add runs fused with the RMSNorm after it (the next block's, or norm_f)."""
         h, mixed, cache = x, None, []
         for layer in self.layers:
-            rows, dtype, h = self._next_rows(h, mixed, layer)
+            rows, dtype, h = self._next_rows(h, mixed, layer, layer.mixer._weight8("in_proj"))
             if return_cache:
                 mixed, layer_cache = layer.mixer(rows, return_cache=True, dtype=dtype)
                 cache.append(layer_cache)
@@ -455,11 +473,13 @@ class Mamba3(nn.Module):
         if cache is not None and len(cache) != depth:
             raise ValueError(f"expected cache for {depth} layers")
         updated: list[_LayerCache] = []
+        # every layer's before the first one's cache moves
+        copies = [layer.mixer._step_copies(x.shape[0]) for layer in self.layers]
         if x.shape[0] <= ops.DECODE_LINEAR_ROWS:
             # few rows: each block's RMSNorm and residual add run inside its two projections
             for i, layer in enumerate(self.layers):
                 layer_cache = None if cache is None else cache[i]
-                x, layer_cache = layer.step(x, layer_cache,
+                x, layer_cache = layer.step(x, layer_cache, copies=copies[i],
                                             inplace=inplace and layer_cache is not None)
                 updated.append(layer_cache)
             return self.norm_f(x), updated
@@ -468,8 +488,8 @@ class Mamba3(nn.Module):
         h, mixed = x, None
         for i, layer in enumerate(self.layers):
             layer_cache = None if cache is None else cache[i]
-            rows, dtype, h = self._next_rows(h, mixed, layer)
-            mixed, layer_cache = layer.mixer.step(rows, layer_cache, dtype=dtype,
+            rows, dtype, h = self._next_rows(h, mixed, layer, copies[i].get("in8"))
+            mixed, layer_cache = layer.mixer.step(rows, layer_cache, dtype=dtype, copies=copies[i],
                                                   inplace=inplace and layer_cache is not None)
             updated.append(layer_cache)
         out, _ = self._add_norm(h, mixed, self.norm_f, torch.promote_types(h.dtype, mixed.dtype),

@@ -126,3 +126,62 @@ def test_a_step_passes_nothing_by(monkeypatch, name, change):
     # (the same products in other orders: a row of in_proj adds 64, one of out_proj 128 of them)
     assert torch.allclose(got, want, rtol=0, atol=256 * 2.0 ** -24 * (want.abs().max().item() + 128))
     assert len(taken) == (2 if change is None else 1)
+
+
+def _stubs(monkeypatch):
+    """The kernels of a step in torch, enough of them for a step off the GPU: the caches count their steps."""
+
+    def step_projection(proj, mixer, cache, inplace):
+        assert inplace
+        for t in cache:
+            t += 1
+        return torch.zeros(proj.shape[0], mixer.nheads, mixer.headdim, dtype=proj.dtype), cache
+
+    def rms_norm8(x, weight, eps, *, add=None, keep_sum=False):
+        return ops.Rows8(torch.zeros(x.shape, dtype=torch.int8), torch.ones(x.shape[:-1])), x if keep_sum else None
+
+    def linear8(rows, weight, residual=None, *, out=None, dtype=None):
+        return torch.zeros(*rows.shape[:-1], weight.shape[0], dtype=dtype)
+
+    monkeypatch.setattr(ops, "step_projection", step_projection)
+    monkeypatch.setattr(ops, "rms_norm8", rms_norm8)
+    monkeypatch.setattr(ops, "linear8", linear8)
+    monkeypatch.setattr(ops, "quantize8_rows", lambda x: rms_norm8(x, None, 0.0)[0])
+
+
+@pytest.mark.parametrize("layer", [0, 1])
+@pytest.mark.parametrize("name", ["in_proj", "out_proj"])
+@pytest.mark.parametrize("maker,rows", [("quantize_prefill", 65), ("quantize_decode", 65), ("quantize_decode", 2)])
+def test_a_refused_step_moves_no_cache(monkeypatch, maker, rows, name, layer):
+    """A stale copy anywhere is refused before the first layer's cache is updated in place."""
+    _stubs(monkeypatch)
+    model = Mamba3(64, depth=2).to(BF16)
+    x = torch.zeros(rows, 1, 64, dtype=BF16)
+    cache = [block.mixer.allocate_cache(rows, device=x.device, dtype=BF16) for block in model.layers]
+    copies = (lambda: model.quantize_decode(32)) if maker == "quantize_decode" else model.quantize_prefill
+    copies()
+    with torch.no_grad():
+        model.step(x, cache, inplace=True)
+        assert all((t == 1).all() for states in cache for t in states)
+        getattr(model.layers[layer].mixer, name).weight.mul_(2)
+        with pytest.raises(RuntimeError, match=f"{name}.weight changed since {maker}"):
+            model.step(x, cache, inplace=True)
+        assert all((t == 1).all() for states in cache for t in states)
+        mixer, states = model.layers[layer].mixer, cache[layer]
+        with pytest.raises(RuntimeError, match=f"{name}.weight changed since {maker}"):
+            mixer.step(x, states, inplace=True)
+        assert all((t == 1).all() for t in states)
+        copies()
+        model.step(x, cache, inplace=True)
+        assert all((t == 2).all() for states in cache for t in states)
+
+
+def test_few_rows_do_not_ask_for_8_bits(monkeypatch):
+    """Steps of up to 64 rows run on the weights as they are, also on changed ones."""
+    _stubs(monkeypatch)
+    model = Mamba3(64, depth=2).to(BF16).quantize_prefill()
+    with torch.no_grad():
+        model.layers[1].mixer.out_proj.weight.mul_(2)
+        cache = [block.mixer.allocate_cache(64, device=torch.device("cpu"), dtype=BF16) for block in model.layers]
+        model.step(torch.zeros(64, 1, 64, dtype=BF16), cache, inplace=True)
+    assert all((t == 1).all() for states in cache for t in states)
