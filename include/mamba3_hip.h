@@ -434,7 +434,7 @@ typedef struct {
   const float* scales;  /* 16-byte aligned */
   m3_tensor residual;   /* [M, N] optional */
   m3_tensor out;        /* [M, N]; may equal residual, overlaps nothing else */
-  void* workspace;      /* 16-byte aligned */
+  void* workspace;      /* 16-byte aligned; overlaps nothing else */
   size_t workspace_bytes;
 } m3_linear8_args;
 

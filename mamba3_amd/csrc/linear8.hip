@@ -677,19 +677,30 @@ int validate(const m3_linear8_args& a) {
   const int64_t tiles = (a.n + 63) / 64, es = elem_size(a.dtype);
   const char* o0 = static_cast<const char*>(a.out.ptr);
   const char* o1 = o0 + ((a.m - 1) * a.out.stride[0] + a.n) * es;
-  const auto meets = [&](const void* p, int64_t bytes) {
+  const auto meets = [](const void* p, int64_t bytes, const char* from, const char* to) {
     const char* p0 = static_cast<const char*>(p);
-    return p0 < o1 && o0 < p0 + bytes;
+    return p0 < to && from < p0 + bytes;
   };
-  if (meets(a.codes, (a.m - 1) * a.codes_stride + a.k) || meets(a.row_scales, a.m * 4) ||
-      meets(a.q, tiles * ((a.k + 127) / 128) * 2 * kTileBytes) || meets(a.scales, tiles * 256)) {
+  const int64_t codes = (a.m - 1) * a.codes_stride + a.k, q = tiles * ((a.k + 127) / 128) * 2 * kTileBytes;
+  const int64_t residual = ((a.m - 1) * a.residual.stride[0] + a.n) * es;
+  if (meets(a.codes, codes, o0, o1) || meets(a.row_scales, a.m * 4, o0, o1) || meets(a.q, q, o0, o1) ||
+      meets(a.scales, tiles * 256, o0, o1)) {
     return fail(M3_EINVAL, "m3_linear8: out overlaps codes, the weight or scales");
   }
-  if (a.workspace != nullptr && meets(a.workspace, static_cast<int64_t>(need(a)))) {
-    return fail(M3_EINVAL, "m3_linear8: out overlaps the workspace");
+  if (const size_t bytes = need(a); a.workspace != nullptr && bytes != 0) {
+    const char* const w0 = static_cast<const char*>(a.workspace);
+    const char* const w1 = w0 + bytes;
+    const char* const what = meets(a.codes, codes, w0, w1)                            ? "codes"
+                             : meets(o0, o1 - o0, w0, w1)                             ? "out"
+                             : meets(a.q, q, w0, w1)                                  ? "the weight"
+                             : present(a.residual) && meets(a.residual.ptr, residual, w0, w1) ? "residual"
+                             : meets(a.row_scales, a.m * 4, w0, w1) || meets(a.scales, tiles * 256, w0, w1)
+                                 ? "scales"
+                                 : nullptr;
+    if (what != nullptr) return fail(M3_EINVAL, "m3_linear8: %s overlaps the workspace", what);
   }
   const bool same = a.residual.ptr == a.out.ptr && (a.m == 1 || a.residual.stride[0] == a.out.stride[0]);
-  if (present(a.residual) && !same && meets(a.residual.ptr, ((a.m - 1) * a.residual.stride[0] + a.n) * es)) {
+  if (present(a.residual) && !same && meets(a.residual.ptr, residual, o0, o1)) {
     return fail(M3_EINVAL, "m3_linear8: out overlaps the residual without being it");
   }
   return M3_OK;

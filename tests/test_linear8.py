@@ -367,3 +367,32 @@ def test_a_graph_decoder_sees_copies_made_after_it():
     many = decoder_for(model, 200)
     model.quantize_prefill()  # of the same weights: the same copies
     many.validate(), few.validate()
+
+
+def test_linear8_s_workspace_overlaps_nothing(lib):
+    """The copy of the codes would be written over what the call reads."""
+    m, n, k = 5000, 64 * 20, 250
+    size = m * 256
+
+    def block(workspace):
+        args = _args(m, n, k)
+        args.codes, args.out.ptr, args.q, args.residual = 1 << 40, 1 << 41, 1 << 42, _hip.Tensor(1 << 44, _hip.BF16, 0, (n, 1))
+        args.row_scales, args.scales = 1 << 45, 1 << 46
+        args.workspace, args.workspace_bytes = workspace, size
+        return args
+
+    need = ctypes.c_size_t(0)
+    for at, bytes_, text in ((1 << 40, (m - 1) * k + k, b"codes"), (1 << 41, m * n * 2, b"out"),
+                             (1 << 42, 20 * 4 * 4096, b"the weight"), (1 << 44, m * n * 2, b"residual"),
+                             (1 << 45, m * 4, b"scales"), (1 << 46, n * 4, b"scales")):
+        for workspace in (at, at - size + 16, (at + bytes_ - 1) // 16 * 16):
+            args = block(workspace)
+            assert lib.m3_linear8_workspace_size(ctypes.byref(args), ctypes.byref(need)) == 1, hex(workspace)
+            assert b"overlaps the workspace" in lib.m3_last_error() and text in lib.m3_last_error()
+        for workspace in (at - size, (at + bytes_ + 15) // 16 * 16):
+            args = block(workspace)
+            assert lib.m3_linear8_workspace_size(ctypes.byref(args), ctypes.byref(need)) == 0, hex(workspace)
+            assert need.value == size
+    args = block(1 << 40)  # not used, and so not looked at, where nothing is copied
+    args.codes_stride = 256
+    assert lib.m3_linear8_workspace_size(ctypes.byref(args), ctypes.byref(need)) == 0 and need.value == 0
