@@ -418,15 +418,17 @@ int m3_rows8_values(const m3_rows8_values_args* args, hipStream_t stream);
  *   q [ceil(N / 64), TK, 4, 64, 16] bytes: byte e of lane l of quarter j holds column 16 (l / 16) + e of
  *     its tile, row 32 (j / 2) + 8 (l % 16 / 4) + 4 (j % 2) + l % 4
  *   scale [64 ceil(N / 64)] FP32, 0 past N
- * What lies in codes between K and the row's stride has no effect. Rows of codes that are not 16-byte aligned, or
- * (exact) end where their memory does, are read with care by the kernels for few rows and copied into the workspace for the
- * others (m3_linear8_workspace_size, 0 where nothing is copied).
+ * What lies in codes between K and the row's stride may be read and has no effect: from the first row's to the
+ * last row's K-th they are one piece of readable memory. Rows of codes that are not 16-byte aligned, or (exact)
+ * end where their memory does, are read with care by the kernels for few rows and copied into the workspace for
+ * the others (m3_linear8_workspace_size, 0 where nothing is copied).
  */
 typedef struct {
   int64_t m, n, k;
   int32_t dtype;        /* of out and residual */
-  int32_t exact;        /* not 0: nothing past a row's K codes may be read; 0: rows that are 16-byte aligned
-                           are readable to the next multiple of 16 */
+  int32_t exact;        /* not 0: nothing past the last row's K codes is read; 0: where rows are 16-byte
+                           aligned, that row is readable to the next multiple of 16. What lies between rows may be
+                           read either way */
   const int8_t* codes;  /* [M, codes_stride] */
   int64_t codes_stride; /* bytes, at least K */
   const float* row_scales; /* [M] */
