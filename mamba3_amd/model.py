@@ -67,6 +67,12 @@ class _RMSNorm(nn.Module):
 class _Mamba3Mixer(nn.Module):
     """One Mamba-3 SISO / MIMO mixer; the scan and the step run in the HIP library."""
 
+    # copies of the projections by name, each with what its weight was then: in 4 bits for decode steps
+    # (quantize_decode) and in 8 bits for the other calls (quantize_prefill). Replaced, never changed in place; of
+    # the class, so that a mixer pickled before there were any has none
+    _decode4: dict[str, tuple[ops.Weight4, tuple[object, ...]]] = {}
+    _prefill8: dict[str, tuple[ops.Weight8, tuple[object, ...]]] = {}
+
     def __init__(self, d_model: int, d_state: int, mimo_rank: int, causal: bool = True) -> None:
         super().__init__()
         self.d_model = d_model
@@ -121,10 +127,7 @@ class _Mamba3Mixer(nn.Module):
             self.register_parameter("direction_logit", None)
         else:
             self.direction_logit = nn.Parameter(torch.zeros(d_model))
-        # 4-bit copies of the projections for decode steps, by name (quantize_decode)
-        self._decode4: dict[str, tuple[ops.Weight4, tuple[object, ...]]] = {}
-        # 8-bit copies for the other calls (quantize_prefill)
-        self._prefill8: dict[str, tuple[ops.Weight8, tuple[object, ...]]] = {}
+        self._decode4, self._prefill8 = {}, {}
 
     def _signed(self, held: dict[str, object]) -> dict[str, tuple]:
         """Copies of the projections by name, each with what its weight is now."""

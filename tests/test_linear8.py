@@ -396,3 +396,21 @@ def test_linear8_s_workspace_overlaps_nothing(lib):
     args = block(1 << 40)  # not used, and so not looked at, where nothing is copied
     args.codes_stride = 256
     assert lib.m3_linear8_workspace_size(ctypes.byref(args), ctypes.byref(need)) == 0 and need.value == 0
+
+
+def test_models_pickled_before_there_were_copies():
+    """A mixer whose state lacks the dicts of copies is one without any."""
+    mixer = Mamba3(64, depth=1).layers[0].mixer
+    for name in ("_decode4", "_prefill8"):
+        del mixer.__dict__[name]
+    twin = copy.deepcopy(mixer)
+    model = Mamba3(64, depth=1)
+    model.layers[0].mixer = twin
+    assert twin._weight8("in_proj") is None and twin._weight4("out_proj") is None
+    with pytest.raises(RuntimeError, match="ROCm devices only"), torch.no_grad():
+        model(torch.zeros(1, 2, 64))
+    with pytest.raises(RuntimeError, match="ROCm devices only"), torch.no_grad():
+        model.step(torch.zeros(70, 1, 64))
+    model.quantize_prefill()
+    assert twin._weight8("in_proj") is not None
+    assert mixer._weight8("in_proj") is None and Mamba3(64, depth=1).layers[0].mixer._prefill8 == {}
