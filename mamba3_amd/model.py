@@ -350,9 +350,9 @@ class _Mamba3Block(nn.Module):
             return hidden_states + output, next_cache
         return hidden_states + mixed
 
-    def step(self, hidden_states, cache, *, inplace: bool = False, copies=None):
+    def step(self, hidden_states, cache, *, inplace: bool = False, **copies):
         return self.mixer.step(hidden_states, cache, inplace=inplace, residual=hidden_states,
-                               norm=self.norm, copies=copies)
+                               norm=self.norm, **copies)
 
 
 class Mamba3(nn.Module):
@@ -416,30 +416,32 @@ class Mamba3(nn.Module):
 
     def _next_rows(self, h: torch.Tensor, mixed: torch.Tensor | None, layer: _Mamba3Block,
                    in8: ops.Weight8 | None):
-        """``(the next mixer's rows, the dtype its in_proj gives, h + mixed)``: normed rows, in 8 bits
-        where the mixer has a copy of its in_proj in them."""
+        """``(the next mixer's rows, its other arguments, h + mixed)``: normed rows, in 8 bits where the mixer
+        has a copy of its in_proj in them, with the dtype that in_proj gives."""
         if (in8 is None
                 or _compute_dtype(h) != layer.mixer.in_proj.weight.dtype
                 and not torch.is_autocast_enabled(h.device.type)):
             normed, h = self._add_norm(h, mixed, layer.norm, self._norm_dtype(h), keep_sum=True)
-            return normed, None, h
+            return normed, {}, h
         if mixed is not None and torch.promote_types(h.dtype, mixed.dtype) != h.dtype:
             h, mixed = h + mixed, None
         rows, s = ops.rms_norm8(h, layer.norm.weight, layer.norm.eps, add=mixed,
                                 keep_sum=mixed is not None)
-        return rows, _compute_dtype(h), h if mixed is None else s
+        return rows, {"dtype": _compute_dtype(h)}, h if mixed is None else s
 
     def _run_layers(self, x: torch.Tensor, *, return_cache: bool):
         """The layer loop of forward / prefill (reference ``model.py:585-607``): each block's
         residual add runs fused with the RMSNorm after it (the next block's, or norm_f)."""
         h, mixed, cache = x, None, []
         for layer in self.layers:
-            rows, dtype, h = self._next_rows(h, mixed, layer, layer.mixer._weight8("in_proj"))
+            mixer = layer.mixer
+            in8 = mixer._weight8("in_proj") if isinstance(mixer, _Mamba3Mixer) else None
+            rows, more, h = self._next_rows(h, mixed, layer, in8)
             if return_cache:
-                mixed, layer_cache = layer.mixer(rows, return_cache=True, dtype=dtype)
+                mixed, layer_cache = mixer(rows, return_cache=True, **more)
                 cache.append(layer_cache)
             else:
-                mixed = layer.mixer(rows, dtype=dtype)
+                mixed = mixer(rows, **more)
         out, _ = self._add_norm(h, mixed, self.norm_f, h.dtype if mixed is None else
                                 torch.promote_types(h.dtype, mixed.dtype), keep_sum=False)
         return out, cache
@@ -477,12 +479,14 @@ class Mamba3(nn.Module):
             raise ValueError(f"expected cache for {depth} layers")
         updated: list[_LayerCache] = []
         # every layer's before the first one's cache moves
-        copies = [layer.mixer._step_copies(x.shape[0]) for layer in self.layers]
+        copies = [layer.mixer._step_copies(x.shape[0]) if isinstance(layer.mixer, _Mamba3Mixer) else {}
+                  for layer in self.layers]
         if x.shape[0] <= ops.DECODE_LINEAR_ROWS:
             # few rows: each block's RMSNorm and residual add run inside its two projections
             for i, layer in enumerate(self.layers):
                 layer_cache = None if cache is None else cache[i]
-                x, layer_cache = layer.step(x, layer_cache, copies=copies[i],
+                more = {"copies": copies[i]} if copies[i] else {}
+                x, layer_cache = layer.step(x, layer_cache, **more,
                                             inplace=inplace and layer_cache is not None)
                 updated.append(layer_cache)
             return self.norm_f(x), updated
@@ -491,8 +495,10 @@ class Mamba3(nn.Module):
         h, mixed = x, None
         for i, layer in enumerate(self.layers):
             layer_cache = None if cache is None else cache[i]
-            rows, dtype, h = self._next_rows(h, mixed, layer, copies[i].get("in8"))
-            mixed, layer_cache = layer.mixer.step(rows, layer_cache, dtype=dtype, copies=copies[i],
+            rows, more, h = self._next_rows(h, mixed, layer, copies[i].get("in8"))
+            if copies[i]:
+                more["copies"] = copies[i]
+            mixed, layer_cache = layer.mixer.step(rows, layer_cache, **more,
                                                   inplace=inplace and layer_cache is not None)
             updated.append(layer_cache)
         out, _ = self._add_norm(h, mixed, self.norm_f, torch.promote_types(h.dtype, mixed.dtype),
@@ -642,7 +648,7 @@ def _layers_in8(model: Mamba3, rows: int) -> list[bool] | None:
     of unchanged weights are equal, so which copies they are does not matter.)"""
     if rows <= ops.DECODE_LINEAR_ROWS:
         return None
-    return [bool(layer.mixer._prefill8) for layer in model.layers]
+    return [bool(getattr(layer.mixer, "_prefill8", None)) for layer in model.layers]
 
 
 class _HipGraphDecoder:

@@ -185,3 +185,29 @@ def test_few_rows_do_not_ask_for_8_bits(monkeypatch):
         cache = [block.mixer.allocate_cache(64, device=torch.device("cpu"), dtype=BF16) for block in model.layers]
         model.step(torch.zeros(64, 1, 64, dtype=BF16), cache, inplace=True)
     assert all((t == 1).all() for states in cache for t in states)
+
+
+class _OwnMixer(torch.nn.Module):
+    """A mixer of someone's own in a layer's place: what it has to take is what it always had to."""
+
+    def forward(self, hidden_states, return_cache=False):
+        return (2 * hidden_states, None) if return_cache else 2 * hidden_states
+
+    def step(self, hidden_states, cache, *, inplace=False, residual=None, norm=None):
+        y = 2 * (hidden_states if norm is None else norm(hidden_states))
+        return y if residual is None else residual + y, cache
+
+
+@pytest.mark.parametrize("call", [lambda m, x: m(x), lambda m, x: m.prefill(x)[0], lambda m, x: m.step(x)[0],
+                                  lambda m, x: m.step(x[:2])[0]])
+def test_mixers_of_one_s_own(call):
+    model = Mamba3(64, depth=2)
+    for layer in model.layers:
+        layer.mixer = _OwnMixer()
+    x = torch.randn(70, 1, 64)
+    with torch.no_grad():
+        got = call(model, x)
+        h = x[:got.shape[0]]
+        for layer in model.layers:
+            h = h + 2 * layer.norm(h)
+        assert torch.equal(got, model.norm_f(h))
