@@ -144,7 +144,7 @@ class _Mamba3Mixer(nn.Module):
         if name not in copies:
             return None
         held, then = copies[name]
-        module = getattr(self, name)
+        module = self._modules[name]
         if not _same_storage(_storage_signature(module.weight), then):
             raise RuntimeError(f"{name}.weight changed since {maker}; call it again")
         if not _plain_linear(module):
@@ -163,9 +163,9 @@ class _Mamba3Mixer(nn.Module):
         decode kernels' in 8. Asked before any cache moves, since a changed weight is refused."""
         copies: dict[str, object] = {}
         if self._decode4:
-            copies.update(in4=self._weight4("in_proj"), out4=self._weight4("out_proj"))
+            copies["in4"], copies["out4"] = self._weight4("in_proj"), self._weight4("out_proj")
         if self._prefill8 and rows > min(ops.DECODE_LINEAR_ROWS, ops.DECODE_LINEAR_OUT_ROWS):
-            copies.update(in8=self._weight8("in_proj"), out8=self._weight8("out_proj"))
+            copies["in8"], copies["out8"] = self._weight8("in_proj"), self._weight8("out_proj")
         return copies
 
     def _project(self, name: str, x: torch.Tensor | ops.Rows8, weight: ops.Weight8 | None,
@@ -293,14 +293,15 @@ class _Mamba3Mixer(nn.Module):
         rows = hidden_states[:, 0]
         small = rows.shape[0] <= ops.DECODE_LINEAR_ROWS
         supported = ops.linear_norm_supported if norm is not None else ops.linear_supported
-        in_proj, in4 = self.in_proj, copies.get("in4")
-        if (small and in4 is not None and rows.dtype == in_proj.weight.dtype
+        in_proj, in4 = self._modules["in_proj"], copies.get("in4")  # (a sixth of an attribute's time)
+        weight = in_proj.weight if small and (in4 is not None or _plain_linear(in_proj)) else None
+        if (weight is not None and in4 is not None and rows.dtype == weight.dtype
                 and ops.linear4_supported(rows, in4)):
             proj = ops.linear4(rows, in4, norm_weight=norm.weight if norm is not None else None,
                                norm_eps=norm.eps if norm is not None else ops.NORM_EPS)
             proj = proj.unsqueeze(1)
-        elif small and _plain_linear(in_proj) and supported(rows, in_proj.weight):
-            proj = ops.linear(rows, in_proj.weight,
+        elif weight is not None and supported(rows, weight):
+            proj = ops.linear(rows, weight,
                               norm_weight=norm.weight if norm is not None else None,
                               norm_eps=norm.eps if norm is not None else ops.NORM_EPS)
             proj = proj.unsqueeze(1)
@@ -313,7 +314,7 @@ class _Mamba3Mixer(nn.Module):
     def _step_from(self, proj: torch.Tensor, cache: _LayerCache | None, inplace: bool,
                    residual: torch.Tensor | None, copies: dict[str, object]):
         """The rest of a step, from ``in_proj``'s output."""
-        batch, out_proj, out4 = proj.shape[0], self.out_proj, copies.get("out4")
+        batch, out4 = proj.shape[0], copies.get("out4")
         if cache is None:
             cache = self.allocate_cache(batch, device=proj.device, dtype=proj.dtype)
         else:
@@ -325,11 +326,12 @@ class _Mamba3Mixer(nn.Module):
                 and (residual is None or residual.dtype == mixed.dtype)):
             res = residual[:, 0] if residual is not None else None
             return ops.linear4(mixed, out4, res).unsqueeze(1), next_cache
-        small = batch <= ops.DECODE_LINEAR_OUT_ROWS
-        if (small and _plain_linear(out_proj) and ops.linear_supported(mixed, out_proj.weight)
+        small, out_proj = batch <= ops.DECODE_LINEAR_OUT_ROWS, self._modules["out_proj"]
+        weight = out_proj.weight if small and _plain_linear(out_proj) else None
+        if (weight is not None and ops.linear_supported(mixed, weight)
                 and (residual is None or residual.dtype == mixed.dtype)):
             res = residual[:, 0] if residual is not None else None
-            return ops.linear(mixed, out_proj.weight, res).unsqueeze(1), next_cache
+            return ops.linear(mixed, weight, res).unsqueeze(1), next_cache
         output = (out_proj(mixed) if small
                   else self._project("out_proj", mixed, copies.get("out8"))).unsqueeze(1)
         if residual is not None:
@@ -622,8 +624,11 @@ def _compute_dtype(x: torch.Tensor) -> torch.dtype:
 def _plain_linear(module: nn.Module) -> bool:
     """Whether calling ``module`` is its weight's product and nothing else, so that a kernel or a copy of the
     weight may stand in for it: ``nn.Linear``'s own forward, without a bias or forward hooks."""
-    return (type(module).forward is nn.Linear.forward and "forward" not in module.__dict__
-            and module.bias is None and not module._forward_hooks and not module._forward_pre_hooks)
+    if type(module).forward is not nn.Linear.forward:
+        return False
+    own = module.__dict__  # a module's attributes take several times as long, twice a layer of a decode step
+    return ("forward" not in own and not own["_forward_hooks"] and not own["_forward_pre_hooks"]
+            and own["_parameters"].get("bias", own) is None)
 
 
 def _require_plain(maker: str, name: str, module: nn.Module) -> None:
