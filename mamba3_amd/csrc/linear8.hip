@@ -14,10 +14,11 @@
 // the launch and a few latencies of memory: 28672 x 8192 at 1 row 39.4 us (6 TB/s, in part from the last-level
 // cache), 8672 x 2048 at 1 row 5.3 us, 2048 x 4096 at 16 rows 5.8 us.
 //
-// linear8_tile_kernel (the rest): below. Bound by the matrix units and their power where K is long: 8192 x 28672 x
-// 8192 takes 1,300 us, 2.96 POP/s, the units busy 77% of the cycles at 1.83 GHz; products of such values alone,
-// without a load, reach 3.95 POP/s here (4.87 of zeros), a library's product of int8 2.30. Where K is short (65536 x
-// 4480 x 1024: 264 to 285 us, units busy 59%), also by what is written (587 MB) and the rounding of the outputs.
+// linear8_tile_kernel (the rest): below. Where K is long 8192 x 28672 x 8192 takes 1,300 to 1,360 us, 2.96 POP/s in
+// the quickest: the matrix units are busy 77% of the cycles at 1.83 GHz, which is nearly the clock that products of such
+// values alone, without a load, run at here (3.95 POP/s; 4.87 of zeros; a library's product of int8 2.30). Bound by
+// what the units wait for in the other 23%. Where K is short (65536 x 4480 x 1024: 264 to 285 us, units busy 59%),
+// also by what is written (587 MB) and the rounding of the outputs.
 #include <hip/hip_runtime.h>
 
 #include "m3_common.hpp"

@@ -14,8 +14,10 @@
 //
 // Bound by memory: the row stays in registers between the two passes over it (its maximum, its codes), so
 // x, add, the sum and the codes each move once. Measured (a large copy reaches 5.0 to 5.5 TB/s): 65536 x 1024 FP32 with
-// a bf16 add and the sum kept 138 us (5.35 TB/s of what moves), 16384 x 2048 bf16 the same way 47.5 us (4.95),
-// 32768 x 4096 bf16 without norm 77.5 us (5.2), one row of 2048 3.5 us.
+// a bf16 add and the sum kept 138 to 145 us (5.35 to 5.1 TB/s of what moves), 16384 x 2048 bf16 the same way 43 to 47.5
+// us (5.5 to 4.95), 32768 x 4096 without norm f16 76 us (5.3), bf16 77 to 97 (5.2 to 4.2), FP32 118 (5.7), one row of 2048
+// 3.5 us. Rows over 8,192 wide do not fit and are walked twice: 8192 x 16384 bf16 107 us (3.8), of FP32 with a bf16
+// add, norm and sum 358 (4.1).
 //
 // m3_rows8_values, what the rows stand for, likewise: 32768 x 4096 to FP32 104 us (6.4 TB/s).
 #include <hip/hip_runtime.h>
